@@ -1,5 +1,7 @@
 """B200-native (sm_100a) W8A8 / FP8 linear family with the reference's
-operator interface.
+operator interface, the low-rank adapters that run beside it, and what training
+them needs: their gradients, the linear's input gradient, and activations kept
+in 8 bits.
 
 The operators load libw8a8.so on first use and raise if it is missing (there
 is no fallback).  Importing the package itself does not load the library, so
@@ -32,12 +34,30 @@ _OPS = (
     "mxfp8_linear",
 )
 
-__all__ = list(_OPS)
+_ADAPTER_OPS = (
+    "int8_linear_backward",
+    "int8_linear_lora",
+    "lora_add",
+    "lora_backward",
+)
+
+_ACTIVATION_OPS = (
+    "act_backward_int8",
+    "act_checkpoint_int8",
+    "checkpointed_activation",
+)
+
+__all__ = [*_OPS, *_ADAPTER_OPS, *_ACTIVATION_OPS]
 
 
 def __getattr__(name):
     if name in _OPS:
-        from . import linear
-
-        return getattr(linear, name)
-    raise AttributeError(name)
+        from . import linear as module
+    elif name in _ADAPTER_OPS:
+        from . import adapters as module
+    elif name in _ACTIVATION_OPS:
+        from . import activation as module
+    else:
+        raise AttributeError(name)
+    value = globals()[name] = getattr(module, name)  # later look-ups skip this function
+    return value

@@ -26,6 +26,8 @@ MAX_RANKS, PEER_FLAG_WORDS = 8, 32
 SCALE_EAGER, SCALE_KITCHEN, SCALE_KITCHEN_CUDA = 0, 1, 2
 DQ_EAGER, DQ_SCALE_PRODUCT, DQ_CHAINED, DQ_SEPARATE = 0, 1, 2, 3
 ACT_NONE, ACT_GELU_TANH = 0, 1
+CKPT_GROUP = 128
+CKPT_GELU_TANH, CKPT_SWIGLU, CKPT_SILU = 1, 2, 3
 STEP_DENOISED, STEP_EULER, STEP_ER_SDE, STEP_CHURN = 0, 1, 2, 3
 
 
@@ -128,6 +130,17 @@ SIGNATURES = {
     "w8a8_fp8_gemm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _CFG, _vp]),
     "w8a8_quantize_mxfp8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "w8a8_mxfp8_gemm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _CFG, _vp]),
+    "w8a8_lora_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i32]),
+    "w8a8_lora_add": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _vp,
+                             _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "w8a8_lora_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _i32,
+                                  _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i64,
+                                  _i64, _vp, _i64, _vp]),
+    "w8a8_input_grad_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
+    "w8a8_input_grad": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i64,
+                               _vp, _i64, _vp]),
+    "w8a8_act_checkpoint": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "w8a8_act_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp]),
     "w8a8_sampler_step": (_i32, [_vp, _vp, _vp, _i32, _i64, _vp, ctypes.POINTER(SamplerStep), _vp,
                                  _vp, _vp, _vp, _vp]),
 }

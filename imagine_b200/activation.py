@@ -1,0 +1,99 @@
+"""Activations that keep their input in 8 bits for the backward pass.
+
+``act_checkpoint_int8`` computes the activation and the checkpoint of its input
+(int8 codes, one fp32 scale for every 128 elements of a row), ``act_backward_int8`` the
+gradient from the checkpoint; ``checkpointed_activation`` is the two as one
+differentiable operator.  The numeric steps run in libw8a8 (include/w8a8.h); there
+is no CPU path.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as N
+from . import linear as L
+from .adapters import _on, _rows
+from .linear import _code, _cuda, _vp
+
+ACTIVATIONS = {"gelu_tanh": N.CKPT_GELU_TANH, "swiglu": N.CKPT_SWIGLU, "silu": N.CKPT_SILU}
+
+
+def _act(act: str) -> tuple:
+    if act not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {act!r}; one of {', '.join(sorted(ACTIVATIONS))}")
+    return ACTIVATIONS[act], 2 if act == "swiglu" else 1
+
+
+def _groups(k: int) -> int:
+    return -(-k // N.CKPT_GROUP)
+
+
+def act_checkpoint_int8(x: torch.Tensor, act: str = "gelu_tanh"):
+    """``act(x)`` and the 8-bit checkpoint of x: ``(y [..., K], q int8, scale fp32)``.
+
+    ``gelu_tanh`` and ``silu`` take x [..., K]; ``swiglu`` takes [..., 2K] rows
+    ``[gate | up]`` and gives ``silu(gate) * up``.  Each half of a row is cut into
+    groups of 128 (the last may be shorter): ``scale = max(amax / 127, 1e-30)``, ``q =
+    round(x / scale)`` (half to even).  q has x's shape, scale [..., halves *
+    ceil(K / 128)].  A group that holds an infinity or a NaN keeps NaN as its scale, and so
+    gives NaN gradients."""
+    code, halves = _act(act)
+    dev = _cuda("x", x).device
+    width = x.shape[-1]
+    if width % halves:
+        raise ValueError(f"swiglu rows are [gate | up]: {width} features do not halve")
+    k = width // halves
+    x2, ldx = _rows(x)
+    m = x2.shape[0]
+    y = torch.empty((*x.shape[:-1], k), dtype=x.dtype, device=dev)
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    scale = torch.empty((*x.shape[:-1], halves * _groups(k)), dtype=torch.float32, device=dev)
+    with _on(dev):
+        N.check(N.LIB.w8a8_act_checkpoint(_vp(x2), _code(x.dtype), ldx, m, k, code, _vp(y), _vp(q),
+                                          _vp(scale), L._stream(dev)))
+    return y, q, scale
+
+
+def act_backward_int8(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
+                      act: str = "gelu_tanh") -> torch.Tensor:
+    """Gradient of ``act_checkpoint_int8``'s input from its checkpoint: ``dy *
+    act'(q * scale)`` in dy's dtype, of q's shape."""
+    code, halves = _act(act)
+    dev = _cuda("dy", dy).device
+    _cuda("q", q, dev)
+    _cuda("scale", scale, dev)
+    k = dy.shape[-1]
+    lead = tuple(dy.shape[:-1])
+    if q.dtype != torch.int8 or tuple(q.shape) != (*lead, halves * k):
+        raise ValueError(f"q must be int8 {(*lead, halves * k)}, got {tuple(q.shape)} of {q.dtype}")
+    if scale.dtype != torch.float32 or tuple(scale.shape) != (*lead, halves * _groups(k)):
+        raise ValueError(f"scale must be fp32 {(*lead, halves * _groups(k))}, got "
+                         f"{tuple(scale.shape)} of {scale.dtype}")
+    dy2, lddy = _rows(dy)
+    q = q.contiguous()
+    scale = scale.contiguous()
+    dx = torch.empty(q.shape, dtype=dy.dtype, device=dev)
+    with _on(dev):
+        N.check(N.LIB.w8a8_act_backward(_vp(dy2), _code(dy.dtype), lddy, dy2.shape[0], k, code, _vp(q),
+                                        _vp(scale), _vp(dx), L._stream(dev)))
+    return dx
+
+
+class _Checkpointed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, act):
+        y, q, scale = act_checkpoint_int8(x, act)
+        ctx.act = act
+        ctx.save_for_backward(q, scale)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return act_backward_int8(dy, *ctx.saved_tensors, ctx.act), None
+
+
+def checkpointed_activation(x: torch.Tensor, act: str = "gelu_tanh") -> torch.Tensor:
+    """``act(x)``, differentiable, keeping x for the backward pass as its 8-bit
+    checkpoint (half of a bf16 input's bytes, and 1/32 more for the scales)."""
+    return _Checkpointed.apply(x, act)

@@ -1,0 +1,309 @@
+"""Low-rank adapters beside the W8A8 linears, and what training them needs.
+
+``lora_add`` adds the adapters of many requests to one shared projection's
+output; ``lora_backward`` gives their gradients, from the projection's input or
+from the int8 codes the W8A8 linear made of it; ``int8_linear_backward`` is the
+frozen linear's input gradient; ``int8_linear_lora`` puts the three together as
+one differentiable operator.  The numeric steps run in libw8a8 through the C ABI
+(include/w8a8.h), as in ``imagine_b200.linear``: there is no CPU path.
+
+``lora_add``, ``lora_backward`` and ``int8_linear_backward`` do not record
+themselves for autograd; ``int8_linear_lora`` does.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _native as N
+from . import linear as L
+from .linear import _code, _cuda, _vp
+
+
+def _on(dev: torch.device):
+    """The device made current for the launch, where it is not already."""
+    if torch.cuda.current_device() == dev.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _rows(t: torch.Tensor) -> tuple:
+    """``t`` as [rows, width] with unit-stride rows that do not overlap (a view
+    where its strides allow, else a copy), and its row stride."""
+    width = t.shape[-1]
+    m = math.prod(t.shape[:-1])
+    t2 = t if t.dim() == 2 else t.reshape(m, width)
+    if (t2.stride(1) != 1 and width > 1) or (m > 1 and t2.stride(0) < width):
+        t2 = t2.contiguous()
+    return t2, (t2.stride(0) if m > 1 else max(width, 1))
+
+
+def _out_rows(name: str, t: torch.Tensor, shape, dtype, dev) -> tuple:
+    """The same for an output, which has to be written in place."""
+    _cuda(name, t, dev)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError(f"{name} must be {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    try:
+        t2 = t.view(math.prod(t.shape[:-1]), t.shape[-1])
+    except RuntimeError as e:
+        raise ValueError(f"{name} must have rows one stride apart") from e
+    width, m = t2.shape[1], t2.shape[0]
+    if t2.numel() and ((t2.stride(1) != 1 and width > 1) or (m > 1 and t2.stride(0) < width)):
+        raise ValueError(f"{name} must have unit-stride rows that do not overlap")
+    return t2, (t2.stride(0) if m > 1 else max(width, 1))
+
+
+def _adapters(a, b, k: int, n: int, dtype, dev) -> tuple:
+    """The stacked adapters, checked, each contiguous: (a, b, S, R)."""
+    _cuda("a", a, dev)
+    _cuda("b", b, dev)
+    if a.dim() != 3 or b.dim() != 3:
+        raise ValueError("a must be [adapters, rank, K] and b [adapters, N, rank]")
+    s, r, ka = a.shape
+    if ka != k or tuple(b.shape) != (s, n, r):
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} do not fit inputs of {k} and "
+                         f"outputs of {n} features")
+    if a.dtype != dtype or b.dtype != dtype:
+        raise ValueError(f"a and b must be {dtype}, got {a.dtype} and {b.dtype}")
+    if s < 1:
+        raise ValueError("at least one adapter is needed")
+    if not 1 <= r <= 128:
+        raise ValueError(f"rank must be 1 to 128, got {r}")
+    # a slice of a larger stack is taken as it lies
+    if a.stride(2) != 1 or a.stride(1) != k or (s > 1 and a.stride(0) < r * k):
+        a = a.contiguous()
+    if b.stride(2) != 1 or b.stride(1) != r or (s > 1 and b.stride(0) < n * r):
+        b = b.contiguous()
+    return a, b, s, r
+
+
+def _index(adapter, lead, m: int, dev) -> tuple:
+    """(index tensor or None, 1 for int64, rows per index).  ``adapter`` has the
+    leading dimensions of the rows it covers: [B, S] for each token, [B] for each sample."""
+    if adapter is None:
+        return None, 0, 1
+    _cuda("adapter", adapter, dev)
+    if adapter.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"adapter must be int32 or int64, got {adapter.dtype}")
+    if tuple(adapter.shape) != tuple(lead[:adapter.dim()]):
+        raise ValueError(f"adapter {tuple(adapter.shape)} must have the leading dimensions of {tuple(lead)}")
+    if not adapter.is_contiguous():
+        adapter = adapter.contiguous()
+    count = adapter.numel()
+    return adapter, int(adapter.dtype == torch.int64), max(1, m // max(count, 1))
+
+
+def _scaling(scaling, s: int, dev):
+    if scaling is None:
+        return None
+    if isinstance(scaling, (int, float)):
+        return torch.full((s,), float(scaling), dtype=torch.float32, device=dev)
+    _cuda("scaling", scaling, dev)
+    if scaling.numel() != s or scaling.dtype != torch.float32:
+        raise ValueError(f"scaling must be fp32 with one value for each of {s} adapters, got "
+                         f"{tuple(scaling.shape)} of {scaling.dtype}")
+    return scaling.reshape(-1).contiguous()
+
+
+def _workspace(nbytes: int, dev):
+    N.check(nbytes if nbytes < 0 else 0)
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+             adapter: Optional[torch.Tensor] = None, scaling=None, *,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The low-rank adapters of a batch's requests, added to the output of the
+    projection they share: ``out = y + scaling[s] * (x a[s]^T) b[s]^T``.
+
+    ``y`` [..., N] is the projection's output for ``x`` [..., K], ``a`` [S, R, K]
+    and ``b`` [S, N, R] the stacked adapters (R 1 to 128; smaller ones padded
+    with zeros), all of one dtype (bf16, f16 or fp32).  ``adapter`` (int32 or int64)
+    is each row's adapter and has x's leading dimensions or the first of them
+    ([B] for [B, S, K]: one for each sample); an index outside [0, S), such as
+    -1, means no adapter and returns y's row.  None: adapter 0 everywhere.
+    ``scaling``: fp32 [S], or one number.  ``out`` may be ``y``, to add in place.
+
+    The contraction over K and the rank are summed in fp32 and the result is
+    rounded once; the same call gives the same bits."""
+    dev = _cuda("x", x).device
+    _cuda("y", y, dev)
+    lead, k, n = x.shape[:-1], x.shape[-1], y.shape[-1]
+    if y.shape[:-1] != lead:
+        raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} must have the same rows")
+    if y.dtype != x.dtype:
+        raise ValueError(f"x is {x.dtype} but y {y.dtype}")
+    code = _code(x.dtype)
+    a, b, s, r = _adapters(a, b, k, n, x.dtype, dev)
+    y2, ldy = _rows(y)
+    x2, ldx = _rows(x)
+    m = y2.shape[0]
+    idx, idx64, per = _index(adapter, lead, m, dev)
+    c = _scaling(scaling, s, dev)
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=dev)
+    o2, ldo = _out_rows("out", out, y.shape, y.dtype, dev)
+    with _on(dev):
+        ws = _workspace(N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 0), dev)
+        N.check(N.LIB.w8a8_lora_add(
+            _vp(y2), ldy, _vp(x2), ldx, code, _vp(a), a.stride(0), _vp(b), b.stride(0), _vp(idx), idx64,
+            per, _vp(c), _vp(o2), ldo, m, n, k, s, r, _vp(ws), ws.numel() if ws is not None else 0,
+            L._stream(dev)))
+    return out
+
+
+def lora_backward(dy: torch.Tensor, x: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor,
+                  adapter: Optional[torch.Tensor] = None, scaling=None, *,
+                  x_scale: Optional[torch.Tensor] = None, dx: Optional[torch.Tensor] = None,
+                  need_dx: bool = True, need_weights: bool = True):
+    """Gradients of ``lora_add`` for ``dy`` [..., N]: ``(dx, da, db)``.
+
+    ``dx = scaling[s] * (dy b[s]) a[s]`` (zero in rows without an adapter),
+    ``da[s]`` and ``db[s]`` the sums over the rows of adapter s (zero without
+    rows), all in dy's dtype.  ``x`` is the forward input, or with ``x_scale`` the
+    int8 codes of ``quantize_int8_rowwise`` (its 8-bit checkpoint; one fp32 scale a
+    row).  A given ``dx`` (the base linear's input gradient) is added to, in place.
+    ``need_dx`` / ``need_weights`` False: None in their place (x may then be None)."""
+    dev = _cuda("dy", dy).device
+    lead, n, k = dy.shape[:-1], dy.shape[-1], a.shape[-1]
+    code = _code(dy.dtype)
+    a, b, s, r = _adapters(a, b, k, n, dy.dtype, dev)
+    dy2, lddy = _rows(dy)
+    m = dy2.shape[0]
+    x2, ldx, xs = None, k, None
+    if need_weights:
+        _cuda("x", x, dev)
+        if tuple(x.shape) != (*lead, k):
+            raise ValueError(f"x {tuple(x.shape)} does not fit dy {tuple(dy.shape)} and inputs of {k} features")
+        if x.dtype != (torch.int8 if x_scale is not None else dy.dtype):
+            raise ValueError(f"x is {x.dtype}: int8 codes come with x_scale, anything else is dy's {dy.dtype}")
+        if x_scale is not None:
+            _cuda("x_scale", x_scale, dev)
+            if x_scale.dtype != torch.float32 or x_scale.numel() != m:
+                raise ValueError(f"x_scale must be fp32 with one value for each of {m} rows")
+            xs = x_scale.reshape(-1).contiguous()
+        x2, ldx = _rows(x)
+    idx, idx64, per = _index(adapter, lead, m, dev)
+    c = _scaling(scaling, s, dev)
+    accumulate = dx is not None
+    if need_dx and dx is None:
+        dx = torch.empty((*lead, k), dtype=dy.dtype, device=dev)
+    d2, lddx = _out_rows("dx", dx, (*lead, k), dy.dtype, dev) if need_dx else (None, k)
+    da = db = None
+    if need_weights:
+        da = torch.empty((s, r, k), dtype=dy.dtype, device=dev)
+        db = torch.empty((s, n, r), dtype=dy.dtype, device=dev)
+    with _on(dev):
+        ws = _workspace(N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 1), dev)
+        N.check(N.LIB.w8a8_lora_backward(
+            _vp(dy2), lddy, _vp(x2), ldx, _vp(xs), code, _vp(a), a.stride(0), _vp(b), b.stride(0),
+            _vp(idx), idx64, per, _vp(c), _vp(d2), lddx, int(accumulate), _vp(da), _vp(db), m, n, k,
+            s, r, _vp(ws), ws.numel() if ws is not None else 0, L._stream(dev)))
+    return (dx if need_dx else None), da, db
+
+
+def int8_linear_backward(dy: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
+                         out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Input gradient of ``int8_linear``: ``dx = dy (weight_scale * weight)`` for
+    ``dy`` [..., N] and the int8 ``weight`` [N, K] with its scales (N or 1), dx
+    [..., K] in dy's dtype.  The quantisation of the input passes the gradient through
+    unchanged (the straight-through estimate)."""
+    dev = _cuda("dy", dy).device
+    _cuda("weight", weight, dev)
+    if weight.dim() != 2 or weight.dtype != torch.int8:
+        raise ValueError("weight must be a 2-D int8 tensor [N, K]")
+    if out_dtype not in (None, dy.dtype):
+        raise ValueError(f"the gradient of {dy.dtype} is {dy.dtype}, not {out_dtype}")
+    n, k = weight.shape
+    if dy.shape[-1] != n:
+        raise ValueError(f"dy has {dy.shape[-1]} features, the weight {n} outputs")
+    ws = weight_scale.to(device=dev, dtype=torch.float32).reshape(-1).contiguous()
+    if ws.numel() not in (1, n):
+        raise ValueError(f"INT8 weight scale must be scalar or per-output-channel, got "
+                         f"{tuple(weight_scale.shape)} for weight shape {tuple(weight.shape)}")
+    code = _code(dy.dtype)
+    dy2, lddy = _rows(dy)
+    w2, ldw = _rows(weight)
+    m = dy2.shape[0]
+    dx = torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dev)
+    with _on(dev):
+        work = _workspace(N.LIB.w8a8_input_grad_workspace_bytes(m, n, k, code), dev)
+        N.check(N.LIB.w8a8_input_grad(
+            _vp(dy2), lddy, _vp(w2), ldw, _vp(ws), ws.numel(), code, _vp(dx), k, m, n, k, _vp(work),
+            work.numel() if work is not None else 0, L._stream(dev)))
+    return dx
+
+
+class _Int8LinearLora(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, weight_scale, bias, a, b, adapter, scaling, keep_input):
+        dev = x.device
+        n, k = weight.shape
+        ws = weight_scale.to(device=dev, dtype=torch.float32).reshape(-1).contiguous()
+        x2, ldx = _rows(x)
+        m = x2.shape[0]
+        w = weight if weight.is_contiguous() else weight.contiguous()
+        q, xs = L.quantize_int8_rowwise(x2)
+        bias = None if bias is None else bias.to(device=dev, dtype=x.dtype).reshape(-1).contiguous()
+        if bias is not None and bias.numel() != n:
+            raise ValueError(f"bias has {bias.numel()} elements for {n} outputs")
+        y = torch.empty((m, n), dtype=x.dtype, device=dev)
+        ep = L._epilogue(ws, bias, None, None, "eager", None, n, n)
+        stream = L._stream(dev)
+        if 1 <= m <= 2:
+            N.check(N.LIB.w8a8_gemv_dequant(_vp(q), _vp(w), _vp(xs), ctypes.byref(ep), _vp(y),
+                                            _code(x.dtype), m, n, k, stream))
+        elif m > 0:
+            L._gemm_dequant(q, w, xs.reshape(-1), ep, y, x.dtype, m, n, k, None, None, stream)
+        y = y.reshape(*x.shape[:-1], n)
+        lora_add(y, x, a, b, adapter, scaling, out=y)
+        kept = (x, None) if keep_input else (q.reshape(x.shape), xs)
+        ctx.save_for_backward(*kept, w, ws, a, b, adapter, scaling)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, xs, w, ws, a, b, adapter, scaling = ctx.saved_tensors
+        need_x, need_a, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[4], ctx.needs_input_grad[5]
+        with _on(dy.device):
+            dx = int8_linear_backward(dy, w, ws) if need_x else None
+            da = db = None
+            if need_x or need_a or need_b:
+                dx, da, db = lora_backward(dy, x, a, b, adapter, scaling, x_scale=xs, dx=dx,
+                                           need_dx=need_x, need_weights=need_a or need_b)
+        return (dx, None, None, None, da if need_a else None, db if need_b else None, None, None, None)
+
+
+def int8_linear_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                     bias: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor,
+                     adapter: Optional[torch.Tensor] = None, scaling=None, *,
+                     keep_input: bool = False) -> torch.Tensor:
+    """``lora_add(int8_linear(x, weight, weight_scale, bias), x, a, b, adapter,
+    scaling)`` with gradients for x, a and b (the int8 weight, its scales and the
+    bias are frozen).
+
+    For the backward pass it keeps the int8 codes that the linear made of x
+    (half of a bf16 input's bytes), from which da and db are taken; with ``keep_input`` it
+    keeps x itself instead.  Operands as in the two operators."""
+    dev = _cuda("x", x).device
+    with _on(dev):
+        _cuda("weight", weight, dev)
+        if weight.dim() != 2 or weight.dtype != torch.int8:
+            raise ValueError("weight must be a 2-D int8 tensor [N, K]")
+        n, k = weight.shape
+        if x.shape[-1] != k:
+            raise ValueError(f"Input and weight inner dimensions must match, got {x.shape[-1]} and {k}")
+        if k == 0:
+            raise ValueError("int8_linear_lora needs K > 0")
+        if weight_scale.numel() not in (1, n):
+            raise ValueError(f"INT8 weight scale must be scalar or per-output-channel, got "
+                             f"{tuple(weight_scale.shape)} for weight shape {tuple(weight.shape)}")
+        _code(x.dtype)
+        _, _, s, _ = _adapters(a, b, k, n, x.dtype, dev)
+        scaling = _scaling(scaling, s, dev)
+        return _Int8LinearLora.apply(x, weight, weight_scale, bias, a, b, adapter, scaling, keep_input)

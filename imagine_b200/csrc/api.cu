@@ -872,4 +872,231 @@ int w8a8_mxfp8_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
   return finish(gemm_launch(g, static_cast<cudaStream_t>(stream)));
 }
 
+// ---- low-rank adapters, their gradients, the linear's input gradient, and
+// ---- activations with an 8-bit checkpoint
+namespace {
+
+constexpr int64_t kMaxDim = 0x7fffff00LL;
+
+bool bad_align(const void* p, int64_t unit) { return reinterpret_cast<uintptr_t>(p) % unit != 0; }
+
+int64_t float_size(int dtype) { return dtype == W8A8_F32 ? 4 : 2; }
+
+int check_lora_shape(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R) {
+  if (M < 0 || N < 0 || K < 0) return fail(W8A8_ERR_VALUE, "lora: negative shape");
+  if (R < 1 || R > 128) {
+    return fail(W8A8_ERR_VALUE, "lora: rank must be 1 to 128, got %lld", static_cast<long long>(R));
+  }
+  if (S < 1 || S > 65535) {
+    return fail(W8A8_ERR_VALUE, "lora: 1 to 65535 adapters, got %lld", static_cast<long long>(S));
+  }
+  if (M > kMaxDim || N > kMaxDim || K > kMaxDim) {
+    return fail(W8A8_ERR_VALUE, "lora: sizes up to %lld", static_cast<long long>(kMaxDim));
+  }
+  const int64_t cols = ((N > K ? N : K) + 127) / 128;
+  if (((M + 63) / 64) * cols > 0x7fffffffLL || cols > 0x7fffffffLL) {
+    return fail(W8A8_ERR_VALUE, "lora: too many output tiles");
+  }
+  return 0;
+}
+
+int check_lora_common(const LoraArgs& g, int64_t workspace_bytes, int backward) {
+  if (!is_float_dtype(g.dtype)) return fail(W8A8_ERR_VALUE, "lora: dtype code %d is not floating", g.dtype);
+  if (g.rows_per_index < 1) return fail(W8A8_ERR_VALUE, "lora: rows_per_index must be >= 1");
+  if ((!g.a && g.K > 0) || (!g.b && g.N > 0)) {
+    return fail(W8A8_ERR_VALUE, "lora: NULL adapter pointer");
+  }
+  if (g.S > 1 && (g.lda < g.R * g.K || g.ldb < g.N * g.R)) {
+    return fail(W8A8_ERR_VALUE, "lora: adapters overlap (slot stride smaller than the adapter)");
+  }
+  const int64_t size = float_size(g.dtype);
+  if (bad_align(g.a, size) || bad_align(g.b, size) || bad_align(g.y, size) || bad_align(g.out, size) ||
+      bad_align(g.x, g.x_scale ? 1 : size) || bad_align(g.scaling, 4) || bad_align(g.x_scale, 4) ||
+      bad_align(g.adapter, g.adapter64 ? 8 : 4)) {
+    return fail(W8A8_ERR_VALUE, "lora: pointer not aligned to its element");
+  }
+  const int64_t need = lora_workspace_bytes(g.M, g.N, g.K, g.S, g.R, backward);
+  if (workspace_bytes < need || (need > 0 && (!g.workspace || bad_align(g.workspace, 256)))) {
+    return fail(W8A8_ERR_VALUE, "lora: workspace of %lld bytes, %lld needed (256-byte aligned)",
+                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  }
+  return 0;
+}
+
+}  // namespace
+
+int64_t w8a8_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R,
+                                  int backward) {
+  if (int rc = check_lora_shape(M, N, K, S, R)) return rc;
+  return lora_workspace_bytes(M, N, K, S, R, backward);
+}
+
+int w8a8_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dtype, const void* a,
+                  int64_t slot_a, const void* b, int64_t slot_b, const void* adapter,
+                  int adapter_is_64, int64_t rows_per_index, const float* scaling, void* out,
+                  int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t S, int64_t R,
+                  void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check_lora_shape(M, N, K, S, R)) return rc;
+  if (M == 0 || N == 0) return finish(0);
+  if (!y || !out || (!x && K > 0)) return fail(W8A8_ERR_VALUE, "NULL tensor pointer");
+  if (ldx < K || ldy < N || ldo < N) return fail(W8A8_ERR_VALUE, "row stride smaller than the row");
+  if (y == out && ldy != ldo) return fail(W8A8_ERR_VALUE, "lora: out is y with another row stride");
+  LoraArgs g{};
+  g.dtype = dtype;
+  g.x = x;
+  g.ldx = ldx;
+  g.y = y;
+  g.ldy = ldy;
+  g.a = a;
+  g.lda = slot_a;
+  g.b = b;
+  g.ldb = slot_b;
+  g.adapter = adapter;
+  g.adapter64 = adapter_is_64 != 0;
+  g.rows_per_index = rows_per_index;
+  g.scaling = scaling;
+  g.out = out;
+  g.ldo = ldo;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.S = S;
+  g.R = R;
+  g.workspace = workspace;
+  if (int rc = check_lora_common(g, workspace_bytes, 0)) return rc;
+  return finish(lora_add_launch(g, static_cast<cudaStream_t>(stream)));
+}
+
+int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                       const float* x_scale, int dtype, const void* a, int64_t slot_a,
+                       const void* b, int64_t slot_b, const void* adapter, int adapter_is_64,
+                       int64_t rows_per_index, const float* scaling, void* dx, int64_t lddx,
+                       int accumulate, void* da, void* db, int64_t M, int64_t N, int64_t K,
+                       int64_t S, int64_t R, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
+  if (int rc = check_lora_shape(M, N, K, S, R)) return rc;
+  if ((da == nullptr) != (db == nullptr)) return fail(W8A8_ERR_VALUE, "lora: da and db go together");
+  if (N == 0 || K == 0) return fail(W8A8_ERR_VALUE, "lora: gradients need N > 0 and K > 0");
+  if (!dx && !da) return finish(0);
+  if (M > 0) {
+    if (!dy || (da && !x)) return fail(W8A8_ERR_VALUE, "NULL tensor pointer");
+    if (lddy < N || (da && ldx < K) || (dx && lddx < K)) {
+      return fail(W8A8_ERR_VALUE, "row stride smaller than the row");
+    }
+  } else if (!da) {
+    return finish(0);
+  }
+  LoraArgs g{};
+  g.dtype = dtype;
+  g.x = x;
+  g.ldx = ldx;
+  g.x_scale = x_scale;
+  g.y = dy;
+  g.ldy = lddy;
+  g.a = a;
+  g.lda = slot_a;
+  g.b = b;
+  g.ldb = slot_b;
+  g.adapter = adapter;
+  g.adapter64 = adapter_is_64 != 0;
+  g.rows_per_index = rows_per_index;
+  g.scaling = scaling;
+  g.out = dx;
+  g.ldo = lddx;
+  g.accumulate = accumulate != 0;
+  g.da = da;
+  g.db = db;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.S = S;
+  g.R = R;
+  g.workspace = workspace;
+  if (int rc = check_lora_common(g, workspace_bytes, 1)) return rc;
+  const int64_t size = float_size(dtype);
+  if (bad_align(da, size) || bad_align(db, size)) {
+    return fail(W8A8_ERR_VALUE, "lora: pointer not aligned to its element");
+  }
+  return finish(lora_backward_launch(g, static_cast<cudaStream_t>(stream)));
+}
+
+int64_t w8a8_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
+  if (M < 0 || N < 0 || K < 0) return fail(W8A8_ERR_VALUE, "negative shape");
+  if (!is_float_dtype(dtype)) return fail(W8A8_ERR_VALUE, "dtype code %d is not floating", dtype);
+  if (M > kMaxDim || N > kMaxDim || K > kMaxDim ||
+      ((M + 63) / 64) * ((K + 127) / 128) > 0x7fffffffLL) {
+    return fail(W8A8_ERR_VALUE, "input_grad: sizes up to %lld", static_cast<long long>(kMaxDim));
+  }
+  return input_grad_workspace_bytes(M, N, K, dtype);
+}
+
+int w8a8_input_grad(const void* dy, int64_t lddy, const int8_t* w, int64_t ldw, const float* ws,
+                    int64_t ws_numel, int dtype, void* dx, int64_t lddx, int64_t M, int64_t N,
+                    int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int64_t need = w8a8_input_grad_workspace_bytes(M, N, K, dtype);
+  if (need < 0) return static_cast<int>(need);
+  if (M == 0 || K == 0) return finish(0);
+  if (!dx || (N > 0 && (!dy || !w || !ws))) return fail(W8A8_ERR_VALUE, "NULL tensor pointer");
+  if (lddy < N || ldw < K || lddx < K) return fail(W8A8_ERR_VALUE, "row stride smaller than the row");
+  if (ws_numel != 1 && ws_numel != N) {
+    return fail(W8A8_ERR_VALUE,
+                "INT8 weight scale must be scalar or per-output-channel, got %lld for N=%lld",
+                static_cast<long long>(ws_numel), static_cast<long long>(N));
+  }
+  const int64_t size = float_size(dtype);
+  if (bad_align(dy, size) || bad_align(dx, size) || bad_align(ws, 4)) {
+    return fail(W8A8_ERR_VALUE, "pointer not aligned to its element");
+  }
+  if (workspace_bytes < need || (need > 0 && (!workspace || bad_align(workspace, 256)))) {
+    return fail(W8A8_ERR_VALUE, "input_grad: workspace of %lld bytes, %lld needed (256-byte aligned)",
+                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  }
+  InputGradArgs g{dtype, dy, lddy, w, ldw, ws, ws_numel, dx, lddx, M, N, K, workspace};
+  return finish(input_grad_launch(g, static_cast<cudaStream_t>(stream)));
+}
+
+namespace {
+int check_act(int dtype, int64_t rows, int64_t cols, int act) {
+  if (rows < 0 || cols < 0) return fail(W8A8_ERR_VALUE, "negative shape");
+  if (!is_float_dtype(dtype)) return fail(W8A8_ERR_VALUE, "dtype code %d is not floating", dtype);
+  if (act < W8A8_CKPT_ACT_GELU_TANH || act > W8A8_CKPT_ACT_SILU) {
+    return fail(W8A8_ERR_VALUE, "unknown checkpointed activation %d", act);
+  }
+  if (rows > kMaxDim || cols > kMaxDim / 2) {
+    return fail(W8A8_ERR_VALUE, "act_checkpoint: sizes up to %lld", static_cast<long long>(kMaxDim));
+  }
+  return 0;
+}
+}  // namespace
+
+int w8a8_act_checkpoint(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, int act,
+                        void* y, int8_t* q, float* scale, void* stream) {
+  if (int rc = check_act(dtype, rows, cols, act)) return rc;
+  if (rows == 0 || cols == 0) return finish(0);
+  if (!x || !y || !q || !scale) return fail(W8A8_ERR_VALUE, "NULL tensor pointer");
+  if (ldx < cols * (act == W8A8_CKPT_ACT_SWIGLU ? 2 : 1)) {
+    return fail(W8A8_ERR_VALUE, "row stride smaller than the row");
+  }
+  const int64_t size = float_size(dtype);
+  if (bad_align(x, size) || bad_align(y, size) || bad_align(scale, 4)) {
+    return fail(W8A8_ERR_VALUE, "pointer not aligned to its element");
+  }
+  return finish(act_checkpoint_launch(x, dtype, ldx, rows, cols, act, y, q, scale,
+                                      static_cast<cudaStream_t>(stream)));
+}
+
+int w8a8_act_backward(const void* dy, int dtype, int64_t lddy, int64_t rows, int64_t cols, int act,
+                      const int8_t* q, const float* scale, void* dx, void* stream) {
+  if (int rc = check_act(dtype, rows, cols, act)) return rc;
+  if (rows == 0 || cols == 0) return finish(0);
+  if (!dy || !q || !scale || !dx) return fail(W8A8_ERR_VALUE, "NULL tensor pointer");
+  if (lddy < cols) return fail(W8A8_ERR_VALUE, "row stride smaller than the row");
+  const int64_t size = float_size(dtype);
+  if (bad_align(dy, size) || bad_align(dx, size) || bad_align(scale, 4)) {
+    return fail(W8A8_ERR_VALUE, "pointer not aligned to its element");
+  }
+  return finish(act_backward_launch(dy, dtype, lddy, rows, cols, act, q, scale, dx,
+                                    static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -1,0 +1,867 @@
+// Low-rank adapters beside a W8A8 projection: many adapters in one batch, and
+// their gradients.
+//
+// Row m uses adapter s = adapter[m / per] of S stacked ones, A[s] [R, K] and
+// B[s] [N, R], c[s] its scaling; an s outside [0, S) means no adapter.
+//   h = x A[s]^T            out = y + c h B[s]^T
+//   g = dy B[s]             dx  = (dx +) c g A[s]
+//   dA[s] = c sum_m g^T x   dB[s] = c sum_m dy^T h      (m over the rows of s)
+// Three kernels do all of it:
+//   shrink  [rows, K] x [K, R]: contracts a row with an adapter (h and g)
+//   expand  [rows, R] x [R, N]: adds the low-rank product to a row (out, dx)
+//   tokens  [R, rows] x [rows, C]: contracts over the rows of an adapter (dA, dB)
+//
+// Arithmetic.  The products run on the tensor cores as bf16 x bf16 -> fp32.  A
+// value that bf16 does not hold is cut into bf16 pieces that add up to it
+// (each piece rounded from what is left): f16 into two, fp32 into three,
+// both exactly.  The rank-side values h and g are sums, kept in fp32, and enter
+// the next product as two pieces (2^-18, far below the rounding of a 16-bit
+// output) or three for fp32 outputs.  Of the products of pieces, those smaller
+// than the last kept bit are dropped (pair()).  int8 codes are exact in bf16;
+// their row scale multiplies h, or the rank side of dA, in fp32.
+//
+// Rows of other adapters, and rows without one, never enter a product as data:
+// they are not loaded, so NaN or infinity there stays there.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "pieces.cuh"
+#include "w8a8_internal.h"
+
+namespace w8a8 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBM = 64;   // rows per tile
+constexpr int kBK = 64;   // contraction per step of shrink
+constexpr int kBN = 128;  // output columns per tile of expand and tokens
+constexpr int kPad = 8;   // bf16 elements of padding a shared-memory row (conflict-free ldmatrix)
+
+// pieces of a rank-side fp32 value next to data of type T
+template <typename T>
+struct RankPieces { static constexpr int n = std::is_same<T, float>::value ? 3 : 2; };
+
+// ---- rows and their adapters
+struct Rows {
+  const void* idx;  // int32 or int64 [ceil(M / per)], or NULL: adapter 0
+  int idx64;
+  int64_t per;      // consecutive rows that share an index
+  int64_t M;
+  int S;
+};
+
+__device__ __forceinline__ int adapter_of(const Rows& r, int64_t row) {
+  if (row >= r.M) return -1;
+  if (!r.idx) return 0;
+  const int64_t i = r.per == 1 ? row : row / r.per;
+  const int64_t v = r.idx64 ? __ldg(static_cast<const long long*>(r.idx) + i)
+                            : static_cast<int64_t>(__ldg(static_cast<const int*>(r.idx) + i));
+  return v >= 0 && v < r.S ? static_cast<int>(v) : -1;
+}
+
+// The adapters of a tile of 64 rows: id[i] each row's, list the distinct ones
+// (in order of appearance), *count how many, *none whether a row has none.
+struct TileIds {
+  int id[kBM];
+  int list[kBM];
+  int count;
+  int none;
+};
+
+__device__ __forceinline__ void tile_ids(const Rows& rows, int64_t row0, TileIds& t) {
+  if (threadIdx.x < 32) {
+    const unsigned all = 0xffffffffu;
+    const int lane = threadIdx.x;
+    const int a = adapter_of(rows, row0 + lane);
+    const int b = adapter_of(rows, row0 + 32 + lane);
+    t.id[lane] = a;
+    t.id[lane + 32] = b;
+    // every lane takes part in every warp operation: their results are tested afterwards
+    const unsigned same_a = __match_any_sync(all, a);
+    const unsigned same_b = __match_any_sync(all, b);
+    const bool first_a = a >= 0 && __ffs(same_a) - 1 == lane;
+    bool first_b = b >= 0 && __ffs(same_b) - 1 == lane;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const int other = __shfl_sync(all, a, j);
+      first_b = first_b && other != b;
+    }
+    const unsigned ma = __ballot_sync(all, first_a);
+    const unsigned mb = __ballot_sync(all, first_b);
+    const unsigned below = (1u << lane) - 1u;
+    if (first_a) t.list[__popc(ma & below)] = a;
+    if (first_b) t.list[__popc(ma) + __popc(mb & below)] = b;
+    const bool n = (a < 0 && row0 + lane < rows.M) || (b < 0 && row0 + 32 + lane < rows.M);
+    const bool any = __any_sync(all, n);
+    if (lane == 0) {
+      t.count = __popc(ma) + __popc(mb);
+      t.none = any;
+    }
+  }
+  __syncthreads();
+}
+
+// ======================================================================== shrink
+// part[split][row][r] = sum over the split's k of x[row, k] W_s[k, r], times the
+// row's scale for int8 codes.  kRank = padded rank (16, 32, 64, 128).
+// kWRows: W_s is stored [r][k] (A); otherwise [k][r] (B, k its N).
+// 8 warps: four of 16 rows, times two that take every other 16 of a step's k.
+template <typename TX, typename TW, int kRank, bool kWRows>
+struct ShrinkTile {
+  static constexpr int kPX = Pieces<TX>::n, kPW = Pieces<TW>::n;
+  static constexpr int kMost = kPX > kPW ? kPX : kPW;
+  static constexpr int kXPlane = kBM * (kBK + kPad);
+  static constexpr int kLdW = kWRows ? kBK + kPad : kRank + kPad;
+  static constexpr int kWPlane = (kWRows ? kRank : kBK) * kLdW;
+  static constexpr int kBytes0 = 2 * (kPX * kXPlane + kPW * kWPlane);
+  static constexpr int kJoin = kBM * kRank * 4;
+  static constexpr int kBytes = kBytes0 > kJoin ? kBytes0 : kJoin;
+};
+
+template <typename TX, typename TW, int kRank, bool kWRows>
+__global__ void __launch_bounds__(kThreads) shrink_kernel(
+    const TX* __restrict__ x, int64_t ldx, const float* __restrict__ xs, const TW* __restrict__ w,
+    int64_t slot, Rows rows, int K, int R, int k_split, int vec_x, int vec_w,
+    float* __restrict__ part) {
+  using Tile = ShrinkTile<TX, TW, kRank, kWRows>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ TileIds ids;
+  __nv_bfloat16* sx = reinterpret_cast<__nv_bfloat16*>(smem);
+  __nv_bfloat16* sw = sx + Tile::kPX * Tile::kXPlane;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int wm = warp & 3, wk = warp >> 2;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kBM;
+  const int k_lo = blockIdx.y * k_split;
+  const int k_hi = min(K, k_lo + k_split);
+  tile_ids(rows, row0, ids);
+
+  constexpr bool kApart = std::is_same<TW, float>::value;
+  constexpr int kGX = kBM * (kBK / 8) / kThreads;                       // 2
+  constexpr int kGWAll = kRank * kBK / 8;                               // 8-element groups of W
+  constexpr int kGW = (kGWAll + kThreads - 1) / kThreads;
+  for (int li = blockIdx.z; li < ids.count; li += gridDim.z) {
+    const int s = ids.list[li];
+    const TW* ws = w + s * slot;
+    float acc[kRank / 8][4];
+#pragma unroll
+    for (int i = 0; i < kRank / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    float low[kApart ? kRank / 8 : 1][4] = {};
+
+    Raw8<TX> rx[kGX];
+    Raw8<TW> rw[kGW];
+    auto fetch = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < kGX; ++i) {
+        const int gi = tid + i * kThreads;
+        const int r = gi / (kBK / 8), c = (gi % (kBK / 8)) * 8;
+        const int valid = ids.id[r] == s ? min(8, k_hi - k0 - c) : 0;
+        load8(rx[i], x + (row0 + r) * ldx + k0 + c, valid, vec_x != 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kGW; ++i) {
+        const int gi = tid + i * kThreads;
+        if (kGWAll % kThreads != 0 && gi >= kGWAll) break;
+        if constexpr (kWRows) {
+          const int r = gi / (kBK / 8), c = (gi % (kBK / 8)) * 8;
+          const int valid = r < R ? min(8, k_hi - k0 - c) : 0;
+          load8(rw[i], ws + static_cast<int64_t>(r) * K + k0 + c, valid, vec_w != 0);
+        } else {
+          const int r = gi / (kRank / 8), c = (gi % (kRank / 8)) * 8;
+          const int valid = k0 + r < k_hi ? min(8, R - c) : 0;
+          load8(rw[i], ws + static_cast<int64_t>(k0 + r) * R + c, valid, vec_w != 0);
+        }
+      }
+    };
+    fetch(k_lo);
+    for (int k0 = k_lo; k0 < k_hi; k0 += kBK) {
+      __syncthreads();  // the previous step's tiles are read
+#pragma unroll
+      for (int i = 0; i < kGX; ++i) {
+        const int gi = tid + i * kThreads;
+        store8(sx + (gi / (kBK / 8)) * (kBK + kPad) + (gi % (kBK / 8)) * 8, Tile::kXPlane, rx[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kGW; ++i) {
+        const int gi = tid + i * kThreads;
+        if (kGWAll % kThreads != 0 && gi >= kGWAll) break;
+        constexpr int kPer = kWRows ? kBK / 8 : kRank / 8;
+        store8(sw + (gi / kPer) * Tile::kLdW + (gi % kPer) * 8, Tile::kWPlane, rw[i]);
+      }
+      __syncthreads();
+      if (k0 + kBK < k_hi) fetch(k0 + kBK);
+#pragma unroll
+      for (int h = 0; h < kBK / 32; ++h) {
+        const int kk = (2 * h + wk) * 16;
+        uint32_t a[Tile::kPX][4];
+#pragma unroll
+        for (int p = 0; p < Tile::kPX; ++p)
+          ldsm4(a[p], at16(sx + p * Tile::kXPlane, wm * 16, kk, kBK + kPad, lane));
+#pragma unroll
+        for (int n = 0; n < kRank / 16; ++n) {
+#pragma unroll
+          for (int pw = 0; pw < Tile::kPW; ++pw) {
+            uint32_t b[4];
+            if constexpr (kWRows) {
+              ldsm4(b, at16h(sw + pw * Tile::kWPlane, n * 16, kk, Tile::kLdW, lane));
+            } else {
+              ldsm4_t(b, at16(sw + pw * Tile::kWPlane, kk, n * 16, Tile::kLdW, lane));
+            }
+#pragma unroll
+            for (int px = 0; px < Tile::kPX; ++px) {
+              if (pair(px, pw, Tile::kMost)) {
+                if constexpr (kApart) {
+                  mma_apart(acc[2 * n], low[2 * n], a[px], b[0], b[1], px + pw == 0);
+                  mma_apart(acc[2 * n + 1], low[2 * n + 1], a[px], b[2], b[3], px + pw == 0);
+                } else {
+                  mma(acc[2 * n], a[px], b[0], b[1]);
+                  mma(acc[2 * n + 1], a[px], b[2], b[3]);
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+    if constexpr (kApart) {
+#pragma unroll
+      for (int i = 0; i < kRank / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += low[i][j];
+    }
+    // join the two halves of the warps through shared memory
+    float* join = reinterpret_cast<float*>(smem);
+    __syncthreads();
+    const int r0 = wm * 16 + (lane >> 2), c0 = (lane & 3) * 2;
+    if (wk == 1) {
+#pragma unroll
+      for (int n = 0; n < kRank / 8; ++n) {
+        *reinterpret_cast<float2*>(join + r0 * kRank + n * 8 + c0) = make_float2(acc[n][0], acc[n][1]);
+        *reinterpret_cast<float2*>(join + (r0 + 8) * kRank + n * 8 + c0) =
+            make_float2(acc[n][2], acc[n][3]);
+      }
+    }
+    __syncthreads();
+    if (wk == 0) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = r0 + half * 8;
+        if (ids.id[r] != s) continue;
+        const int64_t row = row0 + r;
+        const float sc = xs ? __ldg(xs + row) : 1.0f;
+        float* dst = part + (static_cast<int64_t>(blockIdx.y) * rows.M + row) * R;
+#pragma unroll
+        for (int n = 0; n < kRank / 8; ++n) {
+          const int c = n * 8 + c0;
+          const float2 o = *reinterpret_cast<const float2*>(join + r * kRank + c);
+          if (c < R) dst[c] = (acc[n][2 * half] + o.x) * sc;
+          if (c + 1 < R) dst[c + 1] = (acc[n][2 * half + 1] + o.y) * sc;
+        }
+      }
+    }
+  }
+}
+
+// Rank-side values of `rows_n` rows from row0 (those of adapter s; zero elsewhere):
+// the splits' sums in a fixed order, times mul (and the row's scale), as bf16
+// pieces into [row][kRank + kPad] planes.
+template <int kRank, int kP>
+__device__ __forceinline__ void load_rank_side(__nv_bfloat16* dst, const float* __restrict__ part,
+                                               int splits, const Rows& rows, int64_t row0,
+                                               const int* id, int s, int R, float mul,
+                                               const float* __restrict__ row_mul) {
+  constexpr int kLd = kRank + kPad;
+  const int64_t plane = rows.M * R;
+  for (int gi = threadIdx.x; gi < kBM * kRank / 8; gi += kThreads) {
+    const int r = gi / (kRank / 8), c = (gi % (kRank / 8)) * 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (id[r] == s) {
+      const float* p = part + (row0 + r) * R + c;
+      for (int sp = 0; sp < splits; ++sp, p += plane) {
+        if (R % 4 == 0) {
+          const float4 lo = c < R ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
+          const float4 hi =
+              c + 4 < R ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
+          v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+          v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += c + i < R ? __ldg(p + i) : 0.0f;
+        }
+      }
+      const float m = row_mul ? mul * __ldg(row_mul + row0 + r) : mul;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= m;
+    }
+    store_pieces<kP>(dst + r * kLd + c, kBM * kLd, v);
+  }
+}
+
+// ======================================================================== expand
+// out[row, n] = T(y[row, n] + c[s] * sum_r h[row, r] W_s[r, n]), 64 rows x 128
+// columns a block; y NULL: zero.  kWCols: W_s is stored [n][r] (B); otherwise
+// [r][n] (A).  The h of the tile is at most 64 x 128 and W_s at most 128 x 128:
+// one step, no pipeline; several blocks on an SM overlap one's loads with
+// another's stores.
+template <typename T, int kRank, bool kWCols>
+struct ExpandTile {
+  static constexpr int kPH = RankPieces<T>::n, kPW = Pieces<T>::n;
+  static constexpr int kMost = kPH > kPW ? kPH : kPW;
+  static constexpr int kHPlane = kBM * (kRank + kPad);
+  static constexpr int kLdW = kWCols ? kRank + kPad : kBN + kPad;
+  static constexpr int kWPlane = (kWCols ? kBN : kRank) * kLdW;
+  static constexpr int kBytes0 = 2 * (kPH * kHPlane + kPW * kWPlane);
+  static constexpr int kLdO = kBN + 4;
+  static constexpr int kOut = kBM * kLdO * 4;
+  static constexpr int kBytes = kBytes0 > kOut ? kBytes0 : kOut;
+};
+
+template <typename T, int kRank, bool kWCols>
+__global__ void __launch_bounds__(kThreads) expand_kernel(
+    const T* y, int64_t ldy, const float* __restrict__ part, int splits, const T* __restrict__ w,
+    int64_t slot, const float* __restrict__ scaling, Rows rows, int N, int R, int col_tiles, int vec_w,
+    int vec_o, T* out, int64_t ldo) {
+  using Tile = ExpandTile<T, kRank, kWCols>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ TileIds ids;
+  __nv_bfloat16* sh = reinterpret_cast<__nv_bfloat16*>(smem);
+  __nv_bfloat16* sw = sh + Tile::kPH * Tile::kHPlane;
+  float* so = reinterpret_cast<float*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int wm = warp & 3, wn = warp >> 2;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / col_tiles) * kBM;
+  const int col0 = static_cast<int>(blockIdx.x % col_tiles) * kBN;
+  tile_ids(rows, row0, ids);
+
+  // this thread's outputs: rows tid / 16 + 16 i, eight columns
+  const int oc = (tid & 15) * 8;
+  const int valid_c = min(8, N - col0 - oc);
+  Raw8<T> yr[kBM / 16];
+#pragma unroll
+  for (int i = 0; i < kBM / 16; ++i) {
+    const int64_t row = row0 + (tid >> 4) + 16 * i;
+    const int valid = y && row < rows.M ? valid_c : 0;
+    load8(yr[i], y + row * ldy + col0 + oc, valid, vec_o != 0);
+  }
+  auto put = [&](int i, const float* add, float mul) {
+    const int64_t row = row0 + (tid >> 4) + 16 * i;
+    T* dst = out + row * ldo + col0 + oc;
+    Raw8<T> o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float base = to_f(yr[i].e[j]);
+      o.e[j] = add ? from_f<T>(y ? fmaf(mul, add[j], base) : mul * add[j]) : yr[i].e[j];
+    }
+    if (vec_o && valid_c >= 8) {
+#pragma unroll
+      for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) {
+        const uint2* sp = reinterpret_cast<const uint2*>(o.e) + 2 * q;
+        reinterpret_cast<uint4*>(dst)[q] = make_uint4(sp[0].x, sp[0].y, sp[1].x, sp[1].y);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < valid_c) dst[j] = o.e[j];
+    }
+  };
+  if (ids.none && blockIdx.z == 0 && y != out) {
+#pragma unroll
+    for (int i = 0; i < kBM / 16; ++i) {
+      const int r = (tid >> 4) + 16 * i;
+      if (ids.id[r] < 0 && row0 + r < rows.M) put(i, nullptr, 0.0f);
+    }
+  }
+
+  constexpr int kGWAll = kRank * kBN / 8;
+  for (int li = blockIdx.z; li < ids.count; li += gridDim.z) {
+    const int s = ids.list[li];
+    const T* ws = w + s * slot;
+    __syncthreads();  // the previous adapter's outputs are read
+    for (int gi = tid; gi < kGWAll; gi += kThreads) {
+      Raw8<T> raw;
+      if constexpr (kWCols) {
+        const int n = gi / (kRank / 8), c = (gi % (kRank / 8)) * 8;
+        const int valid = col0 + n < N ? min(8, R - c) : 0;
+        load8(raw, ws + static_cast<int64_t>(col0 + n) * R + c, valid, vec_w != 0);
+        store8(sw + n * Tile::kLdW + c, Tile::kWPlane, raw);
+      } else {
+        const int r = gi / (kBN / 8), c = (gi % (kBN / 8)) * 8;
+        const int valid = r < R ? min(8, N - col0 - c) : 0;
+        load8(raw, ws + static_cast<int64_t>(r) * N + col0 + c, valid, vec_w != 0);
+        store8(sw + r * Tile::kLdW + c, Tile::kWPlane, raw);
+      }
+    }
+    load_rank_side<kRank, Tile::kPH>(sh, part, splits, rows, row0, ids.id, s, R, 1.0f, nullptr);
+    __syncthreads();
+    float acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    constexpr bool kApart = std::is_same<T, float>::value;
+    float low[kApart ? 8 : 1][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < kRank; kk += 16) {
+      uint32_t a[Tile::kPH][4];
+#pragma unroll
+      for (int p = 0; p < Tile::kPH; ++p)
+        ldsm4(a[p], at16(sh + p * Tile::kHPlane, wm * 16, kk, kRank + kPad, lane));
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+#pragma unroll
+        for (int pw = 0; pw < Tile::kPW; ++pw) {
+          uint32_t b[4];
+          if constexpr (kWCols) {
+            ldsm4(b, at16h(sw + pw * Tile::kWPlane, wn * 64 + n * 16, kk, Tile::kLdW, lane));
+          } else {
+            ldsm4_t(b, at16(sw + pw * Tile::kWPlane, kk, wn * 64 + n * 16, Tile::kLdW, lane));
+          }
+#pragma unroll
+          for (int ph = 0; ph < Tile::kPH; ++ph) {
+            if (pair(ph, pw, Tile::kMost)) {
+              if constexpr (kApart) {
+                mma_apart(acc[2 * n], low[2 * n], a[ph], b[0], b[1], ph + pw == 0);
+                mma_apart(acc[2 * n + 1], low[2 * n + 1], a[ph], b[2], b[3], ph + pw == 0);
+              } else {
+                mma(acc[2 * n], a[ph], b[0], b[1]);
+                mma(acc[2 * n + 1], a[ph], b[2], b[3]);
+              }
+            }
+          }
+        }
+      }
+    }
+    if constexpr (kApart) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += low[i][j];
+    }
+    __syncthreads();  // the operands are read: the tile takes their place
+    const int r0 = wm * 16 + (lane >> 2), c0 = wn * 64 + (lane & 3) * 2;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      *reinterpret_cast<float2*>(so + r0 * Tile::kLdO + c0 + n * 8) = make_float2(acc[n][0], acc[n][1]);
+      *reinterpret_cast<float2*>(so + (r0 + 8) * Tile::kLdO + c0 + n * 8) =
+          make_float2(acc[n][2], acc[n][3]);
+    }
+    __syncthreads();
+    const float mul = scaling ? __ldg(scaling + s) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kBM / 16; ++i) {
+      const int r = (tid >> 4) + 16 * i;
+      if (ids.id[r] == s) put(i, so + r * Tile::kLdO + oc, mul);
+    }
+  }
+}
+
+// ======================================================================== tokens
+// part[split][s][r][c] (kByCol: [split][s][c][r]) = sum over the split's rows m
+// of adapter s of q[m, r] X[m, c], with q = mul[s] * (row_mul[m]) * the rank side.
+// 128 columns a block, all of the rank; warp w takes columns 16 w .. 16 w + 15.
+// found[split][s] says whether the block wrote anything.
+template <typename TX, typename TO, int kRank, bool kByCol>
+struct TokensTile {
+  static constexpr int kPX = Pieces<TX>::n, kPH = RankPieces<TO>::n;
+  static constexpr int kMost = kPX > kPH ? kPX : kPH;
+  static constexpr int kXPlane = kBM * (kBN + kPad);
+  static constexpr int kHPlane = kBM * (kRank + kPad);
+  static constexpr int kBytes = 2 * (kPX * kXPlane + kPH * kHPlane);
+};
+
+template <typename TX, typename TO, int kRank, bool kByCol>
+__global__ void __launch_bounds__(kThreads) tokens_kernel(
+    const TX* __restrict__ x, int64_t ldx, const float* __restrict__ row_mul,
+    const float* __restrict__ rank_part, int splits, const float* __restrict__ scaling, Rows rows,
+    int C, int R, int64_t rows_split, int vec_x, float* __restrict__ part, int* __restrict__ found) {
+  using Tile = TokensTile<TX, TO, kRank, kByCol>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int id[kBM];
+  __nv_bfloat16* sx = reinterpret_cast<__nv_bfloat16*>(smem);
+  __nv_bfloat16* sh = sx + Tile::kPX * Tile::kXPlane;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int col0 = blockIdx.x * kBN;
+  const int s = blockIdx.z;
+  const int64_t m_lo = static_cast<int64_t>(blockIdx.y) * rows_split;
+  const int64_t m_hi = min(rows.M, m_lo + rows_split);
+  const float mul = scaling ? __ldg(scaling + s) : 1.0f;
+  float acc[kRank / 16][2][4];
+#pragma unroll
+  for (int i = 0; i < kRank / 16; ++i)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
+  constexpr bool kApart = std::is_same<TO, float>::value;
+  float low[kApart ? kRank / 16 : 1][2][4] = {};
+  bool any = false;
+  constexpr int kGX = kBM * (kBN / 8) / kThreads;  // 4
+  for (int64_t m0 = m_lo; m0 < m_hi; m0 += kBM) {
+    int mine = 0;
+    if (tid < kBM) {
+      const int v = m0 + tid < m_hi ? adapter_of(rows, m0 + tid) : -1;
+      id[tid] = v;
+      mine = v == s;
+    }
+    if (!__syncthreads_or(mine)) continue;
+    any = true;
+    Raw8<TX> rx[kGX];
+#pragma unroll
+    for (int i = 0; i < kGX; ++i) {
+      const int gi = tid + i * kThreads;
+      const int r = gi / (kBN / 8), c = (gi % (kBN / 8)) * 8;
+      const int valid = id[r] == s ? min(8, C - col0 - c) : 0;
+      load8(rx[i], x + (m0 + r) * ldx + col0 + c, valid, vec_x != 0);
+    }
+    load_rank_side<kRank, Tile::kPH>(sh, rank_part, splits, rows, m0, id, s, R, mul, row_mul);
+#pragma unroll
+    for (int i = 0; i < kGX; ++i) {
+      const int gi = tid + i * kThreads;
+      store8(sx + (gi / (kBN / 8)) * (kBN + kPad) + (gi % (kBN / 8)) * 8, Tile::kXPlane, rx[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < kBM; kk += 16) {
+      uint32_t b[Tile::kPX][4];
+#pragma unroll
+      for (int p = 0; p < Tile::kPX; ++p)
+        ldsm4_t(b[p], at16(sx + p * Tile::kXPlane, kk, warp * 16, kBN + kPad, lane));
+#pragma unroll
+      for (int i = 0; i < kRank / 16; ++i) {
+#pragma unroll
+        for (int ph = 0; ph < Tile::kPH; ++ph) {
+          uint32_t a[4];
+          ldsm4_t(a, at16h(sh + ph * Tile::kHPlane, kk, i * 16, kRank + kPad, lane));
+#pragma unroll
+          for (int px = 0; px < Tile::kPX; ++px) {
+            if (pair(px, ph, Tile::kMost)) {
+              if constexpr (kApart) {
+                mma_apart(acc[i][0], low[i][0], a, b[px][0], b[px][1], px + ph == 0);
+                mma_apart(acc[i][1], low[i][1], a, b[px][2], b[px][3], px + ph == 0);
+              } else {
+                mma(acc[i][0], a, b[px][0], b[px][1]);
+                mma(acc[i][1], a, b[px][2], b[px][3]);
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();  // tiles and ids are read
+  }
+  if constexpr (kApart) {
+#pragma unroll
+    for (int i = 0; i < kRank / 16; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][n][j] += low[i][n][j];
+  }
+  const int64_t block = static_cast<int64_t>(blockIdx.y) * rows.S + s;
+  if (blockIdx.x == 0 && tid == 0) found[block] = any;
+  if (!any) return;
+  float* dst = part + block * R * C;
+#pragma unroll
+  for (int i = 0; i < kRank / 16; ++i)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = i * 16 + (lane >> 2) + (j >> 1) * 8;
+        const int c = col0 + warp * 16 + n * 8 + (lane & 3) * 2 + (j & 1);
+        if (r < R && c < C) {
+          dst[kByCol ? static_cast<int64_t>(c) * R + r : static_cast<int64_t>(r) * C + c] = acc[i][n][j];
+        }
+      }
+}
+
+// The splits' sums, in a fixed order, rounded to T: dA then dB.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sum_splits_kernel(
+    const float* __restrict__ pa, const int* __restrict__ fa, int splits_a, int64_t na,
+    T* __restrict__ da, const float* __restrict__ pb, const int* __restrict__ fb, int splits_b,
+    int64_t nb, T* __restrict__ db, int S) {
+  // na / nb: elements of one adapter
+  const int64_t total_a = na * S, total = total_a + nb * S;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const bool first = i < total_a;
+    const int64_t j = first ? i : i - total_a;
+    const int64_t per = first ? na : nb;
+    const int s = static_cast<int>(j / per);
+    const float* p = (first ? pa : pb) + j;
+    const int* f = (first ? fa : fb) + s;
+    const int n = first ? splits_a : splits_b;
+    float v = 0.0f;
+    for (int sp = 0; sp < n; ++sp)
+      if (__ldg(f + sp * S)) v += __ldg(p + sp * per * S);
+    (first ? da : db)[j] = from_f<T>(v);
+  }
+}
+
+// ---------------------------------------------------------------- host
+int pad_rank(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
+
+bool aligned(const void* p, int64_t ld, int size) {
+  // rows of eight-element groups that vector loads may take (16 bytes; 8 for int8)
+  const int64_t unit = size == 1 ? 8 : 16;
+  return reinterpret_cast<uintptr_t>(p) % unit == 0 && (ld * size) % unit == 0;
+}
+
+template <typename K>
+int prepare(K kernel, int bytes) {
+  if (bytes > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+      set_error("lora: shared memory of %d bytes refused: %s", bytes, cudaGetErrorString(e));
+      return W8A8_ERR_ACCELERATOR;
+    }
+  }
+  return 0;
+}
+
+int launched(const char* what) {
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error("%s launch failed: %s", what, cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
+}
+
+// How a shrink is cut: enough blocks for two a multiprocessor, at least two
+// steps of the contraction each, and at most 16 pieces (the next kernel adds
+// them up for every tile it makes).
+struct Split {
+  int count;
+  int per;
+};
+Split shrink_split(int64_t M, int K) {
+  const int64_t tiles = (M + kBM - 1) / kBM;
+  const int steps = std::max(1, (K + kBK - 1) / kBK);
+  int64_t want = (2 * device_sm_count() + tiles - 1) / std::max<int64_t>(tiles, 1);
+  want = std::max<int64_t>(1, std::min<int64_t>({want, 16, (steps + 1) / 2}));
+  const int per = static_cast<int>((steps + want - 1) / want);
+  return {(steps + per - 1) / per, per * kBK};
+}
+// Blocks that share out a tile's adapters (a tile of a decode batch has many).
+int parts_of(int64_t M, int S, int blocks) {
+  if (S <= 1) return 1;
+  const int64_t tiles = (M + kBM - 1) / kBM;
+  const int64_t most = std::min<int64_t>({S, M, kBM});
+  const int64_t want = (2 * device_sm_count()) / std::max<int64_t>(1, tiles * blocks);
+  return static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
+}
+// How the rows of a token contraction are cut: two blocks a multiprocessor for
+// one adapter's columns, whole tiles, and at most 64 MiB of partial sums.
+struct RowSplit {
+  int count;
+  int64_t per;
+};
+RowSplit tokens_split(int64_t M, int C, int S, int R) {
+  const int64_t tiles = std::max<int64_t>(1, (M + kBM - 1) / kBM);
+  const int64_t chunks = (C + kBN - 1) / kBN;
+  int64_t want = (2 * device_sm_count() + chunks - 1) / std::max<int64_t>(chunks, 1);
+  const int64_t one = static_cast<int64_t>(S) * R * C * 4;
+  want = std::max<int64_t>(1, std::min<int64_t>({want, tiles, (64ll << 20) / std::max<int64_t>(one, 1)}));
+  const int64_t per = (tiles + want - 1) / want;
+  return {static_cast<int>((tiles + per - 1) / per), per * kBM};
+}
+
+int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
+
+template <typename TX, typename TW, bool kWRows>
+int shrink(const TX* x, int64_t ldx, const float* xs, const TW* w, int64_t slot, const Rows& rows,
+           int K, int R, const Split& sp, float* part, cudaStream_t stream) {
+  const int64_t tiles = (rows.M + kBM - 1) / kBM;
+  const int vx = aligned(x, ldx, sizeof(TX));
+  const int vw = aligned(w, kWRows ? K : R, sizeof(TW)) && aligned(w, slot, sizeof(TW));
+  const dim3 grid(static_cast<unsigned>(tiles), sp.count, parts_of(rows.M, rows.S, sp.count));
+#define SHRINK(RANK)                                                                              \
+  {                                                                                               \
+    auto k = shrink_kernel<TX, TW, RANK, kWRows>;                                                 \
+    constexpr int bytes = ShrinkTile<TX, TW, RANK, kWRows>::kBytes;                               \
+    if (int rc = prepare(k, bytes)) return rc;                                                    \
+    k<<<grid, kThreads, bytes, stream>>>(x, ldx, xs, w, slot, rows, K, R, sp.per, vx, vw, part);  \
+  }
+  switch (pad_rank(R)) {
+    case 16: SHRINK(16) break;
+    case 32: SHRINK(32) break;
+    case 64: SHRINK(64) break;
+    default: SHRINK(128) break;
+  }
+#undef SHRINK
+  return launched("lora shrink");
+}
+
+template <typename T, bool kWCols>
+int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, int64_t slot,
+           const float* scaling, const Rows& rows, int N, int R, T* out, int64_t ldo,
+           cudaStream_t stream) {
+  const int64_t tiles = (rows.M + kBM - 1) / kBM;
+  const int cols = (N + kBN - 1) / kBN;
+  const int vw = aligned(w, kWCols ? R : N, sizeof(T)) && aligned(w, slot, sizeof(T));
+  const int vo = aligned(out, ldo, sizeof(T)) && (!y || aligned(y, ldy, sizeof(T)));
+  const dim3 grid(static_cast<unsigned>(tiles * cols), 1, parts_of(rows.M, rows.S, cols));
+#define EXPAND(RANK)                                                                              \
+  {                                                                                               \
+    auto k = expand_kernel<T, RANK, kWCols>;                                                      \
+    constexpr int bytes = ExpandTile<T, RANK, kWCols>::kBytes;                                    \
+    if (int rc = prepare(k, bytes)) return rc;                                                    \
+    k<<<grid, kThreads, bytes, stream>>>(y, ldy, part, splits, w, slot, scaling, rows, N, R, cols, \
+                                         vw, vo, out, ldo);                                       \
+  }
+  switch (pad_rank(R)) {
+    case 16: EXPAND(16) break;
+    case 32: EXPAND(32) break;
+    case 64: EXPAND(64) break;
+    default: EXPAND(128) break;
+  }
+#undef EXPAND
+  return launched("lora expand");
+}
+
+template <typename TX, typename TO, bool kByCol>
+int tokens(const TX* x, int64_t ldx, const float* row_mul, const float* rank_part, int splits,
+           const float* scaling, const Rows& rows, int C, int R, const RowSplit& sp, float* part,
+           int* found, cudaStream_t stream) {
+  const int vx = aligned(x, ldx, sizeof(TX));
+  const dim3 grid((C + kBN - 1) / kBN, sp.count, rows.S);
+#define TOKENS(RANK)                                                                              \
+  {                                                                                               \
+    auto k = tokens_kernel<TX, TO, RANK, kByCol>;                                                 \
+    constexpr int bytes = TokensTile<TX, TO, RANK, kByCol>::kBytes;                               \
+    if (int rc = prepare(k, bytes)) return rc;                                                    \
+    k<<<grid, kThreads, bytes, stream>>>(x, ldx, row_mul, rank_part, splits, scaling, rows, C, R, \
+                                         sp.per, vx, part, found);                                \
+  }
+  switch (pad_rank(R)) {
+    case 16: TOKENS(16) break;
+    case 32: TOKENS(32) break;
+    case 64: TOKENS(64) break;
+    default: TOKENS(128) break;
+  }
+#undef TOKENS
+  return launched("lora tokens");
+}
+
+template <typename T>
+int add_typed(const LoraArgs& g, cudaStream_t stream) {
+  const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
+  const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
+  const Split sp = shrink_split(g.M, K);
+  float* part = static_cast<float*>(g.workspace);
+  if (int rc = shrink<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
+                                  static_cast<const T*>(g.a), g.lda, rows, K, R, sp, part, stream)) {
+    return rc;
+  }
+  return expand<T, true>(static_cast<const T*>(g.y), g.ldy, part, sp.count,
+                         static_cast<const T*>(g.b), g.ldb, g.scaling, rows, N, R,
+                         static_cast<T*>(g.out), g.ldo, stream);
+}
+
+struct BackwardPlan {
+  Split h, g;
+  RowSplit a, b;
+  int64_t off_g, off_a, off_b, off_found, bytes;
+};
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R) {
+  BackwardPlan p;
+  const int r = static_cast<int>(R), s = static_cast<int>(S);
+  p.h = shrink_split(M, static_cast<int>(K));
+  p.g = shrink_split(M, static_cast<int>(N));
+  p.a = tokens_split(M, static_cast<int>(K), s, r);
+  p.b = tokens_split(M, static_cast<int>(N), s, r);
+  p.off_g = up(p.h.count * M * R * 4);
+  p.off_a = p.off_g + up(p.g.count * M * R * 4);
+  p.off_b = p.off_a + up(p.a.count * S * R * K * 4);
+  p.off_found = p.off_b + up(p.b.count * S * R * N * 4);
+  p.bytes = p.off_found + up((p.a.count + p.b.count) * S * 4);
+  return p;
+}
+
+template <typename T, typename TX>
+int backward_typed(const LoraArgs& g, cudaStream_t stream) {
+  const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
+  const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
+  const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R);
+  uint8_t* ws = static_cast<uint8_t*>(g.workspace);
+  float* ph = reinterpret_cast<float*>(ws);
+  float* pg = reinterpret_cast<float*>(ws + p.off_g);
+  float* pa = reinterpret_cast<float*>(ws + p.off_a);
+  float* pb = reinterpret_cast<float*>(ws + p.off_b);
+  int* fa = reinterpret_cast<int*>(ws + p.off_found);
+  int* fb = fa + p.a.count * g.S;
+  const TX* x = static_cast<const TX*>(g.x);
+  const T* dy = static_cast<const T*>(g.y);
+  const T* a = static_cast<const T*>(g.a);
+  const T* b = static_cast<const T*>(g.b);
+  if (g.M > 0) {
+    if (int rc = shrink<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, rows, N, R, p.g, pg, stream)) return rc;
+    if (g.out) {
+      if (int rc = expand<T, false>(g.accumulate ? static_cast<const T*>(g.out) : nullptr, g.ldo, pg,
+                                    p.g.count, a, g.lda, g.scaling, rows, K, R,
+                                    static_cast<T*>(g.out), g.ldo, stream)) {
+        return rc;
+      }
+    }
+  }
+  if (!g.da) return 0;
+  if (g.M > 0) {
+    if (int rc = shrink<TX, T, true>(x, g.ldx, g.x_scale, a, g.lda, rows, K, R, p.h, ph, stream)) return rc;
+  }
+  if (int rc = tokens<TX, T, false>(x, g.ldx, g.x_scale, pg, p.g.count, g.scaling, rows, K, R, p.a, pa,
+                                    fa, stream)) {
+    return rc;
+  }
+  if (int rc = tokens<T, T, true>(dy, g.ldy, nullptr, ph, p.h.count, g.scaling, rows, N, R, p.b, pb, fb,
+                                  stream)) {
+    return rc;
+  }
+  const int64_t na = g.R * g.K, nb = g.R * g.N;
+  const int64_t blocks = std::min<int64_t>((g.S * (na + nb) + kThreads - 1) / kThreads,
+                                           16ll * device_sm_count());
+  sum_splits_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+      pa, fa, p.a.count, na, static_cast<T*>(g.da), pb, fb, p.b.count, nb, static_cast<T*>(g.db),
+      static_cast<int>(g.S));
+  return launched("lora gradient sum");
+}
+
+}  // namespace
+
+int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, int backward) {
+  if (!backward) return up(shrink_split(M, static_cast<int>(K)).count * M * R * 4);
+  return backward_plan(M, N, K, S, R).bytes;
+}
+
+int lora_add_launch(const LoraArgs& g, cudaStream_t stream) {
+  switch (g.dtype) {
+    case W8A8_BF16: return add_typed<__nv_bfloat16>(g, stream);
+    case W8A8_F16: return add_typed<__half>(g, stream);
+    default: return add_typed<float>(g, stream);
+  }
+}
+
+int lora_backward_launch(const LoraArgs& g, cudaStream_t stream) {
+  const bool codes = g.x_scale != nullptr;
+  switch (g.dtype) {
+    case W8A8_BF16:
+      return codes ? backward_typed<__nv_bfloat16, int8_t>(g, stream)
+                   : backward_typed<__nv_bfloat16, __nv_bfloat16>(g, stream);
+    case W8A8_F16:
+      return codes ? backward_typed<__half, int8_t>(g, stream)
+                   : backward_typed<__half, __half>(g, stream);
+    default:
+      return codes ? backward_typed<float, int8_t>(g, stream)
+                   : backward_typed<float, float>(g, stream);
+  }
+}
+
+}  // namespace w8a8

@@ -156,6 +156,60 @@ int rms_rope_launch(const void* q, const void* k, void* q_out, void* k_out, int 
                     int64_t ldko, const float* freqs, int64_t freq_rows, const void* q_scale,
                     const void* k_scale, float eps, cudaStream_t stream);
 
+// Low-rank adapters (lora.cu).  Forward: y (may be `out`), x, out.  Backward:
+// y is dy, out is dx (NULL: not wanted; accumulate: added to), da / db (both
+// NULL: not wanted), x int8 codes when x_scale is given.
+struct LoraArgs {
+  int dtype;
+  const void* x;
+  int64_t ldx;
+  const float* x_scale;
+  const void* y;
+  int64_t ldy;
+  const void* a;
+  int64_t lda;  // elements from one adapter to the next
+  const void* b;
+  int64_t ldb;
+  const void* adapter;
+  int adapter64;
+  int64_t rows_per_index;
+  const float* scaling;
+  void* out;
+  int64_t ldo;
+  int accumulate;
+  void* da;
+  void* db;
+  int64_t M, N, K, S, R;
+  void* workspace;
+};
+int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, int backward);
+int lora_add_launch(const LoraArgs& g, cudaStream_t stream);
+int lora_backward_launch(const LoraArgs& g, cudaStream_t stream);
+
+// Gradient of the int8 linear's input (linear_backward.cu).
+struct InputGradArgs {
+  int dtype;
+  const void* dy;
+  int64_t lddy;
+  const int8_t* w;
+  int64_t ldw;
+  const float* ws;
+  int64_t ws_numel;
+  void* dx;
+  int64_t lddx;
+  int64_t M, N, K;
+  void* workspace;
+};
+int64_t input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+int input_grad_launch(const InputGradArgs& g, cudaStream_t stream);
+
+// Activation with an 8-bit checkpoint of its input (activation.cu); act codes
+// W8A8_CKPT_ACT_*.
+int act_checkpoint_launch(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, int act,
+                          void* y, int8_t* q, float* scale, cudaStream_t stream);
+int act_backward_launch(const void* dy, int dtype, int64_t lddy, int64_t rows, int64_t cols, int act,
+                        const int8_t* q, const float* scale, void* dx, cudaStream_t stream);
+
 // Error reporting (thread-local), implemented in api.cu.
 void set_error(const char* fmt, ...);
 

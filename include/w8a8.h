@@ -542,6 +542,78 @@ int w8a8_sampler_step(float* x, const void* out_cond, const void* out_uncond, in
                       float* denoised, float* old_denoised, float* old_derivative,
                       const float* noise, void* stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection --------
+ *
+ * No reference counterpart (the reference merges adapters into the weight).
+ * S adapters of rank R (1 to 128) lie stacked: a [S, R, K] and b [S, N, R],
+ * each adapter contiguous, slot_a / slot_b elements from one to the next, all in `dtype`
+ * (F32/F16/BF16).  Row m of the batch uses adapter s =
+ * adapter[m / rows_per_index] (int32, or int64 with adapter_is_64; NULL: 0);
+ * an index outside [0, S) means no adapter.  scaling: fp32 [S] or NULL (ones).
+ * Adapters of smaller rank are padded with zeros.
+ *
+ * w8a8_lora_add: out = y + scaling[s] * (x a[s]^T) b[s]^T, x [M, K], y and out
+ * [M, N] (row strides in elements), each output rounded once; a row without an
+ * adapter is y's row.  out may be y; it may not overlap it otherwise, nor the
+ * other operands.
+ *
+ * w8a8_lora_backward, from dy [M, N]:
+ *   dx [M, K] = (dx when accumulate) + scaling[s] * (dy b[s]) a[s], zero (or
+ *     unchanged) in rows without an adapter; NULL: not wanted
+ *   da [S, R, K] = scaling[s] * sum over the rows of s of (dy b[s])^T x
+ *   db [S, N, R] = scaling[s] * sum over the rows of s of dy^T (x a[s]^T)
+ *     contiguous, in `dtype`, zero for an adapter without rows; both NULL: not wanted
+ * x is `dtype`, or with x_scale (fp32 [M]) the int8 codes of the forward
+ * quantiser (w8a8_quantize_rowwise): the activation's 8-bit checkpoint.
+ * Sums are taken in a fixed order: the same call gives the same bits.
+ *
+ * workspace: at least w8a8_lora_workspace_bytes(M, N, K, S, R, backward)
+ * bytes, 256-byte aligned, any content; calls sharing one must not overlap on
+ * the GPU. */
+int64_t w8a8_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R,
+                                  int backward);
+int w8a8_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dtype, const void* a,
+                  int64_t slot_a, const void* b, int64_t slot_b, const void* adapter,
+                  int adapter_is_64, int64_t rows_per_index, const float* scaling, void* out,
+                  int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t S, int64_t R,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                       const float* x_scale, int dtype, const void* a, int64_t slot_a,
+                       const void* b, int64_t slot_b, const void* adapter, int adapter_is_64,
+                       int64_t rows_per_index, const float* scaling, void* dx, int64_t lddx,
+                       int accumulate, void* da, void* db, int64_t M, int64_t N, int64_t K,
+                       int64_t S, int64_t R, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
+/* ---- gradient of the int8 linear's input ----------------------------------
+ * No reference counterpart (the reference only infers).  dx [M, K] = dy [M, N]
+ * (ws * w) for w int8 [N, K] (row stride ldw) and its scales ws (N or 1); the
+ * quantisation of the input passes the gradient through unchanged.  dy, dx:
+ * `dtype` (F32/F16/BF16).  workspace: w8a8_input_grad_workspace_bytes(M, N, K,
+ * dtype) bytes, 256-byte aligned, any content (may be 0 bytes, then NULL). */
+int64_t w8a8_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+int w8a8_input_grad(const void* dy, int64_t lddy, const int8_t* w, int64_t ldw, const float* ws,
+                    int64_t ws_numel, int dtype, void* dx, int64_t lddx, int64_t M, int64_t N,
+                    int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- activation with an 8-bit checkpoint of its input ----------------------
+ * No reference counterpart.  x [rows, halves * cols] (row stride ldx, halves 2
+ * for SWIGLU's [gate | up] rows, else 1) -> y [rows, cols] = act(x), and of
+ * every group of W8A8_CKPT_GROUP elements of a half (the last may be shorter)
+ * int8 codes q and one fp32 scale = max(amax / 127, 1e-30), q = rne(x /
+ * scale).  q [rows, halves * cols], scale [rows, halves * ceil(cols / 128)];
+ * y, q and scale contiguous.  A group that holds an infinity or a NaN gets the
+ * scale NaN.  w8a8_act_backward: dx [rows, halves * cols] (contiguous) = dy act'(q *
+ * scale). */
+#define W8A8_CKPT_GROUP 128
+#define W8A8_CKPT_ACT_GELU_TANH 1
+#define W8A8_CKPT_ACT_SWIGLU 2
+#define W8A8_CKPT_ACT_SILU 3
+int w8a8_act_checkpoint(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, int act,
+                        void* y, int8_t* q, float* scale, void* stream);
+int w8a8_act_backward(const void* dy, int dtype, int64_t lddy, int64_t rows, int64_t cols, int act,
+                      const int8_t* q, const float* scale, void* dx, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,130 @@
+"""What the adapter, input-gradient and checkpointed-activation operators refuse, on
+the host: nothing is launched."""
+import ctypes
+
+import pytest
+import torch
+
+from imagine_b200 import _native as N
+
+P = 0x10000  # any aligned non-null address: never dereferenced on these paths
+
+
+def _err():
+    return N.LIB.w8a8_last_error().decode()
+
+
+def _add(**kw):
+    d = dict(y=P, ldy=64, x=P, ldx=32, dtype=N.BF16, a=P, slot_a=256, b=P, slot_b=512, adapter=P, is64=0, per=1,
+             scaling=P, out=P, ldo=64, m=10, n=64, k=32, s=2, r=8, ws=P, ws_bytes=1 << 30)
+    d.update(kw)
+    return N.LIB.w8a8_lora_add(d["y"], d["ldy"], d["x"], d["ldx"], d["dtype"], d["a"], d["slot_a"], d["b"], d["slot_b"],
+                               d["adapter"], d["is64"], d["per"], d["scaling"], d["out"], d["ldo"], d["m"], d["n"],
+                               d["k"], d["s"], d["r"], d["ws"], d["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(m=-1), "negative"), (dict(r=0), "rank"), (dict(r=129), "rank"), (dict(s=0), "adapters"),
+    (dict(s=70000), "adapters"), (dict(y=None), "NULL"), (dict(x=None), "NULL"), (dict(out=None), "NULL"),
+    (dict(a=None), "NULL"), (dict(b=None), "NULL"), (dict(ldx=31), "stride"), (dict(ldy=63), "stride"),
+    (dict(ldo=63), "stride"), (dict(ldo=80), "another row stride"), (dict(dtype=N.S8), "floating"),
+    (dict(per=0), "rows_per_index"), (dict(slot_a=255), "overlap"), (dict(slot_b=511), "overlap"),
+    (dict(x=P + 1), "aligned"), (dict(adapter=P + 4, is64=1), "aligned"), (dict(scaling=P + 2), "aligned"),
+    (dict(ws_bytes=16), "workspace"), (dict(ws=None), "workspace"), (dict(ws=P + 16), "workspace"),
+    (dict(m=1 << 40), "sizes"), (dict(m=1 << 30, n=1 << 30), "tiles")])
+def test_lora_add_refuses(kw, word):
+    assert _add(**kw) == N.ERR_VALUE
+    assert word in _err()
+
+
+def test_lora_add_with_nothing_to_do():
+    assert _add(m=0) == 0 and _add(n=0) == 0
+
+
+def _back(**kw):
+    d = dict(dy=P, lddy=64, x=P, ldx=32, xs=None, dtype=N.BF16, a=P, slot_a=256, b=P, slot_b=512, adapter=P, is64=0,
+             per=1, scaling=P, dx=P, lddx=32, acc=0, da=P, db=P, m=10, n=64, k=32, s=2, r=8, ws=P, ws_bytes=1 << 30)
+    d.update(kw)
+    return N.LIB.w8a8_lora_backward(d["dy"], d["lddy"], d["x"], d["ldx"], d["xs"], d["dtype"], d["a"], d["slot_a"],
+                                    d["b"], d["slot_b"], d["adapter"], d["is64"], d["per"], d["scaling"], d["dx"],
+                                    d["lddx"], d["acc"], d["da"], d["db"], d["m"], d["n"], d["k"], d["s"], d["r"],
+                                    d["ws"], d["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(r=200), "rank"), (dict(da=None), "go together"), (dict(db=None), "go together"), (dict(n=0), "N > 0"),
+    (dict(k=0), "N > 0"), (dict(dy=None), "NULL"), (dict(x=None), "NULL"), (dict(lddy=3), "stride"),
+    (dict(ldx=3), "stride"), (dict(lddx=3), "stride"), (dict(dtype=N.E4M3), "floating"), (dict(a=None), "NULL"),
+    (dict(x=P + 1), "aligned"), (dict(xs=P + 1), "aligned"), (dict(dx=P + 1), "aligned"), (dict(da=P + 1), "aligned"),
+    (dict(ws_bytes=100), "workspace")])
+def test_lora_backward_refuses(kw, word):
+    assert _back(**kw) == N.ERR_VALUE
+    assert word in _err()
+    assert _back(dx=None, da=None, db=None) == 0  # nothing wanted
+
+
+def test_workspace_sizes():
+    need = N.LIB.w8a8_lora_workspace_bytes
+    assert need(10, 64, 32, 2, 8, 0) >= 10 * 8 * 4
+    assert need(10, 64, 32, 2, 200, 0) == N.ERR_VALUE and need(-1, 64, 32, 2, 8, 1) == N.ERR_VALUE
+    # partial sums of the adapters' gradients stay bounded
+    assert need(100000, 12288, 12288, 64, 128, 1) < 10 << 30
+    assert N.LIB.w8a8_input_grad_workspace_bytes(10, 64, 32, N.S8) == N.ERR_VALUE
+    assert N.LIB.w8a8_input_grad_workspace_bytes(-1, 64, 32, N.BF16) == N.ERR_VALUE
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dy=None), "NULL"), (dict(w=None), "NULL"), (dict(ws=None), "NULL"), (dict(dx=None), "NULL"),
+    (dict(lddy=63), "stride"), (dict(ldw=31), "stride"), (dict(lddx=31), "stride"), (dict(wsn=3), "per-output"),
+    (dict(dtype=N.S32), "floating"), (dict(dy=P + 1), "aligned"), (dict(work=None, work_bytes=0), "workspace"),
+    (dict(m=-1), "negative")])
+def test_input_grad_refuses(kw, word):
+    d = dict(dy=P, lddy=4096, w=P, ldw=32, ws=P, wsn=4096, dtype=N.BF16, dx=P, lddx=32, m=10, n=4096, k=32, work=P,
+             work_bytes=1 << 30)
+    if "lddy" in kw or "wsn" in kw:
+        d.update(n=64, wsn=64)
+    d.update(kw)
+    rc = N.LIB.w8a8_input_grad(d["dy"], d["lddy"], d["w"], d["ldw"], d["ws"], d["wsn"], d["dtype"], d["dx"], d["lddx"],
+                               d["m"], d["n"], d["k"], d["work"], d["work_bytes"], None)
+    assert rc == N.ERR_VALUE and word in _err()
+
+
+def test_activation_refuses():
+    f, g = N.LIB.w8a8_act_checkpoint, N.LIB.w8a8_act_backward
+    assert f(P, N.BF16, 64, 4, 64, 9, P, P, P, None) == N.ERR_VALUE and "activation" in _err()
+    assert f(P, N.S8, 64, 4, 64, 1, P, P, P, None) == N.ERR_VALUE and "floating" in _err()
+    assert f(P, N.BF16, 64, -4, 64, 1, P, P, P, None) == N.ERR_VALUE
+    assert f(None, N.BF16, 64, 4, 64, 1, P, P, P, None) == N.ERR_VALUE and "NULL" in _err()
+    assert f(P, N.BF16, 64, 4, 64, N.CKPT_SWIGLU, P, P, P, None) == N.ERR_VALUE and "stride" in _err()
+    assert f(P + 1, N.BF16, 64, 4, 64, 1, P, P, P, None) == N.ERR_VALUE and "aligned" in _err()
+    assert g(P, N.BF16, 63, 4, 64, 1, P, P, P, None) == N.ERR_VALUE and "stride" in _err()
+    assert g(P, N.BF16, 64, 4, 64, 1, None, P, P, None) == N.ERR_VALUE and "NULL" in _err()
+    assert f(None, N.BF16, 64, 0, 64, 1, None, None, None, None) == 0
+
+
+def test_cpu_tensors_are_refused():
+    import imagine_b200 as W
+
+    x, y, a, b = torch.zeros(2, 8), torch.zeros(2, 4), torch.zeros(1, 2, 8), torch.zeros(1, 4, 2)
+    w, ws = torch.zeros(4, 8, dtype=torch.int8), torch.ones(4)
+    for call in (lambda: W.lora_add(y, x, a, b), lambda: W.lora_backward(y, x, a, b),
+                 lambda: W.int8_linear_backward(y, w, ws), lambda: W.int8_linear_lora(x, w, ws, None, a, b),
+                 lambda: W.act_checkpoint_int8(x), lambda: W.act_backward_int8(x, x, x),
+                 lambda: W.checkpointed_activation(x)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+    with pytest.raises(ValueError, match="unknown activation"):
+        W.act_checkpoint_int8(x, "relu")
+
+
+def test_argument_helpers():
+    """Host-side checks of shapes, strides and indices (device-independent parts)."""
+    from imagine_b200 import adapters as A
+
+    t = torch.zeros(4, 6)
+    assert A._rows(t)[1] == 6 and A._rows(t[:, :3])[1] == 6 and A._rows(t.t())[0].is_contiguous()
+    assert A._rows(t[:1].expand(3, 6))[0].is_contiguous()  # rows that overlap are copied
+    assert A._rows(torch.zeros(2, 3, 0))[0].shape == (6, 0)
+    assert A._rows(torch.zeros(2, 0, 5))[0].shape == (0, 5)
+    assert A._index(None, (4,), 4, None) == (None, 0, 1)
+    assert A._scaling(None, 3, None) is None
