@@ -8,12 +8,13 @@ is no CPU path.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _native as N
-from . import linear as L
-from .adapters import _on, _rows
-from .linear import _code, _cuda, _vp
+from .adapters import _on, _raw_stream, _rows, _same
+from .linear import _code, _cuda
 
 ACTIVATIONS = {"gelu_tanh": N.CKPT_GELU_TANH, "swiglu": N.CKPT_SWIGLU, "silu": N.CKPT_SILU}
 
@@ -44,13 +45,14 @@ def act_checkpoint_int8(x: torch.Tensor, act: str = "gelu_tanh"):
         raise ValueError(f"swiglu rows are [gate | up]: {width} features do not halve")
     k = width // halves
     x2, ldx = _rows(x)
-    m = x2.shape[0]
-    y = torch.empty((*x.shape[:-1], k), dtype=x.dtype, device=dev)
+    lead, dtype = x.shape[:-1], x.dtype
+    code_t = _code(dtype)
+    y = torch.empty((*lead, k), dtype=dtype, device=dev)
     q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty((*x.shape[:-1], halves * _groups(k)), dtype=torch.float32, device=dev)
+    scale = torch.empty((*lead, halves * _groups(k)), dtype=torch.float32, device=dev)
     with _on(dev):
-        N.check(N.LIB.w8a8_act_checkpoint(_vp(x2), _code(x.dtype), ldx, m, k, code, _vp(y), _vp(q),
-                                          _vp(scale), L._stream(dev)))
+        N.check(N.LIB.w8a8_act_checkpoint(x2.data_ptr(), code_t, ldx, math.prod(lead), k, code, y.data_ptr(),
+                                          q.data_ptr(), scale.data_ptr(), _raw_stream(dev.index)))
     return y, q, scale
 
 
@@ -60,22 +62,24 @@ def act_backward_int8(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
     act'(q * scale)`` in dy's dtype, of q's shape."""
     code, halves = _act(act)
     dev = _cuda("dy", dy).device
-    _cuda("q", q, dev)
-    _cuda("scale", scale, dev)
-    k = dy.shape[-1]
-    lead = tuple(dy.shape[:-1])
-    if q.dtype != torch.int8 or tuple(q.shape) != (*lead, halves * k):
+    _same("q", q, dev)
+    _same("scale", scale, dev)
+    lead, k, dtype = dy.shape[:-1], dy.shape[-1], dy.dtype
+    if q.dtype != torch.int8 or q.shape != (*lead, halves * k):
         raise ValueError(f"q must be int8 {(*lead, halves * k)}, got {tuple(q.shape)} of {q.dtype}")
-    if scale.dtype != torch.float32 or tuple(scale.shape) != (*lead, halves * _groups(k)):
+    if scale.dtype != torch.float32 or scale.shape != (*lead, halves * _groups(k)):
         raise ValueError(f"scale must be fp32 {(*lead, halves * _groups(k))}, got "
                          f"{tuple(scale.shape)} of {scale.dtype}")
+    code_t = _code(dtype)
     dy2, lddy = _rows(dy)
-    q = q.contiguous()
-    scale = scale.contiguous()
-    dx = torch.empty(q.shape, dtype=dy.dtype, device=dev)
+    if not q.is_contiguous():
+        q = q.contiguous()
+    if not scale.is_contiguous():
+        scale = scale.contiguous()
+    dx = torch.empty(q.shape, dtype=dtype, device=dev)
     with _on(dev):
-        N.check(N.LIB.w8a8_act_backward(_vp(dy2), _code(dy.dtype), lddy, dy2.shape[0], k, code, _vp(q),
-                                        _vp(scale), _vp(dx), L._stream(dev)))
+        N.check(N.LIB.w8a8_act_backward(dy2.data_ptr(), code_t, lddy, math.prod(lead), k, code, q.data_ptr(),
+                                        scale.data_ptr(), dx.data_ptr(), _raw_stream(dev.index)))
     return dx
 
 

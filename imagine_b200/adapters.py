@@ -24,17 +24,30 @@ from . import linear as L
 from .linear import _code, _cuda, _vp
 
 
+_NO_SWITCH = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _on(dev: torch.device):
     """The device made current for the launch, where it is not already."""
-    if torch.cuda.current_device() == dev.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    return _NO_SWITCH if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _same(name: str, t, dev: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev.index:
+        _cuda(name, t, dev)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t: torch.Tensor) -> tuple:
-    """``t`` as [rows, width] with unit-stride rows that do not overlap (a view
-    where its strides allow, else a copy), and its row stride."""
+    """``t`` as rows of its last dimension, unit stride, that do not overlap (itself
+    or a view where its strides allow, else a copy), and the row stride."""
     width = t.shape[-1]
+    if t.is_contiguous():
+        return t, max(width, 1)
     m = math.prod(t.shape[:-1])
     t2 = t if t.dim() == 2 else t.reshape(m, width)
     if (t2.stride(1) != 1 and width > 1) or (m > 1 and t2.stride(0) < width):
@@ -42,29 +55,31 @@ def _rows(t: torch.Tensor) -> tuple:
     return t2, (t2.stride(0) if m > 1 else max(width, 1))
 
 
-def _out_rows(name: str, t: torch.Tensor, shape, dtype, dev) -> tuple:
-    """The same for an output, which has to be written in place."""
-    _cuda(name, t, dev)
+def _out_rows(name: str, t: torch.Tensor, shape, dtype, dev) -> int:
+    """The row stride of an output, which has to be written in place."""
+    _same(name, t, dev)
     if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
         raise ValueError(f"{name} must be {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    if t.is_contiguous():
+        return max(t.shape[-1], 1)
+    m, width = math.prod(t.shape[:-1]), t.shape[-1]
     try:
-        t2 = t.view(math.prod(t.shape[:-1]), t.shape[-1])
+        t2 = t.view(m, width)
     except RuntimeError as e:
         raise ValueError(f"{name} must have rows one stride apart") from e
-    width, m = t2.shape[1], t2.shape[0]
-    if t2.numel() and ((t2.stride(1) != 1 and width > 1) or (m > 1 and t2.stride(0) < width)):
+    if (t2.stride(1) != 1 and width > 1) or (m > 1 and t2.stride(0) < width):
         raise ValueError(f"{name} must have unit-stride rows that do not overlap")
-    return t2, (t2.stride(0) if m > 1 else max(width, 1))
+    return t2.stride(0) if m > 1 else max(width, 1)
 
 
 def _adapters(a, b, k: int, n: int, dtype, dev) -> tuple:
-    """The stacked adapters, checked, each contiguous: (a, b, S, R)."""
-    _cuda("a", a, dev)
-    _cuda("b", b, dev)
+    """The stacked adapters, checked: (a, its slot stride, b, its slot stride, S, R)."""
+    _same("a", a, dev)
+    _same("b", b, dev)
     if a.dim() != 3 or b.dim() != 3:
         raise ValueError("a must be [adapters, rank, K] and b [adapters, N, rank]")
     s, r, ka = a.shape
-    if ka != k or tuple(b.shape) != (s, n, r):
+    if ka != k or b.shape != (s, n, r):
         raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} do not fit inputs of {k} and "
                          f"outputs of {n} features")
     if a.dtype != dtype or b.dtype != dtype:
@@ -73,12 +88,19 @@ def _adapters(a, b, k: int, n: int, dtype, dev) -> tuple:
         raise ValueError("at least one adapter is needed")
     if not 1 <= r <= 128:
         raise ValueError(f"rank must be 1 to 128, got {r}")
+    slot_a, slot_b = r * k, n * r
     # a slice of a larger stack is taken as it lies
-    if a.stride(2) != 1 or a.stride(1) != k or (s > 1 and a.stride(0) < r * k):
-        a = a.contiguous()
-    if b.stride(2) != 1 or b.stride(1) != r or (s > 1 and b.stride(0) < n * r):
-        b = b.contiguous()
-    return a, b, s, r
+    if not a.is_contiguous():
+        if a.stride(2) == 1 and a.stride(1) == k and a.stride(0) >= slot_a:
+            slot_a = a.stride(0)
+        else:
+            a = a.contiguous()
+    if not b.is_contiguous():
+        if b.stride(2) == 1 and b.stride(1) == r and b.stride(0) >= slot_b:
+            slot_b = b.stride(0)
+        else:
+            b = b.contiguous()
+    return a, slot_a, b, slot_b, s, r
 
 
 def _index(adapter, lead, m: int, dev) -> tuple:
@@ -86,15 +108,14 @@ def _index(adapter, lead, m: int, dev) -> tuple:
     leading dimensions of the rows it covers: [B, S] for each token, [B] for each sample."""
     if adapter is None:
         return None, 0, 1
-    _cuda("adapter", adapter, dev)
-    if adapter.dtype not in (torch.int32, torch.int64):
+    _same("adapter", adapter, dev)
+    if adapter.dtype != torch.int32 and adapter.dtype != torch.int64:
         raise ValueError(f"adapter must be int32 or int64, got {adapter.dtype}")
-    if tuple(adapter.shape) != tuple(lead[:adapter.dim()]):
+    if adapter.shape != lead[:adapter.dim()]:
         raise ValueError(f"adapter {tuple(adapter.shape)} must have the leading dimensions of {tuple(lead)}")
     if not adapter.is_contiguous():
         adapter = adapter.contiguous()
-    count = adapter.numel()
-    return adapter, int(adapter.dtype == torch.int64), max(1, m // max(count, 1))
+    return adapter, int(adapter.dtype == torch.int64), max(1, m // max(adapter.numel(), 1))
 
 
 def _scaling(scaling, s: int, dev):
@@ -102,11 +123,11 @@ def _scaling(scaling, s: int, dev):
         return None
     if isinstance(scaling, (int, float)):
         return torch.full((s,), float(scaling), dtype=torch.float32, device=dev)
-    _cuda("scaling", scaling, dev)
+    _same("scaling", scaling, dev)
     if scaling.numel() != s or scaling.dtype != torch.float32:
         raise ValueError(f"scaling must be fp32 with one value for each of {s} adapters, got "
                          f"{tuple(scaling.shape)} of {scaling.dtype}")
-    return scaling.reshape(-1).contiguous()
+    return scaling if scaling.is_contiguous() else scaling.contiguous()
 
 
 def _workspace(nbytes: int, dev):
@@ -131,28 +152,31 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     The contraction over K and the rank are summed in fp32 and the result is
     rounded once; the same call gives the same bits."""
     dev = _cuda("x", x).device
-    _cuda("y", y, dev)
-    lead, k, n = x.shape[:-1], x.shape[-1], y.shape[-1]
+    _same("y", y, dev)
+    shape, dtype = x.shape, x.dtype
+    lead, k, n = shape[:-1], shape[-1], y.shape[-1]
     if y.shape[:-1] != lead:
-        raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} must have the same rows")
-    if y.dtype != x.dtype:
-        raise ValueError(f"x is {x.dtype} but y {y.dtype}")
-    code = _code(x.dtype)
-    a, b, s, r = _adapters(a, b, k, n, x.dtype, dev)
+        raise ValueError(f"x {tuple(shape)} and y {tuple(y.shape)} must have the same rows")
+    if y.dtype != dtype:
+        raise ValueError(f"x is {dtype} but y {y.dtype}")
+    code = _code(dtype)
+    a, slot_a, b, slot_b, s, r = _adapters(a, b, k, n, dtype, dev)
     y2, ldy = _rows(y)
     x2, ldx = _rows(x)
-    m = y2.shape[0]
+    m = math.prod(lead)
     idx, idx64, per = _index(adapter, lead, m, dev)
     c = _scaling(scaling, s, dev)
     if out is None:
-        out = torch.empty(y.shape, dtype=y.dtype, device=dev)
-    o2, ldo = _out_rows("out", out, y.shape, y.dtype, dev)
+        out, ldo = torch.empty(y.shape, dtype=dtype, device=dev), max(n, 1)
+    else:
+        ldo = _out_rows("out", out, y.shape, dtype, dev)
     with _on(dev):
-        ws = _workspace(N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 0), dev)
+        nbytes = N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 0)
+        ws = _workspace(nbytes, dev)
         N.check(N.LIB.w8a8_lora_add(
-            _vp(y2), ldy, _vp(x2), ldx, code, _vp(a), a.stride(0), _vp(b), b.stride(0), _vp(idx), idx64,
-            per, _vp(c), _vp(o2), ldo, m, n, k, s, r, _vp(ws), ws.numel() if ws is not None else 0,
-            L._stream(dev)))
+            y2.data_ptr(), ldy, x2.data_ptr(), ldx, code, a.data_ptr(), slot_a, b.data_ptr(), slot_b,
+            _ptr(idx), idx64, per, _ptr(c), out.data_ptr(), ldo, m, n, k, s, r, _ptr(ws), nbytes,
+            _raw_stream(dev.index)))
     return out
 
 
@@ -169,41 +193,45 @@ def lora_backward(dy: torch.Tensor, x: Optional[torch.Tensor], a: torch.Tensor, 
     row).  A given ``dx`` (the base linear's input gradient) is added to, in place.
     ``need_dx`` / ``need_weights`` False: None in their place (x may then be None)."""
     dev = _cuda("dy", dy).device
-    lead, n, k = dy.shape[:-1], dy.shape[-1], a.shape[-1]
-    code = _code(dy.dtype)
-    a, b, s, r = _adapters(a, b, k, n, dy.dtype, dev)
+    lead, n, k, dtype = dy.shape[:-1], dy.shape[-1], a.shape[-1], dy.dtype
+    code = _code(dtype)
+    a, slot_a, b, slot_b, s, r = _adapters(a, b, k, n, dtype, dev)
     dy2, lddy = _rows(dy)
-    m = dy2.shape[0]
+    m = math.prod(lead)
     x2, ldx, xs = None, k, None
     if need_weights:
-        _cuda("x", x, dev)
-        if tuple(x.shape) != (*lead, k):
+        _same("x", x, dev)
+        if x.shape != (*lead, k):
             raise ValueError(f"x {tuple(x.shape)} does not fit dy {tuple(dy.shape)} and inputs of {k} features")
-        if x.dtype != (torch.int8 if x_scale is not None else dy.dtype):
-            raise ValueError(f"x is {x.dtype}: int8 codes come with x_scale, anything else is dy's {dy.dtype}")
+        if x.dtype != (dtype if x_scale is None else torch.int8):
+            raise ValueError(f"x is {x.dtype}: int8 codes come with x_scale, anything else is dy's {dtype}")
         if x_scale is not None:
-            _cuda("x_scale", x_scale, dev)
+            _same("x_scale", x_scale, dev)
             if x_scale.dtype != torch.float32 or x_scale.numel() != m:
                 raise ValueError(f"x_scale must be fp32 with one value for each of {m} rows")
-            xs = x_scale.reshape(-1).contiguous()
+            xs = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
         x2, ldx = _rows(x)
     idx, idx64, per = _index(adapter, lead, m, dev)
     c = _scaling(scaling, s, dev)
-    accumulate = dx is not None
-    if need_dx and dx is None:
-        dx = torch.empty((*lead, k), dtype=dy.dtype, device=dev)
-    d2, lddx = _out_rows("dx", dx, (*lead, k), dy.dtype, dev) if need_dx else (None, k)
+    lddx, accumulate = k, 0
+    if not need_dx:
+        dx = None
+    elif dx is None:
+        dx = torch.empty((*lead, k), dtype=dtype, device=dev)
+    else:
+        lddx, accumulate = _out_rows("dx", dx, (*lead, k), dtype, dev), 1
     da = db = None
     if need_weights:
-        da = torch.empty((s, r, k), dtype=dy.dtype, device=dev)
-        db = torch.empty((s, n, r), dtype=dy.dtype, device=dev)
+        da = torch.empty((s, r, k), dtype=dtype, device=dev)
+        db = torch.empty((s, n, r), dtype=dtype, device=dev)
     with _on(dev):
-        ws = _workspace(N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 1), dev)
+        nbytes = N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 1)
+        ws = _workspace(nbytes, dev)
         N.check(N.LIB.w8a8_lora_backward(
-            _vp(dy2), lddy, _vp(x2), ldx, _vp(xs), code, _vp(a), a.stride(0), _vp(b), b.stride(0),
-            _vp(idx), idx64, per, _vp(c), _vp(d2), lddx, int(accumulate), _vp(da), _vp(db), m, n, k,
-            s, r, _vp(ws), ws.numel() if ws is not None else 0, L._stream(dev)))
-    return (dx if need_dx else None), da, db
+            dy2.data_ptr(), lddy, _ptr(x2), ldx, _ptr(xs), code, a.data_ptr(), slot_a, b.data_ptr(),
+            slot_b, _ptr(idx), idx64, per, _ptr(c), _ptr(dx), lddx, accumulate, _ptr(da), _ptr(db), m,
+            n, k, s, r, _ptr(ws), nbytes, _raw_stream(dev.index)))
+    return dx, da, db
 
 
 def int8_linear_backward(dy: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
@@ -213,7 +241,7 @@ def int8_linear_backward(dy: torch.Tensor, weight: torch.Tensor, weight_scale: t
     [..., K] in dy's dtype.  The quantisation of the input passes the gradient through
     unchanged (the straight-through estimate)."""
     dev = _cuda("dy", dy).device
-    _cuda("weight", weight, dev)
+    _same("weight", weight, dev)
     if weight.dim() != 2 or weight.dtype != torch.int8:
         raise ValueError("weight must be a 2-D int8 tensor [N, K]")
     if out_dtype not in (None, dy.dtype):
@@ -221,20 +249,24 @@ def int8_linear_backward(dy: torch.Tensor, weight: torch.Tensor, weight_scale: t
     n, k = weight.shape
     if dy.shape[-1] != n:
         raise ValueError(f"dy has {dy.shape[-1]} features, the weight {n} outputs")
-    ws = weight_scale.to(device=dev, dtype=torch.float32).reshape(-1).contiguous()
-    if ws.numel() not in (1, n):
+    ws = weight_scale
+    if ws.get_device() != dev.index or ws.dtype != torch.float32 or not ws.is_contiguous():
+        ws = ws.to(device=dev, dtype=torch.float32).contiguous()
+    if ws.numel() != n and ws.numel() != 1:
         raise ValueError(f"INT8 weight scale must be scalar or per-output-channel, got "
                          f"{tuple(weight_scale.shape)} for weight shape {tuple(weight.shape)}")
     code = _code(dy.dtype)
     dy2, lddy = _rows(dy)
     w2, ldw = _rows(weight)
-    m = dy2.shape[0]
-    dx = torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dev)
+    lead = dy.shape[:-1]
+    m = math.prod(lead)
+    dx = torch.empty((*lead, k), dtype=dy.dtype, device=dev)
     with _on(dev):
-        work = _workspace(N.LIB.w8a8_input_grad_workspace_bytes(m, n, k, code), dev)
+        nbytes = N.LIB.w8a8_input_grad_workspace_bytes(m, n, k, code)
+        work = _workspace(nbytes, dev)
         N.check(N.LIB.w8a8_input_grad(
-            _vp(dy2), lddy, _vp(w2), ldw, _vp(ws), ws.numel(), code, _vp(dx), k, m, n, k, _vp(work),
-            work.numel() if work is not None else 0, L._stream(dev)))
+            dy2.data_ptr(), lddy, w2.data_ptr(), ldw, ws.data_ptr(), ws.numel(), code, dx.data_ptr(),
+            max(k, 1), m, n, k, _ptr(work), nbytes, _raw_stream(dev.index)))
     return dx
 
 
@@ -244,8 +276,8 @@ class _Int8LinearLora(torch.autograd.Function):
         dev = x.device
         n, k = weight.shape
         ws = weight_scale.to(device=dev, dtype=torch.float32).reshape(-1).contiguous()
-        x2, ldx = _rows(x)
-        m = x2.shape[0]
+        m = math.prod(x.shape[:-1])
+        x2 = _rows(x)[0].reshape(m, k)
         w = weight if weight.is_contiguous() else weight.contiguous()
         q, xs = L.quantize_int8_rowwise(x2)
         bias = None if bias is None else bias.to(device=dev, dtype=x.dtype).reshape(-1).contiguous()
@@ -304,6 +336,6 @@ def int8_linear_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
             raise ValueError(f"INT8 weight scale must be scalar or per-output-channel, got "
                              f"{tuple(weight_scale.shape)} for weight shape {tuple(weight.shape)}")
         _code(x.dtype)
-        _, _, s, _ = _adapters(a, b, k, n, x.dtype, dev)
-        scaling = _scaling(scaling, s, dev)
+        _adapters(a, b, k, n, x.dtype, dev)
+        scaling = _scaling(scaling, a.shape[0], dev)
         return _Int8LinearLora.apply(x, weight, weight_scale, bias, a, b, adapter, scaling, keep_input)

@@ -13,9 +13,11 @@
 // sigmoid from e = exp(-|z|) alone: s = 1 / (1 + e) or e / (1 + e), and
 // s (1 - s) = e / (1 + e)^2, with no cancellation and no overflow.
 //
-// Both passes read and write every byte once and are bound by HBM: a group is
-// 16 lanes of 8 elements (one 16-byte load a lane at 16 bits), so the absolute
-// maximum is four shuffles.
+// Both passes read and write every byte once.  At 16 bits they are held by HBM only
+// if an element costs fewer than about twenty instructions, hence the arithmetic
+// on pairs, and a group in four lanes of 32 elements each (four 16-byte loads in
+// flight): the scale's two divisions, the index arithmetic and the shuffles are
+// paid once for 32 elements.  With 16 lanes of 8 the forward pass was issue-bound.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -32,94 +34,224 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroup = 128;
-constexpr int kLanes = 16;  // lanes per group, eight elements each
-
-// e = exp(-|z|) and r = 1 / (1 + e).  The 16-bit types take the approximate
-// exponential and reciprocal (2^-21, far below their rounding).
-template <typename T>
-__device__ __forceinline__ void exp_recip(float z, float& e, float& r) {
-  if constexpr (std::is_same<T, float>::value) {
-    e = expf(-fabsf(z));
-    r = __fdiv_rn(1.0f, 1.0f + e);
-  } else {
-    e = __expf(-fabsf(z));
-    r = __fdividef(1.0f, 1.0f + e);
-  }
-}
+constexpr int kLanes = 4;   // lanes per group
+constexpr int kChunks = 4;  // chunks of eight elements a lane: lane l has chunks l, l + 4, l + 8, l + 12
 
 constexpr float kC0 = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kC1 = 0.044715f;
-
-template <typename T>
-__device__ __forceinline__ float gelu(float x) {
-  float e, r;
-  const float z = 2.0f * kC0 * (x + kC1 * x * x * x);
-  exp_recip<T>(z, e, r);
-  return x * (z >= 0.0f ? r : e * r);
-}
-template <typename T>
-__device__ __forceinline__ float gelu_slope(float x) {
-  float e, r;
-  const float x2 = x * x;
-  const float z = 2.0f * kC0 * (x + kC1 * x2 * x);
-  exp_recip<T>(z, e, r);
-  const float s = z >= 0.0f ? r : e * r;
-  // beyond |x| = 16 the second term is below 1e-100; x2 may overflow there
-  const float t = fabsf(x) > 16.0f ? 0.0f : x * e * r * r * (2.0f * kC0) * (1.0f + 3.0f * kC1 * x2);
-  return x != x ? x : s + t;
-}
-template <typename T>
-__device__ __forceinline__ float silu(float x) {
-  float e, r;
-  exp_recip<T>(x, e, r);
-  return x * (x >= 0.0f ? r : e * r);
-}
-// sigmoid(x) and the slope of silu
-template <typename T>
-__device__ __forceinline__ float silu_slope(float x, float& s) {
-  float e, r;
-  exp_recip<T>(x, e, r);
-  s = x >= 0.0f ? r : e * r;
-  const float other = x >= 0.0f ? e * r : r;  // 1 - s
-  return s + x * s * other;
-}
+constexpr float kLog2e = 1.4426950408889634f;
 
 enum Act : int { kGelu = 1, kSwiglu = 2, kSilu = 3 };
 
-// One group (this thread's eight elements v): codes and scale.  A group with
-// an infinity or a NaN keeps NaN as its scale, so that its gradient is NaN.
-__device__ __forceinline__ uint2 quant_group(const float (&v)[8], float& scale) {
-  // as integers, so that NaN is the largest
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (m >= 0x7F800000u) {
-    scale = __uint_as_float(0x7FC00000u);
-    return make_uint2(0, 0);
+// ---- fp32: the accurate exponential and an IEEE division
+__device__ __forceinline__ void exp_recip(float z, float& e, float& r) {
+  e = expf(-fabsf(z));
+  r = __fdiv_rn(1.0f, 1.0f + e);
+}
+// sigmoid's argument and that argument's slope
+template <int kAct>
+__device__ __forceinline__ void argument(float x, float& z, float& dz) {
+  if constexpr (kAct == kGelu) {
+    const float x2 = x * x;
+    z = 2.0f * kC0 * (x + kC1 * x2 * x);
+    dz = 2.0f * kC0 * (1.0f + 3.0f * kC1 * x2);
+  } else {
+    z = x;
+    dz = 1.0f;
   }
-  scale = fmaxf(__fdiv_rn(__uint_as_float(m), 127.0f), 1.0e-30f);
-  const float recip = __frcp_rn(scale);
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // rne(x / scale) from the product with the reciprocal, which is within
-    // 2^-22 of the quotient (below 4e-5): only next to a half does the divide decide
-    const float y = v[i] * recip;
-    const float n = rintf(y);
-    int q = static_cast<int>(n);
-    if (fabsf(y - n) > 0.4999f) q = __float2int_rn(__fdiv_rn(v[i], scale));
-    w[i >> 2] |= static_cast<uint32_t>(q & 0xFF) << (8 * (i & 3));
+}
+template <int kAct>
+__device__ __forceinline__ float act_one(float x) {
+  float z, dz, e, r;
+  argument<kAct>(x, z, dz);
+  exp_recip(z, e, r);
+  return x * (z >= 0.0f ? r : e * r);
+}
+// The slope of x sigmoid(z(x)), and sigmoid(z) itself.
+template <int kAct>
+__device__ __forceinline__ float slope_one(float x, float& s) {
+  float z, dz, e, r;
+  // beyond 16 gelu's second term is below 1e-100 and x^2 may overflow
+  const float c = kAct == kGelu ? (x != x ? x : fminf(fmaxf(x, -16.0f), 16.0f)) : x;
+  argument<kAct>(c, z, dz);
+  exp_recip(z, e, r);
+  s = z >= 0.0f ? r : e * r;
+  const float t = c * (e * r * r) * dz;
+  return s + (fabsf(z) > 200.0f ? 0.0f : t);  // exp(-200) |z|: 0 in fp32; an infinite x times 0
+}
+
+// ---- 16-bit types: two elements an instruction (f32x2), approximate
+// exponential and reciprocal (2^-22, far below the output's rounding).
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float v) { return pk(v, v); }
+
+// z log2(e)
+template <int kAct>
+__device__ __forceinline__ uint64_t argument_two(uint64_t x) {
+  if constexpr (kAct == kGelu) {
+    constexpr float k = 2.0f * kC0 * kLog2e;
+    return mul2(x, fma2(mul2(x, x), both(k * kC1), both(k)));
+  } else {
+    return mul2(x, both(kLog2e));
   }
-  return make_uint2(w[0], w[1]);
+}
+// With e = exp(-|z|): er = e / (1 + e) and r = 1 / (1 + e); the sigmoid is r where z >= 0, else er
+__device__ __forceinline__ void exp_recip_two(uint64_t z, uint64_t& er, uint64_t& r, uint64_t& s) {
+  // the exponential 2^24 too large, so that flushing its subnormals to zero loses
+  // nothing that bf16 holds (ftz: one instruction instead of four)
+  const uint64_t e = mul2(pk(ex2(24.0f - fabsf(lo(z))), ex2(24.0f - fabsf(hi(z)))), both(5.9604644775390625e-8f));
+  const uint64_t d = add2(e, both(1.0f));
+  r = pk(rcp(lo(d)), rcp(hi(d)));
+  er = mul2(e, r);
+  s = pk(lo(z) >= 0.0f ? lo(r) : lo(er), hi(z) >= 0.0f ? hi(r) : hi(er));
+}
+template <int kAct>
+__device__ __forceinline__ uint64_t act_two(uint64_t x) {
+  uint64_t er, r, s;
+  exp_recip_two(argument_two<kAct>(x), er, r, s);
+  return mul2(x, s);
+}
+// The slope of x sigmoid(z(x)), and sigmoid(z) itself.
+template <int kAct>
+__device__ __forceinline__ uint64_t slope_two(uint64_t x, uint64_t& s) {
+  uint64_t er, r;
+  if constexpr (kAct == kGelu) {
+    // beyond |x| = 16 the second term is below 1e-100 whatever its factor: x^2 held
+    // at 256 keeps the factor finite
+    constexpr float k = 2.0f * kC0;
+    const uint64_t x2 = mul2(x, x);
+    const uint64_t m = pk(fminf(lo(x2), 256.0f), fminf(hi(x2), 256.0f));
+    exp_recip_two(mul2(x, fma2(m, both(k * kC1 * kLog2e), both(k * kLog2e))), er, r, s);
+    return fma2(mul2(x, mul2(er, r)), fma2(m, both(3.0f * k * kC1), both(k)), s);
+  } else {
+    exp_recip_two(argument_two<kAct>(x), er, r, s);
+    return fma2(x, mul2(er, r), s);
+  }
+}
+
+// The scale of a group from the bits of its absolute maximum, and its reciprocal.
+// A group with an infinity or a NaN keeps NaN as its scale, so that its
+// gradient is NaN, and codes of zero.
+__device__ __forceinline__ float group_scale(uint32_t amax, float& recip) {
+  if (amax >= 0x7F800000u) {
+    recip = 0.0f;
+    return __uint_as_float(0x7FC00000u);
+  }
+  const float scale = fmaxf(__fdiv_rn(__uint_as_float(amax), 127.0f), 1.0e-30f);
+  recip = __frcp_rn(scale);
+  return scale;
+}
+
+// Codes of eight elements: rne(x / scale) from the product with the reciprocal,
+// which is within 2^-22 of the quotient (below 4e-5 in all): only next to a half does
+// the divide decide.  Adding 1.5 * 2^23 rounds to an integer, whose low byte is
+// the code.
+__device__ __forceinline__ uint2 codes_of(const uint64_t (&v)[4], float scale, float recip) {
+  const uint64_t magic = both(12582912.0f);
+  uint64_t n[4];
+  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t y = mul2(v[i], both(recip));
+    n[i] = add2(y, magic);
+    const uint64_t d = sub2(y, sub2(n[i], magic));
+    off = fmaxf(off, fmaxf(fabsf(lo(d)), fabsf(hi(d))));
+  }
+  if (off > 0.49995f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = add2(pk(__fdiv_rn(lo(v[i]), scale), __fdiv_rn(hi(v[i]), scale)), magic);
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t p = __byte_perm(static_cast<uint32_t>(n[2 * i]), static_cast<uint32_t>(n[2 * i] >> 32), 0x0040);
+    const uint32_t q = __byte_perm(static_cast<uint32_t>(n[2 * i + 1]), static_cast<uint32_t>(n[2 * i + 1] >> 32), 0x0040);
+    w[i] = __byte_perm(p, q, 0x5410);
+  }
+  // a spoiled group's codes are 0 (its elements times a reciprocal of 0 may be NaN)
+  return scale == scale ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
+}
+
+// |x| of eight elements: the largest, as the bits of its fp32 value (NaN is the largest of all).
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max(const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 2) {
+    const uint2* u = reinterpret_cast<const uint2*>(r.e);
+    const uint32_t k = 0x7FFF7FFFu;
+    return __vmaxu2(__vmaxu2(u[0].x & k, u[0].y & k), __vmaxu2(u[1].x & k, u[1].y & k));
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(r.e[i]) & 0x7FFFFFFFu);
+    return m;
+  }
+}
+// The group's, over its lanes.
+template <typename T>
+__device__ __forceinline__ uint32_t group_max(uint32_t m) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, m, o);
+    m = sizeof(T) == 2 ? __vmaxu2(m, other) : max(m, other);
+  }
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t h = static_cast<uint16_t>(max(m & 0xFFFFu, m >> 16));
+    if constexpr (std::is_same<T, __half>::value) {
+      m = __float_as_uint(__half2float(__ushort_as_half(h)));
+    } else {
+      m = static_cast<uint32_t>(h) << 16;
+    }
+  }
+  return m;
 }
 
 template <typename T>
-__device__ __forceinline__ void store8_out(T* p, const float (&v)[8], int valid, bool vec) {
+__device__ __forceinline__ void widen(uint64_t (&v)[4], const Raw8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const uint32_t u = reinterpret_cast<const uint32_t*>(r.e)[i];
+      v[i] = pk(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+    } else {
+      v[i] = pk(to_f(r.e[2 * i]), to_f(r.e[2 * i + 1]));
+    }
+  }
+}
+// Eight codes times their scale.  A code's float comes from its byte placed in
+// the mantissa of 2^23 (an integer conversion takes a quarter of the rate).
+__device__ __forceinline__ void widen_codes(uint64_t (&v)[4], const Raw8<int8_t>& r, float scale) {
+  const uint2 u = *reinterpret_cast<const uint2*>(r.e);
+  const uint32_t x[2] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u};
+  const uint64_t base = both(-8388736.0f);  // -(2^23 + 128)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __byte_perm(x[i >> 1], 0x4B000000u, (i & 1) ? 0x7542 : 0x7540);
+    const uint32_t b = __byte_perm(x[i >> 1], 0x4B000000u, (i & 1) ? 0x7543 : 0x7541);
+    v[i] = mul2(add2(pk(__uint_as_float(a), __uint_as_float(b)), base), both(scale));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_two(T* p, const uint64_t (&v)[4], int valid, bool vec) {
   Raw8<T> o;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o.e[i] = from_f<T>(v[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      reinterpret_cast<uint32_t*>(o.e)[i] = pack_bf16(lo(v[i]), hi(v[i]));
+    } else {
+      o.e[2 * i] = from_f<T>(lo(v[i]));
+      o.e[2 * i + 1] = from_f<T>(hi(v[i]));
+    }
+  }
   if (vec && valid >= 8) {
 #pragma unroll
     for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) {
@@ -143,101 +275,164 @@ __device__ __forceinline__ void store_codes(int8_t* p, uint2 w, int valid, bool 
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void load_f8(float (&v)[8], const T* p, int valid, bool vec) {
-  Raw8<T> r;
-  load8(r, p, valid, vec);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f(r.e[i]);
+// Quotient of an item number below 2^31 by the number of groups in a row: one wide
+// multiplication by m = ceil(2^(31 + l) / d), 2^l >= d, whose excess over the
+// true factor is below 2^l and moves no quotient of a number below 2^31.
+struct Groups {
+  uint32_t count;
+  uint64_t m;
+  int shift;
+  __device__ __forceinline__ uint32_t row_of(uint32_t item) const {
+    return static_cast<uint32_t>((static_cast<uint64_t>(item) * m) >> shift);
+  }
+};
+Groups groups_of(int K) {
+  Groups g;
+  g.count = static_cast<uint32_t>((K + kGroup - 1) / kGroup);
+  int l = 0;
+  while ((1ull << l) < g.count) ++l;
+  g.shift = 31 + l;
+  g.m = ((1ull << g.shift) + g.count - 1) / g.count;
+  return g;
 }
 
-// Forward.  Item = one group of one row (of both halves when gated); 16 lanes each.
+struct Item {
+  int64_t row;
+  int c;       // the lane's first chunk; chunk j is 32 j further
+  int left;    // elements of the row (or half) from c on, 0 for no item
+  uint32_t g;
+};
+__device__ __forceinline__ Item item_at(uint64_t item, uint32_t items, const Groups& groups, int K) {
+  Item t;
+  const bool live = item < items;
+  const uint32_t i = live ? static_cast<uint32_t>(item) : 0;
+  const uint32_t row = groups.row_of(i);
+  t.row = row;
+  t.g = i - row * groups.count;
+  t.c = static_cast<int>(t.g) * kGroup + (threadIdx.x % kLanes) * 8;
+  t.left = live ? K - t.c : 0;
+  return t;
+}
+constexpr int kStep = kLanes * 8;  // elements from one of a lane's chunks to the next
+
+// Forward.  Item = one group of one row (of both halves when gated).  Every lane
+// of a warp makes the same number of steps (shuffles).
 template <typename T, int kAct>
 __global__ void __launch_bounds__(kThreads) act_checkpoint_kernel(
-    const T* __restrict__ x, int64_t ldx, int64_t rows, int K, int groups, int vec, T* __restrict__ y,
-    int8_t* __restrict__ q, float* __restrict__ scale) {
+    const T* __restrict__ x, int64_t ldx, uint32_t items, int K, Groups groups, int vec,
+    T* __restrict__ y, int8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int kHalves = kAct == kSwiglu ? 2 : 1;
-  const int64_t items = rows * groups;
-  const int sub = threadIdx.x % kLanes;
-  // whole half-warps pair up: both run the same number of steps (shuffles)
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes); base < items;
-       base += static_cast<int64_t>(gridDim.x) * (kThreads / kLanes)) {
-    const int64_t item = base + threadIdx.x / kLanes;
-    const bool live = item < items;
-    const int64_t row = live ? item / groups : 0;
-    const int g = live ? static_cast<int>(item - row * groups) : 0;
-    const int c = g * kGroup + sub * 8;
-    const int valid = live ? min(8, K - c) : 0;
-    float v[kHalves][8];
+  constexpr uint32_t kPerBlock = kThreads / kLanes;
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * kPerBlock; base < items;
+       base += static_cast<uint64_t>(gridDim.x) * kPerBlock) {
+    const Item it = item_at(base + threadIdx.x / kLanes, items, groups, K);
+    Raw8<T> raw[kHalves][kChunks];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) load_f8(v[h], x + row * ldx + h * static_cast<int64_t>(K) + c, valid, vec != 0);
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+        load8(raw[h][j], x + it.row * ldx + h * static_cast<int64_t>(K) + it.c + j * kStep,
+              min(8, it.left - j * kStep), vec != 0);
+    float s[kHalves], recip[kHalves];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
-      float s;
-      const uint2 w = quant_group(v[h], s);
-      if (valid > 0) store_codes(q + (row * kHalves + h) * K + c, w, valid, vec != 0);
-      if (live && sub == 0) scale[(row * kHalves + h) * groups + g] = s;
-    }
-    float o[8];
+      uint32_t m = abs_max(raw[h][0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (kAct == kGelu) o[i] = gelu<T>(v[0][i]);
-      if constexpr (kAct == kSilu) o[i] = silu<T>(v[0][i]);
-      if constexpr (kAct == kSwiglu) o[i] = silu<T>(v[0][i]) * v[kHalves - 1][i];
+      for (int j = 1; j < kChunks; ++j) {
+        const uint32_t o = abs_max(raw[h][j]);
+        m = sizeof(T) == 2 ? __vmaxu2(m, o) : max(m, o);
+      }
+      s[h] = group_scale(group_max<T>(m), recip[h]);
+      if (it.left > 0 && threadIdx.x % kLanes == 0) scale[(it.row * kHalves + h) * groups.count + it.g] = s[h];
     }
-    if (valid > 0) store8_out(y + row * K + c, o, valid, vec != 0);
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      const int valid = it.left - j * kStep;
+      if (valid <= 0) break;
+      const int c = it.c + j * kStep;
+      uint64_t v[kHalves][4], o[4];
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        widen(v[h], raw[h][j]);
+        store_codes(q + (it.row * kHalves + h) * K + c, codes_of(v[h], s[h], recip[h]), valid, vec != 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        constexpr int kOne = kAct == kGelu ? kGelu : kSilu;
+        if constexpr (std::is_same<T, float>::value) {
+          o[i] = pk(act_one<kOne>(lo(v[0][i])), act_one<kOne>(hi(v[0][i])));
+        } else {
+          o[i] = act_two<kOne>(v[0][i]);
+        }
+        if constexpr (kAct == kSwiglu) o[i] = mul2(o[i], v[kHalves - 1][i]);
+      }
+      store_two(y + it.row * K + c, o, valid, vec != 0);
+    }
   }
 }
 
 // Backward: dx [rows, halves * K] from dy [rows, K] and the checkpoint.
 template <typename T, int kAct>
 __global__ void __launch_bounds__(kThreads) act_backward_kernel(
-    const T* __restrict__ dy, int64_t lddy, int64_t rows, int K, int groups, int vec,
+    const T* __restrict__ dy, int64_t lddy, uint32_t items, int K, Groups groups, int vec,
     const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ dx) {
   constexpr int kHalves = kAct == kSwiglu ? 2 : 1;
-  const int64_t items = rows * groups;
-  const int sub = threadIdx.x % kLanes;
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
-       item < items; item += static_cast<int64_t>(gridDim.x) * (kThreads / kLanes)) {
-    const int64_t row = item / groups;
-    const int g = static_cast<int>(item - row * groups);
-    const int c = g * kGroup + sub * 8;
-    const int valid = min(8, K - c);
-    if (valid <= 0) continue;
-    float d[8], v[kHalves][8], o[kHalves][8];
-    load_f8(d, dy + row * lddy + c, valid, vec != 0);
+  constexpr uint32_t kPerBlock = kThreads / kLanes;
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * kPerBlock; base < items;
+       base += static_cast<uint64_t>(gridDim.x) * kPerBlock) {
+    const Item it = item_at(base + threadIdx.x / kLanes, items, groups, K);
+    Raw8<T> rd[kChunks];
+    Raw8<int8_t> rq[kHalves][kChunks];
+    float sc[kHalves];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      load_f8(v[h], q + (row * kHalves + h) * K + c, valid, vec != 0);
-      const float s = __ldg(scale + (row * kHalves + h) * groups + g);
+    for (int h = 0; h < kHalves; ++h) sc[h] = __ldg(scale + (it.row * kHalves + h) * groups.count + it.g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[h][i] *= s;
+    for (int j = 0; j < kChunks; ++j) {
+      const int valid = min(8, it.left - j * kStep);
+      load8(rd[j], dy + it.row * lddy + it.c + j * kStep, valid, vec != 0);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+        load8(rq[h][j], q + (it.row * kHalves + h) * K + it.c + j * kStep, valid, vec != 0);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (kAct == kGelu) o[0][i] = d[i] * gelu_slope<T>(v[0][i]);
-      if constexpr (kAct == kSilu) {
-        float s;
-        o[0][i] = d[i] * silu_slope<T>(v[0][i], s);
-      }
-      if constexpr (kAct == kSwiglu) {
-        float s;
-        const float slope = silu_slope<T>(v[0][i], s);
-        o[0][i] = d[i] * v[kHalves - 1][i] * slope;
-        o[kHalves - 1][i] = d[i] * v[0][i] * s;
-      }
-    }
+    for (int j = 0; j < kChunks; ++j) {
+      const int valid = it.left - j * kStep;
+      if (valid <= 0) break;
+      uint64_t d[4], v[kHalves][4], o[kHalves][4];
+      widen(d, rd[j]);
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h)
-      store8_out(dx + (row * kHalves + h) * K + c, o[h], valid, vec != 0);
+      for (int h = 0; h < kHalves; ++h) widen_codes(v[h], rq[h][j], sc[h]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        constexpr int kOne = kAct == kGelu ? kGelu : kSilu;
+        uint64_t s, slope;
+        if constexpr (std::is_same<T, float>::value) {
+          float s0, s1;
+          const float a0 = slope_one<kOne>(lo(v[0][i]), s0), a1 = slope_one<kOne>(hi(v[0][i]), s1);
+          slope = pk(a0, a1);
+          s = pk(s0, s1);
+        } else {
+          slope = slope_two<kOne>(v[0][i], s);
+        }
+        if constexpr (kAct == kSwiglu) {
+          o[0][i] = mul2(mul2(d[i], v[kHalves - 1][i]), slope);
+          o[kHalves - 1][i] = mul2(mul2(d[i], v[0][i]), s);
+        } else {
+          o[0][i] = mul2(d[i], slope);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+        store_two(dx + (it.row * kHalves + h) * K + it.c + j * kStep, o[h], valid, vec != 0);
+    }
   }
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 unsigned blocks_for(int64_t items) {
-  const int64_t need = (items + kThreads / kLanes - 1) / (kThreads / kLanes);
-  return static_cast<unsigned>(std::min<int64_t>(need, 32ll * device_sm_count()));
+  const int64_t per = kThreads / kLanes;
+  return static_cast<unsigned>(std::min<int64_t>((items + per - 1) / per, 8ll * device_sm_count()));
 }
 
 int launched(const char* what) {
@@ -249,39 +444,60 @@ int launched(const char* what) {
   return 0;
 }
 
+// Rows a launch takes: item numbers stay below 2^31.
+int64_t rows_per_launch(const Groups& g) { return std::max<int64_t>(1, ((1ll << 31) - 1) / g.count); }
+
 template <typename T>
 int checkpoint_typed(const void* x, int64_t ldx, int64_t rows, int K, int act, void* y, int8_t* q,
                      float* scale, cudaStream_t stream) {
-  const int groups = (K + kGroup - 1) / kGroup;
+  const Groups groups = groups_of(K);
+  const int64_t halves = act == kSwiglu ? 2 : 1;
   // every group starts on a vector boundary: rows, halves and codes alike
   const int vec = K % 8 == 0 && aligned16(x) && (ldx * static_cast<int64_t>(sizeof(T))) % 16 == 0 &&
                   aligned16(y) && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  const unsigned grid = blocks_for(rows * groups);
   const T* xp = static_cast<const T*>(x);
   T* yp = static_cast<T*>(y);
-  switch (act) {
-    case kGelu: act_checkpoint_kernel<T, kGelu><<<grid, kThreads, 0, stream>>>(xp, ldx, rows, K, groups, vec, yp, q, scale); break;
-    case kSilu: act_checkpoint_kernel<T, kSilu><<<grid, kThreads, 0, stream>>>(xp, ldx, rows, K, groups, vec, yp, q, scale); break;
-    default: act_checkpoint_kernel<T, kSwiglu><<<grid, kThreads, 0, stream>>>(xp, ldx, rows, K, groups, vec, yp, q, scale); break;
+  for (int64_t r = 0; r < rows; r += rows_per_launch(groups)) {
+    const uint32_t items = static_cast<uint32_t>(std::min(rows - r, rows_per_launch(groups)) * groups.count);
+#define CHECKPOINT(ACT)                                                                           \
+  act_checkpoint_kernel<T, ACT><<<blocks_for(items), kThreads, 0, stream>>>(      \
+      xp + r * ldx, ldx, items, K, groups, vec, yp + r * K, q + r * halves * K,                   \
+      scale + r * halves * groups.count)
+    switch (act) {
+      case kGelu: CHECKPOINT(kGelu); break;
+      case kSilu: CHECKPOINT(kSilu); break;
+      default: CHECKPOINT(kSwiglu); break;
+    }
+#undef CHECKPOINT
+    if (int rc = launched("act_checkpoint")) return rc;
   }
-  return launched("act_checkpoint");
+  return 0;
 }
 
 template <typename T>
 int backward_typed(const void* dy, int64_t lddy, int64_t rows, int K, int act, const int8_t* q,
                    const float* scale, void* dx, cudaStream_t stream) {
-  const int groups = (K + kGroup - 1) / kGroup;
+  const Groups groups = groups_of(K);
+  const int64_t halves = act == kSwiglu ? 2 : 1;
   const int vec = K % 8 == 0 && aligned16(dy) && (lddy * static_cast<int64_t>(sizeof(T))) % 16 == 0 &&
                   aligned16(dx) && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  const unsigned grid = blocks_for(rows * groups);
   const T* dp = static_cast<const T*>(dy);
   T* xp = static_cast<T*>(dx);
-  switch (act) {
-    case kGelu: act_backward_kernel<T, kGelu><<<grid, kThreads, 0, stream>>>(dp, lddy, rows, K, groups, vec, q, scale, xp); break;
-    case kSilu: act_backward_kernel<T, kSilu><<<grid, kThreads, 0, stream>>>(dp, lddy, rows, K, groups, vec, q, scale, xp); break;
-    default: act_backward_kernel<T, kSwiglu><<<grid, kThreads, 0, stream>>>(dp, lddy, rows, K, groups, vec, q, scale, xp); break;
+  for (int64_t r = 0; r < rows; r += rows_per_launch(groups)) {
+    const uint32_t items = static_cast<uint32_t>(std::min(rows - r, rows_per_launch(groups)) * groups.count);
+#define BACKWARD(ACT)                                                                             \
+  act_backward_kernel<T, ACT><<<blocks_for(items), kThreads, 0, stream>>>(        \
+      dp + r * lddy, lddy, items, K, groups, vec, q + r * halves * K,                             \
+      scale + r * halves * groups.count, xp + r * halves * K)
+    switch (act) {
+      case kGelu: BACKWARD(kGelu); break;
+      case kSilu: BACKWARD(kSilu); break;
+      default: BACKWARD(kSwiglu); break;
+    }
+#undef BACKWARD
+    if (int rc = launched("act_backward")) return rc;
   }
-  return launched("act_backward");
+  return 0;
 }
 
 }  // namespace

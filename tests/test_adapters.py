@@ -124,7 +124,8 @@ def test_argument_helpers():
     t = torch.zeros(4, 6)
     assert A._rows(t)[1] == 6 and A._rows(t[:, :3])[1] == 6 and A._rows(t.t())[0].is_contiguous()
     assert A._rows(t[:1].expand(3, 6))[0].is_contiguous()  # rows that overlap are copied
-    assert A._rows(torch.zeros(2, 3, 0))[0].shape == (6, 0)
-    assert A._rows(torch.zeros(2, 0, 5))[0].shape == (0, 5)
+    assert A._rows(torch.zeros(2, 3, 0))[1] == 1 and A._rows(torch.zeros(2, 0, 5))[1] == 5
+    assert A._rows(torch.zeros(1, 9)[:, ::2])[0].is_contiguous()  # elements apart are copied
+    assert A._rows(torch.zeros(3, 2, 8)[:, :, :4])[1] == 8  # samples whose rows stay one stride apart
     assert A._index(None, (4,), 4, None) == (None, 0, 1)
     assert A._scaling(None, 3, None) is None
