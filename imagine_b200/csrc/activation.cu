@@ -110,7 +110,9 @@ __device__ __forceinline__ void exp_recip_two(uint64_t z, uint64_t& er, uint64_t
   // nothing that bf16 holds (ftz: one instruction instead of four)
   const uint64_t e = mul2(pk(ex2(24.0f - fabsf(lo(z))), ex2(24.0f - fabsf(hi(z)))), both(5.9604644775390625e-8f));
   const uint64_t d = add2(e, both(1.0f));
-  r = pk(rcp(lo(d)), rcp(hi(d)));
+  // both reciprocals from that of the product, which lies in [1, 4]: the special
+  // function unit (a quarter of the rate) is the busiest
+  r = mul2(both(rcp(lo(d) * hi(d))), pk(hi(d), lo(d)));
   er = mul2(e, r);
   s = pk(lo(z) >= 0.0f ? lo(r) : lo(er), hi(z) >= 0.0f ? hi(r) : hi(er));
 }
@@ -317,114 +319,110 @@ constexpr int kStep = kLanes * 8;  // elements from one of a lane's chunks to th
 
 // Forward.  Item = one group of one row (of both halves when gated).  Every lane
 // of a warp makes the same number of steps (shuffles).
-template <typename T, int kAct>
-__global__ void __launch_bounds__(kThreads) act_checkpoint_kernel(
+// kWhole: rows (or halves) of whole groups on vector boundaries, the usual case, in which nothing
+// has to be looked at element by element.
+template <typename T, int kAct, bool kWhole>
+__global__ void __launch_bounds__(kThreads, kAct == kSwiglu || sizeof(T) == 4 ? 1 : 4) act_checkpoint_kernel(
     const T* __restrict__ x, int64_t ldx, uint32_t items, int K, Groups groups, int vec,
     T* __restrict__ y, int8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int kHalves = kAct == kSwiglu ? 2 : 1;
   constexpr uint32_t kPerBlock = kThreads / kLanes;
-  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * kPerBlock; base < items;
-       base += static_cast<uint64_t>(gridDim.x) * kPerBlock) {
-    const Item it = item_at(base + threadIdx.x / kLanes, items, groups, K);
-    Raw8<T> raw[kHalves][kChunks];
+  const Item it = item_at(static_cast<uint64_t>(blockIdx.x) * kPerBlock + threadIdx.x / kLanes, items, groups, K);
+  Raw8<T> raw[kHalves][kChunks];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h)
+  for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-      for (int j = 0; j < kChunks; ++j)
-        load8(raw[h][j], x + it.row * ldx + h * static_cast<int64_t>(K) + it.c + j * kStep,
-              min(8, it.left - j * kStep), vec != 0);
-    float s[kHalves], recip[kHalves];
+    for (int j = 0; j < kChunks; ++j)
+      load8(raw[h][j], x + it.row * ldx + h * static_cast<int64_t>(K) + it.c + j * kStep,
+            kWhole ? (it.left > 0 ? 8 : 0) : min(8, it.left - j * kStep), kWhole || vec != 0);
+  float s[kHalves], recip[kHalves];
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) {
+    uint32_t m = abs_max(raw[h][0]);
+#pragma unroll
+    for (int j = 1; j < kChunks; ++j) {
+      const uint32_t o = abs_max(raw[h][j]);
+      m = sizeof(T) == 2 ? __vmaxu2(m, o) : max(m, o);
+    }
+    s[h] = group_scale(group_max<T>(m), recip[h]);
+    if (it.left > 0 && threadIdx.x % kLanes == 0) scale[(it.row * kHalves + h) * groups.count + it.g] = s[h];
+  }
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    const int valid = kWhole ? 8 : it.left - j * kStep;
+    if (kWhole ? it.left <= 0 : valid <= 0) break;
+    const int c = it.c + j * kStep;
+    uint64_t v[kHalves][4], o[4];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
-      uint32_t m = abs_max(raw[h][0]);
-#pragma unroll
-      for (int j = 1; j < kChunks; ++j) {
-        const uint32_t o = abs_max(raw[h][j]);
-        m = sizeof(T) == 2 ? __vmaxu2(m, o) : max(m, o);
-      }
-      s[h] = group_scale(group_max<T>(m), recip[h]);
-      if (it.left > 0 && threadIdx.x % kLanes == 0) scale[(it.row * kHalves + h) * groups.count + it.g] = s[h];
+      widen(v[h], raw[h][j]);
+      store_codes(q + (it.row * kHalves + h) * K + c, codes_of(v[h], s[h], recip[h]), valid, kWhole || vec != 0);
     }
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      const int valid = it.left - j * kStep;
-      if (valid <= 0) break;
-      const int c = it.c + j * kStep;
-      uint64_t v[kHalves][4], o[4];
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        widen(v[h], raw[h][j]);
-        store_codes(q + (it.row * kHalves + h) * K + c, codes_of(v[h], s[h], recip[h]), valid, vec != 0);
+    for (int i = 0; i < 4; ++i) {
+      constexpr int kOne = kAct == kGelu ? kGelu : kSilu;
+      if constexpr (std::is_same<T, float>::value) {
+        o[i] = pk(act_one<kOne>(lo(v[0][i])), act_one<kOne>(hi(v[0][i])));
+      } else {
+        o[i] = act_two<kOne>(v[0][i]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        constexpr int kOne = kAct == kGelu ? kGelu : kSilu;
-        if constexpr (std::is_same<T, float>::value) {
-          o[i] = pk(act_one<kOne>(lo(v[0][i])), act_one<kOne>(hi(v[0][i])));
-        } else {
-          o[i] = act_two<kOne>(v[0][i]);
-        }
-        if constexpr (kAct == kSwiglu) o[i] = mul2(o[i], v[kHalves - 1][i]);
-      }
-      store_two(y + it.row * K + c, o, valid, vec != 0);
+      if constexpr (kAct == kSwiglu) o[i] = mul2(o[i], v[kHalves - 1][i]);
     }
+    store_two(y + it.row * K + c, o, valid, kWhole || vec != 0);
   }
 }
 
 // Backward: dx [rows, halves * K] from dy [rows, K] and the checkpoint.
-template <typename T, int kAct>
+template <typename T, int kAct, bool kWhole>
 __global__ void __launch_bounds__(kThreads) act_backward_kernel(
     const T* __restrict__ dy, int64_t lddy, uint32_t items, int K, Groups groups, int vec,
     const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ dx) {
   constexpr int kHalves = kAct == kSwiglu ? 2 : 1;
   constexpr uint32_t kPerBlock = kThreads / kLanes;
-  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * kPerBlock; base < items;
-       base += static_cast<uint64_t>(gridDim.x) * kPerBlock) {
-    const Item it = item_at(base + threadIdx.x / kLanes, items, groups, K);
-    Raw8<T> rd[kChunks];
-    Raw8<int8_t> rq[kHalves][kChunks];
-    float sc[kHalves];
+  const Item it = item_at(static_cast<uint64_t>(blockIdx.x) * kPerBlock + threadIdx.x / kLanes, items, groups, K);
+  Raw8<T> rd[kChunks];
+  Raw8<int8_t> rq[kHalves][kChunks];
+  float sc[kHalves];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) sc[h] = __ldg(scale + (it.row * kHalves + h) * groups.count + it.g);
+  for (int h = 0; h < kHalves; ++h) sc[h] = __ldg(scale + (it.row * kHalves + h) * groups.count + it.g);
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      const int valid = min(8, it.left - j * kStep);
-      load8(rd[j], dy + it.row * lddy + it.c + j * kStep, valid, vec != 0);
+  for (int j = 0; j < kChunks; ++j) {
+    const int valid = kWhole ? (it.left > 0 ? 8 : 0) : min(8, it.left - j * kStep);
+    load8(rd[j], dy + it.row * lddy + it.c + j * kStep, valid, kWhole || vec != 0);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h)
-        load8(rq[h][j], q + (it.row * kHalves + h) * K + it.c + j * kStep, valid, vec != 0);
-    }
+    for (int h = 0; h < kHalves; ++h)
+      load8(rq[h][j], q + (it.row * kHalves + h) * K + it.c + j * kStep, valid, kWhole || vec != 0);
+  }
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      const int valid = it.left - j * kStep;
-      if (valid <= 0) break;
-      uint64_t d[4], v[kHalves][4], o[kHalves][4];
-      widen(d, rd[j]);
+  for (int j = 0; j < kChunks; ++j) {
+    const int valid = kWhole ? 8 : it.left - j * kStep;
+    if (kWhole ? it.left <= 0 : valid <= 0) break;
+    uint64_t d[4], v[kHalves][4], o[kHalves][4];
+    widen(d, rd[j]);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) widen_codes(v[h], rq[h][j], sc[h]);
+    for (int h = 0; h < kHalves; ++h) widen_codes(v[h], rq[h][j], sc[h]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        constexpr int kOne = kAct == kGelu ? kGelu : kSilu;
-        uint64_t s, slope;
-        if constexpr (std::is_same<T, float>::value) {
-          float s0, s1;
-          const float a0 = slope_one<kOne>(lo(v[0][i]), s0), a1 = slope_one<kOne>(hi(v[0][i]), s1);
-          slope = pk(a0, a1);
-          s = pk(s0, s1);
-        } else {
-          slope = slope_two<kOne>(v[0][i], s);
-        }
-        if constexpr (kAct == kSwiglu) {
-          o[0][i] = mul2(mul2(d[i], v[kHalves - 1][i]), slope);
-          o[kHalves - 1][i] = mul2(mul2(d[i], v[0][i]), s);
-        } else {
-          o[0][i] = mul2(d[i], slope);
-        }
+    for (int i = 0; i < 4; ++i) {
+      constexpr int kOne = kAct == kGelu ? kGelu : kSilu;
+      uint64_t s, slope;
+      if constexpr (std::is_same<T, float>::value) {
+        float s0, s1;
+        const float a0 = slope_one<kOne>(lo(v[0][i]), s0), a1 = slope_one<kOne>(hi(v[0][i]), s1);
+        slope = pk(a0, a1);
+        s = pk(s0, s1);
+      } else {
+        slope = slope_two<kOne>(v[0][i], s);
       }
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h)
-        store_two(dx + (it.row * kHalves + h) * K + it.c + j * kStep, o[h], valid, vec != 0);
+      if constexpr (kAct == kSwiglu) {
+        o[0][i] = mul2(mul2(d[i], v[kHalves - 1][i]), slope);
+        o[kHalves - 1][i] = mul2(mul2(d[i], v[0][i]), s);
+      } else {
+        o[0][i] = mul2(d[i], slope);
+      }
     }
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+      store_two(dx + (it.row * kHalves + h) * K + it.c + j * kStep, o[h], valid, kWhole || vec != 0);
   }
 }
 
@@ -432,7 +430,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 unsigned blocks_for(int64_t items) {
   const int64_t per = kThreads / kLanes;
-  return static_cast<unsigned>(std::min<int64_t>((items + per - 1) / per, 8ll * device_sm_count()));
+  return static_cast<unsigned>((items + per - 1) / per);  // below 2^31 / 64
 }
 
 int launched(const char* what) {
@@ -455,18 +453,19 @@ int checkpoint_typed(const void* x, int64_t ldx, int64_t rows, int K, int act, v
   // every group starts on a vector boundary: rows, halves and codes alike
   const int vec = K % 8 == 0 && aligned16(x) && (ldx * static_cast<int64_t>(sizeof(T))) % 16 == 0 &&
                   aligned16(y) && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const bool whole = vec && K % kGroup == 0;
   const T* xp = static_cast<const T*>(x);
   T* yp = static_cast<T*>(y);
   for (int64_t r = 0; r < rows; r += rows_per_launch(groups)) {
     const uint32_t items = static_cast<uint32_t>(std::min(rows - r, rows_per_launch(groups)) * groups.count);
-#define CHECKPOINT(ACT)                                                                           \
-  act_checkpoint_kernel<T, ACT><<<blocks_for(items), kThreads, 0, stream>>>(      \
+#define CHECKPOINT(ACT, WHOLE)                                                                           \
+  act_checkpoint_kernel<T, ACT, WHOLE><<<blocks_for(items), kThreads, 0, stream>>>(      \
       xp + r * ldx, ldx, items, K, groups, vec, yp + r * K, q + r * halves * K,                   \
       scale + r * halves * groups.count)
     switch (act) {
-      case kGelu: CHECKPOINT(kGelu); break;
-      case kSilu: CHECKPOINT(kSilu); break;
-      default: CHECKPOINT(kSwiglu); break;
+      case kGelu: if (whole) CHECKPOINT(kGelu, true); else CHECKPOINT(kGelu, false); break;
+      case kSilu: if (whole) CHECKPOINT(kSilu, true); else CHECKPOINT(kSilu, false); break;
+      default: if (whole) CHECKPOINT(kSwiglu, true); else CHECKPOINT(kSwiglu, false); break;
     }
 #undef CHECKPOINT
     if (int rc = launched("act_checkpoint")) return rc;
@@ -481,18 +480,19 @@ int backward_typed(const void* dy, int64_t lddy, int64_t rows, int K, int act, c
   const int64_t halves = act == kSwiglu ? 2 : 1;
   const int vec = K % 8 == 0 && aligned16(dy) && (lddy * static_cast<int64_t>(sizeof(T))) % 16 == 0 &&
                   aligned16(dx) && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const bool whole = vec && K % kGroup == 0;
   const T* dp = static_cast<const T*>(dy);
   T* xp = static_cast<T*>(dx);
   for (int64_t r = 0; r < rows; r += rows_per_launch(groups)) {
     const uint32_t items = static_cast<uint32_t>(std::min(rows - r, rows_per_launch(groups)) * groups.count);
-#define BACKWARD(ACT)                                                                             \
-  act_backward_kernel<T, ACT><<<blocks_for(items), kThreads, 0, stream>>>(        \
+#define BACKWARD(ACT, WHOLE)                                                                             \
+  act_backward_kernel<T, ACT, WHOLE><<<blocks_for(items), kThreads, 0, stream>>>(        \
       dp + r * lddy, lddy, items, K, groups, vec, q + r * halves * K,                             \
       scale + r * halves * groups.count, xp + r * halves * K)
     switch (act) {
-      case kGelu: BACKWARD(kGelu); break;
-      case kSilu: BACKWARD(kSilu); break;
-      default: BACKWARD(kSwiglu); break;
+      case kGelu: if (whole) BACKWARD(kGelu, true); else BACKWARD(kGelu, false); break;
+      case kSilu: if (whole) BACKWARD(kSilu, true); else BACKWARD(kSilu, false); break;
+      default: if (whole) BACKWARD(kSwiglu, true); else BACKWARD(kSwiglu, false); break;
     }
 #undef BACKWARD
     if (int rc = launched("act_backward")) return rc;
