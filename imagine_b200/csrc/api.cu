@@ -115,7 +115,12 @@ int w8a8_abi_version(void) { return 103; }
 
 int w8a8_device_error(void* stream) {
   int v = 0;
-  const int rc = read_and_clear_device_error(static_cast<cudaStream_t>(stream), &v);
+  int rc = read_and_clear_device_error(static_cast<cudaStream_t>(stream), &v);
+  if (rc == 0) {
+    int w = 0;
+    rc = read_and_clear_input_grad_error(static_cast<cudaStream_t>(stream), &w);
+    if (v == 0) v = w;
+  }
   if (rc != 0) {
     g_last_accel = rc;
     return fail(W8A8_ERR_ACCELERATOR, "reading the device error word failed: %s",

@@ -6,20 +6,49 @@
 // weight would have), two for f16 and three for fp32 (pieces.cuh), which keeps
 // each type's own precision.
 //
-// Tile: 64 rows x 128 columns, 64 of the contraction a step, 8 warps (four of
-// 16 rows, two of 64 columns).  With few tiles the contraction is cut over
-// blocks and the fp32 partial sums are added in a fixed order.
+// Two kernels:
+//   input_grad_kernel     mma.sync tiles of 64 rows x 128 columns, for fp32, for
+//                         few rows and for weights whose rows are not 4-byte aligned
+//   input_grad_tc_kernel  tcgen05, pairs of CTAs on 256 x 256 tiles, for the rest
+// With few tiles the contraction is cut over blocks and the fp32 partial sums
+// are added in a fixed order.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <mutex>
 #include <type_traits>
 
 #include "pieces.cuh"
+#include "quant_common.cuh"
+#include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
 
 namespace w8a8 {
+
+// Why a bounded wait of input_grad_tc_kernel gave up (DeviceError).
+__device__ int g_input_grad_error;
+
+int read_and_clear_input_grad_error(cudaStream_t stream, int* value) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_input_grad_error, sizeof(int), 0,
+                                            cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (v != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_input_grad_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice,
+                                stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  *value = v;
+  return 0;
+}
+
 namespace {
 
 constexpr int kThreads = 256;
@@ -146,13 +175,37 @@ __global__ void __launch_bounds__(kThreads) input_grad_kernel(
     }
 }
 
+// dx from the fp32 partial sums of its cuts, in a fixed order; four elements a
+// thread where the rows allow it.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sum_parts_kernel(const float* __restrict__ part,
-                                                             int parts, int64_t M, int K,
+                                                             int parts, int64_t M, int K, int vec,
                                                              T* __restrict__ dx, int64_t lddx) {
   const int64_t total = M * K;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+  const int64_t start = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  if (vec) {
+    for (int64_t i = start * 4; i < total; i += step * 4) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int p = 0; p < parts; ++p) {
+        const float4 o = __ldg(reinterpret_cast<const float4*>(part + p * total + i));
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
+      }
+      const int64_t row = i / K;
+      T* dst = dx + row * lddx + (i - row * K);
+      const T o[4] = {from_f<T>(v.x), from_f<T>(v.y), from_f<T>(v.z), from_f<T>(v.w)};
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+      } else {
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+      }
+    }
+    return;
+  }
+  for (int64_t i = start; i < total; i += step) {
     float v = 0.0f;
     for (int p = 0; p < parts; ++p) v += __ldg(part + p * total + i);
     const int64_t row = i / K;
@@ -160,17 +213,407 @@ __global__ void __launch_bounds__(kThreads) sum_parts_kernel(const float* __rest
   }
 }
 
-// Blocks for two a multiprocessor, at least four steps each, at most 16 pieces.
+template <typename T>
+void sum_parts(const float* part, int parts, const InputGradArgs& g, cudaStream_t stream) {
+  const int K = static_cast<int>(g.K);
+  const int vec = K % 4 == 0 && reinterpret_cast<uintptr_t>(g.dx) % (4 * sizeof(T)) == 0 && g.lddx % 4 == 0;
+  const int64_t items = g.M * K / (vec ? 4 : 1);
+  const int64_t blocks = std::min<int64_t>((items + kThreads - 1) / kThreads, 16ll * device_sm_count());
+  sum_parts_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(part, parts, g.M, K, vec,
+                                                                             static_cast<T*>(g.dx), g.lddx);
+}
+
+// At most two blocks a multiprocessor (all resident), at least four steps each, at
+// most 16 pieces.
 struct NSplit {
   int count, per;
 };
 NSplit n_split_of(int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = ((M + kBM - 1) / kBM) * ((K + kBC - 1) / kBC);
   const int64_t steps = std::max<int64_t>(1, (N + kBN - 1) / kBN);
-  int64_t want = (2ll * device_sm_count() + tiles - 1) / std::max<int64_t>(1, tiles);
+  int64_t want = 2ll * device_sm_count() / std::max<int64_t>(1, tiles);
   want = std::max<int64_t>(1, std::min<int64_t>({want, 16, steps / 4}));
   const int64_t per = (steps + want - 1) / want;
   return {static_cast<int>((steps + per - 1) / per), static_cast<int>(per * kBN)};
+}
+
+// ================================================================ tcgen05
+// D[256 x 256] of a CTA pair: rows of dy (or of its pieces) times 256 columns
+// of w, 64 of the contraction a stage, six stages.  The weights come as bf16,
+// transposed to [K][n] once per call by widen_weights_kernel (16 us for 12288 x
+// 4096, against 380 us of products at 5856 rows).  Per CTA:
+//   warp 4     TMA: its 128 rows of dy and its 128 columns of w (both K-major,
+//              128-byte swizzle)
+//   warp 5     MMA issue (the pair's leader), two TMEM accumulators of 256 columns
+//   warps 0-3  epilogue: TMEM -> registers -> dx (or a split's fp32 partial sums)
+// Twelve warps that converted the int8 weights inside this kernel, registers to
+// swizzled shared memory, held it to 643 us where the MMAs alone take 381: every
+// row tile converts the weights again, 500 instructions a warp and stage.
+constexpr int kTmaWarp = 4, kMmaWarp = 5;
+constexpr int kTcThreads = 192;
+constexpr int kTcRows = 128, kTcCols = 256, kTcK = 64, kTcStages = 6;
+constexpr int kTcTile = kTcRows * kTcK * 2;  // bytes of A, and of B, of a stage and CTA
+constexpr int kTcSmem = 1024 + kTcStages * 2 * kTcTile + 256;
+
+__device__ __forceinline__ void mma_bf16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+struct TcArgs {
+  int64_t M;
+  int N, K;
+  int n_blocks;   // blocks of 64 of N; the contraction runs over pieces * n_blocks
+  int kb_total;
+  int col_tiles, row_tiles, splits;
+  void* dx;
+  int64_t lddx;
+  int vec_o;
+  float* part;    // splits > 1
+};
+
+// Unit u: split, then tiles in groups of eight row tiles (the CTAs that run
+// together share rows of dy and columns of w in L2).
+__device__ __forceinline__ void tc_unit(const TcArgs& g, int unit, int& mb, int& cb, int& kb_lo,
+                                        int& kb_hi, int& split) {
+  const int tiles = g.col_tiles * g.row_tiles;
+  split = unit / tiles;
+  const int tile = unit - split * tiles;
+  constexpr int kGroup = 8;
+  const int per = kGroup * g.col_tiles;
+  const int grp = tile / per;
+  const int rows = min(kGroup, g.row_tiles - grp * kGroup);
+  const int r = tile - grp * per;
+  mb = grp * kGroup + r % rows;
+  cb = r / rows;
+  kb_lo = static_cast<int>(static_cast<int64_t>(split) * g.kb_total / g.splits);
+  kb_hi = static_cast<int>(static_cast<int64_t>(split + 1) * g.kb_total / g.splits);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    input_grad_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                         const TcArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* s_a = smem;
+  uint8_t* s_b = smem + kTcStages * kTcTile;
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_b + kTcStages * kTcTile);
+  uint64_t* empty = full + kTcStages;
+  uint64_t* tfull = empty + kTcStages;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* abortv = abort_flag;
+  int* err = &g_input_grad_error;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int units = g.col_tiles * g.row_tiles * g.splits;
+  const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kTcStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 8);  // four epilogue warps of each CTA
+    }
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == kTmaWarp && lane == 0) {
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc<512, 2>(tmem_slot);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int unit = first; ok && unit < units; unit += step) {
+        int mb, cb, lo, hi, split;
+        tc_unit(g, unit, mb, cb, lo, hi, split);
+        const int row = (mb * 2 + static_cast<int>(rank)) * kTcRows;
+        const int col = (cb * 2 + static_cast<int>(rank)) * kTcRows;
+        for (int kb = lo; kb < hi; ++kb, ++it) {
+          const int s = static_cast<int>(it % kTcStages);
+          if (!mbar_wait(&empty[s], ((it / kTcStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          // both CTAs' bytes are counted on the leader's barrier
+          if (leader) mbar_arrive_expect_tx(&full[s], 4 * kTcTile);
+          const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+          tma_load_2d_pair(s_a + s * kTcTile, &tm_a, bar, kb * kTcK, row);
+          tma_load_2d_pair(s_b + s * kTcTile, &tm_b, bar, (kb % g.n_blocks) * kTcK, col);
+        }
+      }
+      if (!ok) {  // let loads already in flight land (bounded)
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000) {
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0 && leader) {
+      constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10)  // f32 = bf16 x bf16
+                                 | (static_cast<uint32_t>(kTcCols >> 3) << 17) |
+                                 (static_cast<uint32_t>(2 * kTcRows >> 4) << 24);
+      uint32_t it = 0, tl = 0;
+      bool ok = true;
+      for (int unit = first; ok && unit < units; unit += step, ++tl) {
+        int mb, cb, lo, hi, split;
+        tc_unit(g, unit, mb, cb, lo, hi, split);
+        const uint32_t acc = tl & 1u;
+        if (!mbar_wait(&tempty[acc], ((tl >> 1) & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty)) break;
+        tc_fence_after();
+        for (int kb = lo; kb < hi; ++kb, ++it) {
+          const int s = static_cast<int>(it % kTcStages);
+          if (!mbar_wait(&full[s], (it / kTcStages) & 1u, abortv, err, kDevTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(s_a + s * kTcTile), b0 = smem_u32(s_b + s * kTcTile);
+#pragma unroll
+          for (int k = 0; k < kTcK / 16; ++k) {
+            mma_bf16_pair(tmem + acc * kTcCols, smem_desc_k_sw128(a0 + k * 32),
+                          smem_desc_k_sw128(b0 + k * 32), idesc, (kb != lo || k != 0) ? 1u : 0u);
+          }
+          umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 0));
+          umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 1));
+        }
+        if (ok) {
+          umma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 0));
+          umma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 1));
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    uint32_t tl = 0;
+    for (int unit = first; unit < units; unit += step, ++tl) {
+      int mb, cb, lo, hi, split;
+      tc_unit(g, unit, mb, cb, lo, hi, split);
+      const uint32_t acc = tl & 1u;
+      const bool done = mbar_wait(&tfull[acc], (tl >> 1) & 1u, abortv, err, kDevTimeoutTmemFull);
+      if (!__all_sync(0xffffffffu, done)) break;
+      tc_fence_after();
+      const int64_t row = static_cast<int64_t>(mb * 2 + static_cast<int>(rank)) * kTcRows + warp * 32 + lane;
+      for (int c = 0; c < kTcCols / 32; ++c) {
+        const int col = cb * kTcCols + c * 32;
+        if (col >= g.K) break;
+        uint32_t v[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + acc * kTcCols + c * 32, v);
+        tmem_ld_wait();
+        if (row >= g.M) {
+        } else if (g.part) {
+          float* p = g.part + (static_cast<int64_t>(split) * g.M + row) * g.K + col;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            if (g.K % 4 == 0 && col + j < g.K) {
+              *reinterpret_cast<uint4*>(p + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (col + j + q < g.K) p[j + q] = __uint_as_float(v[j + q]);
+            }
+          }
+        } else {
+          T* p = static_cast<T*>(g.dx) + row * g.lddx + col;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            T o[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) o[q] = from_f<T>(__uint_as_float(v[j + q]));
+            if (g.vec_o && col + j + 8 <= g.K) {
+              const uint32_t* u = reinterpret_cast<const uint32_t*>(o);
+              *reinterpret_cast<uint4*>(p + j) = make_uint4(u[0], u[1], u[2], u[3]);
+            } else {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                if (col + j + q < g.K) p[j + q] = o[q];
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+    }
+  }
+  __syncthreads();
+  cluster_sync();  // the peer is done with its TMEM and these barriers
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc<512, 2>(tmem);
+  }
+}
+
+// bf16(w ws) (ws NULL: w itself, which bf16 holds) transposed to out[K][n_pad],
+// zero past N.  A block takes 128 rows by 64 columns; a thread 8 rows by 4
+// columns: eight words, from which byte permutations make the floats (a byte in
+// the mantissa of 2^23), four 16-byte pieces of output rows, exchanged through
+// shared memory so that the stores run along n.
+__global__ void __launch_bounds__(kThreads) widen_weights_kernel(
+    const int8_t* __restrict__ w, int64_t ldw, const float* __restrict__ ws, int ws_one, int N, int K,
+    int n_pad, int k_tiles, int vec, __nv_bfloat16* __restrict__ out) {
+  __shared__ __align__(16) uint4 tile[64][16];
+  const int n0 = static_cast<int>(blockIdx.x / k_tiles) * 128, k0 = static_cast<int>(blockIdx.x % k_tiles) * 64;
+  const int kc = threadIdx.x & 15, ng = threadIdx.x >> 4;
+  const int col = k0 + 4 * kc;
+  uint32_t x[8];
+  uint64_t sc[4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int n = n0 + ng * 8 + j;
+    uint32_t v = 0;
+    if (n < N) {
+      const int8_t* p = w + n * ldw + col;
+      if (vec && col + 4 <= K) {
+        v = __ldg(reinterpret_cast<const uint32_t*>(p));
+      } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (col + b < K) v |= static_cast<uint32_t>(static_cast<uint8_t>(p[b])) << (8 * b);
+      }
+    }
+    x[j] = v ^ 0x80808080u;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + ng * 8 + 2 * j;
+    sc[j] = pk(ws && n < N ? __ldg(ws + (ws_one ? 0 : n)) : 1.0f,
+               ws && n + 1 < N ? __ldg(ws + (ws_one ? 0 : n + 1)) : 1.0f);
+  }
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    uint32_t o[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint64_t f = pk(__uint_as_float(__byte_perm(x[2 * p], 0x4B000000u, 0x7540 + b)),
+                            __uint_as_float(__byte_perm(x[2 * p + 1], 0x4B000000u, 0x7540 + b)));
+      const uint64_t v = mul2(add2(f, pk(-8388736.0f, -8388736.0f)), sc[p]);  // -(2^23 + 128)
+      o[p] = pack_bf16(lo(v), hi(v));
+    }
+    const int k = 4 * kc + b;
+    tile[k][ng ^ kc] = make_uint4(o[0], o[1], o[2], o[3]);  // 16 threads, 16 different pieces of a row
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = static_cast<int>(threadIdx.x) + i * kThreads;
+    const int k = at >> 4, c = at & 15;
+    const int n = n0 + c * 8;
+    if (k0 + k < K && n < n_pad)
+      *reinterpret_cast<uint4*>(out + static_cast<int64_t>(k0 + k) * n_pad + n) = tile[k][c ^ (k >> 2)];
+  }
+}
+
+// bf16 pieces of dy ws as planes [row][piece][n_pad], zero past N: the operand
+// of input_grad_tc_kernel for f16.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pieces_kernel(const T* __restrict__ dy, int64_t lddy,
+                                                          const float* __restrict__ ws, int ws_one,
+                                                          int64_t M, int N, int n_pad, int vec,
+                                                          __nv_bfloat16* __restrict__ out) {
+  constexpr int kP = Pieces<T>::n;
+  const int64_t total = M * (n_pad / 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t row = i / (n_pad / 8);
+    const int c = static_cast<int>(i - row * (n_pad / 8)) * 8;
+    const int valid = min(8, N - c);
+    Raw8<T> r;
+    load8(r, dy + row * lddy + c, valid, vec != 0);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = to_f(r.e[j]);
+      if (j < valid) v[j] *= __ldg(ws + (ws_one ? 0 : c + j));
+    }
+    store_pieces<kP>(out + row * kP * n_pad + c, n_pad, v);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess) {
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }
+  });
+  return fn;
+}
+
+// bf16 rows [rows][ld], `inner` of them used, in boxes of 128 rows x 64.
+bool map_rows(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld) {
+  auto fn = tensor_map_encoder();
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[2] = {kTcK, kTcRows}, ones[2] = {1, 1};
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Whether input_grad_tc_kernel takes a call: 16-bit types (fp32 needs its sums
+// apart), more rows than one mma.sync tile and, for bf16, rows of dy that TMA
+// can read.
+bool tc_shape(int64_t M, int64_t N, int64_t K, int dtype) {
+  return dtype != W8A8_F32 && M > kBM && N > 0;
+}
+bool rows_of_16_bytes(const InputGradArgs& g) {
+  return reinterpret_cast<uintptr_t>(g.dy) % 16 == 0 && (g.lddy * 2) % 16 == 0;
+}
+bool tc_operands(const InputGradArgs& g) {
+  return g.dtype != W8A8_BF16 || rows_of_16_bytes(g);
+}
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct TcPlan {
+  int n_blocks, kb_total, row_tiles, col_tiles, splits;
+  int64_t pieces_bytes, weight_bytes, part_bytes;
+};
+// The contraction is cut until every pair of multiprocessors has a unit, with
+// at least sixteen stages a unit (the pipeline's fill and the sum of the parts).
+TcPlan tc_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+  TcPlan p;
+  const int pieces = dtype == W8A8_F16 ? 2 : 1;
+  p.n_blocks = static_cast<int>((N + kTcK - 1) / kTcK);
+  p.kb_total = pieces * p.n_blocks;
+  p.row_tiles = static_cast<int>((M + 2 * kTcRows - 1) / (2 * kTcRows));
+  p.col_tiles = static_cast<int>((K + kTcCols - 1) / kTcCols);
+  const int64_t tiles = static_cast<int64_t>(p.row_tiles) * p.col_tiles;
+  const int64_t pairs = device_sm_count() / 2;
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pairs / tiles, p.kb_total / 16)));
+  p.pieces_bytes = pieces > 1 ? round_up(M * pieces * p.n_blocks * kTcK * 2, 256) : 0;
+  p.weight_bytes = round_up(K * p.n_blocks * kTcK * 2, 256);
+  p.part_bytes = p.splits > 1 ? p.splits * M * K * 4 : 0;
+  return p;
 }
 
 int launched(const char* what) {
@@ -178,6 +621,90 @@ int launched(const char* what) {
   if (e != cudaSuccess) {
     set_error("%s launch failed: %s", what, cudaGetErrorString(e));
     return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
+}
+
+template <typename T>
+int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
+  const TcPlan p = tc_plan(g.M, g.N, g.K, g.dtype);
+  const int N = static_cast<int>(g.N), K = static_cast<int>(g.K);
+  const int n_pad = p.n_blocks * kTcK;
+  constexpr int kP = Pieces<T>::n;
+  constexpr bool direct = kP == 1;  // bf16: TMA takes dy as it lies
+  uint8_t* work = static_cast<uint8_t*>(g.workspace);
+  // the scales go into the pieces of dy where there are pieces, else into w
+  if constexpr (!direct) {
+    const int vec = rows_of_16_bytes(g);
+    const int64_t total = g.M * (n_pad / 8);
+    const int64_t blocks = std::min<int64_t>((total + kThreads - 1) / kThreads, 16ll * device_sm_count());
+    pieces_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+        static_cast<const T*>(g.dy), g.lddy, g.ws, g.ws_numel == 1, g.M, N, n_pad, vec,
+        reinterpret_cast<__nv_bfloat16*>(work));
+    if (int rc = launched("input gradient pieces")) return rc;
+  }
+  uint8_t* wide = work + p.pieces_bytes;
+  const int k_tiles = (K + 63) / 64;
+  widen_weights_kernel<<<static_cast<unsigned>(static_cast<int64_t>((N + 127) / 128) * k_tiles), kThreads, 0,
+                         stream>>>(g.w, g.ldw, direct ? g.ws : nullptr, g.ws_numel == 1, N, K, n_pad, k_tiles,
+                                   reinterpret_cast<uintptr_t>(g.w) % 4 == 0 && g.ldw % 4 == 0,
+                                   reinterpret_cast<__nv_bfloat16*>(wide));
+  if (int rc = launched("input gradient weights")) return rc;
+  CUtensorMap map_a, map_b;
+  const int64_t inner = direct ? g.N : static_cast<int64_t>(kP) * n_pad;
+  if (!map_rows(&map_a, direct ? g.dy : work, inner, g.M, direct ? g.lddy : inner) ||
+      !map_rows(&map_b, wide, n_pad, g.K, n_pad)) {
+    set_error("cuTensorMapEncodeTiled rejected the operands (M=%lld N=%lld K=%lld)",
+              static_cast<long long>(g.M), static_cast<long long>(g.N), static_cast<long long>(g.K));
+    return W8A8_ERR_RUNTIME;
+  }
+  TcArgs a{};
+  a.M = g.M;
+  a.N = N;
+  a.K = K;
+  a.n_blocks = p.n_blocks;
+  a.kb_total = p.kb_total;
+  a.row_tiles = p.row_tiles;
+  a.col_tiles = p.col_tiles;
+  a.splits = p.splits;
+  a.dx = g.dx;
+  a.lddx = g.lddx;
+  a.vec_o = reinterpret_cast<uintptr_t>(g.dx) % 16 == 0 && (g.lddx * 2) % 16 == 0;
+  a.part = p.splits > 1 ? reinterpret_cast<float*>(wide + p.weight_bytes) : nullptr;
+  auto kern = input_grad_tc_kernel<T>;
+  static bool set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !set[dev]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem);
+    if (e != cudaSuccess) {
+      set_error("cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
+      return W8A8_ERR_ACCELERATOR;
+    }
+    if (dev < 64) set[dev] = true;
+  }
+  const int64_t units = static_cast<int64_t>(p.row_tiles) * p.col_tiles * p.splits;
+  cudaLaunchConfig_t lc{};
+  lc.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(units, device_sm_count() / 2)));
+  lc.blockDim = dim3(kTcThreads);
+  lc.dynamicSmemBytes = kTcSmem;
+  lc.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, kern, map_a, map_b, a);
+  if (e != cudaSuccess) {
+    set_error("input gradient launch failed: %s", cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  if (a.part) {
+    sum_parts<T>(a.part, p.splits, g, stream);
+    return launched("input gradient sum");
   }
   return 0;
 }
@@ -203,10 +730,7 @@ int typed(const InputGradArgs& g, cudaStream_t stream) {
       vdy, vw, vo, static_cast<T*>(g.dx), g.lddx, part);
   if (int rc = launched("input gradient")) return rc;
   if (part) {
-    const int64_t blocks =
-        std::min<int64_t>((g.M * K + kThreads - 1) / kThreads, 16ll * device_sm_count());
-    sum_parts_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-        part, sp.count, g.M, K, static_cast<T*>(g.dx), g.lddx);
+    sum_parts<T>(part, sp.count, g, stream);
     return launched("input gradient sum");
   }
   return 0;
@@ -215,15 +739,20 @@ int typed(const InputGradArgs& g, cudaStream_t stream) {
 }  // namespace
 
 int64_t input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
-  (void)dtype;
   const NSplit sp = n_split_of(M, N, K);
-  return sp.count > 1 ? sp.count * M * K * 4 : 0;
+  int64_t bytes = sp.count > 1 ? sp.count * M * K * 4 : 0;
+  if (tc_shape(M, N, K, dtype)) {
+    const TcPlan p = tc_plan(M, N, K, dtype);
+    bytes = std::max(bytes, p.pieces_bytes + p.weight_bytes + p.part_bytes);
+  }
+  return bytes;
 }
 
 int input_grad_launch(const InputGradArgs& g, cudaStream_t stream) {
+  const bool tc = tc_shape(g.M, g.N, g.K, g.dtype) && tc_operands(g);
   switch (g.dtype) {
-    case W8A8_BF16: return typed<__nv_bfloat16>(g, stream);
-    case W8A8_F16: return typed<__half>(g, stream);
+    case W8A8_BF16: return tc ? tc_typed<__nv_bfloat16>(g, stream) : typed<__nv_bfloat16>(g, stream);
+    case W8A8_F16: return tc ? tc_typed<__half>(g, stream) : typed<__half>(g, stream);
     default: return typed<float>(g, stream);
   }
 }

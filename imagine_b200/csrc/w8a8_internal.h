@@ -200,6 +200,8 @@ struct InputGradArgs {
   int64_t M, N, K;
   void* workspace;
 };
+// The device word in which its tcgen05 kernel's waits record that they gave up.
+int read_and_clear_input_grad_error(cudaStream_t stream, int* value);
 int64_t input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
 int input_grad_launch(const InputGradArgs& g, cudaStream_t stream);
 
