@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "pieces.cuh"
+#include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
 
 namespace w8a8 {
@@ -305,11 +306,11 @@ __device__ __forceinline__ void load_rank_side(__nv_bfloat16* dst, const float* 
 }
 
 // ======================================================================== expand
-// out[row, n] = T(y[row, n] + c[s] * sum_r h[row, r] W_s[r, n]), 64 rows x 128
-// columns a block; y NULL: zero.  kWCols: W_s is stored [n][r] (B); otherwise
-// [r][n] (A).  The h of the tile is at most 64 x 128 and W_s at most 128 x 128:
-// one step, no pipeline; several blocks on an SM overlap one's loads with
-// another's stores.
+// out[row, n] = T(y[row, n] + c[s] * sum_r h[row, r] W_s[r, n]); y NULL: zero.
+// kWCols: W_s is stored [n][r] (B); otherwise [r][n] (A).
+// A block keeps the rank side of 64 rows and goes through its range of columns,
+// 128 at a time; the next tile's W_s and y are fetched into registers while this
+// one is multiplied.  Bound by reading y and writing out.
 template <typename T, int kRank, bool kWCols>
 struct ExpandTile {
   static constexpr int kPH = RankPieces<T>::n, kPW = Pieces<T>::n;
@@ -317,49 +318,48 @@ struct ExpandTile {
   static constexpr int kHPlane = kBM * (kRank + kPad);
   static constexpr int kLdW = kWCols ? kRank + kPad : kBN + kPad;
   static constexpr int kWPlane = (kWCols ? kBN : kRank) * kLdW;
-  static constexpr int kBytes0 = 2 * (kPH * kHPlane + kPW * kWPlane);
   static constexpr int kLdO = kBN + 4;
-  static constexpr int kOut = kBM * kLdO * 4;
-  static constexpr int kBytes = kBytes0 > kOut ? kBytes0 : kOut;
+  static constexpr int kOperands = 2 * (kPH * kHPlane + kPW * kWPlane);
+  static constexpr int kBytes = kOperands + kBM * kLdO * 4;
 };
 
 template <typename T, int kRank, bool kWCols>
-__global__ void __launch_bounds__(kThreads) expand_kernel(
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && kRank <= 64 ? 2 : 1) expand_kernel(
     const T* y, int64_t ldy, const float* __restrict__ part, int splits, const T* __restrict__ w,
-    int64_t slot, const float* __restrict__ scaling, Rows rows, int N, int R, int col_tiles, int vec_w,
-    int vec_o, T* out, int64_t ldo) {
+    int64_t slot, const float* __restrict__ scaling, Rows rows, int N, int R, int col_parts,
+    int cols_part, int vec_w, int vec_o, T* out, int64_t ldo) {
   using Tile = ExpandTile<T, kRank, kWCols>;
+  constexpr bool kApart = std::is_same<T, float>::value;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ TileIds ids;
   __nv_bfloat16* sh = reinterpret_cast<__nv_bfloat16*>(smem);
   __nv_bfloat16* sw = sh + Tile::kPH * Tile::kHPlane;
-  float* so = reinterpret_cast<float*>(smem);
+  float* so = reinterpret_cast<float*>(smem + Tile::kOperands);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wm = warp & 3, wn = warp >> 2;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x / col_tiles) * kBM;
-  const int col0 = static_cast<int>(blockIdx.x % col_tiles) * kBN;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / col_parts) * kBM;
+  const int c_lo = static_cast<int>(blockIdx.x % col_parts) * cols_part;
+  const int c_hi = min(N, c_lo + cols_part);
   tile_ids(rows, row0, ids);
 
-  // this thread's outputs: rows tid / 16 + 16 i, eight columns
+  // this thread's outputs of a tile: rows tid / 16 + 16 i, eight columns
+  constexpr int kRowsT = kBM / 16;
   const int oc = (tid & 15) * 8;
-  const int valid_c = min(8, N - col0 - oc);
-  Raw8<T> yr[kBM / 16];
+  constexpr int kGWAll = kRank * kBN / 8;
+  constexpr int kGW = (kGWAll + kThreads - 1) / kThreads;
+  Raw8<T> y_next[kRowsT], w_next[kGW];
+  auto fetch_y = [&](int col0) {
+    if (!y) return;
 #pragma unroll
-  for (int i = 0; i < kBM / 16; ++i) {
-    const int64_t row = row0 + (tid >> 4) + 16 * i;
-    const int valid = y && row < rows.M ? valid_c : 0;
-    load8(yr[i], y + row * ldy + col0 + oc, valid, vec_o != 0);
-  }
-  auto put = [&](int i, const float* add, float mul) {
-    const int64_t row = row0 + (tid >> 4) + 16 * i;
-    T* dst = out + row * ldo + col0 + oc;
-    Raw8<T> o;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float base = to_f(yr[i].e[j]);
-      o.e[j] = add ? from_f<T>(y ? fmaf(mul, add[j], base) : mul * add[j]) : yr[i].e[j];
+    for (int i = 0; i < kRowsT; ++i) {
+      const int64_t row = row0 + (tid >> 4) + 16 * i;
+      load8(y_next[i], y + row * ldy + col0 + oc, row < rows.M ? min(8, c_hi - col0 - oc) : 0, vec_o != 0);
     }
-    if (vec_o && valid_c >= 8) {
+  };
+  auto put = [&](int64_t row, int col0, const Raw8<T>& o) {
+    T* dst = out + row * ldo + col0 + oc;
+    const int valid = c_hi - col0 - oc;
+    if (vec_o && valid >= 8) {
 #pragma unroll
       for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) {
         const uint2* sp = reinterpret_cast<const uint2*>(o.e) + 2 * q;
@@ -368,98 +368,220 @@ __global__ void __launch_bounds__(kThreads) expand_kernel(
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < valid_c) dst[j] = o.e[j];
+        if (j < valid) dst[j] = o.e[j];
     }
   };
+  // rows without an adapter: y as it is (zero without y)
   if (ids.none && blockIdx.z == 0 && y != out) {
+    for (int col0 = c_lo; col0 < c_hi; col0 += kBN) {
+      fetch_y(col0);
 #pragma unroll
-    for (int i = 0; i < kBM / 16; ++i) {
-      const int r = (tid >> 4) + 16 * i;
-      if (ids.id[r] < 0 && row0 + r < rows.M) put(i, nullptr, 0.0f);
+      for (int i = 0; i < kRowsT; ++i) {
+        const int r = (tid >> 4) + 16 * i;
+        if (!y) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y_next[i].e[j] = T(0.0f);
+        }
+        if (ids.id[r] < 0 && row0 + r < rows.M) put(row0 + r, col0, y_next[i]);
+      }
     }
   }
-
-  constexpr int kGWAll = kRank * kBN / 8;
   for (int li = blockIdx.z; li < ids.count; li += gridDim.z) {
     const int s = ids.list[li];
     const T* ws = w + s * slot;
-    __syncthreads();  // the previous adapter's outputs are read
-    for (int gi = tid; gi < kGWAll; gi += kThreads) {
-      Raw8<T> raw;
-      if constexpr (kWCols) {
-        const int n = gi / (kRank / 8), c = (gi % (kRank / 8)) * 8;
-        const int valid = col0 + n < N ? min(8, R - c) : 0;
-        load8(raw, ws + static_cast<int64_t>(col0 + n) * R + c, valid, vec_w != 0);
-        store8(sw + n * Tile::kLdW + c, Tile::kWPlane, raw);
-      } else {
-        const int r = gi / (kBN / 8), c = (gi % (kBN / 8)) * 8;
-        const int valid = r < R ? min(8, N - col0 - c) : 0;
-        load8(raw, ws + static_cast<int64_t>(r) * N + col0 + c, valid, vec_w != 0);
-        store8(sw + r * Tile::kLdW + c, Tile::kWPlane, raw);
+    const float mul = scaling ? __ldg(scaling + s) : 1.0f;
+    auto fetch_w = [&](int col0) {
+#pragma unroll
+      for (int i = 0; i < kGW; ++i) {
+        const int gi = tid + i * kThreads;
+        if (kGWAll % kThreads != 0 && gi >= kGWAll) break;
+        if constexpr (kWCols) {
+          const int n = gi / (kRank / 8), c = (gi % (kRank / 8)) * 8;
+          load8(w_next[i], ws + static_cast<int64_t>(col0 + n) * R + c, col0 + n < c_hi ? min(8, R - c) : 0,
+                vec_w != 0);
+        } else {
+          const int r = gi / (kBN / 8), c = (gi % (kBN / 8)) * 8;
+          load8(w_next[i], ws + static_cast<int64_t>(r) * N + col0 + c, r < R ? min(8, c_hi - col0 - c) : 0,
+                vec_w != 0);
+        }
       }
-    }
+    };
+    fetch_w(c_lo);
+    fetch_y(c_lo);
+    __syncthreads();  // the previous adapter's rank side is read
     load_rank_side<kRank, Tile::kPH>(sh, part, splits, rows, row0, ids.id, s, R, 1.0f, nullptr);
-    __syncthreads();
-    float acc[8][4];
+    for (int col0 = c_lo; col0 < c_hi; col0 += kBN) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kGW; ++i) {
+        const int gi = tid + i * kThreads;
+        if (kGWAll % kThreads != 0 && gi >= kGWAll) break;
+        constexpr int kPer = kWCols ? kRank / 8 : kBN / 8;
+        store8(sw + (gi / kPer) * Tile::kLdW + (gi % kPer) * 8, Tile::kWPlane, w_next[i]);
+      }
+      Raw8<T> y_now[kRowsT];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    constexpr bool kApart = std::is_same<T, float>::value;
-    float low[kApart ? 8 : 1][4] = {};
+      for (int i = 0; i < kRowsT; ++i) y_now[i] = y_next[i];
+      __syncthreads();
+      if (col0 + kBN < c_hi) {
+        fetch_w(col0 + kBN);
+        fetch_y(col0 + kBN);
+      }
+      float acc[8][4];
 #pragma unroll
-    for (int kk = 0; kk < kRank; kk += 16) {
-      uint32_t a[Tile::kPH][4];
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int p = 0; p < Tile::kPH; ++p)
-        ldsm4(a[p], at16(sh + p * Tile::kHPlane, wm * 16, kk, kRank + kPad, lane));
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+      float low[kApart ? 8 : 1][4] = {};
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int kk = 0; kk < kRank; kk += 16) {
+        uint32_t a[Tile::kPH][4];
 #pragma unroll
-        for (int pw = 0; pw < Tile::kPW; ++pw) {
-          uint32_t b[4];
-          if constexpr (kWCols) {
-            ldsm4(b, at16h(sw + pw * Tile::kWPlane, wn * 64 + n * 16, kk, Tile::kLdW, lane));
-          } else {
-            ldsm4_t(b, at16(sw + pw * Tile::kWPlane, kk, wn * 64 + n * 16, Tile::kLdW, lane));
-          }
+        for (int p = 0; p < Tile::kPH; ++p)
+          ldsm4(a[p], at16(sh + p * Tile::kHPlane, wm * 16, kk, kRank + kPad, lane));
 #pragma unroll
-          for (int ph = 0; ph < Tile::kPH; ++ph) {
-            if (pair(ph, pw, Tile::kMost)) {
-              if constexpr (kApart) {
-                mma_apart(acc[2 * n], low[2 * n], a[ph], b[0], b[1], ph + pw == 0);
-                mma_apart(acc[2 * n + 1], low[2 * n + 1], a[ph], b[2], b[3], ph + pw == 0);
-              } else {
-                mma(acc[2 * n], a[ph], b[0], b[1]);
-                mma(acc[2 * n + 1], a[ph], b[2], b[3]);
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+          for (int pw = 0; pw < Tile::kPW; ++pw) {
+            uint32_t b[4];
+            if constexpr (kWCols) {
+              ldsm4(b, at16h(sw + pw * Tile::kWPlane, wn * 64 + n * 16, kk, Tile::kLdW, lane));
+            } else {
+              ldsm4_t(b, at16(sw + pw * Tile::kWPlane, kk, wn * 64 + n * 16, Tile::kLdW, lane));
+            }
+#pragma unroll
+            for (int ph = 0; ph < Tile::kPH; ++ph) {
+              if (pair(ph, pw, Tile::kMost)) {
+                if constexpr (kApart) {
+                  mma_apart(acc[2 * n], low[2 * n], a[ph], b[0], b[1], ph + pw == 0);
+                  mma_apart(acc[2 * n + 1], low[2 * n + 1], a[ph], b[2], b[3], ph + pw == 0);
+                } else {
+                  mma(acc[2 * n], a[ph], b[0], b[1]);
+                  mma(acc[2 * n + 1], a[ph], b[2], b[3]);
+                }
               }
             }
           }
         }
       }
-    }
-    if constexpr (kApart) {
+      if constexpr (kApart) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += low[i][j];
-    }
-    __syncthreads();  // the operands are read: the tile takes their place
-    const int r0 = wm * 16 + (lane >> 2), c0 = wn * 64 + (lane & 3) * 2;
+          for (int j = 0; j < 4; ++j) acc[i][j] += low[i][j];
+      }
+      const int r0 = wm * 16 + (lane >> 2), c0 = wn * 64 + (lane & 3) * 2;
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      *reinterpret_cast<float2*>(so + r0 * Tile::kLdO + c0 + n * 8) = make_float2(acc[n][0], acc[n][1]);
-      *reinterpret_cast<float2*>(so + (r0 + 8) * Tile::kLdO + c0 + n * 8) =
-          make_float2(acc[n][2], acc[n][3]);
-    }
-    __syncthreads();
-    const float mul = scaling ? __ldg(scaling + s) : 1.0f;
+      for (int n = 0; n < 8; ++n) {
+        *reinterpret_cast<float2*>(so + r0 * Tile::kLdO + c0 + n * 8) = make_float2(acc[n][0], acc[n][1]);
+        *reinterpret_cast<float2*>(so + (r0 + 8) * Tile::kLdO + c0 + n * 8) =
+            make_float2(acc[n][2], acc[n][3]);
+      }
+      __syncthreads();  // the products are staged, and W_s is read
 #pragma unroll
-    for (int i = 0; i < kBM / 16; ++i) {
-      const int r = (tid >> 4) + 16 * i;
-      if (ids.id[r] == s) put(i, so + r * Tile::kLdO + oc, mul);
+      for (int i = 0; i < kRowsT; ++i) {
+        const int r = (tid >> 4) + 16 * i;
+        if (ids.id[r] != s) continue;
+        const float* add = so + r * Tile::kLdO + oc;
+        Raw8<T> o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          o.e[j] = from_f<T>(y ? fmaf(mul, add[j], to_f(y_now[i].e[j])) : mul * add[j]);
+        put(row0 + r, col0, o);
+      }
     }
   }
+}
+
+// ======================================================================== few rows
+// Decode steps: each row with an adapter of its own, so a tile would hold one row.
+// CUDA cores, a block for each (rank, row) and then for each (256 columns, row);
+// what has to be read is the adapters' weights, once, and latency counts.  The
+// second kernel starts while the first runs (programmatic dependent launch): its
+// weights and y are on their way when h arrives.
+// 64 rows, 32 adapters of rank 32, 4096 -> 12288: see the measurements at few_rows().
+template <typename T>
+__global__ void __launch_bounds__(kThreads) shrink_row_kernel(const T* __restrict__ x, int64_t ldx,
+                                                              const T* __restrict__ a, int64_t slot,
+                                                              Rows rows, int K, int R, int vec,
+                                                              float* __restrict__ h) {
+  griddep_launch_dependents();
+  __shared__ float sums[kThreads / 32];
+  const int r = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  const int s = adapter_of(rows, row);
+  if (s < 0) return;
+  const T* xr = x + row * ldx;
+  const T* ar = a + s * slot + static_cast<int64_t>(r) * K;
+  float v = 0.0f;
+#pragma unroll 4
+  for (int k = threadIdx.x * 8; k < K; k += kThreads * 8) {
+    Raw8<T> p, q;
+    load8(p, xr + k, K - k, vec != 0);
+    load8(q, ar + k, K - k, vec != 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v = fmaf(to_f(p.e[i]), to_f(q.e[i]), v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) t += sums[i];
+    h[row * R + r] = t;
+  }
+}
+
+// kVec: rows of B of whole eight-element vectors.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kThreads) expand_row_kernel(const T* y, int64_t ldy, const float* h,
+                                                              const T* __restrict__ b, int64_t slot,
+                                                              const float* __restrict__ scaling,
+                                                              Rows rows, int N, int R, T* out,
+                                                              int64_t ldo) {
+  __shared__ float sh[128];
+  const int n = blockIdx.x * kThreads + threadIdx.x;
+  const int64_t row = blockIdx.y;
+  const int s = adapter_of(rows, row);
+  const float base = n < N ? to_f(y[row * ldy + n]) : 0.0f;
+  const T* br = b + (s < 0 ? 0 : s * slot) + static_cast<int64_t>(n) * R;
+  constexpr int kAhead = 4;  // vectors of B fetched before h is there
+  Raw8<T> w[kAhead];
+  if (kVec && s >= 0 && n < N) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i * 8 < R) load8(w[i], br + i * 8, 8, true);
+  }
+  const float mul = s >= 0 && scaling ? __ldg(scaling + s) : 1.0f;
+  griddep_wait();
+  if (s >= 0 && threadIdx.x < R) sh[threadIdx.x] = __ldcg(h + row * R + threadIdx.x);
+  __syncthreads();
+  if (n >= N) return;
+  T* dst = out + row * ldo + n;
+  if (s < 0) {
+    if (y != out) *dst = y[row * ldy + n];
+    return;
+  }
+  float v = 0.0f;
+  if constexpr (kVec) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i * 8 < R) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v = fmaf(sh[i * 8 + j], to_f(w[i].e[j]), v);
+      }
+    }
+    for (int c = kAhead * 8; c < R; c += 8) {
+      Raw8<T> q;
+      load8(q, br + c, 8, true);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = fmaf(sh[c + j], to_f(q.e[j]), v);
+    }
+  } else {
+    for (int c = 0; c < R; ++c) v = fmaf(sh[c], to_f(br[c]), v);
+  }
+  *dst = from_f<T>(fmaf(mul, v, base));
 }
 
 // ======================================================================== tokens
@@ -582,27 +704,49 @@ __global__ void __launch_bounds__(kThreads) tokens_kernel(
       }
 }
 
-// The splits' sums, in a fixed order, rounded to T: dA then dB.
+// The splits' sums, in a fixed order, rounded to T: dA (blockIdx.z 0) or dB of
+// adapter blockIdx.y, four elements a thread where the adapter's size allows it.
+struct SumArgs {
+  const float* part;
+  const int* found;
+  int splits;
+  int64_t per;  // elements of one adapter
+  void* out;
+};
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sum_splits_kernel(
-    const float* __restrict__ pa, const int* __restrict__ fa, int splits_a, int64_t na,
-    T* __restrict__ da, const float* __restrict__ pb, const int* __restrict__ fb, int splits_b,
-    int64_t nb, T* __restrict__ db, int S) {
-  // na / nb: elements of one adapter
-  const int64_t total_a = na * S, total = total_a + nb * S;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const bool first = i < total_a;
-    const int64_t j = first ? i : i - total_a;
-    const int64_t per = first ? na : nb;
-    const int s = static_cast<int>(j / per);
-    const float* p = (first ? pa : pb) + j;
-    const int* f = (first ? fa : fb) + s;
-    const int n = first ? splits_a : splits_b;
+__global__ void __launch_bounds__(kThreads) sum_splits_kernel(SumArgs ga, SumArgs gb, int S) {
+  const SumArgs g = blockIdx.z ? gb : ga;
+  const int s = blockIdx.y;
+  const int64_t plane = g.per * S;
+  const float* p0 = g.part + s * g.per;
+  T* out = static_cast<T*>(g.out) + s * g.per;
+  const int64_t start = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  if (g.per % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % (4 * sizeof(T)) == 0) {
+    for (int64_t i = start * 4; i < g.per; i += step * 4) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int sp = 0; sp < g.splits; ++sp) {
+        if (!__ldg(g.found + sp * S + s)) continue;
+        const float4 o = __ldg(reinterpret_cast<const float4*>(p0 + sp * plane + i));
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
+      }
+      const T o[4] = {from_f<T>(v.x), from_f<T>(v.y), from_f<T>(v.z), from_f<T>(v.w)};
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint2*>(out + i) = *reinterpret_cast<const uint2*>(o);
+      } else {
+        *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(o);
+      }
+    }
+    return;
+  }
+  for (int64_t i = start; i < g.per; i += step) {
     float v = 0.0f;
-    for (int sp = 0; sp < n; ++sp)
-      if (__ldg(f + sp * S)) v += __ldg(p + sp * per * S);
-    (first ? da : db)[j] = from_f<T>(v);
+    for (int sp = 0; sp < g.splits; ++sp)
+      if (__ldg(g.found + sp * S + s)) v += __ldg(p0 + sp * plane + i);
+    out[i] = from_f<T>(v);
   }
 }
 
@@ -617,7 +761,7 @@ bool aligned(const void* p, int64_t ld, int size) {
 
 template <typename K>
 int prepare(K kernel, int bytes) {
-  if (bytes > 48 * 1024) {
+  if (bytes > 40 * 1024) {  // 48 KiB without opting in, the static part included
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) {
       set_error("lora: shared memory of %d bytes refused: %s", bytes, cudaGetErrorString(e));
@@ -706,17 +850,22 @@ int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, i
            const float* scaling, const Rows& rows, int N, int R, T* out, int64_t ldo,
            cudaStream_t stream) {
   const int64_t tiles = (rows.M + kBM - 1) / kBM;
-  const int cols = (N + kBN - 1) / kBN;
+  const int col_tiles = (N + kBN - 1) / kBN;
   const int vw = aligned(w, kWCols ? R : N, sizeof(T)) && aligned(w, slot, sizeof(T));
   const int vo = aligned(out, ldo, sizeof(T)) && (!y || aligned(y, ldy, sizeof(T)));
-  const dim3 grid(static_cast<unsigned>(tiles * cols), 1, parts_of(rows.M, rows.S, cols));
+  // Ranges of columns: six blocks a multiprocessor (three at a time), so that a
+  // block has several tiles to overlap and the last wave is short.
+  int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(col_tiles, 6ll * device_sm_count() / tiles)));
+  const int per = (col_tiles + parts - 1) / parts;
+  parts = (col_tiles + per - 1) / per;
+  const dim3 grid(static_cast<unsigned>(tiles * parts), 1, parts_of(rows.M, rows.S, parts));
 #define EXPAND(RANK)                                                                              \
   {                                                                                               \
     auto k = expand_kernel<T, RANK, kWCols>;                                                      \
     constexpr int bytes = ExpandTile<T, RANK, kWCols>::kBytes;                                    \
     if (int rc = prepare(k, bytes)) return rc;                                                    \
-    k<<<grid, kThreads, bytes, stream>>>(y, ldy, part, splits, w, slot, scaling, rows, N, R, cols, \
-                                         vw, vo, out, ldo);                                       \
+    k<<<grid, kThreads, bytes, stream>>>(y, ldy, part, splits, w, slot, scaling, rows, N, R, parts, \
+                                         per * kBN, vw, vo, out, ldo);                            \
   }
   switch (pad_rank(R)) {
     case 16: EXPAND(16) break;
@@ -752,12 +901,48 @@ int tokens(const TX* x, int64_t ldx, const float* row_mul, const float* rank_par
   return launched("lora tokens");
 }
 
+// Up to one tile of rows.
+bool few_rows(int64_t M) { return M <= kBM; }
+
+template <typename T>
+int add_few_rows(const LoraArgs& g, const Rows& rows, float* h, cudaStream_t stream) {
+  const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
+  const T* x = static_cast<const T*>(g.x);
+  const T* a = static_cast<const T*>(g.a);
+  const T* b = static_cast<const T*>(g.b);
+  const T* y = static_cast<const T*>(g.y);
+  const int vec = aligned(x, g.ldx, sizeof(T)) && aligned(a, K, sizeof(T)) && aligned(a, g.lda, sizeof(T));
+  const unsigned m = static_cast<unsigned>(g.M);
+  shrink_row_kernel<T><<<dim3(R, m), kThreads, 0, stream>>>(x, g.ldx, a, g.lda, rows, K, R, vec, h);
+  if (int rc = launched("lora shrink")) return rc;
+  cudaLaunchConfig_t lc{};
+  lc.gridDim = dim3((N + kThreads - 1) / kThreads, m);
+  lc.blockDim = dim3(kThreads);
+  lc.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  const bool whole = R % 8 == 0 && aligned(b, R, sizeof(T)) && aligned(b, g.ldb, sizeof(T));
+  const cudaError_t e =
+      cudaLaunchKernelEx(&lc, whole ? expand_row_kernel<T, true> : expand_row_kernel<T, false>, y, g.ldy,
+                         static_cast<const float*>(h), b, g.ldb, g.scaling, rows, N, R,
+                         static_cast<T*>(g.out), g.ldo);
+  if (e != cudaSuccess) {
+    set_error("lora expand launch failed: %s", cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
+}
+
 template <typename T>
 int add_typed(const LoraArgs& g, cudaStream_t stream) {
   const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
   const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
-  const Split sp = shrink_split(g.M, K);
   float* part = static_cast<float*>(g.workspace);
+  if (few_rows(g.M)) return add_few_rows<T>(g, rows, part, stream);
+  const Split sp = shrink_split(g.M, K);
   if (int rc = shrink<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
                                   static_cast<const T*>(g.a), g.lda, rows, K, R, sp, part, stream)) {
     return rc;
@@ -825,12 +1010,12 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
                                   stream)) {
     return rc;
   }
-  const int64_t na = g.R * g.K, nb = g.R * g.N;
-  const int64_t blocks = std::min<int64_t>((g.S * (na + nb) + kThreads - 1) / kThreads,
-                                           16ll * device_sm_count());
-  sum_splits_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-      pa, fa, p.a.count, na, static_cast<T*>(g.da), pb, fb, p.b.count, nb, static_cast<T*>(g.db),
-      static_cast<int>(g.S));
+  const SumArgs sa{pa, fa, p.a.count, g.R * g.K, g.da}, sb{pb, fb, p.b.count, g.R * g.N, g.db};
+  const int64_t most = std::max(sa.per, sb.per);
+  const int64_t want = (most + 4 * kThreads - 1) / (4 * kThreads);
+  const int64_t cap = std::max<int64_t>(1, 8ll * device_sm_count() / g.S);
+  sum_splits_kernel<T><<<dim3(static_cast<unsigned>(std::min(want, cap)), static_cast<unsigned>(g.S), 2),
+                         kThreads, 0, stream>>>(sa, sb, static_cast<int>(g.S));
   return launched("lora gradient sum");
 }
 
