@@ -24,8 +24,8 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libw8a8.so")
 
 SOURCES = ["api.cu", "quantize.cu", "convrot.cu", "gemm_sm100.cu", "gemm_splitk_static.cu", "gemv.cu",
-           "mxfp8.cu", "rope.cu", "sampler.cu", "lora.cu", "linear_backward.cu", "activation.cu"]
-HEADERS = ["sm100_ptx.cuh", "epilogue.cuh", "quant_common.cuh", "pieces.cuh", "w8a8_internal.h"]
+           "mxfp8.cu", "rope.cu", "sampler.cu", "lora.cu", "lora_sm100.cu", "linear_backward.cu", "activation.cu"]
+HEADERS = ["sm100_ptx.cuh", "epilogue.cuh", "quant_common.cuh", "pieces.cuh", "lora_rows.cuh", "w8a8_internal.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3",

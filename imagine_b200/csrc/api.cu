@@ -120,6 +120,8 @@ int w8a8_device_error(void* stream) {
     int w = 0;
     rc = read_and_clear_input_grad_error(static_cast<cudaStream_t>(stream), &w);
     if (v == 0) v = w;
+    if (rc == 0) rc = read_and_clear_lora_error(static_cast<cudaStream_t>(stream), &w);
+    if (v == 0) v = w;
   }
   if (rc != 0) {
     g_last_accel = rc;

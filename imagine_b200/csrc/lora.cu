@@ -29,6 +29,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "lora_rows.cuh"
 #include "pieces.cuh"
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
@@ -37,7 +38,6 @@ namespace w8a8 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBM = 64;   // rows per tile
 constexpr int kBK = 64;   // contraction per step of shrink
 constexpr int kBN = 128;  // output columns per tile of expand and tokens
 constexpr int kPad = 8;   // bf16 elements of padding a shared-memory row (conflict-free ldmatrix)
@@ -45,66 +45,6 @@ constexpr int kPad = 8;   // bf16 elements of padding a shared-memory row (confl
 // pieces of a rank-side fp32 value next to data of type T
 template <typename T>
 struct RankPieces { static constexpr int n = std::is_same<T, float>::value ? 3 : 2; };
-
-// ---- rows and their adapters
-struct Rows {
-  const void* idx;  // int32 or int64 [ceil(M / per)], or NULL: adapter 0
-  int idx64;
-  int64_t per;      // consecutive rows that share an index
-  int64_t M;
-  int S;
-};
-
-__device__ __forceinline__ int adapter_of(const Rows& r, int64_t row) {
-  if (row >= r.M) return -1;
-  if (!r.idx) return 0;
-  const int64_t i = r.per == 1 ? row : row / r.per;
-  const int64_t v = r.idx64 ? __ldg(static_cast<const long long*>(r.idx) + i)
-                            : static_cast<int64_t>(__ldg(static_cast<const int*>(r.idx) + i));
-  return v >= 0 && v < r.S ? static_cast<int>(v) : -1;
-}
-
-// The adapters of a tile of 64 rows: id[i] each row's, list the distinct ones
-// (in order of appearance), *count how many, *none whether a row has none.
-struct TileIds {
-  int id[kBM];
-  int list[kBM];
-  int count;
-  int none;
-};
-
-__device__ __forceinline__ void tile_ids(const Rows& rows, int64_t row0, TileIds& t) {
-  if (threadIdx.x < 32) {
-    const unsigned all = 0xffffffffu;
-    const int lane = threadIdx.x;
-    const int a = adapter_of(rows, row0 + lane);
-    const int b = adapter_of(rows, row0 + 32 + lane);
-    t.id[lane] = a;
-    t.id[lane + 32] = b;
-    // every lane takes part in every warp operation: their results are tested afterwards
-    const unsigned same_a = __match_any_sync(all, a);
-    const unsigned same_b = __match_any_sync(all, b);
-    const bool first_a = a >= 0 && __ffs(same_a) - 1 == lane;
-    bool first_b = b >= 0 && __ffs(same_b) - 1 == lane;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const int other = __shfl_sync(all, a, j);
-      first_b = first_b && other != b;
-    }
-    const unsigned ma = __ballot_sync(all, first_a);
-    const unsigned mb = __ballot_sync(all, first_b);
-    const unsigned below = (1u << lane) - 1u;
-    if (first_a) t.list[__popc(ma & below)] = a;
-    if (first_b) t.list[__popc(ma) + __popc(mb & below)] = b;
-    const bool n = (a < 0 && row0 + lane < rows.M) || (b < 0 && row0 + 32 + lane < rows.M);
-    const bool any = __any_sync(all, n);
-    if (lane == 0) {
-      t.count = __popc(ma) + __popc(mb);
-      t.none = any;
-    }
-  }
-  __syncthreads();
-}
 
 // ======================================================================== shrink
 // part[split][row][r] = sum over the split's k of x[row, k] W_s[k, r], times the
@@ -821,6 +761,47 @@ RowSplit tokens_split(int64_t M, int C, int S, int R) {
 
 int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 
+// ---- the tcgen05 form (lora_sm100.cu): long bf16 batches of a few adapters whose
+// operands TMA can take (16-byte rows).
+constexpr int64_t kTcRows = 256;
+bool tc_shape(const LoraArgs& g) {
+  return g.dtype == W8A8_BF16 && g.M >= kTcRows && g.S <= 64 && g.K % 8 == 0 && g.N % 8 == 0 && g.R % 8 == 0 &&
+         g.K > 0 && g.N > 0;
+}
+bool tc_rows(const void* p, int64_t ld, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0;
+}
+bool tc_x(const LoraArgs& g) { return tc_rows(g.x, g.ldx, g.x_scale ? 1 : 2); }
+bool tc_weights(const void* p, int64_t slot, int64_t width, int64_t S) {
+  return tc_rows(p, width, 2) && (S == 1 || (slot * 2) % 16 == 0);
+}
+// Two blocks a multiprocessor, at least four steps each.
+Split shrink_tc_split(int64_t M, int K) {
+  const int64_t tiles = std::max<int64_t>(1, (M + 127) / 128);
+  const int steps = std::max(1, (K + 63) / 64);
+  const int64_t want =
+      std::max<int64_t>(1, std::min<int64_t>({2ll * device_sm_count() / tiles, 16, (steps + 3) / 4}));
+  const int per = static_cast<int>((steps + want - 1) / want);
+  return {(steps + per - 1) / per, per * 64};
+}
+// One block a multiprocessor for 256 columns each; a block lists at most 2048 tiles.
+RowSplit tokens_tc_split(int64_t M, int C) {
+  const int64_t tiles = std::max<int64_t>(1, (M + kBM - 1) / kBM);
+  const int64_t chunks = std::max<int64_t>(1, (C + 255) / 256);
+  int64_t want = std::max<int64_t>(1, std::min<int64_t>(device_sm_count() / chunks, tiles));
+  want = std::max(want, (tiles + 2047) / 2048);
+  const int64_t per = (tiles + want - 1) / want;
+  return {static_cast<int>((tiles + per - 1) / per), per * kBM};
+}
+int shrink_tc(const LoraArgs& g, const void* x, int64_t ldx, bool codes, const float* x_scale, const void* w,
+              int64_t slot, bool w_rows, int64_t K, const Split& sp, float* part, cudaStream_t stream) {
+  const int64_t blocks = (g.M + 127) / 128 * sp.count;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.S, 2ll * device_sm_count() / blocks));
+  return lora_shrink_tc({x, codes, ldx, x_scale, w, w_rows, slot, g.M, K, g.S, g.R, sp.count, sp.per / 64,
+                         static_cast<int>(parts), part},
+                        {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
+}
+
 template <typename TX, typename TW, bool kWRows>
 int shrink(const TX* x, int64_t ldx, const float* xs, const TW* w, int64_t slot, const Rows& rows,
            int K, int R, const Split& sp, float* part, cudaStream_t stream) {
@@ -942,9 +923,12 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
   const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
   float* part = static_cast<float*>(g.workspace);
   if (few_rows(g.M)) return add_few_rows<T>(g, rows, part, stream);
-  const Split sp = shrink_split(g.M, K);
-  if (int rc = shrink<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
-                                  static_cast<const T*>(g.a), g.lda, rows, K, R, sp, part, stream)) {
+  Split sp = shrink_split(g.M, K);
+  if (tc_shape(g) && tc_x(g) && tc_weights(g.a, g.lda, K, g.S)) {
+    sp = shrink_tc_split(g.M, K);
+    if (int rc = shrink_tc(g, g.x, g.ldx, false, nullptr, g.a, g.lda, true, K, sp, part, stream)) return rc;
+  } else if (int rc = shrink<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
+                                         static_cast<const T*>(g.a), g.lda, rows, K, R, sp, part, stream)) {
     return rc;
   }
   return expand<T, true>(static_cast<const T*>(g.y), g.ldy, part, sp.count,
@@ -955,20 +939,25 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
 struct BackwardPlan {
   Split h, g;
   RowSplit a, b;
-  int64_t off_g, off_a, off_b, off_found, bytes;
+  int64_t off_g, off_a, off_b, off_found, off_pa, off_pb, off_info, bytes;
 };
-BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R) {
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, bool tc) {
   BackwardPlan p;
-  const int r = static_cast<int>(R), s = static_cast<int>(S);
-  p.h = shrink_split(M, static_cast<int>(K));
-  p.g = shrink_split(M, static_cast<int>(N));
-  p.a = tokens_split(M, static_cast<int>(K), s, r);
-  p.b = tokens_split(M, static_cast<int>(N), s, r);
+  const int r = static_cast<int>(R), s = static_cast<int>(S), k = static_cast<int>(K), n = static_cast<int>(N);
+  p.h = tc ? shrink_tc_split(M, k) : shrink_split(M, k);
+  p.g = tc ? shrink_tc_split(M, n) : shrink_split(M, n);
+  p.a = tc ? tokens_tc_split(M, k) : tokens_split(M, k, s, r);
+  p.b = tc ? tokens_tc_split(M, n) : tokens_split(M, n, s, r);
   p.off_g = up(p.h.count * M * R * 4);
   p.off_a = p.off_g + up(p.g.count * M * R * 4);
   p.off_b = p.off_a + up(p.a.count * S * R * K * 4);
   p.off_found = p.off_b + up(p.b.count * S * R * N * 4);
-  p.bytes = p.off_found + up((p.a.count + p.b.count) * S * 4);
+  p.off_pa = p.off_found + up((p.a.count + p.b.count) * S * 4);
+  const int64_t tiles = (M + kBM - 1) / kBM;
+  const int64_t pieces = tc ? up(2 * pad_rank(r) * tiles * kBM * 2) : 0;
+  p.off_pb = p.off_pa + pieces;
+  p.off_info = p.off_pb + pieces;
+  p.bytes = p.off_info + (tc ? up(S * tiles) : 0);
   return p;
 }
 
@@ -976,7 +965,9 @@ template <typename T, typename TX>
 int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
   const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
-  const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R);
+  const bool tc = tc_shape(g) && tc_x(g) && tc_rows(g.y, g.ldy, 2) && tc_weights(g.a, g.lda, g.K, g.S) &&
+                  tc_weights(g.b, g.ldb, g.R, g.S);
+  const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R, tc);
   uint8_t* ws = static_cast<uint8_t*>(g.workspace);
   float* ph = reinterpret_cast<float*>(ws);
   float* pg = reinterpret_cast<float*>(ws + p.off_g);
@@ -989,7 +980,11 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   const T* a = static_cast<const T*>(g.a);
   const T* b = static_cast<const T*>(g.b);
   if (g.M > 0) {
-    if (int rc = shrink<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, rows, N, R, p.g, pg, stream)) return rc;
+    if (tc) {
+      if (int rc = shrink_tc(g, dy, g.ldy, false, nullptr, b, g.ldb, false, N, p.g, pg, stream)) return rc;
+    } else if (int rc = shrink<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, rows, N, R, p.g, pg, stream)) {
+      return rc;
+    }
     if (g.out) {
       if (int rc = expand<T, false>(g.accumulate ? static_cast<const T*>(g.out) : nullptr, g.ldo, pg,
                                     p.g.count, a, g.lda, g.scaling, rows, K, R,
@@ -999,16 +994,35 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
     }
   }
   if (!g.da) return 0;
-  if (g.M > 0) {
-    if (int rc = shrink<TX, T, true>(x, g.ldx, g.x_scale, a, g.lda, rows, K, R, p.h, ph, stream)) return rc;
-  }
-  if (int rc = tokens<TX, T, false>(x, g.ldx, g.x_scale, pg, p.g.count, g.scaling, rows, K, R, p.a, pa,
-                                    fa, stream)) {
-    return rc;
-  }
-  if (int rc = tokens<T, T, true>(dy, g.ldy, nullptr, ph, p.h.count, g.scaling, rows, N, R, p.b, pb, fb,
-                                  stream)) {
-    return rc;
+  if (tc) {
+    const LoraRows lr{g.adapter, g.adapter64, g.rows_per_index, g.M, g.S};
+    void *qa = ws + p.off_pa, *qb = ws + p.off_pb;
+    uint8_t* info = ws + p.off_info;
+    if (int rc = shrink_tc(g, x, g.ldx, g.x_scale != nullptr, g.x_scale, a, g.lda, true, K, p.h, ph, stream)) return rc;
+    if (int rc = lora_rank_pieces({pg, p.g.count, g.x_scale, qa, ph, p.h.count, qb, g.scaling, R, info}, lr, stream)) {
+      return rc;
+    }
+    const int per_a = static_cast<int>(p.a.per / kBM), per_b = static_cast<int>(p.b.per / kBM);
+    if (int rc = lora_tokens_tc({x, g.x_scale != nullptr, g.ldx, qa, g.M, g.K, g.S, g.R, 0, p.a.count, per_a,
+                                 info, pa, fa}, lr, stream)) {
+      return rc;
+    }
+    if (int rc = lora_tokens_tc({dy, 0, g.ldy, qb, g.M, g.N, g.S, g.R, 1, p.b.count, per_b, info, pb, fb}, lr,
+                                stream)) {
+      return rc;
+    }
+  } else {
+    if (g.M > 0) {
+      if (int rc = shrink<TX, T, true>(x, g.ldx, g.x_scale, a, g.lda, rows, K, R, p.h, ph, stream)) return rc;
+    }
+    if (int rc = tokens<TX, T, false>(x, g.ldx, g.x_scale, pg, p.g.count, g.scaling, rows, K, R, p.a, pa,
+                                      fa, stream)) {
+      return rc;
+    }
+    if (int rc = tokens<T, T, true>(dy, g.ldy, nullptr, ph, p.h.count, g.scaling, rows, N, R, p.b, pb, fb,
+                                    stream)) {
+      return rc;
+    }
   }
   const SumArgs sa{pa, fa, p.a.count, g.R * g.K, g.da}, sb{pb, fb, p.b.count, g.R * g.N, g.db};
   const int64_t most = std::max(sa.per, sb.per);
@@ -1022,8 +1036,11 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
 }  // namespace
 
 int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, int backward) {
-  if (!backward) return up(shrink_split(M, static_cast<int>(K)).count * M * R * 4);
-  return backward_plan(M, N, K, S, R).bytes;
+  // either form of the kernels may run: which one depends on pointers and strides too
+  const int k = static_cast<int>(K);
+  if (!backward) return up(std::max(shrink_split(M, k).count, shrink_tc_split(M, k).count) * M * R * 4);
+  return std::max(backward_plan(M, N, K, S, R, false).bytes,
+                  M >= kTcRows ? backward_plan(M, N, K, S, R, true).bytes : 0);
 }
 
 int lora_add_launch(const LoraArgs& g, cudaStream_t stream) {

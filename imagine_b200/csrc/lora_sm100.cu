@@ -1,0 +1,734 @@
+// The adapter contractions of long bf16 batches on tcgen05.
+//
+//   shrink_tc   part[split][row][r] = sum over the split's k of x[row, k] W_s[k, r]
+//               a tile of 128 rows is the M side, the rank the N side
+//   tokens_tc   part[split][s][r][c] (or [c][r]) = sum over the split's rows m of
+//               adapter s of q[m, r] x[m, c]: 128 columns are the M side, read
+//               from the same row-major tiles by their transposed (MN-major)
+//               descriptors; the rank-side values come as bf16 pieces, [r][m]
+//
+// Every operand arrives by TMA in 128-byte swizzled rows; a rank below 64 is
+// padded by the copies' zero fill.  The tensor core's rate leaves both bound by
+// reading x (mma.sync, at 510 TFLOP/s, would hold a rank of 64 with two pieces to a
+// third of it).  int8 codes (an 8-bit checkpoint as x) land as bytes and are
+// widened to bf16 by four warps on the way.
+//
+// Waits are bounded (sm100_ptx.cuh): a wait that gives up records its code, every
+// role of the block falls through, and TMEM is released.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+#include <type_traits>
+
+#include "lora_rows.cuh"
+#include "pieces.cuh"
+#include "quant_common.cuh"
+#include "sm100_ptx.cuh"
+#include "w8a8_internal.h"
+
+namespace w8a8 {
+
+__device__ int g_lora_error;
+
+int read_and_clear_lora_error(cudaStream_t stream, int* value) {
+  int v = 0;
+  cudaError_t e =
+      cudaMemcpyFromSymbolAsync(&v, g_lora_error, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (v != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_lora_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  *value = v;
+  return 0;
+}
+
+namespace {
+
+constexpr int kThreads = 192;  // warps 0-3: widen, mask, epilogue; 4: TMA; 5: MMA
+constexpr int kTmaWarp = 4, kMmaWarp = 5;
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of an operand whose M (or N) elements run along the 128-byte rows:
+// row = one k, 64 elements; eight rows a swizzle atom (1024 bytes, the stride
+// offset); the next 64 elements `chunk` bytes further (the leading offset).
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t chunk) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((chunk >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+// f32 = bf16 x bf16, M 128; a_mn / b_mn: that operand's M / N runs along the rows.
+__host__ __device__ constexpr uint32_t idesc_bf16(int n, int a_mn, int b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+         (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+constexpr uint32_t tmem_cols(int n) { return n <= 32 ? 32u : n <= 64 ? 64u : n <= 128 ? 128u : 256u; }
+
+// Sixteen codes to sixteen bf16 (two 16-byte vectors).
+__device__ __forceinline__ void widen16(const uint4& q, uint4& lo8, uint4& hi8) {
+  const uint32_t w[4] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u, q.z ^ 0x80808080u, q.w ^ 0x80808080u};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = __byte_perm(w[i >> 1], 0x4B000000u, (i & 1) ? 0x7542 : 0x7540);
+    const uint32_t b = __byte_perm(w[i >> 1], 0x4B000000u, (i & 1) ? 0x7543 : 0x7541);
+    const uint64_t f = add2(pk(__uint_as_float(a), __uint_as_float(b)), pk(-8388736.0f, -8388736.0f));
+    o[i] = pack_bf16(lo(f), hi(f));
+  }
+  lo8 = make_uint4(o[0], o[1], o[2], o[3]);
+  hi8 = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+struct Bars {
+  uint64_t full[8], ready[8], empty[8], done, drained;
+  uint32_t tmem;
+  int abort_flag;
+};
+
+// ======================================================================== shrink
+constexpr int kSRows = 128, kSK = 64;
+constexpr int kXTile = kSRows * kSK * 2;  // 16 KB
+template <bool kCodes, int kRank>
+struct ShrinkTc {
+  static constexpr int kW = kRank == 128 ? 16384 : 8192;
+  static constexpr int kRaw = kCodes ? kSRows * kSK : 0;
+  static constexpr int kStage = kXTile + kW + kRaw;
+  static constexpr int kStages = 98304 / kStage;  // two blocks a multiprocessor
+  static constexpr int kBytes = 1024 + kStages * kStage + 512 + 1280;
+};
+
+// tm_x: rows of x, boxes 64 x 128 (bf16, swizzled; codes: as they are).  tm_w:
+// the adapters, boxes 64 k x kRank of [S][R][K] (kWRows), or 64 r x 64 n of [S][N][R].
+template <bool kCodes, int kRank, bool kWRows>
+__global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
+    const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, Rows rows,
+    const float* __restrict__ row_mul, int K, int R, int kb_split, float* __restrict__ part) {
+  using C = ShrinkTc<kCodes, kRank>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* s_x = smem;
+  uint8_t* s_w = s_x + C::kStages * kXTile;
+  uint8_t* s_raw = s_w + C::kStages * C::kW;
+  Bars* bars = reinterpret_cast<Bars*>(s_raw + C::kStages * C::kRaw);
+  int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
+  int* list = id + kSRows;
+  __shared__ int count;
+  volatile int* abortv = &bars->abort_flag;
+  int* err = &g_lora_error;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kSRows;
+  const int kb_all = (K + kSK - 1) / kSK;
+  const int kb_lo = blockIdx.y * kb_split, kb_hi = min(kb_all, kb_lo + kb_split);
+
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->ready[s], 4);
+      mbar_init(&bars->empty[s], 1);
+    }
+    mbar_init(&bars->done, 1);
+    mbar_init(&bars->drained, 4);
+    bars->abort_flag = 0;
+    fence_mbarrier_init();
+    count = 0;
+  }
+  if (tid < kSRows) id[tid] = adapter_of(rows, row0 + tid);
+  if (warp == kTmaWarp && lane == 0) {
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc<tmem_cols(kRank)>(&bars->tmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // the distinct adapters, in order of appearance (a row is first if none before it has its adapter)
+  if (warp == 0) {
+    int n = 0;
+    for (int base = 0; base < kSRows; base += 32) {
+      const int mine = id[base + lane];
+      bool first = mine >= 0;
+      for (int j = 0; j < base; ++j) first = first && id[j] != mine;
+      const unsigned same = __match_any_sync(0xffffffffu, mine);
+      first = first && __ffs(same) - 1 == lane;
+      const unsigned m = __ballot_sync(0xffffffffu, first);
+      if (first) list[n + __popc(m & ((1u << lane) - 1u))] = mine;
+      n += __popc(m);
+    }
+    if (lane == 0) count = n;
+  }
+  __syncthreads();
+  const int passes = count;
+  const uint32_t tmem = bars->tmem;
+
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int li = blockIdx.z; ok && li < passes; li += gridDim.z) {
+        for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
+          const int s = static_cast<int>(it % C::kStages);
+          if (!mbar_wait(&bars->empty[s], ((it / C::kStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          constexpr uint32_t w_bytes = kWRows ? kRank * 128 : (kRank == 128 ? 2 : 1) * 64 * 128;
+          mbar_arrive_expect_tx(&bars->full[s], (kCodes ? C::kRaw : kXTile) + w_bytes);
+          tma_load_2d(kCodes ? s_raw + s * C::kRaw : s_x + s * kXTile, &tm_x, &bars->full[s], kb * kSK,
+                      static_cast<int>(row0));
+          uint8_t* w = s_w + s * C::kW;
+          if constexpr (kWRows) {
+            tma_load_3d(w, &tm_w, &bars->full[s], kb * kSK, 0, list[li]);
+          } else {
+            tma_load_3d(w, &tm_w, &bars->full[s], 0, kb * kSK, list[li]);
+            if constexpr (kRank == 128) tma_load_3d(w + 8192, &tm_w, &bars->full[s], 64, kb * kSK, list[li]);
+          }
+        }
+      }
+      if (!ok) {  // let loads already in flight land (bounded)
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000) {
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16(kRank, 0, kWRows ? 0 : 1);
+      uint32_t it = 0, pass = 0;
+      bool ok = true;
+      for (int li = blockIdx.z; ok && li < passes; li += gridDim.z, ++pass) {
+        if (!mbar_wait(&bars->drained, (pass & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty)) break;
+        tc_fence_after();
+        for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
+          const int s = static_cast<int>(it % C::kStages);
+          const uint32_t ph = (it / C::kStages) & 1u;
+          if (!mbar_wait(&bars->full[s], ph, abortv, err, kDevTimeoutFull) ||
+              (kCodes && !mbar_wait(&bars->ready[s], ph, abortv, err, kDevTimeoutFull))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(s_x + s * kXTile), b0 = smem_u32(s_w + s * C::kW);
+#pragma unroll
+          for (int k = 0; k < kSK / 16; ++k) {
+            mma_bf16(tmem, smem_desc_k_sw128(a0 + k * 32),
+                     kWRows ? smem_desc_k_sw128(b0 + k * 32) : smem_desc_mn_sw128(b0 + k * 2048, 8192), idesc,
+                     (kb != kb_lo || k != 0) ? 1u : 0u);
+          }
+          umma_commit(&bars->empty[s]);
+        }
+        if (ok) umma_commit(&bars->done);
+      }
+    }
+  } else {
+    uint32_t it = 0, pass = 0;
+    bool ok = true;
+    for (int li = blockIdx.z; ok && li < passes; li += gridDim.z, ++pass) {
+      if constexpr (kCodes) {
+        // 128 rows x 64 codes: thread = row
+        for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
+          const int s = static_cast<int>(it % C::kStages);
+          const bool there =
+              mbar_wait(&bars->full[s], (it / C::kStages) & 1u, abortv, err, kDevTimeoutFull);
+          if (!__all_sync(0xffffffffu, there)) {
+            ok = false;
+            break;
+          }
+          const uint8_t* raw = s_raw + s * C::kRaw;
+          uint8_t* x = s_x + s * kXTile;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // four neighbours share a row of 64 bytes
+            const int r = (tid >> 2) + 32 * i, c = tid & 3;
+            uint4 a, b;
+            widen16(*reinterpret_cast<const uint4*>(raw + r * 64 + c * 16), a, b);
+            *reinterpret_cast<uint4*>(x + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = a;
+            *reinterpret_cast<uint4*>(x + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = b;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->ready[s]);
+        }
+        if (!ok) break;
+      }
+      const bool there = mbar_wait(&bars->done, pass & 1u, abortv, err, kDevTimeoutTmemFull);
+      if (!__all_sync(0xffffffffu, there)) break;
+      tc_fence_after();
+      const int r = warp * 32 + lane;
+      const bool mine = id[r] == list[li];
+      const int64_t row = row0 + r;
+      const float mul = mine && row_mul ? __ldg(row_mul + row) : 1.0f;
+      float* dst = part + (static_cast<int64_t>(blockIdx.y) * rows.M + row) * R;
+#pragma unroll
+      for (int c = 0; c < kRank; c += 32) {
+        uint32_t v[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, v);
+        tmem_ld_wait();
+        if (mine) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {  // R % 8 == 0
+            if (c + j < R) {
+              *reinterpret_cast<float4*>(dst + c + j) =
+                  make_float4(__uint_as_float(v[j]) * mul, __uint_as_float(v[j + 1]) * mul,
+                              __uint_as_float(v[j + 2]) * mul, __uint_as_float(v[j + 3]) * mul);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->drained);
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc<tmem_cols(kRank)>(tmem);
+  }
+}
+
+// ======================================================================== pieces
+// The rank side as tokens_tc reads it: out[piece][r][m] = bf16 pieces of
+// mul[s] * row_mul[m] * (the splits' sum), zero in rows without an adapter, past M and
+// past R; and info[s][tile]: 0 no row of adapter s in the tile of 64, 2 only such rows,
+// 1 others too.  blockIdx.y: which of the two rank sides.
+constexpr int kTile = 64;
+struct RankSide {
+  const float* part;
+  int splits;
+  const float* row_mul;
+  __nv_bfloat16* out;
+};
+template <int kRank>
+__global__ void __launch_bounds__(256) rank_pieces_kernel(RankSide a, RankSide b,
+                                                          const float* __restrict__ scaling, Rows rows,
+                                                          int R, int64_t m_pad, uint8_t* __restrict__ info) {
+  __shared__ float v[kTile][kRank + 1];
+  __shared__ TileIds ids;
+  const RankSide g = blockIdx.y ? b : a;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kTile;
+  tile_ids(rows, row0, ids);
+  for (int i = threadIdx.x; i < kTile * kRank; i += 256) {
+    const int r = i / kRank, c = i % kRank;
+    float sum = 0.0f;
+    if (ids.id[r] >= 0 && c < R) {
+      const float* p = g.part + (row0 + r) * R + c;
+      for (int sp = 0; sp < g.splits; ++sp) sum += __ldg(p + sp * rows.M * R);
+      if (scaling) sum *= __ldg(scaling + ids.id[r]);
+      if (g.row_mul) sum *= __ldg(g.row_mul + row0 + r);
+    }
+    v[r][c] = sum;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRank * (kTile / 2); i += 256) {
+    const int c = i / (kTile / 2), r = (i % (kTile / 2)) * 2;
+    float x = v[r][c], y = v[r + 1][c];
+    const float x0 = next_piece(x), y0 = next_piece(y);
+    *reinterpret_cast<uint32_t*>(g.out + c * m_pad + row0 + r) = pack_bf16(x0, y0);
+    *reinterpret_cast<uint32_t*>(g.out + (kRank + c) * m_pad + row0 + r) = pack_bf16(x, y);
+  }
+  if (blockIdx.y == 0) {
+    for (int s = threadIdx.x; s < rows.S; s += 256) {
+      int f = 0;
+      for (int i = 0; i < ids.count; ++i) f = ids.list[i] == s ? 1 : f;
+      if (f && ids.count == 1 && !ids.none) f = 2;
+      info[static_cast<int64_t>(s) * gridDim.x + blockIdx.x] = static_cast<uint8_t>(f);
+    }
+  }
+}
+
+// ======================================================================== tokens
+constexpr int kTCols = 256;
+constexpr int kTilesMost = 2048;  // tiles of 64 rows a block goes through
+template <bool kCodes, int kRank>
+struct TokensTc {
+  static constexpr int kX = kTile * kTCols * 2;            // four boxes of 64 columns, 32 KB
+  static constexpr int kH = 2 * kRank * kTile * 2;
+  static constexpr int kRaw = kCodes ? kTile * kTCols : 0;
+  static constexpr int kStage = kX + kH + kRaw;
+  static constexpr int kStagesRaw = (227 * 1024 - 1024 - 512 - kTilesMost) / kStage;
+  static constexpr int kStages = kStagesRaw > 6 ? 6 : kStagesRaw;
+  static constexpr int kBytes = 1024 + kStages * kStage + 512 + kTilesMost;
+  static_assert(kStages >= 2 && kH % 1024 == 0, "tiles");
+};
+
+// tm_x: boxes of 64 columns x 64 rows (codes: 256 x 64 bytes).  tm_h: the pieces,
+// [2 kRank][m_pad], boxes 64 x 2 kRank.
+template <bool kCodes, int kRank, bool kByCol>
+__global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
+    const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_h, Rows rows, int C, int R,
+    int tiles, int tiles_split, const uint8_t* __restrict__ info, float* __restrict__ part,
+    int* __restrict__ found) {
+  using T = TokensTc<kCodes, kRank>;
+  // two accumulators of kRank columns, read 32 columns at a time
+  constexpr uint32_t kTokenCols = tmem_cols(kRank < 32 ? 64 : 2 * kRank);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* s_x = smem;
+  uint8_t* s_h = s_x + T::kStages * T::kX;
+  uint8_t* s_raw = s_h + T::kStages * T::kH;
+  Bars* bars = reinterpret_cast<Bars*>(s_raw + T::kStages * T::kRaw);
+  uint8_t* live = reinterpret_cast<uint8_t*>(bars) + 512;
+  volatile int* abortv = &bars->abort_flag;
+  int* err = &g_lora_error;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int col0 = blockIdx.x * kTCols, s = blockIdx.z;
+  const int t_lo = blockIdx.y * tiles_split, n_tiles = min(tiles - t_lo, tiles_split);
+  const int64_t block = static_cast<int64_t>(blockIdx.y) * rows.S + s;
+
+  int mine = 0;
+  for (int i = tid; i < n_tiles; i += kThreads) {
+    const uint8_t f = __ldg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
+    live[i] = f;
+    mine |= f;
+  }
+  const int any = __syncthreads_or(mine);
+  if (blockIdx.x == 0 && tid == 0) found[block] = any != 0;
+  if (!any) return;
+
+  if (tid == 0) {
+    for (int i = 0; i < T::kStages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->ready[i], 4);
+      mbar_init(&bars->empty[i], 1);
+    }
+    mbar_init(&bars->done, 1);
+    bars->abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == kTmaWarp && lane == 0) {
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_h);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc<kTokenCols>(&bars->tmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = 0; ok && t < n_tiles; ++t) {
+        if (!live[t]) continue;
+        const int st = static_cast<int>(it % T::kStages);
+        if (!mbar_wait(&bars->empty[st], ((it / T::kStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+          ok = false;
+          break;
+        }
+        const int m = (t_lo + t) * kTile;
+        mbar_arrive_expect_tx(&bars->full[st], (kCodes ? T::kRaw : T::kX) + T::kH);
+        if constexpr (kCodes) {
+          tma_load_2d(s_raw + st * T::kRaw, &tm_x, &bars->full[st], col0, m);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            tma_load_2d(s_x + st * T::kX + c * 8192, &tm_x, &bars->full[st], col0 + c * 64, m);
+        }
+        tma_load_2d(s_h + st * T::kH, &tm_h, &bars->full[st], m, 0);
+        ++it;
+      }
+      if (!ok) {  // let loads already in flight land (bounded)
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000) {
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16(kRank, 1, 0);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = 0; t < n_tiles; ++t) {
+        if (!live[t]) continue;
+        const int st = static_cast<int>(it % T::kStages);
+        const uint32_t ph = (it / T::kStages) & 1u;
+        if (!mbar_wait(&bars->full[st], ph, abortv, err, kDevTimeoutFull) ||
+            !mbar_wait(&bars->ready[st], ph, abortv, err, kDevTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a0 = smem_u32(s_x + st * T::kX), b0 = smem_u32(s_h + st * T::kH);
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k) {
+            const uint64_t ad = smem_desc_mn_sw128(a0 + blk * 16384 + k * 2048, 8192);
+            mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + k * 32), idesc, (it != 0 || k != 0) ? 1u : 0u);
+            mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + kRank * 128 + k * 32), idesc, 1u);
+          }
+        }
+        umma_commit(&bars->empty[st]);
+        ++it;
+      }
+      if (ok) umma_commit(&bars->done);
+    }
+  } else {
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int f = live[t];
+      if (!f) continue;
+      const int st = static_cast<int>(it % T::kStages);
+      const bool there = mbar_wait(&bars->full[st], (it / T::kStages) & 1u, abortv, err, kDevTimeoutFull);
+      if (!__all_sync(0xffffffffu, there)) {
+        ok = false;
+        break;
+      }
+      const int64_t m0 = static_cast<int64_t>(t_lo + t) * kTile;
+      uint8_t* x = s_x + st * T::kX;
+      if constexpr (kCodes) {
+        // 64 rows x 256 codes: 16 neighbours a row
+        const uint8_t* raw = s_raw + st * T::kRaw;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = (tid >> 4) + 8 * i, c = tid & 15;  // 16 codes of the box c / 4
+          uint4 lo8, hi8;
+          widen16(*reinterpret_cast<const uint4*>(raw + r * kTCols + c * 16), lo8, hi8);
+          uint8_t* row = x + (c >> 2) * 8192 + r * 128;
+          const int at = 2 * (c & 3);
+          *reinterpret_cast<uint4*>(row + ((at ^ (r & 7)) << 4)) = lo8;
+          *reinterpret_cast<uint4*>(row + (((at + 1) ^ (r & 7)) << 4)) = hi8;
+        }
+      }
+      if (f == 1) {
+        // rows of other adapters (whatever they hold) leave the products: their
+        // values and their rank side are zeroed
+        const int r = tid & 63, half = tid >> 6;
+        if (adapter_of(rows, m0 + r) != s) {
+          if (!kCodes) {
+            for (int c = half * 2; c < half * 2 + 2; ++c)
+              for (int q = 0; q < 8; ++q)
+                *reinterpret_cast<uint4*>(x + c * 8192 + r * 128 + q * 16) = make_uint4(0, 0, 0, 0);
+          }
+          uint8_t* h = s_h + st * T::kH;
+          for (int k = half * kRank; k < (half + 1) * kRank; ++k)
+            *reinterpret_cast<uint16_t*>(h + k * 128 + (((r >> 3) ^ (k & 7)) << 4) + (r & 7) * 2) = 0;
+        }
+      }
+      if (kCodes || f == 1) fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->ready[st]);
+      ++it;
+    }
+    if (ok) {
+      const bool there = mbar_wait(&bars->done, 0, abortv, err, kDevTimeoutTmemFull);
+      if (__all_sync(0xffffffffu, there)) {
+        tc_fence_after();
+        float* dst = part + block * R * C;
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+          const int c = col0 + blk * 128 + warp * 32 + lane;
+#pragma unroll
+          for (int k = 0; k < kRank; k += 32) {
+            uint32_t v[32];
+            __syncwarp();
+            tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + blk * kRank + k, v);
+            tmem_ld_wait();
+            if (c < C) {
+              if constexpr (kByCol) {
+                float* p = dst + static_cast<int64_t>(c) * R + k;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)  // R % 8 == 0
+                  if (k + j < R && j < kRank)
+                    *reinterpret_cast<uint4*>(p + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (k + j < R && j < kRank) dst[static_cast<int64_t>(k + j) * C + c] = __uint_as_float(v[j]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc<kTokenCols>(tmem);
+  }
+}
+
+// ---------------------------------------------------------------- host
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess) {
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }
+  });
+  return fn;
+}
+
+// A map of `rank` dimensions (innermost first), element strides of the outer ones.
+bool map_of(CUtensorMap* map, bool bytes, int rank, const void* base, const int64_t* dims,
+            const int64_t* strides, const uint32_t* box, bool swizzled) {
+  auto fn = encoder();
+  cuuint64_t d[3], st[2];
+  cuuint32_t bx[3], ones[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    bx[i] = box[i];
+    if (i) st[i - 1] = static_cast<cuuint64_t>(strides[i - 1]) * (bytes ? 1 : 2);
+  }
+  return fn && fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                  const_cast<void*>(base), d, st, bx, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int refused(const char* what) {
+  set_error("cuTensorMapEncodeTiled rejected the operands of %s", what);
+  return W8A8_ERR_RUNTIME;
+}
+
+template <typename K>
+int opt_in(K kernel, int bytes) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    set_error("lora: shared memory of %d bytes refused: %s", bytes, cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
+}
+
+int launched(const char* what) {
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error("%s launch failed: %s", what, cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
+}
+
+template <bool kCodes, int kRank, bool kWRows>
+int shrink_rank(const ShrinkTcArgs& g, const Rows& rows, cudaStream_t stream) {
+  CUtensorMap tx, tw;
+  const int64_t xd[2] = {g.K, g.M}, xs[1] = {g.ldx};
+  const uint32_t xb[2] = {kSK, kSRows};
+  const int64_t wd[3] = {kWRows ? g.K : g.R, kWRows ? g.R : g.K, g.S};
+  const int64_t wst[2] = {kWRows ? g.K : g.R, g.S > 1 ? g.slot : g.R * g.K};
+  const uint32_t wb[3] = {64, kWRows ? static_cast<uint32_t>(kRank) : 64u, 1};
+  if (!map_of(&tx, kCodes, 2, g.x, xd, xs, xb, !kCodes) || !map_of(&tw, false, 3, g.w, wd, wst, wb, true)) {
+    return refused("the adapters' contraction");
+  }
+  auto k = shrink_tc_kernel<kCodes, kRank, kWRows>;
+  constexpr int bytes = ShrinkTc<kCodes, kRank>::kBytes;
+  if (int rc = opt_in(k, bytes)) return rc;
+  const dim3 grid(static_cast<unsigned>((g.M + kSRows - 1) / kSRows), g.splits, g.parts);
+  k<<<grid, kThreads, bytes, stream>>>(tx, tw, rows, g.x_scale, static_cast<int>(g.K), static_cast<int>(g.R),
+                                       g.kb_split, g.part);
+  return launched("lora shrink");
+}
+
+template <bool kCodes, bool kWRows>
+int shrink_codes(const ShrinkTcArgs& g, const Rows& rows, cudaStream_t stream) {
+  if (g.R <= 16) return shrink_rank<kCodes, 16, kWRows>(g, rows, stream);
+  if (g.R <= 32) return shrink_rank<kCodes, 32, kWRows>(g, rows, stream);
+  if (g.R <= 64) return shrink_rank<kCodes, 64, kWRows>(g, rows, stream);
+  return shrink_rank<kCodes, 128, kWRows>(g, rows, stream);
+}
+
+template <bool kCodes, int kRank, bool kByCol>
+int tokens_rank(const TokensTcArgs& g, const Rows& rows, cudaStream_t stream) {
+  CUtensorMap tx, th;
+  const int64_t tiles = (g.M + kTile - 1) / kTile;
+  const int64_t xd[2] = {g.C, g.M}, xs[1] = {g.ldx};
+  const uint32_t xb[2] = {kCodes ? 256u : 64u, kTile};
+  const int64_t hd[2] = {tiles * kTile, 2 * kRank}, hs[1] = {tiles * kTile};
+  const uint32_t hb[2] = {kTile, 2 * kRank};
+  if (!map_of(&tx, kCodes, 2, g.x, xd, xs, xb, !kCodes) || !map_of(&th, false, 2, g.pieces, hd, hs, hb, true)) {
+    return refused("the adapters' gradient");
+  }
+  auto k = tokens_tc_kernel<kCodes, kRank, kByCol>;
+  constexpr int bytes = TokensTc<kCodes, kRank>::kBytes;
+  if (int rc = opt_in(k, bytes)) return rc;
+  const dim3 grid(static_cast<unsigned>((g.C + kTCols - 1) / kTCols), g.splits, static_cast<unsigned>(g.S));
+  k<<<grid, kThreads, bytes, stream>>>(tx, th, rows, static_cast<int>(g.C), static_cast<int>(g.R),
+                                       static_cast<int>(tiles), g.tiles_split, g.info, g.part, g.found);
+  return launched("lora tokens");
+}
+
+template <bool kCodes, bool kByCol>
+int tokens_codes(const TokensTcArgs& g, const Rows& rows, cudaStream_t stream) {
+  if (g.R <= 16) return tokens_rank<kCodes, 16, kByCol>(g, rows, stream);
+  if (g.R <= 32) return tokens_rank<kCodes, 32, kByCol>(g, rows, stream);
+  if (g.R <= 64) return tokens_rank<kCodes, 64, kByCol>(g, rows, stream);
+  return tokens_rank<kCodes, 128, kByCol>(g, rows, stream);
+}
+
+template <int kRank>
+int pieces_rank(const RankPiecesArgs& g, const Rows& rows, cudaStream_t stream) {
+  const int64_t tiles = (rows.M + kTile - 1) / kTile;
+  const RankSide a{g.part_a, g.splits_a, g.row_mul_a, static_cast<__nv_bfloat16*>(g.out_a)};
+  const RankSide b{g.part_b, g.splits_b, nullptr, static_cast<__nv_bfloat16*>(g.out_b)};
+  rank_pieces_kernel<kRank><<<dim3(static_cast<unsigned>(tiles), 2), 256, 0, stream>>>(
+      a, b, g.scaling, rows, g.R, tiles * kTile, g.info);
+  return launched("lora rank pieces");
+}
+
+}  // namespace
+
+int lora_shrink_tc(const ShrinkTcArgs& g, const LoraRows& r, cudaStream_t stream) {
+  const Rows rows = rows_of(r);
+  if (g.codes) {
+    return g.w_rows ? shrink_codes<true, true>(g, rows, stream) : shrink_codes<true, false>(g, rows, stream);
+  }
+  return g.w_rows ? shrink_codes<false, true>(g, rows, stream) : shrink_codes<false, false>(g, rows, stream);
+}
+
+int lora_tokens_tc(const TokensTcArgs& g, const LoraRows& r, cudaStream_t stream) {
+  const Rows rows = rows_of(r);
+  if (g.codes) return tokens_codes<true, false>(g, rows, stream);
+  return g.by_col ? tokens_codes<false, true>(g, rows, stream) : tokens_codes<false, false>(g, rows, stream);
+}
+
+int lora_rank_pieces(const RankPiecesArgs& g, const LoraRows& r, cudaStream_t stream) {
+  const Rows rows = rows_of(r);
+  if (g.R <= 16) return pieces_rank<16>(g, rows, stream);
+  if (g.R <= 32) return pieces_rank<32>(g, rows, stream);
+  if (g.R <= 64) return pieces_rank<64>(g, rows, stream);
+  return pieces_rank<128>(g, rows, stream);
+}
+
+}  // namespace w8a8

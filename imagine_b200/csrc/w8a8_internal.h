@@ -182,6 +182,52 @@ struct LoraArgs {
   int64_t M, N, K, S, R;
   void* workspace;
 };
+// The tcgen05 form for long bf16 batches (lora_sm100.cu).
+struct LoraRows {
+  const void* idx;
+  int idx64;
+  int64_t per, M, S;
+};
+struct ShrinkTcArgs {
+  const void* x;  // bf16, or int8 codes
+  int codes;
+  int64_t ldx;
+  const float* x_scale;
+  const void* w;
+  int w_rows;     // 1: [S][R][K]; 0: [S][K][R] (K being B's N)
+  int64_t slot;
+  int64_t M, K, S, R;
+  int splits, kb_split, parts;
+  float* part;
+};
+struct TokensTcArgs {
+  const void* x;
+  int codes;
+  int64_t ldx;
+  const void* pieces;
+  int64_t M, C, S, R;
+  int by_col;
+  int splits, tiles_split;
+  const uint8_t* info;
+  float* part;
+  int* found;
+};
+struct RankPiecesArgs {
+  const float* part_a;  // the rank side that meets x (its row scale in row_mul_a), and dy
+  int splits_a;
+  const float* row_mul_a;
+  void* out_a;
+  const float* part_b;
+  int splits_b;
+  void* out_b;
+  const float* scaling;
+  int R;
+  uint8_t* info;
+};
+int lora_shrink_tc(const ShrinkTcArgs& g, const LoraRows& rows, cudaStream_t stream);
+int lora_tokens_tc(const TokensTcArgs& g, const LoraRows& rows, cudaStream_t stream);
+int lora_rank_pieces(const RankPiecesArgs& g, const LoraRows& rows, cudaStream_t stream);
+int read_and_clear_lora_error(cudaStream_t stream, int* value);
 int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, int backward);
 int lora_add_launch(const LoraArgs& g, cudaStream_t stream);
 int lora_backward_launch(const LoraArgs& g, cudaStream_t stream);
