@@ -931,6 +931,10 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
                                          static_cast<const T*>(g.a), g.lda, rows, K, R, sp, part, stream)) {
     return rc;
   }
+  if (tc_shape(g) && tc_rows(g.y, g.ldy, 2) && tc_rows(g.out, g.ldo, 2) && tc_weights(g.b, g.ldb, R, g.S)) {
+    return lora_expand_tc({g.y, g.ldy, part, sp.count, g.b, 1, g.ldb, g.scaling, g.out, g.ldo, g.M, g.N, g.S, g.R},
+                          {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
+  }
   return expand<T, true>(static_cast<const T*>(g.y), g.ldy, part, sp.count,
                          static_cast<const T*>(g.b), g.ldb, g.scaling, rows, N, R,
                          static_cast<T*>(g.out), g.ldo, stream);
@@ -985,7 +989,13 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
     } else if (int rc = shrink<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, rows, N, R, p.g, pg, stream)) {
       return rc;
     }
-    if (g.out) {
+    if (g.out && tc && tc_rows(g.out, g.ldo, 2)) {
+      if (int rc = lora_expand_tc({g.accumulate ? g.out : nullptr, g.ldo, pg, p.g.count, a, 0, g.lda, g.scaling,
+                                   g.out, g.ldo, g.M, g.K, g.S, g.R},
+                                  {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream)) {
+        return rc;
+      }
+    } else if (g.out) {
       if (int rc = expand<T, false>(g.accumulate ? static_cast<const T*>(g.out) : nullptr, g.ldo, pg,
                                     p.g.count, a, g.lda, g.scaling, rows, K, R,
                                     static_cast<T*>(g.out), g.ldo, stream)) {

@@ -2,6 +2,7 @@
 //
 //   shrink_tc   part[split][row][r] = sum over the split's k of x[row, k] W_s[k, r]
 //               a tile of 128 rows is the M side, the rank the N side
+//   expand_tc   out[row][n] = y[row][n] + c[s] * sum over r of h[row, r] W_s[r, n]
 //   tokens_tc   part[split][s][r][c] (or [c][r]) = sum over the split's rows m of
 //               adapter s of q[m, r] x[m, c]: 128 columns are the M side, read
 //               from the same row-major tiles by their transposed (MN-major)
@@ -103,6 +104,24 @@ __device__ __forceinline__ void widen16(const uint4& q, uint4& lo8, uint4& hi8) 
   hi8 = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
+// The distinct adapters of 128 rows in order of appearance, by one warp (a row is
+// first if none before it has its adapter).
+__device__ __forceinline__ void list_adapters(const int* id, int* list, int& count) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (int base = 0; base < 128; base += 32) {
+    const int mine = id[base + lane];
+    bool first = mine >= 0;
+    for (int j = 0; j < base; ++j) first = first && id[j] != mine;
+    const unsigned same = __match_any_sync(0xffffffffu, mine);
+    first = first && __ffs(same) - 1 == lane;
+    const unsigned m = __ballot_sync(0xffffffffu, first);
+    if (first) list[n + __popc(m & ((1u << lane) - 1u))] = mine;
+    n += __popc(m);
+  }
+  if (lane == 0) count = n;
+}
+
 struct Bars {
   uint64_t full[8], ready[8], empty[8], done, drained;
   uint32_t tmem;
@@ -169,21 +188,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // the distinct adapters, in order of appearance (a row is first if none before it has its adapter)
-  if (warp == 0) {
-    int n = 0;
-    for (int base = 0; base < kSRows; base += 32) {
-      const int mine = id[base + lane];
-      bool first = mine >= 0;
-      for (int j = 0; j < base; ++j) first = first && id[j] != mine;
-      const unsigned same = __match_any_sync(0xffffffffu, mine);
-      first = first && __ffs(same) - 1 == lane;
-      const unsigned m = __ballot_sync(0xffffffffu, first);
-      if (first) list[n + __popc(m & ((1u << lane) - 1u))] = mine;
-      n += __popc(m);
-    }
-    if (lane == 0) count = n;
-  }
+  if (warp == 0) list_adapters(id, list, count);
   __syncthreads();
   const int passes = count;
   const uint32_t tmem = bars->tmem;
@@ -585,6 +590,274 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
   }
 }
 
+// ======================================================================== expand
+// out[row, n] = bf16(y[row, n] + c[s] * sum_r h[row, r] W_s[r, n]); y NULL: zero.
+// A block keeps the pieces of h of 128 rows in shared memory and goes through its
+// columns 64 at a time: W_s and y arrive by TMA, the product lies in one of two
+// accumulators, the epilogue adds it to y in place in shared memory and a TMA store
+// takes the tile away.  Three stages, two blocks a multiprocessor: bound by
+// reading y and writing out.
+// A tile whose rows have different adapters (or none) is done adapter by adapter,
+// each storing its own rows only.
+constexpr int kERows = 128, kECols = 64;
+template <int kRank>
+struct ExpandTc {
+  static constexpr int kBlks = kRank > 64 ? 2 : 1;             // blocks of 64 of the rank
+  static constexpr int kHBlk = kERows * 128;                   // 16 KB
+  static constexpr int kH = 2 * kBlks * kHBlk;
+  static constexpr int kW = kBlks * kECols * 128;              // 8 KB a block, either way round
+  static constexpr int kY = kERows * kECols * 2;
+  static constexpr int kStage = kW + kY;
+  static constexpr int kStages = kBlks == 2 ? 4 : 3;
+  static constexpr int kBytes = 1024 + kH + kStages * kStage + 512 + 1024;
+};
+
+template <int kRank, bool kWCols>
+__global__ void __launch_bounds__(kThreads) expand_tc_kernel(
+    const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_w,
+    const __grid_constant__ CUtensorMap tm_out, const __nv_bfloat16* y, int64_t ldy, __nv_bfloat16* out,
+    int64_t ldo, const float* __restrict__ part, int splits, const float* __restrict__ scaling, Rows rows, int N,
+    int R, int col_parts, int tiles_part) {
+  using C = ExpandTc<kRank>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* s_h = smem;
+  uint8_t* s_y = s_h + C::kH;
+  uint8_t* s_w = s_y + C::kStages * C::kY;
+  Bars* bars = reinterpret_cast<Bars*>(s_w + C::kStages * C::kW);
+  uint64_t* tfull = bars->ready;       // two accumulators
+  uint64_t* tempty = bars->ready + 2;
+  uint64_t* h_there = &bars->done;
+  int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
+  int* list = id + kERows;
+  __shared__ int count, none;
+  volatile int* abortv = &bars->abort_flag;
+  int* err = &g_lora_error;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / col_parts) * kERows;
+  const int all_tiles = (N + kECols - 1) / kECols;
+  const int t_lo = static_cast<int>(blockIdx.x % col_parts) * tiles_part, t_hi = min(all_tiles, t_lo + tiles_part);
+
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 5);  // the MMAs, and four epilogue warps
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 4);
+    }
+    mbar_init(h_there, 4);
+    bars->abort_flag = 0;
+    fence_mbarrier_init();
+    none = 0;
+  }
+  __syncthreads();
+  if (tid < kERows) {
+    const int v = adapter_of(rows, row0 + tid);
+    id[tid] = v;
+    if (v < 0 && row0 + tid < rows.M) none = 1;
+  }
+  if (warp == kTmaWarp && lane == 0) {
+    tma_prefetch_desc(&tm_y);
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_out);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc<2 * kECols>(&bars->tmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) list_adapters(id, list, count);
+  __syncthreads();
+  const int passes = count;
+  const bool pure = passes == 1 && !none;
+  const uint32_t tmem = bars->tmem;
+
+  if (warp == kTmaWarp) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int li = 0; ok && li < passes; ++li) {
+        for (int t = t_lo; t < t_hi; ++t, ++it) {
+          const int s = static_cast<int>(it % C::kStages);
+          if (!mbar_wait(&bars->empty[s], ((it / C::kStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          constexpr uint32_t w_bytes = kWCols ? C::kW : kRank * 128;
+          mbar_arrive_expect_tx(&bars->full[s], w_bytes + (y ? C::kY : 0));
+          uint8_t* w = s_w + s * C::kW;
+          if constexpr (kWCols) {
+#pragma unroll
+            for (int b = 0; b < C::kBlks; ++b)
+              tma_load_3d(w + b * 8192, &tm_w, &bars->full[s], b * 64, t * kECols, list[li]);
+          } else {
+            tma_load_3d(w, &tm_w, &bars->full[s], t * kECols, 0, list[li]);
+          }
+          if (y) tma_load_2d(s_y + s * C::kY, &tm_y, &bars->full[s], t * kECols, static_cast<int>(row0));
+        }
+      }
+      if (!ok) {  // let loads already in flight land (bounded)
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000) {
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16(kECols, 0, kWCols ? 0 : 1);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int li = 0; ok && li < passes; ++li) {
+        if (!mbar_wait(h_there, static_cast<uint32_t>(li) & 1u, abortv, err, kDevTimeoutFull)) break;
+        for (int t = t_lo; t < t_hi; ++t, ++it) {
+          const int s = static_cast<int>(it % C::kStages);
+          const uint32_t acc = it & 1u;
+          if (!mbar_wait(&tempty[acc], ((it >> 1) & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty) ||
+              !mbar_wait(&bars->full[s], (it / C::kStages) & 1u, abortv, err, kDevTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t h0 = smem_u32(s_h), w0 = smem_u32(s_w + s * C::kW);
+#pragma unroll
+          for (int k = 0; k < kRank / 16; ++k) {
+            const int blk = k / 4, off = (k % 4) * 32;
+            const uint64_t bd = kWCols ? smem_desc_k_sw128(w0 + blk * 8192 + off) : smem_desc_mn_sw128(w0 + k * 2048, 8192);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              mma_bf16(tmem + acc * kECols, smem_desc_k_sw128(h0 + (p * C::kBlks + blk) * C::kHBlk + off), bd, idesc,
+                       (k != 0 || p != 0) ? 1u : 0u);
+            }
+          }
+          umma_commit(&bars->empty[s]);
+          umma_commit(&tfull[acc]);
+        }
+      }
+    }
+  } else {
+    const int r = warp * 32 + lane;
+    const int64_t row = row0 + r;
+    if (!pure && none && y != out) {
+      // rows without an adapter: y as it is (zero without y), a warp a row
+      for (int i = 0; i < 32; ++i) {
+        const int64_t m = row0 + warp * 32 + i;
+        if (id[warp * 32 + i] >= 0 || m >= rows.M) continue;
+        for (int c = t_lo * kECols + lane * 8; c < min(N, t_hi * kECols); c += 256) {  // N % 8 == 0
+          *reinterpret_cast<uint4*>(out + m * ldo + c) =
+              y ? *reinterpret_cast<const uint4*>(y + m * ldy + c) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    uint32_t it = 0;
+    bool ok = true;
+    int to_free = -1;  // the stage whose store may still be reading
+    for (int li = 0; ok && li < passes; ++li) {
+      const int s_id = list[li];
+      const bool mine = id[r] == s_id;
+      const float mul = scaling ? __ldg(scaling + s_id) : 1.0f;
+      // the row's h as pieces (zero in rows of other adapters); the previous adapter's
+      // products are done, their last accumulator has been read
+      const float* p0 = part + row * R;
+#pragma unroll 1
+      for (int c = 0; c < kRank; c += 8) {
+        float v[8] = {};
+        if (mine && c < R) {  // R % 8 == 0
+          for (int sp = 0; sp < splits; ++sp) {
+            const float4* q = reinterpret_cast<const float4*>(p0 + sp * rows.M * R + c);
+            const float4 a = __ldg(q), b = __ldg(q + 1);
+            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+            v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+          }
+        }
+        uint4 piece[2];
+        uint32_t* u = reinterpret_cast<uint32_t*>(piece);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x0 = next_piece(v[2 * j]), x1 = next_piece(v[2 * j + 1]);
+          u[j] = pack_bf16(x0, x1);
+          u[4 + j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        }
+        const int blk = c >> 6, ch = (c >> 3) & 7;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          *reinterpret_cast<uint4*>(s_h + (p * C::kBlks + blk) * C::kHBlk + r * 128 + ((ch ^ (r & 7)) << 4)) = piece[p];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(h_there);
+      for (int t = t_lo; t < t_hi; ++t, ++it) {
+        const int s = static_cast<int>(it % C::kStages);
+        const uint32_t acc = it & 1u;
+        const bool there = mbar_wait(&tfull[acc], (it >> 1) & 1u, abortv, err, kDevTimeoutTmemFull) &&
+                           mbar_wait(&bars->full[s], (it / C::kStages) & 1u, abortv, err, kDevTimeoutFull);
+        if (!__all_sync(0xffffffffu, there)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t v[2][32];
+        const uint32_t at = tmem + (static_cast<uint32_t>(warp * 32) << 16) + acc * kECols;
+        tmem_ld_32x32b_x32(at, v[0]);
+        tmem_ld_32x32b_x32(at + 32, v[1]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[acc]);
+        uint8_t* yr = s_y + s * C::kY + r * 128;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint4* cell = reinterpret_cast<uint4*>(yr + ((c ^ (r & 7)) << 4));
+          const uint4 b = y ? *cell : make_uint4(0, 0, 0, 0);
+          const uint32_t w4[4] = {b.x, b.y, b.z, b.w};
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x0 = __uint_as_float(v[c >> 2][(c & 3) * 8 + 2 * j]);
+            const float x1 = __uint_as_float(v[c >> 2][(c & 3) * 8 + 2 * j + 1]);
+            o[j] = pack_bf16(fmaf(mul, x0, __uint_as_float(w4[j] << 16)),
+                             fmaf(mul, x1, __uint_as_float(w4[j] & 0xFFFF0000u)));
+          }
+          const uint4 ov = make_uint4(o[0], o[1], o[2], o[3]);
+          if (pure) {
+            *cell = ov;
+          } else if (mine) {
+            const int col = t * kECols + c * 8;
+            if (col < N) *reinterpret_cast<uint4*>(out + row * ldo + col) = ov;
+          }
+        }
+        if (pure) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 + warp * 32 < rows.M)
+              tma_store_2d(&tm_out, s_y + s * C::kY + warp * 4096, t * kECols, static_cast<int>(row0) + warp * 32);
+            tma_store_commit();
+            if (to_free >= 0) {
+              tma_store_wait_read<1>();  // the tile before this one has left shared memory
+              mbar_arrive(&bars->empty[to_free]);
+            }
+            to_free = s;
+          }
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->empty[s]);
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait_all<0>();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc<2 * kECols>(tmem);
+  }
+}
+
 // ---------------------------------------------------------------- host
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -697,6 +970,44 @@ int tokens_codes(const TokensTcArgs& g, const Rows& rows, cudaStream_t stream) {
   return tokens_rank<kCodes, 128, kByCol>(g, rows, stream);
 }
 
+template <int kRank, bool kWCols>
+int expand_rank(const ExpandTcArgs& g, const Rows& rows, cudaStream_t stream) {
+  CUtensorMap ty, tw, to;
+  const int64_t od[2] = {g.N, g.M}, os[1] = {g.ldo}, ys[1] = {g.ldy};
+  const uint32_t yb[2] = {kECols, kERows}, ob[2] = {kECols, 32};
+  const int64_t wd[3] = {kWCols ? g.R : g.N, kWCols ? g.N : g.R, g.S};
+  const int64_t wst[2] = {kWCols ? g.R : g.N, g.S > 1 ? g.slot : g.R * g.N};
+  const uint32_t wb[3] = {64, kWCols ? 64u : static_cast<uint32_t>(kRank), 1};
+  if (!map_of(&to, false, 2, g.out, od, os, ob, true) ||
+      !map_of(&ty, false, 2, g.y ? g.y : g.out, od, g.y ? ys : os, yb, true) ||
+      !map_of(&tw, false, 3, g.w, wd, wst, wb, true)) {
+    return refused("the adapters' product");
+  }
+  auto k = expand_tc_kernel<kRank, kWCols>;
+  constexpr int bytes = ExpandTc<kRank>::kBytes;
+  if (int rc = opt_in(k, bytes)) return rc;
+  // one wave of blocks, two a multiprocessor (one at rank 128)
+  const int64_t tiles = (g.M + kERows - 1) / kERows;
+  const int64_t cols = (g.N + kECols - 1) / kECols;
+  const int64_t slots = static_cast<int64_t>(kRank > 64 ? 1 : 2) * device_sm_count();
+  int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cols, slots / tiles));
+  const int64_t per = (cols + parts - 1) / parts;
+  parts = (cols + per - 1) / per;
+  k<<<static_cast<unsigned>(tiles * parts), kThreads, bytes, stream>>>(
+      ty, tw, to, static_cast<const __nv_bfloat16*>(g.y), g.ldy, static_cast<__nv_bfloat16*>(g.out), g.ldo, g.part,
+      g.splits, g.scaling, rows, static_cast<int>(g.N), static_cast<int>(g.R), static_cast<int>(parts),
+      static_cast<int>(per));
+  return launched("lora expand");
+}
+
+template <bool kWCols>
+int expand_cols(const ExpandTcArgs& g, const Rows& rows, cudaStream_t stream) {
+  if (g.R <= 16) return expand_rank<16, kWCols>(g, rows, stream);
+  if (g.R <= 32) return expand_rank<32, kWCols>(g, rows, stream);
+  if (g.R <= 64) return expand_rank<64, kWCols>(g, rows, stream);
+  return expand_rank<128, kWCols>(g, rows, stream);
+}
+
 template <int kRank>
 int pieces_rank(const RankPiecesArgs& g, const Rows& rows, cudaStream_t stream) {
   const int64_t tiles = (rows.M + kTile - 1) / kTile;
@@ -721,6 +1032,11 @@ int lora_tokens_tc(const TokensTcArgs& g, const LoraRows& r, cudaStream_t stream
   const Rows rows = rows_of(r);
   if (g.codes) return tokens_codes<true, false>(g, rows, stream);
   return g.by_col ? tokens_codes<false, true>(g, rows, stream) : tokens_codes<false, false>(g, rows, stream);
+}
+
+int lora_expand_tc(const ExpandTcArgs& g, const LoraRows& r, cudaStream_t stream) {
+  const Rows rows = rows_of(r);
+  return g.w_cols ? expand_cols<true>(g, rows, stream) : expand_cols<false>(g, rows, stream);
 }
 
 int lora_rank_pieces(const RankPiecesArgs& g, const LoraRows& r, cudaStream_t stream) {

@@ -200,6 +200,19 @@ struct ShrinkTcArgs {
   int splits, kb_split, parts;
   float* part;
 };
+struct ExpandTcArgs {
+  const void* y;  // or NULL
+  int64_t ldy;
+  const float* part;
+  int splits;
+  const void* w;
+  int w_cols;     // 1: [S][N][R]; 0: [S][R][N] (N being A's K)
+  int64_t slot;
+  const float* scaling;
+  void* out;
+  int64_t ldo;
+  int64_t M, N, S, R;
+};
 struct TokensTcArgs {
   const void* x;
   int codes;
@@ -225,6 +238,7 @@ struct RankPiecesArgs {
   uint8_t* info;
 };
 int lora_shrink_tc(const ShrinkTcArgs& g, const LoraRows& rows, cudaStream_t stream);
+int lora_expand_tc(const ExpandTcArgs& g, const LoraRows& rows, cudaStream_t stream);
 int lora_tokens_tc(const TokensTcArgs& g, const LoraRows& rows, cudaStream_t stream);
 int lora_rank_pieces(const RankPiecesArgs& g, const LoraRows& rows, cudaStream_t stream);
 int read_and_clear_lora_error(cudaStream_t stream, int* value);
