@@ -123,21 +123,26 @@ __device__ __forceinline__ void list_adapters(const int* id, int* list, int& cou
 }
 
 struct Bars {
-  uint64_t full[8], ready[8], empty[8], done, drained;
+  uint64_t full[8], ready[8], empty[8], acc[8], done, drained;
   uint32_t tmem;
   int abort_flag;
 };
 
 // ======================================================================== shrink
+// A tile whose rows have several adapters is multiplied by each of them while it is
+// there, into accumulators of their own, as many at a time as TMEM has columns for.
 constexpr int kSRows = 128, kSK = 64;
 constexpr int kXTile = kSRows * kSK * 2;  // 16 KB
 template <bool kCodes, int kRank>
 struct ShrinkTc {
   static constexpr int kW = kRank == 128 ? 16384 : 8192;
   static constexpr int kRaw = kCodes ? kSRows * kSK : 0;
-  static constexpr int kStage = kXTile + kW + kRaw;
-  static constexpr int kStages = 98304 / kStage;  // two blocks a multiprocessor
-  static constexpr int kBytes = 1024 + kStages * kStage + 512 + 1280;
+  static constexpr int kWStages = kRank == 128 ? 2 : kCodes ? 2 : 4;
+  static constexpr int kXStages = kCodes ? 3 : 4;
+  static constexpr int kBytes = 1024 + kXStages * (kXTile + kRaw) + kWStages * kW + 512 + 1280;
+  static constexpr uint32_t kCols = 256;                  // accumulator columns a block takes
+  static constexpr int kAtOnce = static_cast<int>(kCols) / kRank;
+  static_assert(2 * kBytes + 2048 <= 228 * 1024, "two blocks a multiprocessor");
 };
 
 // tm_x: rows of x, boxes 64 x 128 (bf16, swizzled; codes: as they are).  tm_w:
@@ -151,9 +156,11 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* s_x = smem;
-  uint8_t* s_w = s_x + C::kStages * kXTile;
-  uint8_t* s_raw = s_w + C::kStages * C::kW;
-  Bars* bars = reinterpret_cast<Bars*>(s_raw + C::kStages * C::kRaw);
+  uint8_t* s_w = s_x + C::kXStages * kXTile;
+  uint8_t* s_raw = s_w + C::kWStages * C::kW;
+  Bars* bars = reinterpret_cast<Bars*>(s_raw + C::kXStages * C::kRaw);
+  uint64_t* w_full = bars->full + 4;
+  uint64_t* w_empty = bars->empty + 4;
   int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
   int* list = id + kSRows;
   __shared__ int count;
@@ -165,10 +172,14 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   const int kb_lo = blockIdx.y * kb_split, kb_hi = min(kb_all, kb_lo + kb_split);
 
   if (tid == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
+    for (int s = 0; s < C::kXStages; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->ready[s], 4);
       mbar_init(&bars->empty[s], 1);
+    }
+    for (int s = 0; s < C::kWStages; ++s) {
+      mbar_init(&w_full[s], 1);
+      mbar_init(&w_empty[s], 1);
     }
     mbar_init(&bars->done, 1);
     mbar_init(&bars->drained, 4);
@@ -176,44 +187,69 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
     fence_mbarrier_init();
     count = 0;
   }
-  if (tid < kSRows) id[tid] = adapter_of(rows, row0 + tid);
+  int v = -1;
+  if (tid < kSRows) {
+    v = adapter_of(rows, row0 + tid);
+    id[tid] = v;
+  }
   if (warp == kTmaWarp && lane == 0) {
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_w);
   }
   if (warp == kMmaWarp) {
-    tmem_alloc<tmem_cols(kRank)>(&bars->tmem);
+    tmem_alloc<C::kCols>(&bars->tmem);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) list_adapters(id, list, count);
+  const bool one = __syncthreads_and(tid >= kSRows || row0 + tid >= rows.M || v == id[0]);
+  if (one) {
+    if (tid == 0) {
+      list[0] = id[0];
+      count = id[0] >= 0 ? 1 : 0;
+    }
+  } else if (warp == 0) {
+    list_adapters(id, list, count);
+  }
   __syncthreads();
-  const int passes = count;
+  const int total = count;
   const uint32_t tmem = bars->tmem;
+  // this block's adapters of the tile: those from blockIdx.z on, gridDim.z apart, kAtOnce a pass
+  const int mine_n = total > static_cast<int>(blockIdx.z) ? (total - blockIdx.z + gridDim.z - 1) / gridDim.z : 0;
+  auto adapter = [&](int i) { return list[blockIdx.z + i * gridDim.z]; };
 
   if (warp == kTmaWarp) {
     if (lane == 0) {
-      uint32_t it = 0;
+      uint32_t it = 0, wt = 0;
       bool ok = true;
-      for (int li = blockIdx.z; ok && li < passes; li += gridDim.z) {
-        for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
-          const int s = static_cast<int>(it % C::kStages);
-          if (!mbar_wait(&bars->empty[s], ((it / C::kStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+      for (int i0 = 0; ok && i0 < mine_n; i0 += C::kAtOnce) {
+        const int n = min(C::kAtOnce, mine_n - i0);
+        for (int kb = kb_lo; ok && kb < kb_hi; ++kb, ++it) {
+          const int s = static_cast<int>(it % C::kXStages);
+          if (!mbar_wait(&bars->empty[s], ((it / C::kXStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
             ok = false;
             break;
           }
-          constexpr uint32_t w_bytes = kWRows ? kRank * 128 : (kRank == 128 ? 2 : 1) * 64 * 128;
-          mbar_arrive_expect_tx(&bars->full[s], (kCodes ? C::kRaw : kXTile) + w_bytes);
+          mbar_arrive_expect_tx(&bars->full[s], kCodes ? C::kRaw : kXTile);
           tma_load_2d(kCodes ? s_raw + s * C::kRaw : s_x + s * kXTile, &tm_x, &bars->full[s], kb * kSK,
                       static_cast<int>(row0));
-          uint8_t* w = s_w + s * C::kW;
-          if constexpr (kWRows) {
-            tma_load_3d(w, &tm_w, &bars->full[s], kb * kSK, 0, list[li]);
-          } else {
-            tma_load_3d(w, &tm_w, &bars->full[s], 0, kb * kSK, list[li]);
-            if constexpr (kRank == 128) tma_load_3d(w + 8192, &tm_w, &bars->full[s], 64, kb * kSK, list[li]);
+          for (int i = 0; i < n; ++i, ++wt) {
+            const int ws = static_cast<int>(wt % C::kWStages);
+            if (!mbar_wait(&w_empty[ws], ((wt / C::kWStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+              ok = false;
+              break;
+            }
+            constexpr uint32_t w_bytes = kWRows ? kRank * 128 : (kRank == 128 ? 2 : 1) * 64 * 128;
+            mbar_arrive_expect_tx(&w_full[ws], w_bytes);
+            uint8_t* w = s_w + ws * C::kW;
+            const int ad = adapter(i0 + i);
+            if constexpr (kWRows) {
+              tma_load_3d(w, &tm_w, &w_full[ws], kb * kSK, 0, ad);
+            } else {
+              tma_load_3d(w, &tm_w, &w_full[ws], 0, kb * kSK, ad);
+              if constexpr (kRank == 128) tma_load_3d(w + 8192, &tm_w, &w_full[ws], 64, kb * kSK, ad);
+            }
           }
         }
       }
@@ -226,28 +262,38 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   } else if (warp == kMmaWarp) {
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_bf16(kRank, 0, kWRows ? 0 : 1);
-      uint32_t it = 0, pass = 0;
+      uint32_t it = 0, wt = 0, pass = 0;
       bool ok = true;
-      for (int li = blockIdx.z; ok && li < passes; li += gridDim.z, ++pass) {
+      for (int i0 = 0; ok && i0 < mine_n; i0 += C::kAtOnce, ++pass) {
+        const int n = min(C::kAtOnce, mine_n - i0);
         if (!mbar_wait(&bars->drained, (pass & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty)) break;
         tc_fence_after();
-        for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
-          const int s = static_cast<int>(it % C::kStages);
-          const uint32_t ph = (it / C::kStages) & 1u;
+        for (int kb = kb_lo; ok && kb < kb_hi; ++kb, ++it) {
+          const int s = static_cast<int>(it % C::kXStages);
+          const uint32_t ph = (it / C::kXStages) & 1u;
           if (!mbar_wait(&bars->full[s], ph, abortv, err, kDevTimeoutFull) ||
               (kCodes && !mbar_wait(&bars->ready[s], ph, abortv, err, kDevTimeoutFull))) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(s_x + s * kXTile), b0 = smem_u32(s_w + s * C::kW);
+          const uint32_t a0 = smem_u32(s_x + s * kXTile);
+          for (int i = 0; i < n; ++i, ++wt) {
+            const int ws = static_cast<int>(wt % C::kWStages);
+            if (!mbar_wait(&w_full[ws], (wt / C::kWStages) & 1u, abortv, err, kDevTimeoutFull)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t b0 = smem_u32(s_w + ws * C::kW);
 #pragma unroll
-          for (int k = 0; k < kSK / 16; ++k) {
-            mma_bf16(tmem, smem_desc_k_sw128(a0 + k * 32),
-                     kWRows ? smem_desc_k_sw128(b0 + k * 32) : smem_desc_mn_sw128(b0 + k * 2048, 8192), idesc,
-                     (kb != kb_lo || k != 0) ? 1u : 0u);
+            for (int k = 0; k < kSK / 16; ++k) {
+              mma_bf16(tmem + i * kRank, smem_desc_k_sw128(a0 + k * 32),
+                       kWRows ? smem_desc_k_sw128(b0 + k * 32) : smem_desc_mn_sw128(b0 + k * 2048, 8192), idesc,
+                       (kb != kb_lo || k != 0) ? 1u : 0u);
+            }
+            umma_commit(&w_empty[ws]);
           }
-          umma_commit(&bars->empty[s]);
+          if (ok) umma_commit(&bars->empty[s]);
         }
         if (ok) umma_commit(&bars->done);
       }
@@ -255,13 +301,14 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   } else {
     uint32_t it = 0, pass = 0;
     bool ok = true;
-    for (int li = blockIdx.z; ok && li < passes; li += gridDim.z, ++pass) {
+    for (int i0 = 0; ok && i0 < mine_n; i0 += C::kAtOnce, ++pass) {
+      const int n = min(C::kAtOnce, mine_n - i0);
       if constexpr (kCodes) {
-        // 128 rows x 64 codes: thread = row
+        // 128 rows x 64 codes: four neighbours share a row of 64 bytes
         for (int kb = kb_lo; kb < kb_hi; ++kb, ++it) {
-          const int s = static_cast<int>(it % C::kStages);
+          const int s = static_cast<int>(it % C::kXStages);
           const bool there =
-              mbar_wait(&bars->full[s], (it / C::kStages) & 1u, abortv, err, kDevTimeoutFull);
+              mbar_wait(&bars->full[s], (it / C::kXStages) & 1u, abortv, err, kDevTimeoutFull);
           if (!__all_sync(0xffffffffu, there)) {
             ok = false;
             break;
@@ -270,12 +317,11 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
           uint8_t* x = s_x + s * kXTile;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            // four neighbours share a row of 64 bytes
             const int r = (tid >> 2) + 32 * i, c = tid & 3;
-            uint4 a, b;
-            widen16(*reinterpret_cast<const uint4*>(raw + r * 64 + c * 16), a, b);
-            *reinterpret_cast<uint4*>(x + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = a;
-            *reinterpret_cast<uint4*>(x + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = b;
+            uint4 lo8, hi8;
+            widen16(*reinterpret_cast<const uint4*>(raw + r * 64 + c * 16), lo8, hi8);
+            *reinterpret_cast<uint4*>(x + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = lo8;
+            *reinterpret_cast<uint4*>(x + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = hi8;
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -287,23 +333,25 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
       if (!__all_sync(0xffffffffu, there)) break;
       tc_fence_after();
       const int r = warp * 32 + lane;
-      const bool mine = id[r] == list[li];
       const int64_t row = row0 + r;
-      const float mul = mine && row_mul ? __ldg(row_mul + row) : 1.0f;
+      const float mul = id[r] >= 0 && row_mul ? __ldg(row_mul + row) : 1.0f;
       float* dst = part + (static_cast<int64_t>(blockIdx.y) * rows.M + row) * R;
+      for (int i = 0; i < n; ++i) {
+        const bool mine = id[r] == adapter(i0 + i);
 #pragma unroll
-      for (int c = 0; c < kRank; c += 32) {
-        uint32_t v[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, v);
-        tmem_ld_wait();
-        if (mine) {
+        for (int c = 0; c < kRank; c += 32) {
+          uint32_t d[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + i * kRank + c, d);
+          tmem_ld_wait();
+          if (mine) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {  // R % 8 == 0
-            if (c + j < R) {
-              *reinterpret_cast<float4*>(dst + c + j) =
-                  make_float4(__uint_as_float(v[j]) * mul, __uint_as_float(v[j + 1]) * mul,
-                              __uint_as_float(v[j + 2]) * mul, __uint_as_float(v[j + 3]) * mul);
+            for (int j = 0; j < 32; j += 4) {  // R % 8 == 0
+              if (c + j < R && j < kRank) {
+                *reinterpret_cast<float4*>(dst + c + j) =
+                    make_float4(__uint_as_float(d[j]) * mul, __uint_as_float(d[j + 1]) * mul,
+                                __uint_as_float(d[j + 2]) * mul, __uint_as_float(d[j + 3]) * mul);
+              }
             }
           }
         }
@@ -316,7 +364,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc<tmem_cols(kRank)>(tmem);
+    tmem_dealloc<C::kCols>(tmem);
   }
 }
 
@@ -372,7 +420,8 @@ __global__ void __launch_bounds__(256) rank_pieces_kernel(RankSide a, RankSide b
 
 // ======================================================================== tokens
 constexpr int kTCols = 256;
-constexpr int kTilesMost = 2048;  // tiles of 64 rows a block goes through
+constexpr int kTilesMost = 2048;   // tiles of 64 rows a block goes through
+constexpr int kAdaptersMost = 64;  // adapters of a call
 template <bool kCodes, int kRank>
 struct TokensTc {
   static constexpr int kX = kTile * kTCols * 2;            // four boxes of 64 columns, 32 KB
@@ -403,22 +452,12 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
   uint8_t* s_raw = s_h + T::kStages * T::kH;
   Bars* bars = reinterpret_cast<Bars*>(s_raw + T::kStages * T::kRaw);
   uint8_t* live = reinterpret_cast<uint8_t*>(bars) + 512;
+  __shared__ uint8_t present[kAdaptersMost];
   volatile int* abortv = &bars->abort_flag;
   int* err = &g_lora_error;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int col0 = blockIdx.x * kTCols, s = blockIdx.z;
+  const int col0 = blockIdx.x * kTCols;
   const int t_lo = blockIdx.y * tiles_split, n_tiles = min(tiles - t_lo, tiles_split);
-  const int64_t block = static_cast<int64_t>(blockIdx.y) * rows.S + s;
-
-  int mine = 0;
-  for (int i = tid; i < n_tiles; i += kThreads) {
-    const uint8_t f = __ldg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
-    live[i] = f;
-    mine |= f;
-  }
-  const int any = __syncthreads_or(mine);
-  if (blockIdx.x == 0 && tid == 0) found[block] = any != 0;
-  if (!any) return;
 
   if (tid == 0) {
     for (int i = 0; i < T::kStages; ++i) {
@@ -429,6 +468,16 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
     mbar_init(&bars->done, 1);
     bars->abort_flag = 0;
     fence_mbarrier_init();
+  }
+  // which adapters these rows have
+  for (int s = warp; s < rows.S; s += kThreads / 32) {
+    int any = 0;
+    for (int i = lane; i < n_tiles; i += 32) any |= __ldg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
+    any = __any_sync(0xffffffffu, any);
+    if (lane == 0) {
+      present[s] = static_cast<uint8_t>(any);
+      if (blockIdx.x == 0) found[static_cast<int64_t>(blockIdx.y) * rows.S + s] = any;
+    }
   }
   if (warp == kTmaWarp && lane == 0) {
     tma_prefetch_desc(&tm_x);
@@ -443,145 +492,154 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
 
-  if (warp == kTmaWarp) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = 0; ok && t < n_tiles; ++t) {
-        if (!live[t]) continue;
-        const int st = static_cast<int>(it % T::kStages);
-        if (!mbar_wait(&bars->empty[st], ((it / T::kStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
-          ok = false;
-          break;
-        }
-        const int m = (t_lo + t) * kTile;
-        mbar_arrive_expect_tx(&bars->full[st], (kCodes ? T::kRaw : T::kX) + T::kH);
-        if constexpr (kCodes) {
-          tma_load_2d(s_raw + st * T::kRaw, &tm_x, &bars->full[st], col0, m);
-        } else {
+  // one adapter after the other: its tiles, then its sums are written
+  uint32_t it = 0, segment = 0;
+  for (int s = 0; s < rows.S; ++s) {
+    if (!present[s]) continue;
+    for (int i = tid; i < n_tiles; i += kThreads) live[i] = __ldg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kTmaWarp) {
+      if (lane == 0) {
+        bool ok = true;
+        for (int t = 0; ok && t < n_tiles; ++t) {
+          if (!live[t]) continue;
+          const int st = static_cast<int>(it % T::kStages);
+          if (!mbar_wait(&bars->empty[st], ((it / T::kStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          const int m = (t_lo + t) * kTile;
+          mbar_arrive_expect_tx(&bars->full[st], (kCodes ? T::kRaw : T::kX) + T::kH);
+          if constexpr (kCodes) {
+            tma_load_2d(s_raw + st * T::kRaw, &tm_x, &bars->full[st], col0, m);
+          } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            tma_load_2d(s_x + st * T::kX + c * 8192, &tm_x, &bars->full[st], col0 + c * 64, m);
+            for (int c = 0; c < 4; ++c)
+              tma_load_2d(s_x + st * T::kX + c * 8192, &tm_x, &bars->full[st], col0 + c * 64, m);
+          }
+          tma_load_2d(s_h + st * T::kH, &tm_h, &bars->full[st], m, 0);
+          ++it;
         }
-        tma_load_2d(s_h + st * T::kH, &tm_h, &bars->full[st], m, 0);
-        ++it;
-      }
-      if (!ok) {  // let loads already in flight land (bounded)
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 1000000) {
+        if (!ok) {  // let loads already in flight land (bounded)
+          const uint64_t t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 1000000) {
+          }
         }
       }
-    }
-  } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16(kRank, 1, 0);
-      uint32_t it = 0;
+    } else if (warp == kMmaWarp) {
+      if (lane == 0) {
+        constexpr uint32_t idesc = idesc_bf16(kRank, 1, 0);
+        bool ok = true, first = true;
+        for (int t = 0; t < n_tiles; ++t) {
+          if (!live[t]) continue;
+          const int st = static_cast<int>(it % T::kStages);
+          const uint32_t ph = (it / T::kStages) & 1u;
+          if (!mbar_wait(&bars->full[st], ph, abortv, err, kDevTimeoutFull) ||
+              !mbar_wait(&bars->ready[st], ph, abortv, err, kDevTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(s_x + st * T::kX), b0 = smem_u32(s_h + st * T::kH);
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k) {
+              const uint64_t ad = smem_desc_mn_sw128(a0 + blk * 16384 + k * 2048, 8192);
+              mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + k * 32), idesc, (!first || k != 0) ? 1u : 0u);
+              mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + kRank * 128 + k * 32), idesc, 1u);
+            }
+          }
+          umma_commit(&bars->empty[st]);
+          first = false;
+          ++it;
+        }
+        if (ok) umma_commit(&bars->done);
+      }
+    } else {
       bool ok = true;
       for (int t = 0; t < n_tiles; ++t) {
-        if (!live[t]) continue;
+        const int f = live[t];
+        if (!f) continue;
         const int st = static_cast<int>(it % T::kStages);
-        const uint32_t ph = (it / T::kStages) & 1u;
-        if (!mbar_wait(&bars->full[st], ph, abortv, err, kDevTimeoutFull) ||
-            !mbar_wait(&bars->ready[st], ph, abortv, err, kDevTimeoutFull)) {
+        const bool there = mbar_wait(&bars->full[st], (it / T::kStages) & 1u, abortv, err, kDevTimeoutFull);
+        if (!__all_sync(0xffffffffu, there)) {
           ok = false;
           break;
         }
-        tc_fence_after();
-        const uint32_t a0 = smem_u32(s_x + st * T::kX), b0 = smem_u32(s_h + st * T::kH);
+        const int64_t m0 = static_cast<int64_t>(t_lo + t) * kTile;
+        uint8_t* x = s_x + st * T::kX;
+        if constexpr (kCodes) {
+          // 64 rows x 256 codes: 16 neighbours a row
+          const uint8_t* raw = s_raw + st * T::kRaw;
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k) {
-            const uint64_t ad = smem_desc_mn_sw128(a0 + blk * 16384 + k * 2048, 8192);
-            mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + k * 32), idesc, (it != 0 || k != 0) ? 1u : 0u);
-            mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + kRank * 128 + k * 32), idesc, 1u);
+          for (int i = 0; i < 8; ++i) {
+            const int r = (tid >> 4) + 8 * i, c = tid & 15;  // 16 codes of the box c / 4
+            uint4 lo8, hi8;
+            widen16(*reinterpret_cast<const uint4*>(raw + r * kTCols + c * 16), lo8, hi8);
+            uint8_t* row = x + (c >> 2) * 8192 + r * 128;
+            const int at = 2 * (c & 3);
+            *reinterpret_cast<uint4*>(row + ((at ^ (r & 7)) << 4)) = lo8;
+            *reinterpret_cast<uint4*>(row + (((at + 1) ^ (r & 7)) << 4)) = hi8;
           }
         }
-        umma_commit(&bars->empty[st]);
+        if (f == 1) {
+          // rows of other adapters (whatever they hold) leave the products: their
+          // values and their rank side are zeroed
+          const int r = tid & 63, half = tid >> 6;
+          if (adapter_of(rows, m0 + r) != s) {
+            if (!kCodes) {
+              for (int c = half * 2; c < half * 2 + 2; ++c)
+                for (int q = 0; q < 8; ++q)
+                  *reinterpret_cast<uint4*>(x + c * 8192 + r * 128 + q * 16) = make_uint4(0, 0, 0, 0);
+            }
+            uint8_t* h = s_h + st * T::kH;
+            for (int k = half * kRank; k < (half + 1) * kRank; ++k)
+              *reinterpret_cast<uint16_t*>(h + k * 128 + (((r >> 3) ^ (k & 7)) << 4) + (r & 7) * 2) = 0;
+          }
+        }
+        if (kCodes || f == 1) fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ready[st]);
         ++it;
       }
-      if (ok) umma_commit(&bars->done);
-    }
-  } else {
-    uint32_t it = 0;
-    bool ok = true;
-    for (int t = 0; t < n_tiles; ++t) {
-      const int f = live[t];
-      if (!f) continue;
-      const int st = static_cast<int>(it % T::kStages);
-      const bool there = mbar_wait(&bars->full[st], (it / T::kStages) & 1u, abortv, err, kDevTimeoutFull);
-      if (!__all_sync(0xffffffffu, there)) {
-        ok = false;
-        break;
-      }
-      const int64_t m0 = static_cast<int64_t>(t_lo + t) * kTile;
-      uint8_t* x = s_x + st * T::kX;
-      if constexpr (kCodes) {
-        // 64 rows x 256 codes: 16 neighbours a row
-        const uint8_t* raw = s_raw + st * T::kRaw;
+      if (ok) {
+        const bool there = mbar_wait(&bars->done, segment & 1u, abortv, err, kDevTimeoutTmemFull);
+        if (__all_sync(0xffffffffu, there)) {
+          tc_fence_after();
+          float* dst = part + (static_cast<int64_t>(blockIdx.y) * rows.S + s) * R * C;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = (tid >> 4) + 8 * i, c = tid & 15;  // 16 codes of the box c / 4
-          uint4 lo8, hi8;
-          widen16(*reinterpret_cast<const uint4*>(raw + r * kTCols + c * 16), lo8, hi8);
-          uint8_t* row = x + (c >> 2) * 8192 + r * 128;
-          const int at = 2 * (c & 3);
-          *reinterpret_cast<uint4*>(row + ((at ^ (r & 7)) << 4)) = lo8;
-          *reinterpret_cast<uint4*>(row + (((at + 1) ^ (r & 7)) << 4)) = hi8;
-        }
-      }
-      if (f == 1) {
-        // rows of other adapters (whatever they hold) leave the products: their
-        // values and their rank side are zeroed
-        const int r = tid & 63, half = tid >> 6;
-        if (adapter_of(rows, m0 + r) != s) {
-          if (!kCodes) {
-            for (int c = half * 2; c < half * 2 + 2; ++c)
-              for (int q = 0; q < 8; ++q)
-                *reinterpret_cast<uint4*>(x + c * 8192 + r * 128 + q * 16) = make_uint4(0, 0, 0, 0);
-          }
-          uint8_t* h = s_h + st * T::kH;
-          for (int k = half * kRank; k < (half + 1) * kRank; ++k)
-            *reinterpret_cast<uint16_t*>(h + k * 128 + (((r >> 3) ^ (k & 7)) << 4) + (r & 7) * 2) = 0;
-        }
-      }
-      if (kCodes || f == 1) fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ready[st]);
-      ++it;
-    }
-    if (ok) {
-      const bool there = mbar_wait(&bars->done, 0, abortv, err, kDevTimeoutTmemFull);
-      if (__all_sync(0xffffffffu, there)) {
-        tc_fence_after();
-        float* dst = part + block * R * C;
+          for (int blk = 0; blk < 2; ++blk) {
+            const int c = col0 + blk * 128 + warp * 32 + lane;
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-          const int c = col0 + blk * 128 + warp * 32 + lane;
+            for (int k = 0; k < kRank; k += 32) {
+              uint32_t v[32];
+              __syncwarp();
+              tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + blk * kRank + k, v);
+              tmem_ld_wait();
+              if (c < C) {
+                if constexpr (kByCol) {
+                  float* p = dst + static_cast<int64_t>(c) * R + k;
 #pragma unroll
-          for (int k = 0; k < kRank; k += 32) {
-            uint32_t v[32];
-            __syncwarp();
-            tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + blk * kRank + k, v);
-            tmem_ld_wait();
-            if (c < C) {
-              if constexpr (kByCol) {
-                float* p = dst + static_cast<int64_t>(c) * R + k;
+                  for (int j = 0; j < 32; j += 4)  // R % 8 == 0
+                    if (k + j < R && j < kRank)
+                      *reinterpret_cast<uint4*>(p + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)  // R % 8 == 0
-                  if (k + j < R && j < kRank)
-                    *reinterpret_cast<uint4*>(p + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (k + j < R && j < kRank) dst[static_cast<int64_t>(k + j) * C + c] = __uint_as_float(v[j]);
+                  for (int j = 0; j < 32; ++j)
+                    if (k + j < R && j < kRank) dst[static_cast<int64_t>(k + j) * C + c] = __uint_as_float(v[j]);
+                }
               }
             }
           }
+          tc_fence_before();
         }
-        tc_fence_before();
       }
     }
+    ++segment;
+    __syncthreads();  // the accumulators and the list are read
+    if (*abortv) break;
   }
   __syncthreads();
   if (warp == kMmaWarp) {
@@ -592,14 +650,18 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
 
 // ======================================================================== expand
 // out[row, n] = bf16(y[row, n] + c[s] * sum_r h[row, r] W_s[r, n]); y NULL: zero.
-// A block keeps the pieces of h of 128 rows in shared memory and goes through its
-// columns 64 at a time: W_s and y arrive by TMA, the product lies in one of two
-// accumulators, the epilogue adds it to y in place in shared memory and a TMA store
-// takes the tile away.  Three stages, two blocks a multiprocessor: bound by
-// reading y and writing out.
-// A tile whose rows have different adapters (or none) is done adapter by adapter,
-// each storing its own rows only.
+// One block a multiprocessor takes an equal share of all 128 x 64 tiles, row tile by
+// row tile: a segment is its run of columns in one row tile, whose h it keeps as
+// pieces in shared memory.  W_s and y arrive by TMA, seven stages ahead; the
+// products lie in four accumulators; two groups of four warps take the tiles in
+// turn, add the product to y in place in shared memory, and a TMA store takes the
+// tile away.  Bound by reading y and writing out.
+// Three stages and one group of warps, twice a multiprocessor, waited for the loads:
+// 178 us on 11712 x 12288 at rank 64.
+// Every row of a tile keeps the h of its own adapter; a tile whose rows have
+// different ones is multiplied by each adapter's W_s and a row takes its own's.
 constexpr int kERows = 128, kECols = 64;
+constexpr int kEThreads = 320, kETmaWarp = 8, kEMmaWarp = 9;
 template <int kRank>
 struct ExpandTc {
   static constexpr int kBlks = kRank > 64 ? 2 : 1;             // blocks of 64 of the rank
@@ -607,254 +669,291 @@ struct ExpandTc {
   static constexpr int kH = 2 * kBlks * kHBlk;
   static constexpr int kW = kBlks * kECols * 128;              // 8 KB a block, either way round
   static constexpr int kY = kERows * kECols * 2;
-  static constexpr int kStage = kW + kY;
-  static constexpr int kStages = kBlks == 2 ? 4 : 3;
-  static constexpr int kBytes = 1024 + kH + kStages * kStage + 512 + 1024;
+  static constexpr int kYStages = kBlks == 2 ? 6 : 8;
+  static constexpr int kWStages = kBlks == 2 ? 3 : 4;
+  static constexpr int kBytes = 1024 + kH + kYStages * kY + kWStages * kW + 512 + 1024;
+  static_assert(kBytes <= 232448, "shared memory");
 };
 
 template <int kRank, bool kWCols>
-__global__ void __launch_bounds__(kThreads) expand_tc_kernel(
+__global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
     const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_w,
-    const __grid_constant__ CUtensorMap tm_out, const __nv_bfloat16* y, int64_t ldy, __nv_bfloat16* out,
-    int64_t ldo, const float* __restrict__ part, int splits, const float* __restrict__ scaling, Rows rows, int N,
-    int R, int col_parts, int tiles_part) {
+    const __grid_constant__ CUtensorMap tm_out, const __nv_bfloat16* y, __nv_bfloat16* out,
+    const float* __restrict__ part, int splits, const float* __restrict__ scaling, Rows rows, int N,
+    int R) {
   using C = ExpandTc<kRank>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* s_h = smem;
   uint8_t* s_y = s_h + C::kH;
-  uint8_t* s_w = s_y + C::kStages * C::kY;
-  Bars* bars = reinterpret_cast<Bars*>(s_w + C::kStages * C::kW);
-  uint64_t* tfull = bars->ready;       // two accumulators
-  uint64_t* tempty = bars->ready + 2;
+  uint8_t* s_w = s_y + C::kYStages * C::kY;
+  Bars* bars = reinterpret_cast<Bars*>(s_w + C::kWStages * C::kW);
+  uint64_t* y_full = bars->full;       // 8
+  uint64_t* y_empty = bars->empty;     // 8
+  uint64_t* w_full = bars->ready;      // 4
+  uint64_t* w_empty = bars->ready + 4; // 4
+  uint64_t* tfull = bars->acc;         // four accumulators
+  uint64_t* tempty = bars->acc + 4;
   uint64_t* h_there = &bars->done;
   int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
   int* list = id + kERows;
-  __shared__ int count, none;
+  __shared__ int count;
   volatile int* abortv = &bars->abort_flag;
   int* err = &g_lora_error;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x / col_parts) * kERows;
-  const int all_tiles = (N + kECols - 1) / kECols;
-  const int t_lo = static_cast<int>(blockIdx.x % col_parts) * tiles_part, t_hi = min(all_tiles, t_lo + tiles_part);
+  const int col_tiles = (N + kECols - 1) / kECols;
+  const int64_t tiles = (rows.M + kERows - 1) / kERows * col_tiles;
+  const int64_t g_lo = tiles * blockIdx.x / gridDim.x, g_hi = tiles * (blockIdx.x + 1) / gridDim.x;
 
   if (tid == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&bars->full[s], 1);
-      mbar_init(&bars->empty[s], 5);  // the MMAs, and four epilogue warps
+    for (int s = 0; s < C::kYStages; ++s) {
+      mbar_init(&y_full[s], 1);
+      mbar_init(&y_empty[s], 4);  // the four warps that take the tile
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int s = 0; s < C::kWStages; ++s) {
+      mbar_init(&w_full[s], 1);
+      mbar_init(&w_empty[s], 1);
+    }
+    for (int b = 0; b < 4; ++b) {
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 4);
     }
-    mbar_init(h_there, 4);
+    mbar_init(h_there, 8);
     bars->abort_flag = 0;
     fence_mbarrier_init();
-    none = 0;
   }
-  __syncthreads();
-  if (tid < kERows) {
-    const int v = adapter_of(rows, row0 + tid);
-    id[tid] = v;
-    if (v < 0 && row0 + tid < rows.M) none = 1;
-  }
-  if (warp == kTmaWarp && lane == 0) {
+  if (warp == kETmaWarp && lane == 0) {
     tma_prefetch_desc(&tm_y);
     tma_prefetch_desc(&tm_w);
     tma_prefetch_desc(&tm_out);
   }
-  if (warp == kMmaWarp) {
-    tmem_alloc<2 * kECols>(&bars->tmem);
+  if (warp == kEMmaWarp) {
+    tmem_alloc<4 * kECols>(&bars->tmem);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) list_adapters(id, list, count);
-  __syncthreads();
-  const int passes = count;
-  const bool pure = passes == 1 && !none;
   const uint32_t tmem = bars->tmem;
+  uint32_t yt = 0;       // tiles this block has gone through
+  uint32_t wt = 0;       // products (a tile times an adapter)
+  uint32_t h_count = 0;  // times h has been laid down
+  int to_free = -1;      // the stage whose store may still be reading
 
-  if (warp == kTmaWarp) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int li = 0; ok && li < passes; ++li) {
-        for (int t = t_lo; t < t_hi; ++t, ++it) {
-          const int s = static_cast<int>(it % C::kStages);
-          if (!mbar_wait(&bars->empty[s], ((it / C::kStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+  for (int64_t g = g_lo; g < g_hi;) {
+    const int64_t rt = g / col_tiles;
+    const int t_lo = static_cast<int>(g - rt * col_tiles);
+    const int t_hi = static_cast<int>(min(static_cast<int64_t>(col_tiles), t_lo + (g_hi - g)));
+    g += t_hi - t_lo;
+    const int64_t row0 = rt * kERows;
+    // the adapters of the rows; usually one
+    int v = -1;
+    if (tid < kERows) {
+      v = adapter_of(rows, row0 + tid);
+      id[tid] = v;
+    }
+    __syncthreads();
+    const bool one = __syncthreads_and(tid >= kERows || row0 + tid >= rows.M || v == id[0]);
+    if (one) {
+      if (tid == 0) {
+        list[0] = id[0];
+        count = id[0] >= 0 ? 1 : 0;
+      }
+    } else if (warp == 0) {
+      list_adapters(id, list, count);
+    }
+    __syncthreads();
+    const int n = count;
+    if (n == 0 && y == out) continue;  // nothing to add (the ids are not read again)
+
+    if (warp == kETmaWarp) {
+      if (lane == 0) {
+        bool ok = true;
+        for (int t = t_lo; ok && t < t_hi; ++t, ++yt) {
+          const int s = static_cast<int>(yt % C::kYStages);
+          if (!mbar_wait(&y_empty[s], ((yt / C::kYStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
             ok = false;
             break;
           }
-          constexpr uint32_t w_bytes = kWCols ? C::kW : kRank * 128;
-          mbar_arrive_expect_tx(&bars->full[s], w_bytes + (y ? C::kY : 0));
-          uint8_t* w = s_w + s * C::kW;
-          if constexpr (kWCols) {
-#pragma unroll
-            for (int b = 0; b < C::kBlks; ++b)
-              tma_load_3d(w + b * 8192, &tm_w, &bars->full[s], b * 64, t * kECols, list[li]);
+          if (y) {
+            mbar_arrive_expect_tx(&y_full[s], C::kY);
+            tma_load_2d(s_y + s * C::kY, &tm_y, &y_full[s], t * kECols, static_cast<int>(row0));
           } else {
-            tma_load_3d(w, &tm_w, &bars->full[s], t * kECols, 0, list[li]);
+            mbar_arrive(&y_full[s]);
           }
-          if (y) tma_load_2d(s_y + s * C::kY, &tm_y, &bars->full[s], t * kECols, static_cast<int>(row0));
+          for (int li = 0; li < n; ++li, ++wt) {
+            const int ws = static_cast<int>(wt % C::kWStages);
+            if (!mbar_wait(&w_empty[ws], ((wt / C::kWStages) & 1u) ^ 1u, abortv, err, kDevTimeoutEmpty)) {
+              ok = false;
+              break;
+            }
+            constexpr uint32_t w_bytes = kWCols ? C::kW : kRank * 128;
+            mbar_arrive_expect_tx(&w_full[ws], w_bytes);
+            uint8_t* w = s_w + ws * C::kW;
+            if constexpr (kWCols) {
+#pragma unroll
+              for (int b = 0; b < C::kBlks; ++b)
+                tma_load_3d(w + b * 8192, &tm_w, &w_full[ws], b * 64, t * kECols, list[li]);
+            } else {
+              tma_load_3d(w, &tm_w, &w_full[ws], t * kECols, 0, list[li]);
+            }
+          }
+        }
+        if (!ok) {  // let loads already in flight land (bounded)
+          const uint64_t t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 1000000) {
+          }
         }
       }
-      if (!ok) {  // let loads already in flight land (bounded)
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 1000000) {
-        }
-      }
-    }
-  } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16(kECols, 0, kWCols ? 0 : 1);
-      uint32_t it = 0;
-      bool ok = true;
-      for (int li = 0; ok && li < passes; ++li) {
-        if (!mbar_wait(h_there, static_cast<uint32_t>(li) & 1u, abortv, err, kDevTimeoutFull)) break;
-        for (int t = t_lo; t < t_hi; ++t, ++it) {
-          const int s = static_cast<int>(it % C::kStages);
-          const uint32_t acc = it & 1u;
-          if (!mbar_wait(&tempty[acc], ((it >> 1) & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty) ||
-              !mbar_wait(&bars->full[s], (it / C::kStages) & 1u, abortv, err, kDevTimeoutFull)) {
-            ok = false;
+    } else if (warp == kEMmaWarp) {
+      if (lane == 0) {
+        constexpr uint32_t idesc = idesc_bf16(kECols, 0, kWCols ? 0 : 1);
+        bool ok = mbar_wait(h_there, h_count & 1u, abortv, err, kDevTimeoutFull);
+        ++h_count;
+        const uint32_t end = wt + static_cast<uint32_t>(t_hi - t_lo) * static_cast<uint32_t>(n);
+        for (; ok && wt != end; ++wt) {
+          const int ws = static_cast<int>(wt % C::kWStages);
+          const uint32_t acc = wt & 3u;
+          if (!mbar_wait(&tempty[acc], ((wt >> 2) & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty) ||
+              !mbar_wait(&w_full[ws], (wt / C::kWStages) & 1u, abortv, err, kDevTimeoutFull)) {
             break;
           }
           tc_fence_after();
-          const uint32_t h0 = smem_u32(s_h), w0 = smem_u32(s_w + s * C::kW);
+          const uint32_t h0 = smem_u32(s_h), w0 = smem_u32(s_w + ws * C::kW);
 #pragma unroll
           for (int k = 0; k < kRank / 16; ++k) {
             const int blk = k / 4, off = (k % 4) * 32;
-            const uint64_t bd = kWCols ? smem_desc_k_sw128(w0 + blk * 8192 + off) : smem_desc_mn_sw128(w0 + k * 2048, 8192);
+            const uint64_t bd =
+                kWCols ? smem_desc_k_sw128(w0 + blk * 8192 + off) : smem_desc_mn_sw128(w0 + k * 2048, 8192);
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-              mma_bf16(tmem + acc * kECols, smem_desc_k_sw128(h0 + (p * C::kBlks + blk) * C::kHBlk + off), bd, idesc,
-                       (k != 0 || p != 0) ? 1u : 0u);
+              mma_bf16(tmem + acc * kECols, smem_desc_k_sw128(h0 + (p * C::kBlks + blk) * C::kHBlk + off), bd,
+                       idesc, (k != 0 || p != 0) ? 1u : 0u);
             }
           }
-          umma_commit(&bars->empty[s]);
+          umma_commit(&w_empty[ws]);
           umma_commit(&tfull[acc]);
         }
       }
-    }
-  } else {
-    const int r = warp * 32 + lane;
-    const int64_t row = row0 + r;
-    if (!pure && none && y != out) {
-      // rows without an adapter: y as it is (zero without y), a warp a row
-      for (int i = 0; i < 32; ++i) {
-        const int64_t m = row0 + warp * 32 + i;
-        if (id[warp * 32 + i] >= 0 || m >= rows.M) continue;
-        for (int c = t_lo * kECols + lane * 8; c < min(N, t_hi * kECols); c += 256) {  // N % 8 == 0
-          *reinterpret_cast<uint4*>(out + m * ldo + c) =
-              y ? *reinterpret_cast<const uint4*>(y + m * ldy + c) : make_uint4(0, 0, 0, 0);
-        }
-      }
-    }
-    uint32_t it = 0;
-    bool ok = true;
-    int to_free = -1;  // the stage whose store may still be reading
-    for (int li = 0; ok && li < passes; ++li) {
-      const int s_id = list[li];
-      const bool mine = id[r] == s_id;
-      const float mul = scaling ? __ldg(scaling + s_id) : 1.0f;
-      // the row's h as pieces (zero in rows of other adapters); the previous adapter's
-      // products are done, their last accumulator has been read
+    } else {
+      const int quad = warp & 3, group = warp >> 2;
+      const int r = quad * 32 + lane;
+      const int64_t row = row0 + r;
+      const int own = id[r];
+      // the row's h as pieces, a group half of the rank each (zero without an adapter);
+      // the products with the last one are done (see the barrier below)
       const float* p0 = part + row * R;
-#pragma unroll 1
-      for (int c = 0; c < kRank; c += 8) {
-        float v[8] = {};
-        if (mine && c < R) {  // R % 8 == 0
+#pragma unroll 4
+      for (int c = group * (kRank / 2); c < (group + 1) * (kRank / 2); c += 8) {
+        float x[8] = {};
+        if (own >= 0 && c < R) {  // R % 8 == 0
+#pragma unroll 3
           for (int sp = 0; sp < splits; ++sp) {
             const float4* q = reinterpret_cast<const float4*>(p0 + sp * rows.M * R + c);
             const float4 a = __ldg(q), b = __ldg(q + 1);
-            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-            v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+            x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
+            x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
           }
         }
         uint4 piece[2];
         uint32_t* u = reinterpret_cast<uint32_t*>(piece);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float x0 = next_piece(v[2 * j]), x1 = next_piece(v[2 * j + 1]);
+          const float x0 = next_piece(x[2 * j]), x1 = next_piece(x[2 * j + 1]);
           u[j] = pack_bf16(x0, x1);
-          u[4 + j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+          u[4 + j] = pack_bf16(x[2 * j], x[2 * j + 1]);
         }
         const int blk = c >> 6, ch = (c >> 3) & 7;
 #pragma unroll
         for (int p = 0; p < 2; ++p)
-          *reinterpret_cast<uint4*>(s_h + (p * C::kBlks + blk) * C::kHBlk + r * 128 + ((ch ^ (r & 7)) << 4)) = piece[p];
+          *reinterpret_cast<uint4*>(s_h + (p * C::kBlks + blk) * C::kHBlk + r * 128 + ((ch ^ (r & 7)) << 4)) =
+              piece[p];
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(h_there);
-      for (int t = t_lo; t < t_hi; ++t, ++it) {
-        const int s = static_cast<int>(it % C::kStages);
-        const uint32_t acc = it & 1u;
-        const bool there = mbar_wait(&tfull[acc], (it >> 1) & 1u, abortv, err, kDevTimeoutTmemFull) &&
-                           mbar_wait(&bars->full[s], (it / C::kStages) & 1u, abortv, err, kDevTimeoutFull);
+      const float mul = own >= 0 && scaling ? __ldg(scaling + own) : 1.0f;
+      bool ok = true;
+      for (int t = t_lo; ok && t < t_hi; ++t, ++yt, wt += static_cast<uint32_t>(n)) {
+        if (static_cast<int>(yt & 1u) != group) continue;
+        const int s = static_cast<int>(yt % C::kYStages);
+        bool there = mbar_wait(&y_full[s], (yt / C::kYStages) & 1u, abortv, err, kDevTimeoutFull);
         if (!__all_sync(0xffffffffu, there)) {
           ok = false;
           break;
         }
-        tc_fence_after();
-        uint32_t v[2][32];
-        const uint32_t at = tmem + (static_cast<uint32_t>(warp * 32) << 16) + acc * kECols;
-        tmem_ld_32x32b_x32(at, v[0]);
-        tmem_ld_32x32b_x32(at + 32, v[1]);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[acc]);
         uint8_t* yr = s_y + s * C::kY + r * 128;
+        if (!y && own < 0) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint4* cell = reinterpret_cast<uint4*>(yr + ((c ^ (r & 7)) << 4));
-          const uint4 b = y ? *cell : make_uint4(0, 0, 0, 0);
-          const uint32_t w4[4] = {b.x, b.y, b.z, b.w};
-          uint32_t o[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x0 = __uint_as_float(v[c >> 2][(c & 3) * 8 + 2 * j]);
-            const float x1 = __uint_as_float(v[c >> 2][(c & 3) * 8 + 2 * j + 1]);
-            o[j] = pack_bf16(fmaf(mul, x0, __uint_as_float(w4[j] << 16)),
-                             fmaf(mul, x1, __uint_as_float(w4[j] & 0xFFFF0000u)));
-          }
-          const uint4 ov = make_uint4(o[0], o[1], o[2], o[3]);
-          if (pure) {
-            *cell = ov;
-          } else if (mine) {
-            const int col = t * kECols + c * 8;
-            if (col < N) *reinterpret_cast<uint4*>(out + row * ldo + col) = ov;
-          }
+          for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(yr + (c << 4)) = make_uint4(0, 0, 0, 0);
         }
-        if (pure) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (row0 + warp * 32 < rows.M)
-              tma_store_2d(&tm_out, s_y + s * C::kY + warp * 4096, t * kECols, static_cast<int>(row0) + warp * 32);
-            tma_store_commit();
-            if (to_free >= 0) {
-              tma_store_wait_read<1>();  // the tile before this one has left shared memory
-              mbar_arrive(&bars->empty[to_free]);
-            }
-            to_free = s;
+        for (int li = 0; li < n; ++li) {
+          const uint32_t j = wt + static_cast<uint32_t>(li);
+          const uint32_t acc = j & 3u;
+          there = mbar_wait(&tfull[acc], (j >> 2) & 1u, abortv, err, kDevTimeoutTmemFull);
+          if (!__all_sync(0xffffffffu, there)) {
+            ok = false;
+            break;
           }
-        } else {
+          tc_fence_after();
+          uint32_t d[2][32];
+          const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) + acc * kECols;
+          tmem_ld_32x32b_x32(at, d[0]);
+          tmem_ld_32x32b_x32(at + 32, d[1]);
+          tmem_ld_wait();
+          tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->empty[s]);
+          if (lane == 0) mbar_arrive(&tempty[acc]);
+          if (own == list[li]) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint4* cell = reinterpret_cast<uint4*>(yr + ((c ^ (r & 7)) << 4));
+              const uint4 b = y ? *cell : make_uint4(0, 0, 0, 0);
+              const uint32_t w4[4] = {b.x, b.y, b.z, b.w};
+              uint32_t o[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float x0 = __uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * q]);
+                const float x1 = __uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * q + 1]);
+                o[q] = pack_bf16(fmaf(mul, x0, __uint_as_float(w4[q] << 16)),
+                                 fmaf(mul, x1, __uint_as_float(w4[q] & 0xFFFF0000u)));
+              }
+              *cell = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (row0 + quad * 32 < rows.M)
+            tma_store_2d(&tm_out, s_y + s * C::kY + quad * 4096, t * kECols, static_cast<int>(row0) + quad * 32);
+          tma_store_commit();
+          if (to_free >= 0) {
+            tma_store_wait_read<1>();  // this group's tile before has left shared memory
+            mbar_arrive(&y_empty[to_free]);
+          }
+          to_free = s;
         }
       }
+      // both groups have seen the products of all their tiles: h may be replaced
+      named_bar_sync(1, 256);
+      if (lane == 0 && to_free >= 0) {
+        tma_store_wait_read<0>();
+        mbar_arrive(&y_empty[to_free]);
+        to_free = -1;
+      }
     }
-    if (lane == 0) tma_store_wait_all<0>();
+    __syncthreads();  // the segment's ids are read
+    if (*abortv) break;
   }
+  if (warp < kETmaWarp && lane == 0) tma_store_wait_all<0>();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kEMmaWarp) {
     tc_fence_after();
-    tmem_dealloc<2 * kECols>(tmem);
+    tmem_dealloc<4 * kECols>(tmem);
   }
 }
 
@@ -956,7 +1055,7 @@ int tokens_rank(const TokensTcArgs& g, const Rows& rows, cudaStream_t stream) {
   auto k = tokens_tc_kernel<kCodes, kRank, kByCol>;
   constexpr int bytes = TokensTc<kCodes, kRank>::kBytes;
   if (int rc = opt_in(k, bytes)) return rc;
-  const dim3 grid(static_cast<unsigned>((g.C + kTCols - 1) / kTCols), g.splits, static_cast<unsigned>(g.S));
+  const dim3 grid(static_cast<unsigned>((g.C + kTCols - 1) / kTCols), g.splits);
   k<<<grid, kThreads, bytes, stream>>>(tx, th, rows, static_cast<int>(g.C), static_cast<int>(g.R),
                                        static_cast<int>(tiles), g.tiles_split, g.info, g.part, g.found);
   return launched("lora tokens");
@@ -986,17 +1085,10 @@ int expand_rank(const ExpandTcArgs& g, const Rows& rows, cudaStream_t stream) {
   auto k = expand_tc_kernel<kRank, kWCols>;
   constexpr int bytes = ExpandTc<kRank>::kBytes;
   if (int rc = opt_in(k, bytes)) return rc;
-  // one wave of blocks, two a multiprocessor (one at rank 128)
-  const int64_t tiles = (g.M + kERows - 1) / kERows;
-  const int64_t cols = (g.N + kECols - 1) / kECols;
-  const int64_t slots = static_cast<int64_t>(kRank > 64 ? 1 : 2) * device_sm_count();
-  int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cols, slots / tiles));
-  const int64_t per = (cols + parts - 1) / parts;
-  parts = (cols + per - 1) / per;
-  k<<<static_cast<unsigned>(tiles * parts), kThreads, bytes, stream>>>(
-      ty, tw, to, static_cast<const __nv_bfloat16*>(g.y), g.ldy, static_cast<__nv_bfloat16*>(g.out), g.ldo, g.part,
-      g.splits, g.scaling, rows, static_cast<int>(g.N), static_cast<int>(g.R), static_cast<int>(parts),
-      static_cast<int>(per));
+  const int64_t tiles = (g.M + kERows - 1) / kERows * ((g.N + kECols - 1) / kECols);
+  k<<<static_cast<unsigned>(std::min<int64_t>(tiles, device_sm_count())), kEThreads, bytes, stream>>>(
+      ty, tw, to, static_cast<const __nv_bfloat16*>(g.y), static_cast<__nv_bfloat16*>(g.out), g.part,
+      g.splits, g.scaling, rows, static_cast<int>(g.N), static_cast<int>(g.R));
   return launched("lora expand");
 }
 
