@@ -794,11 +794,11 @@ RowSplit tokens_tc_split(int64_t M, int C) {
   return {static_cast<int>((tiles + per - 1) / per), per * kBM};
 }
 int shrink_tc(const LoraArgs& g, const void* x, int64_t ldx, bool codes, const float* x_scale, const void* w,
-              int64_t slot, bool w_rows, int64_t K, const Split& sp, float* part, cudaStream_t stream) {
+              int64_t slot, bool w_rows, int64_t K, const Split& sp, float* part, int* counts, cudaStream_t stream) {
   const int64_t blocks = (g.M + 127) / 128 * sp.count;
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.S, 2ll * device_sm_count() / blocks));
   return lora_shrink_tc({x, codes, ldx, x_scale, w, w_rows, slot, g.M, K, g.S, g.R, sp.count, sp.per / 64,
-                         static_cast<int>(parts), part},
+                         static_cast<int>(parts), part, counts},
                         {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
 }
 
@@ -924,15 +924,17 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
   float* part = static_cast<float*>(g.workspace);
   if (few_rows(g.M)) return add_few_rows<T>(g, rows, part, stream);
   Split sp = shrink_split(g.M, K);
+  int* counts = nullptr;
   if (tc_shape(g) && tc_x(g) && tc_weights(g.a, g.lda, K, g.S)) {
     sp = shrink_tc_split(g.M, K);
-    if (int rc = shrink_tc(g, g.x, g.ldx, false, nullptr, g.a, g.lda, true, K, sp, part, stream)) return rc;
+    counts = reinterpret_cast<int*>(part + sp.count * g.M * g.R);
+    if (int rc = shrink_tc(g, g.x, g.ldx, false, nullptr, g.a, g.lda, true, K, sp, part, counts, stream)) return rc;
   } else if (int rc = shrink<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
                                          static_cast<const T*>(g.a), g.lda, rows, K, R, sp, part, stream)) {
     return rc;
   }
-  if (tc_shape(g) && tc_rows(g.y, g.ldy, 2) && tc_rows(g.out, g.ldo, 2) && tc_weights(g.b, g.ldb, R, g.S)) {
-    return lora_expand_tc({g.y, g.ldy, part, sp.count, g.b, 1, g.ldb, g.scaling, g.out, g.ldo, g.M, g.N, g.S, g.R},
+  if (counts && tc_rows(g.y, g.ldy, 2) && tc_rows(g.out, g.ldo, 2) && tc_weights(g.b, g.ldb, R, g.S)) {
+    return lora_expand_tc({g.y, g.ldy, counts, part, sp.count, g.b, 1, g.ldb, g.scaling, g.out, g.ldo, g.M, g.N, g.S, g.R},
                           {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
   }
   return expand<T, true>(static_cast<const T*>(g.y), g.ldy, part, sp.count,
@@ -943,7 +945,7 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
 struct BackwardPlan {
   Split h, g;
   RowSplit a, b;
-  int64_t off_g, off_a, off_b, off_found, off_pa, off_pb, off_info, bytes;
+  int64_t off_g, off_a, off_b, off_found, off_pa, off_pb, off_info, off_counts, bytes;
 };
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, bool tc) {
   BackwardPlan p;
@@ -961,7 +963,8 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R
   const int64_t pieces = tc ? up(2 * pad_rank(r) * tiles * kBM * 2) : 0;
   p.off_pb = p.off_pa + pieces;
   p.off_info = p.off_pb + pieces;
-  p.bytes = p.off_info + (tc ? up(S * tiles) : 0);
+  p.off_counts = p.off_info + (tc ? up(S * tiles) : 0);
+  p.bytes = p.off_counts + (tc ? up((M + 127) / 128 * 4) : 0);
   return p;
 }
 
@@ -979,18 +982,19 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   float* pb = reinterpret_cast<float*>(ws + p.off_b);
   int* fa = reinterpret_cast<int*>(ws + p.off_found);
   int* fb = fa + p.a.count * g.S;
+  int* counts = reinterpret_cast<int*>(ws + p.off_counts);
   const TX* x = static_cast<const TX*>(g.x);
   const T* dy = static_cast<const T*>(g.y);
   const T* a = static_cast<const T*>(g.a);
   const T* b = static_cast<const T*>(g.b);
   if (g.M > 0) {
     if (tc) {
-      if (int rc = shrink_tc(g, dy, g.ldy, false, nullptr, b, g.ldb, false, N, p.g, pg, stream)) return rc;
+      if (int rc = shrink_tc(g, dy, g.ldy, false, nullptr, b, g.ldb, false, N, p.g, pg, counts, stream)) return rc;
     } else if (int rc = shrink<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, rows, N, R, p.g, pg, stream)) {
       return rc;
     }
     if (g.out && tc && tc_rows(g.out, g.ldo, 2)) {
-      if (int rc = lora_expand_tc({g.accumulate ? g.out : nullptr, g.ldo, pg, p.g.count, a, 0, g.lda, g.scaling,
+      if (int rc = lora_expand_tc({g.accumulate ? g.out : nullptr, g.ldo, counts, pg, p.g.count, a, 0, g.lda, g.scaling,
                                    g.out, g.ldo, g.M, g.K, g.S, g.R},
                                   {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream)) {
         return rc;
@@ -1008,7 +1012,7 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
     const LoraRows lr{g.adapter, g.adapter64, g.rows_per_index, g.M, g.S};
     void *qa = ws + p.off_pa, *qb = ws + p.off_pb;
     uint8_t* info = ws + p.off_info;
-    if (int rc = shrink_tc(g, x, g.ldx, g.x_scale != nullptr, g.x_scale, a, g.lda, true, K, p.h, ph, stream)) return rc;
+    if (int rc = shrink_tc(g, x, g.ldx, g.x_scale != nullptr, g.x_scale, a, g.lda, true, K, p.h, ph, counts, stream)) return rc;
     if (int rc = lora_rank_pieces({pg, p.g.count, g.x_scale, qa, ph, p.h.count, qb, g.scaling, R, info}, lr, stream)) {
       return rc;
     }
@@ -1048,7 +1052,9 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
 int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, int backward) {
   // either form of the kernels may run: which one depends on pointers and strides too
   const int k = static_cast<int>(K);
-  if (!backward) return up(std::max(shrink_split(M, k).count, shrink_tc_split(M, k).count) * M * R * 4);
+  if (!backward) {
+    return up(std::max(shrink_split(M, k).count, shrink_tc_split(M, k).count) * M * R * 4 + (M + 127) / 128 * 4);
+  }
   return std::max(backward_plan(M, N, K, S, R, false).bytes,
                   M >= kTcRows ? backward_plan(M, N, K, S, R, true).bytes : 0);
 }

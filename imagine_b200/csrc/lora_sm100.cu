@@ -122,11 +122,20 @@ __device__ __forceinline__ void list_adapters(const int* id, int* list, int& cou
   if (lane == 0) count = n;
 }
 
+// After a wait that gave up: copies already in flight land first (bounded).
+__device__ __forceinline__ void let_copies_land() {
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 1000000) {
+  }
+}
+
 struct Bars {
-  uint64_t full[8], ready[8], empty[8], acc[8], done, drained;
+  uint64_t full[16], ready[16], empty[16], acc[8], w_full[16], w_empty[16], done, drained;
   uint32_t tmem;
   int abort_flag;
 };
+constexpr int kBarBytes = 768;
+static_assert(sizeof(Bars) <= kBarBytes, "barriers");
 
 // ======================================================================== shrink
 // A tile whose rows have several adapters is multiplied by each of them while it is
@@ -139,7 +148,7 @@ struct ShrinkTc {
   static constexpr int kRaw = kCodes ? kSRows * kSK : 0;
   static constexpr int kWStages = kRank == 128 ? 2 : kCodes ? 2 : 4;
   static constexpr int kXStages = kCodes ? 3 : 4;
-  static constexpr int kBytes = 1024 + kXStages * (kXTile + kRaw) + kWStages * kW + 512 + 1280;
+  static constexpr int kBytes = 1024 + kXStages * (kXTile + kRaw) + kWStages * kW + kBarBytes + 1280;
   static constexpr uint32_t kCols = 256;                  // accumulator columns a block takes
   static constexpr int kAtOnce = static_cast<int>(kCols) / kRank;
   static_assert(2 * kBytes + 2048 <= 228 * 1024, "two blocks a multiprocessor");
@@ -150,7 +159,8 @@ struct ShrinkTc {
 template <bool kCodes, int kRank, bool kWRows>
 __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
     const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, Rows rows,
-    const float* __restrict__ row_mul, int K, int R, int kb_split, float* __restrict__ part) {
+    const float* __restrict__ row_mul, int K, int R, int kb_split, float* __restrict__ part,
+    int* __restrict__ counts) {
   using C = ShrinkTc<kCodes, kRank>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -161,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   Bars* bars = reinterpret_cast<Bars*>(s_raw + C::kXStages * C::kRaw);
   uint64_t* w_full = bars->full + 4;
   uint64_t* w_empty = bars->empty + 4;
-  int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
+  int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + kBarBytes);
   int* list = id + kSRows;
   __shared__ int count;
   volatile int* abortv = &bars->abort_flag;
@@ -214,6 +224,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   }
   __syncthreads();
   const int total = count;
+  if (tid == 0 && blockIdx.y == 0 && blockIdx.z == 0) counts[blockIdx.x] = total;  // for expand_tc_kernel
   const uint32_t tmem = bars->tmem;
   // this block's adapters of the tile: those from blockIdx.z on, gridDim.z apart, kAtOnce a pass
   const int mine_n = total > static_cast<int>(blockIdx.z) ? (total - blockIdx.z + gridDim.z - 1) / gridDim.z : 0;
@@ -253,11 +264,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
           }
         }
       }
-      if (!ok) {  // let loads already in flight land (bounded)
-        const uint64_t t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 1000000) {
-        }
-      }
+      if (!ok) let_copies_land();
     }
   } else if (warp == kMmaWarp) {
     if (lane == 0) {
@@ -389,24 +396,52 @@ __global__ void __launch_bounds__(256) rank_pieces_kernel(RankSide a, RankSide b
   const RankSide g = blockIdx.y ? b : a;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kTile;
   tile_ids(rows, row0, ids);
-  for (int i = threadIdx.x; i < kTile * kRank; i += 256) {
-    const int r = i / kRank, c = i % kRank;
-    float sum = 0.0f;
-    if (ids.id[r] >= 0 && c < R) {
+  constexpr int kVecs = kRank / 4;
+  constexpr int kEach = kTile * kVecs / 256;  // 1 .. 8 vectors a thread
+  const int64_t plane = rows.M * R;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int at = threadIdx.x + i * 256;
+    const int r = at / kVecs, c = (at % kVecs) * 4;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int own = ids.id[r];
+    if (own >= 0 && c < R) {  // R % 8 == 0
       const float* p = g.part + (row0 + r) * R + c;
-      for (int sp = 0; sp < g.splits; ++sp) sum += __ldg(p + sp * rows.M * R);
-      if (scaling) sum *= __ldg(scaling + ids.id[r]);
-      if (g.row_mul) sum *= __ldg(g.row_mul + row0 + r);
+#pragma unroll 4
+      for (int sp = 0; sp < g.splits; ++sp) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(p + sp * plane));
+        sum.x += q.x;
+        sum.y += q.y;
+        sum.z += q.z;
+        sum.w += q.w;
+      }
+      float mul = scaling ? __ldg(scaling + own) : 1.0f;
+      if (g.row_mul) mul *= __ldg(g.row_mul + row0 + r);
+      sum.x *= mul;
+      sum.y *= mul;
+      sum.z *= mul;
+      sum.w *= mul;
     }
-    v[r][c] = sum;
+    v[r][c] = sum.x;
+    v[r][c + 1] = sum.y;
+    v[r][c + 2] = sum.z;
+    v[r][c + 3] = sum.w;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kRank * (kTile / 2); i += 256) {
-    const int c = i / (kTile / 2), r = (i % (kTile / 2)) * 2;
-    float x = v[r][c], y = v[r + 1][c];
-    const float x0 = next_piece(x), y0 = next_piece(y);
-    *reinterpret_cast<uint32_t*>(g.out + c * m_pad + row0 + r) = pack_bf16(x0, y0);
-    *reinterpret_cast<uint32_t*>(g.out + (kRank + c) * m_pad + row0 + r) = pack_bf16(x, y);
+#pragma unroll
+  for (int i = threadIdx.x; i < kRank * (kTile / 8); i += 256) {
+    const int c = i / (kTile / 8), r = (i % (kTile / 8)) * 8;
+    uint4 first, second;
+    uint32_t *f = reinterpret_cast<uint32_t*>(&first), *s = reinterpret_cast<uint32_t*>(&second);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x = v[r + 2 * j][c], y = v[r + 2 * j + 1][c];
+      const float x0 = next_piece(x), y0 = next_piece(y);
+      f[j] = pack_bf16(x0, y0);
+      s[j] = pack_bf16(x, y);
+    }
+    *reinterpret_cast<uint4*>(g.out + c * m_pad + row0 + r) = first;
+    *reinterpret_cast<uint4*>(g.out + (kRank + c) * m_pad + row0 + r) = second;
   }
   if (blockIdx.y == 0) {
     for (int s = threadIdx.x; s < rows.S; s += 256) {
@@ -428,9 +463,9 @@ struct TokensTc {
   static constexpr int kH = 2 * kRank * kTile * 2;
   static constexpr int kRaw = kCodes ? kTile * kTCols : 0;
   static constexpr int kStage = kX + kH + kRaw;
-  static constexpr int kStagesRaw = (227 * 1024 - 1024 - 512 - kTilesMost) / kStage;
+  static constexpr int kStagesRaw = (227 * 1024 - 1024 - kBarBytes - kTilesMost) / kStage;
   static constexpr int kStages = kStagesRaw > 6 ? 6 : kStagesRaw;
-  static constexpr int kBytes = 1024 + kStages * kStage + 512 + kTilesMost;
+  static constexpr int kBytes = 1024 + kStages * kStage + kBarBytes + kTilesMost;
   static_assert(kStages >= 2 && kH % 1024 == 0, "tiles");
 };
 
@@ -442,8 +477,8 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
     int tiles, int tiles_split, const uint8_t* __restrict__ info, float* __restrict__ part,
     int* __restrict__ found) {
   using T = TokensTc<kCodes, kRank>;
-  // two accumulators of kRank columns, read 32 columns at a time
-  constexpr uint32_t kTokenCols = tmem_cols(kRank < 32 ? 64 : 2 * kRank);
+  // two accumulators of 2 kRank columns (the sums with the first pieces, then the second)
+  constexpr uint32_t kTokenCols = 4 * kRank;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -451,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
   uint8_t* s_h = s_x + T::kStages * T::kX;
   uint8_t* s_raw = s_h + T::kStages * T::kH;
   Bars* bars = reinterpret_cast<Bars*>(s_raw + T::kStages * T::kRaw);
-  uint8_t* live = reinterpret_cast<uint8_t*>(bars) + 512;
+  uint8_t* live = reinterpret_cast<uint8_t*>(bars) + kBarBytes;
   __shared__ uint8_t present[kAdaptersMost];
   volatile int* abortv = &bars->abort_flag;
   int* err = &g_lora_error;
@@ -521,15 +556,11 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
           tma_load_2d(s_h + st * T::kH, &tm_h, &bars->full[st], m, 0);
           ++it;
         }
-        if (!ok) {  // let loads already in flight land (bounded)
-          const uint64_t t0 = globaltimer_ns();
-          while (globaltimer_ns() - t0 < 1000000) {
-          }
-        }
+        if (!ok) let_copies_land();
       }
     } else if (warp == kMmaWarp) {
       if (lane == 0) {
-        constexpr uint32_t idesc = idesc_bf16(kRank, 1, 0);
+        constexpr uint32_t idesc = idesc_bf16(2 * kRank, 1, 0);
         bool ok = true, first = true;
         for (int t = 0; t < n_tiles; ++t) {
           if (!live[t]) continue;
@@ -546,9 +577,9 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
           for (int blk = 0; blk < 2; ++blk) {
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k) {
-              const uint64_t ad = smem_desc_mn_sw128(a0 + blk * 16384 + k * 2048, 8192);
-              mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + k * 32), idesc, (!first || k != 0) ? 1u : 0u);
-              mma_bf16(tmem + blk * kRank, ad, smem_desc_k_sw128(b0 + kRank * 128 + k * 32), idesc, 1u);
+              // both pieces side by side: the columns are read once for them
+              mma_bf16(tmem + blk * 2 * kRank, smem_desc_mn_sw128(a0 + blk * 16384 + k * 2048, 8192),
+                       smem_desc_k_sw128(b0 + k * 32), idesc, (!first || k != 0) ? 1u : 0u);
             }
           }
           umma_commit(&bars->empty[st]);
@@ -614,10 +645,17 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
             const int c = col0 + blk * 128 + warp * 32 + lane;
 #pragma unroll
             for (int k = 0; k < kRank; k += 32) {
-              uint32_t v[32];
+              uint32_t v[32], w[32];
               __syncwarp();
-              tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + blk * kRank + k, v);
+              const uint32_t at = tmem + (static_cast<uint32_t>(warp * 32) << 16) + blk * 2 * kRank + k;
+              tmem_ld_32x32b_x32(at, v);
+              if constexpr (kRank >= 32) tmem_ld_32x32b_x32(at + kRank, w);
               tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const uint32_t second = kRank >= 32 ? w[j] : v[(j + 16) & 31];
+                v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(second));
+              }
               if (c < C) {
                 if constexpr (kByCol) {
                   float* p = dst + static_cast<int64_t>(c) * R + k;
@@ -651,7 +689,8 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
 // ======================================================================== expand
 // out[row, n] = bf16(y[row, n] + c[s] * sum_r h[row, r] W_s[r, n]); y NULL: zero.
 // One block a multiprocessor takes an equal share of all 128 x 64 tiles, row tile by
-// row tile: a segment is its run of columns in one row tile, whose h it keeps as
+// row tile, a tile counted as often as it takes (its adapters are counted by the
+// shrink kernel): a segment is its run of columns in one row tile, whose h it keeps as
 // pieces in shared memory.  W_s and y arrive by TMA, seven stages ahead; the
 // products lie in four accumulators; two groups of four warps take the tiles in
 // turn, add the product to y in place in shared memory, and a TMA store takes the
@@ -671,15 +710,19 @@ struct ExpandTc {
   static constexpr int kY = kERows * kECols * 2;
   static constexpr int kYStages = kBlks == 2 ? 6 : 8;
   static constexpr int kWStages = kBlks == 2 ? 3 : 4;
-  static constexpr int kBytes = 1024 + kH + kYStages * kY + kWStages * kW + 512 + 1024;
+  static constexpr int kBytes = 1024 + kH + kYStages * kY + kWStages * kW + kBarBytes + 1024;
   static_assert(kBytes <= 232448, "shared memory");
 };
+
+// What a tile of rows with so many adapters costs: a second product takes the thread
+// that issues them 1100 cycles, where HBM needs 1260 for the tile.
+__device__ __forceinline__ int tile_cost(int adapters) { return adapters <= 1 ? 4 : 3 * adapters + 1; }
 
 template <int kRank, bool kWCols>
 __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
     const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_w,
     const __grid_constant__ CUtensorMap tm_out, const __nv_bfloat16* y, __nv_bfloat16* out,
-    const float* __restrict__ part, int splits, const float* __restrict__ scaling, Rows rows, int N,
+    const int* __restrict__ counts, const float* __restrict__ part, int splits, const float* __restrict__ scaling, Rows rows, int N,
     int R) {
   using C = ExpandTc<kRank>;
   extern __shared__ uint8_t smem_raw[];
@@ -696,16 +739,15 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   uint64_t* tfull = bars->acc;         // four accumulators
   uint64_t* tempty = bars->acc + 4;
   uint64_t* h_there = &bars->done;
-  int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 512);
+  int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + kBarBytes);
   int* list = id + kERows;
   __shared__ int count;
+  __shared__ int64_t scan[kEThreads / 32], share[2], start_tile, start_at;
   volatile int* abortv = &bars->abort_flag;
   int* err = &g_lora_error;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int col_tiles = (N + kECols - 1) / kECols;
-  const int64_t tiles = (rows.M + kERows - 1) / kERows * col_tiles;
-  const int64_t g_lo = tiles * blockIdx.x / gridDim.x, g_hi = tiles * (blockIdx.x + 1) / gridDim.x;
-
+  const int64_t row_tiles = (rows.M + kERows - 1) / kERows;
   if (tid == 0) {
     for (int s = 0; s < C::kYStages; ++s) {
       mbar_init(&y_full[s], 1);
@@ -741,11 +783,53 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   uint32_t h_count = 0;  // times h has been laid down
   int to_free = -1;      // the stage whose store may still be reading
 
-  for (int64_t g = g_lo; g < g_hi;) {
-    const int64_t rt = g / col_tiles;
-    const int t_lo = static_cast<int>(g - rt * col_tiles);
-    const int t_hi = static_cast<int>(min(static_cast<int64_t>(col_tiles), t_lo + (g_hi - g)));
-    g += t_hi - t_lo;
+  // this block's share [lo, hi) of the whole cost, and the row tile it starts in: a
+  // thread adds up a run of row tiles, a scan over the block gives the run's start
+  {
+    const int64_t run = (row_tiles + kEThreads - 1) / kEThreads;
+    const int64_t first = min(row_tiles, tid * run), last = min(row_tiles, first + run);
+    int64_t mine = 0;
+    for (int64_t i = first; i < last; ++i) mine += tile_cost(__ldg(counts + i));
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    if (lane == 31) scan[warp] = upto;
+    __syncthreads();
+    int64_t before = upto - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kEThreads / 32; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    total *= col_tiles;
+    const int64_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+    int64_t at = before * col_tiles;
+    for (int64_t i = first; i < last; ++i) {
+      const int64_t end = at + static_cast<int64_t>(tile_cost(__ldg(counts + i))) * col_tiles;
+      if (lo >= at && lo < end) {
+        start_tile = i;
+        start_at = at;
+      }
+      at = end;
+    }
+    if (tid == 0) {
+      share[0] = lo;
+      share[1] = hi;
+    }
+  }
+  __syncthreads();
+  const int64_t lo = share[0], hi = share[1];
+  int64_t at = start_at;
+  for (int64_t rt = start_tile; rt < row_tiles && at < hi; ++rt) {
+    // the row tile's tiles that start in the share
+    const int64_t cost = tile_cost(__ldg(counts + rt));
+    const int t_lo = static_cast<int>(lo <= at ? 0 : min(static_cast<int64_t>(col_tiles), (lo - at + cost - 1) / cost));
+    const int t_hi = static_cast<int>(min(static_cast<int64_t>(col_tiles), (hi - at + cost - 1) / cost));
+    at += cost * col_tiles;
+    if (t_lo >= t_hi) continue;
     const int64_t row0 = rt * kERows;
     // the adapters of the rows; usually one
     int v = -1;
@@ -800,11 +884,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
             }
           }
         }
-        if (!ok) {  // let loads already in flight land (bounded)
-          const uint64_t t0 = globaltimer_ns();
-          while (globaltimer_ns() - t0 < 1000000) {
-          }
-        }
+        if (!ok) let_copies_land();
       }
     } else if (warp == kEMmaWarp) {
       if (lane == 0) {
@@ -895,6 +975,10 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
           if (!__all_sync(0xffffffffu, there)) {
             ok = false;
             break;
+          }
+          if (!__any_sync(0xffffffffu, own == list[li])) {  // none of these 32 rows
+            if (lane == 0) mbar_arrive(&tempty[acc]);
+            continue;
           }
           tc_fence_after();
           uint32_t d[2][32];
@@ -1029,7 +1113,7 @@ int shrink_rank(const ShrinkTcArgs& g, const Rows& rows, cudaStream_t stream) {
   if (int rc = opt_in(k, bytes)) return rc;
   const dim3 grid(static_cast<unsigned>((g.M + kSRows - 1) / kSRows), g.splits, g.parts);
   k<<<grid, kThreads, bytes, stream>>>(tx, tw, rows, g.x_scale, static_cast<int>(g.K), static_cast<int>(g.R),
-                                       g.kb_split, g.part);
+                                       g.kb_split, g.part, g.counts);
   return launched("lora shrink");
 }
 
@@ -1087,7 +1171,7 @@ int expand_rank(const ExpandTcArgs& g, const Rows& rows, cudaStream_t stream) {
   if (int rc = opt_in(k, bytes)) return rc;
   const int64_t tiles = (g.M + kERows - 1) / kERows * ((g.N + kECols - 1) / kECols);
   k<<<static_cast<unsigned>(std::min<int64_t>(tiles, device_sm_count())), kEThreads, bytes, stream>>>(
-      ty, tw, to, static_cast<const __nv_bfloat16*>(g.y), static_cast<__nv_bfloat16*>(g.out), g.part,
+      ty, tw, to, static_cast<const __nv_bfloat16*>(g.y), static_cast<__nv_bfloat16*>(g.out), g.counts, g.part,
       g.splits, g.scaling, rows, static_cast<int>(g.N), static_cast<int>(g.R));
   return launched("lora expand");
 }

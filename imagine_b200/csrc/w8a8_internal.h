@@ -199,10 +199,12 @@ struct ShrinkTcArgs {
   int64_t M, K, S, R;
   int splits, kb_split, parts;
   float* part;
+  int* counts;    // out: the adapters of every 128 rows
 };
 struct ExpandTcArgs {
   const void* y;  // or NULL
   int64_t ldy;
+  const int* counts;  // from the shrink
   const float* part;
   int splits;
   const void* w;
