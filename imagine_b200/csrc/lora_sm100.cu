@@ -53,8 +53,9 @@ int read_and_clear_lora_error(cudaStream_t stream, int* value) {
 
 namespace {
 
-constexpr int kThreads = 192;  // warps 0-3: widen, mask, epilogue; 4: TMA; 5: MMA
-constexpr int kTmaWarp = 4, kMmaWarp = 5;
+// warps 0-7: widen codes, mask (0-3 also the epilogue); 8: TMA; 9: MMA
+constexpr int kThreads = 320;
+constexpr int kTmaWarp = 8, kMmaWarp = 9;
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* map, uint64_t* bar, int x, int y, int z) {
   asm volatile(
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   if (tid == 0) {
     for (int s = 0; s < C::kXStages; ++s) {
       mbar_init(&bars->full[s], 1);
-      mbar_init(&bars->ready[s], 4);
+      mbar_init(&bars->ready[s], 8);
       mbar_init(&bars->empty[s], 1);
     }
     for (int s = 0; s < C::kWStages; ++s) {
@@ -323,8 +324,8 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
           const uint8_t* raw = s_raw + s * C::kRaw;
           uint8_t* x = s_x + s * kXTile;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = (tid >> 2) + 32 * i, c = tid & 3;
+          for (int i = 0; i < 2; ++i) {
+            const int r = (tid >> 2) + 64 * i, c = tid & 3;
             uint4 lo8, hi8;
             widen16(*reinterpret_cast<const uint4*>(raw + r * 64 + c * 16), lo8, hi8);
             *reinterpret_cast<uint4*>(x + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = lo8;
@@ -336,6 +337,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
         }
         if (!ok) break;
       }
+      if (warp >= 4) continue;
       const bool there = mbar_wait(&bars->done, pass & 1u, abortv, err, kDevTimeoutTmemFull);
       if (!__all_sync(0xffffffffu, there)) break;
       tc_fence_after();
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
   if (tid == 0) {
     for (int i = 0; i < T::kStages; ++i) {
       mbar_init(&bars->full[i], 1);
-      mbar_init(&bars->ready[i], 4);
+      mbar_init(&bars->ready[i], 8);
       mbar_init(&bars->empty[i], 1);
     }
     mbar_init(&bars->done, 1);
@@ -605,8 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
           // 64 rows x 256 codes: 16 neighbours a row
           const uint8_t* raw = s_raw + st * T::kRaw;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = (tid >> 4) + 8 * i, c = tid & 15;  // 16 codes of the box c / 4
+          for (int i = 0; i < 4; ++i) {
+            const int r = (tid >> 4) + 16 * i, c = tid & 15;  // 16 codes of the box c / 4
             uint4 lo8, hi8;
             widen16(*reinterpret_cast<const uint4*>(raw + r * kTCols + c * 16), lo8, hi8);
             uint8_t* row = x + (c >> 2) * 8192 + r * 128;
@@ -618,15 +620,14 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
         if (f == 1) {
           // rows of other adapters (whatever they hold) leave the products: their
           // values and their rank side are zeroed
-          const int r = tid & 63, half = tid >> 6;
+          const int r = tid & 63, quarter = tid >> 6;
           if (adapter_of(rows, m0 + r) != s) {
             if (!kCodes) {
-              for (int c = half * 2; c < half * 2 + 2; ++c)
-                for (int q = 0; q < 8; ++q)
-                  *reinterpret_cast<uint4*>(x + c * 8192 + r * 128 + q * 16) = make_uint4(0, 0, 0, 0);
+              for (int q = 0; q < 8; ++q)
+                *reinterpret_cast<uint4*>(x + quarter * 8192 + r * 128 + q * 16) = make_uint4(0, 0, 0, 0);
             }
             uint8_t* h = s_h + st * T::kH;
-            for (int k = half * kRank; k < (half + 1) * kRank; ++k)
+            for (int k = quarter * (kRank / 2); k < (quarter + 1) * (kRank / 2); ++k)
               *reinterpret_cast<uint16_t*>(h + k * 128 + (((r >> 3) ^ (k & 7)) << 4) + (r & 7) * 2) = 0;
           }
         }
@@ -635,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
         if (lane == 0) mbar_arrive(&bars->ready[st]);
         ++it;
       }
-      if (ok) {
+      if (ok && warp < 4) {
         const bool there = mbar_wait(&bars->done, segment & 1u, abortv, err, kDevTimeoutTmemFull);
         if (__all_sync(0xffffffffu, there)) {
           tc_fence_after();
