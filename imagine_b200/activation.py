@@ -47,9 +47,10 @@ def act_checkpoint_int8(x: torch.Tensor, act: str = "gelu_tanh"):
     x2, ldx = _rows(x)
     lead, dtype = x.shape[:-1], x.dtype
     code_t = _code(dtype)
-    y = torch.empty((*lead, k), dtype=dtype, device=dev)
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty((*lead, halves * _groups(k)), dtype=torch.float32, device=dev)
+    whole = x2 is x  # contiguous: the results may be made like it
+    y = torch.empty_like(x) if whole and halves == 1 else x.new_empty((*lead, k))
+    q = torch.empty_like(x, dtype=torch.int8) if whole else x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty((*lead, halves * _groups(k)), dtype=torch.float32)
     with _on(dev):
         N.check(N.LIB.w8a8_act_checkpoint(x2.data_ptr(), code_t, ldx, math.prod(lead), k, code, y.data_ptr(),
                                           q.data_ptr(), scale.data_ptr(), _raw_stream(dev.index)))
@@ -76,7 +77,7 @@ def act_backward_int8(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
         q = q.contiguous()
     if not scale.is_contiguous():
         scale = scale.contiguous()
-    dx = torch.empty(q.shape, dtype=dtype, device=dev)
+    dx = torch.empty_like(q, dtype=dtype)
     with _on(dev):
         N.check(N.LIB.w8a8_act_backward(dy2.data_ptr(), code_t, lddy, math.prod(lead), k, code, q.data_ptr(),
                                         scale.data_ptr(), dx.data_ptr(), _raw_stream(dev.index)))

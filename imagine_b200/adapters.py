@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -130,8 +131,22 @@ def _scaling(scaling, s: int, dev):
     return scaling if scaling.is_contiguous() else scaling.contiguous()
 
 
-def _workspace(nbytes: int, dev):
+# Workspace sizes: functions of the shape and the device alone (current when they are asked for).
+@functools.lru_cache(maxsize=4096)
+def _lora_bytes(device: int, m: int, n: int, k: int, s: int, r: int, backward: int) -> int:
+    nbytes = N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, backward)
     N.check(nbytes if nbytes < 0 else 0)
+    return nbytes
+
+
+@functools.lru_cache(maxsize=4096)
+def _input_grad_bytes(device: int, m: int, n: int, k: int, code: int) -> int:
+    nbytes = N.LIB.w8a8_input_grad_workspace_bytes(m, n, k, code)
+    N.check(nbytes if nbytes < 0 else 0)
+    return nbytes
+
+
+def _workspace(nbytes: int, dev):
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
@@ -167,11 +182,11 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     idx, idx64, per = _index(adapter, lead, m, dev)
     c = _scaling(scaling, s, dev)
     if out is None:
-        out, ldo = torch.empty(y.shape, dtype=dtype, device=dev), max(n, 1)
+        out, ldo = (torch.empty_like(y) if y2 is y else y.new_empty(y.shape)), max(n, 1)
     else:
         ldo = _out_rows("out", out, y.shape, dtype, dev)
     with _on(dev):
-        nbytes = N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 0)
+        nbytes = _lora_bytes(dev.index, m, n, k, s, r, 0)
         ws = _workspace(nbytes, dev)
         N.check(N.LIB.w8a8_lora_add(
             y2.data_ptr(), ldy, x2.data_ptr(), ldx, code, a.data_ptr(), slot_a, b.data_ptr(), slot_b,
@@ -217,15 +232,15 @@ def lora_backward(dy: torch.Tensor, x: Optional[torch.Tensor], a: torch.Tensor, 
     if not need_dx:
         dx = None
     elif dx is None:
-        dx = torch.empty((*lead, k), dtype=dtype, device=dev)
+        dx = dy.new_empty((*lead, k))
     else:
         lddx, accumulate = _out_rows("dx", dx, (*lead, k), dtype, dev), 1
     da = db = None
     if need_weights:
-        da = torch.empty((s, r, k), dtype=dtype, device=dev)
-        db = torch.empty((s, n, r), dtype=dtype, device=dev)
+        da = torch.empty_like(a) if slot_a == r * k else dy.new_empty((s, r, k))
+        db = torch.empty_like(b) if slot_b == n * r else dy.new_empty((s, n, r))
     with _on(dev):
-        nbytes = N.LIB.w8a8_lora_workspace_bytes(m, n, k, s, r, 1)
+        nbytes = _lora_bytes(dev.index, m, n, k, s, r, 1)
         ws = _workspace(nbytes, dev)
         N.check(N.LIB.w8a8_lora_backward(
             dy2.data_ptr(), lddy, _ptr(x2), ldx, _ptr(xs), code, a.data_ptr(), slot_a, b.data_ptr(),
@@ -260,9 +275,9 @@ def int8_linear_backward(dy: torch.Tensor, weight: torch.Tensor, weight_scale: t
     w2, ldw = _rows(weight)
     lead = dy.shape[:-1]
     m = math.prod(lead)
-    dx = torch.empty((*lead, k), dtype=dy.dtype, device=dev)
+    dx = dy.new_empty((*lead, k))
     with _on(dev):
-        nbytes = N.LIB.w8a8_input_grad_workspace_bytes(m, n, k, code)
+        nbytes = _input_grad_bytes(dev.index, m, n, k, code)
         work = _workspace(nbytes, dev)
         N.check(N.LIB.w8a8_input_grad(
             dy2.data_ptr(), lddy, w2.data_ptr(), ldw, ws.data_ptr(), ws.numel(), code, dx.data_ptr(),

@@ -63,11 +63,24 @@ struct ShrinkTile {
   static constexpr int kBytes = kBytes0 > kJoin ? kBytes0 : kJoin;
 };
 
+template <typename TX, typename TW>
+struct ShrinkArgs {
+  const TX* x;
+  int64_t ldx;
+  const float* xs;
+  const TW* w;
+  int64_t slot;
+  int K, k_split, vec_x, vec_w;
+  float* part;
+};
 template <typename TX, typename TW, int kRank, bool kWRows>
-__global__ void __launch_bounds__(kThreads) shrink_kernel(
-    const TX* __restrict__ x, int64_t ldx, const float* __restrict__ xs, const TW* __restrict__ w,
-    int64_t slot, Rows rows, int K, int R, int k_split, int vec_x, int vec_w,
-    float* __restrict__ part) {
+__device__ __forceinline__ void shrink_tile(const ShrinkArgs<TX, TW>& g, const Rows& rows, int R, int split) {
+  const TX* __restrict__ x = g.x;
+  const TW* __restrict__ w = g.w;
+  const float* __restrict__ xs = g.xs;
+  float* __restrict__ part = g.part;
+  const int64_t ldx = g.ldx, slot = g.slot;
+  const int K = g.K, k_split = g.k_split, vec_x = g.vec_x, vec_w = g.vec_w;
   using Tile = ShrinkTile<TX, TW, kRank, kWRows>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ TileIds ids;
@@ -76,7 +89,7 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wm = warp & 3, wk = warp >> 2;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kBM;
-  const int k_lo = blockIdx.y * k_split;
+  const int k_lo = split * k_split;
   const int k_hi = min(K, k_lo + k_split);
   tile_ids(rows, row0, ids);
 
@@ -195,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(
         if (ids.id[r] != s) continue;
         const int64_t row = row0 + r;
         const float sc = xs ? __ldg(xs + row) : 1.0f;
-        float* dst = part + (static_cast<int64_t>(blockIdx.y) * rows.M + row) * R;
+        float* dst = part + (static_cast<int64_t>(split) * rows.M + row) * R;
 #pragma unroll
         for (int n = 0; n < kRank / 8; ++n) {
           const int c = n * 8 + c0;
@@ -205,6 +218,21 @@ __global__ void __launch_bounds__(kThreads) shrink_kernel(
         }
       }
     }
+  }
+}
+
+template <typename TX, typename TW, int kRank, bool kWRows>
+__global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs<TX, TW> g, Rows rows, int R) {
+  shrink_tile<TX, TW, kRank, kWRows>(g, rows, R, blockIdx.y);
+}
+// dy times B and x times A in one launch: blockIdx.y below `first` is the former.
+template <typename TX, typename T, int kRank>
+__global__ void __launch_bounds__(kThreads) shrink_pair_kernel(ShrinkArgs<T, T> dy, ShrinkArgs<TX, T> x, int first,
+                                                               Rows rows, int R) {
+  if (static_cast<int>(blockIdx.y) < first) {
+    shrink_tile<T, T, kRank, false>(dy, rows, R, blockIdx.y);
+  } else {
+    shrink_tile<TX, T, kRank, true>(x, rows, R, blockIdx.y - first);
   }
 }
 
@@ -538,20 +566,40 @@ struct TokensTile {
   static constexpr int kBytes = 2 * (kPX * kXPlane + kPH * kHPlane);
 };
 
+template <typename TX>
+struct TokensArgs {
+  const TX* x;
+  int64_t ldx;
+  const float* row_mul;
+  const float* rank_part;
+  int splits;           // of the rank side
+  int C;
+  int64_t rows_split;
+  int count;            // splits of the rows
+  int chunks;           // of 128 columns
+  int vec_x;
+  float* part;
+  int* found;
+};
 template <typename TX, typename TO, int kRank, bool kByCol>
-__global__ void __launch_bounds__(kThreads) tokens_kernel(
-    const TX* __restrict__ x, int64_t ldx, const float* __restrict__ row_mul,
-    const float* __restrict__ rank_part, int splits, const float* __restrict__ scaling, Rows rows,
-    int C, int R, int64_t rows_split, int vec_x, float* __restrict__ part, int* __restrict__ found) {
+__device__ __forceinline__ void tokens_tile(const TokensArgs<TX>& g, const float* __restrict__ scaling,
+                                            const Rows& rows, int R, int chunk, int split) {
+  const TX* __restrict__ x = g.x;
+  const float* __restrict__ row_mul = g.row_mul;
+  const float* __restrict__ rank_part = g.rank_part;
+  float* __restrict__ part = g.part;
+  int* __restrict__ found = g.found;
+  const int64_t ldx = g.ldx, rows_split = g.rows_split;
+  const int splits = g.splits, C = g.C, vec_x = g.vec_x;
   using Tile = TokensTile<TX, TO, kRank, kByCol>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int id[kBM];
   __nv_bfloat16* sx = reinterpret_cast<__nv_bfloat16*>(smem);
   __nv_bfloat16* sh = sx + Tile::kPX * Tile::kXPlane;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int col0 = blockIdx.x * kBN;
+  const int col0 = chunk * kBN;
   const int s = blockIdx.z;
-  const int64_t m_lo = static_cast<int64_t>(blockIdx.y) * rows_split;
+  const int64_t m_lo = static_cast<int64_t>(split) * rows_split;
   const int64_t m_hi = min(rows.M, m_lo + rows_split);
   const float mul = scaling ? __ldg(scaling + s) : 1.0f;
   float acc[kRank / 16][2][4];
@@ -626,8 +674,8 @@ __global__ void __launch_bounds__(kThreads) tokens_kernel(
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][n][j] += low[i][n][j];
   }
-  const int64_t block = static_cast<int64_t>(blockIdx.y) * rows.S + s;
-  if (blockIdx.x == 0 && tid == 0) found[block] = any;
+  const int64_t block = static_cast<int64_t>(split) * rows.S + s;
+  if (chunk == 0 && tid == 0) found[block] = any;
   if (!any) return;
   float* dst = part + block * R * C;
 #pragma unroll
@@ -642,6 +690,19 @@ __global__ void __launch_bounds__(kThreads) tokens_kernel(
           dst[kByCol ? static_cast<int64_t>(c) * R + r : static_cast<int64_t>(r) * C + c] = acc[i][n][j];
         }
       }
+}
+
+// Both gradients in one launch: blocks below a.chunks * a.count are dA's.
+template <typename TX, typename T, int kRank>
+__global__ void __launch_bounds__(kThreads) tokens_pair_kernel(TokensArgs<TX> a, TokensArgs<T> b,
+                                                               const float* __restrict__ scaling, Rows rows, int R) {
+  const int first = a.chunks * a.count;
+  const int i = static_cast<int>(blockIdx.x);
+  if (i < first) {
+    tokens_tile<TX, T, kRank, false>(a, scaling, rows, R, i % a.chunks, i / a.chunks);
+  } else {
+    tokens_tile<T, T, kRank, true>(b, scaling, rows, R, (i - first) % b.chunks, (i - first) / b.chunks);
+  }
 }
 
 // The splits' sums, in a fixed order, rounded to T: dA (blockIdx.z 0) or dB of
@@ -803,25 +864,51 @@ int shrink_tc(const LoraArgs& g, const void* x, int64_t ldx, bool codes, const f
 }
 
 template <typename TX, typename TW, bool kWRows>
-int shrink(const TX* x, int64_t ldx, const float* xs, const TW* w, int64_t slot, const Rows& rows,
-           int K, int R, const Split& sp, float* part, cudaStream_t stream) {
-  const int64_t tiles = (rows.M + kBM - 1) / kBM;
+ShrinkArgs<TX, TW> shrink_args(const TX* x, int64_t ldx, const float* xs, const TW* w, int64_t slot, int K, int R,
+                               const Split& sp, float* part) {
   const int vx = aligned(x, ldx, sizeof(TX));
   const int vw = aligned(w, kWRows ? K : R, sizeof(TW)) && aligned(w, slot, sizeof(TW));
-  const dim3 grid(static_cast<unsigned>(tiles), sp.count, parts_of(rows.M, rows.S, sp.count));
-#define SHRINK(RANK)                                                                              \
-  {                                                                                               \
-    auto k = shrink_kernel<TX, TW, RANK, kWRows>;                                                 \
-    constexpr int bytes = ShrinkTile<TX, TW, RANK, kWRows>::kBytes;                               \
-    if (int rc = prepare(k, bytes)) return rc;                                                    \
-    k<<<grid, kThreads, bytes, stream>>>(x, ldx, xs, w, slot, rows, K, R, sp.per, vx, vw, part);  \
+  return {x, ldx, xs, w, slot, K, sp.per, vx, vw, part};
+}
+
+#define BY_RANK(F)                 \
+  switch (pad_rank(R)) {           \
+    case 16: F(16) break;          \
+    case 32: F(32) break;          \
+    case 64: F(64) break;          \
+    default: F(128) break;         \
   }
-  switch (pad_rank(R)) {
-    case 16: SHRINK(16) break;
-    case 32: SHRINK(32) break;
-    case 64: SHRINK(64) break;
-    default: SHRINK(128) break;
+
+template <typename T>
+int shrink(const ShrinkArgs<T, T>& g, bool w_rows, int splits, const Rows& rows, int R, cudaStream_t stream) {
+  const int64_t tiles = (rows.M + kBM - 1) / kBM;
+  const dim3 grid(static_cast<unsigned>(tiles), splits, parts_of(rows.M, rows.S, splits));
+#define SHRINK(RANK)                                                       \
+  {                                                                        \
+    auto k = w_rows ? shrink_kernel<T, T, RANK, true> : shrink_kernel<T, T, RANK, false>; \
+    const int bytes = w_rows ? ShrinkTile<T, T, RANK, true>::kBytes : ShrinkTile<T, T, RANK, false>::kBytes; \
+    if (int rc = prepare(k, bytes)) return rc;                             \
+    k<<<grid, kThreads, bytes, stream>>>(g, rows, R);                      \
   }
+  BY_RANK(SHRINK)
+#undef SHRINK
+  return launched("lora shrink");
+}
+
+template <typename TX, typename T>
+int shrink_pair(const ShrinkArgs<T, T>& dy, int splits_dy, const ShrinkArgs<TX, T>& x, int splits_x, const Rows& rows,
+                int R, cudaStream_t stream) {
+  const int64_t tiles = (rows.M + kBM - 1) / kBM;
+  const int splits = splits_dy + splits_x;
+  const dim3 grid(static_cast<unsigned>(tiles), splits, parts_of(rows.M, rows.S, splits));
+#define SHRINK(RANK)                                                       \
+  {                                                                        \
+    auto k = shrink_pair_kernel<TX, T, RANK>;                              \
+    constexpr int bytes = std::max(ShrinkTile<T, T, RANK, false>::kBytes, ShrinkTile<TX, T, RANK, true>::kBytes); \
+    if (int rc = prepare(k, bytes)) return rc;                             \
+    k<<<grid, kThreads, bytes, stream>>>(dy, x, splits_dy, rows, R);       \
+  }
+  BY_RANK(SHRINK)
 #undef SHRINK
   return launched("lora shrink");
 }
@@ -858,26 +945,18 @@ int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, i
   return launched("lora expand");
 }
 
-template <typename TX, typename TO, bool kByCol>
-int tokens(const TX* x, int64_t ldx, const float* row_mul, const float* rank_part, int splits,
-           const float* scaling, const Rows& rows, int C, int R, const RowSplit& sp, float* part,
-           int* found, cudaStream_t stream) {
-  const int vx = aligned(x, ldx, sizeof(TX));
-  const dim3 grid((C + kBN - 1) / kBN, sp.count, rows.S);
-#define TOKENS(RANK)                                                                              \
-  {                                                                                               \
-    auto k = tokens_kernel<TX, TO, RANK, kByCol>;                                                 \
-    constexpr int bytes = TokensTile<TX, TO, RANK, kByCol>::kBytes;                               \
-    if (int rc = prepare(k, bytes)) return rc;                                                    \
-    k<<<grid, kThreads, bytes, stream>>>(x, ldx, row_mul, rank_part, splits, scaling, rows, C, R, \
-                                         sp.per, vx, part, found);                                \
+template <typename TX, typename T>
+int tokens_pair(const TokensArgs<TX>& a, const TokensArgs<T>& b, const float* scaling, const Rows& rows, int R,
+                cudaStream_t stream) {
+  const dim3 grid(a.chunks * a.count + b.chunks * b.count, 1, rows.S);
+#define TOKENS(RANK)                                                       \
+  {                                                                        \
+    auto k = tokens_pair_kernel<TX, T, RANK>;                              \
+    constexpr int bytes = std::max(TokensTile<TX, T, RANK, false>::kBytes, TokensTile<T, T, RANK, true>::kBytes); \
+    if (int rc = prepare(k, bytes)) return rc;                             \
+    k<<<grid, kThreads, bytes, stream>>>(a, b, scaling, rows, R);          \
   }
-  switch (pad_rank(R)) {
-    case 16: TOKENS(16) break;
-    case 32: TOKENS(32) break;
-    case 64: TOKENS(64) break;
-    default: TOKENS(128) break;
-  }
+  BY_RANK(TOKENS)
 #undef TOKENS
   return launched("lora tokens");
 }
@@ -929,8 +1008,9 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
     sp = shrink_tc_split(g.M, K);
     counts = reinterpret_cast<int*>(part + sp.count * g.M * g.R);
     if (int rc = shrink_tc(g, g.x, g.ldx, false, nullptr, g.a, g.lda, true, K, sp, part, counts, stream)) return rc;
-  } else if (int rc = shrink<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
-                                         static_cast<const T*>(g.a), g.lda, rows, K, R, sp, part, stream)) {
+  } else if (int rc = shrink<T>(shrink_args<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
+                                                        static_cast<const T*>(g.a), g.lda, K, R, sp, part),
+                                true, sp.count, rows, R, stream)) {
     return rc;
   }
   if (counts && tc_rows(g.y, g.ldy, 2) && tc_rows(g.out, g.ldo, 2) && tc_weights(g.b, g.ldb, R, g.S)) {
@@ -990,8 +1070,13 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   if (g.M > 0) {
     if (tc) {
       if (int rc = shrink_tc(g, dy, g.ldy, false, nullptr, b, g.ldb, false, N, p.g, pg, counts, stream)) return rc;
-    } else if (int rc = shrink<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, rows, N, R, p.g, pg, stream)) {
-      return rc;
+    } else {
+      const auto sg = shrink_args<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, N, R, p.g, pg);
+      const auto sh = shrink_args<TX, T, true>(x, g.ldx, g.x_scale, a, g.lda, K, R, p.h, ph);
+      if (int rc = g.da ? shrink_pair<TX, T>(sg, p.g.count, sh, p.h.count, rows, R, stream)
+                        : shrink<T>(sg, false, p.g.count, rows, R, stream)) {
+        return rc;
+      }
     }
     if (g.out && tc && tc_rows(g.out, g.ldo, 2)) {
       if (int rc = lora_expand_tc({g.accumulate ? g.out : nullptr, g.ldo, counts, pg, p.g.count, a, 0, g.lda, g.scaling,
@@ -1026,17 +1111,11 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
       return rc;
     }
   } else {
-    if (g.M > 0) {
-      if (int rc = shrink<TX, T, true>(x, g.ldx, g.x_scale, a, g.lda, rows, K, R, p.h, ph, stream)) return rc;
-    }
-    if (int rc = tokens<TX, T, false>(x, g.ldx, g.x_scale, pg, p.g.count, g.scaling, rows, K, R, p.a, pa,
-                                      fa, stream)) {
-      return rc;
-    }
-    if (int rc = tokens<T, T, true>(dy, g.ldy, nullptr, ph, p.h.count, g.scaling, rows, N, R, p.b, pb, fb,
-                                    stream)) {
-      return rc;
-    }
+    const TokensArgs<TX> ta{x, g.ldx, g.x_scale, pg, p.g.count, K, p.a.per, p.a.count, (K + kBN - 1) / kBN,
+                            aligned(x, g.ldx, sizeof(TX)), pa, fa};
+    const TokensArgs<T> tb{dy, g.ldy, nullptr, ph, p.h.count, N, p.b.per, p.b.count, (N + kBN - 1) / kBN,
+                           aligned(dy, g.ldy, sizeof(T)), pb, fb};
+    if (int rc = tokens_pair<TX, T>(ta, tb, g.scaling, rows, R, stream)) return rc;
   }
   const SumArgs sa{pa, fa, p.a.count, g.R * g.K, g.da}, sb{pb, fb, p.b.count, g.R * g.N, g.db};
   const int64_t most = std::max(sa.per, sb.per);
