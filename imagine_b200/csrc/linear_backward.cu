@@ -6,10 +6,12 @@
 // weight would have), two for f16 and three for fp32 (pieces.cuh), which keeps
 // each type's own precision.
 //
-// Two kernels:
-//   input_grad_kernel     mma.sync tiles of 64 rows x 128 columns, for fp32, for
-//                         few rows and for weights whose rows are not 4-byte aligned
-//   input_grad_tc_kernel  tcgen05, pairs of CTAs on 256 x 256 tiles, for the rest
+// Three kernels:
+//   input_grad_few_kernel  up to 16 rows: w from HBM straight into mma.sync fragments
+//   input_grad_tc_kernel   16-bit types: tcgen05, pairs of CTAs on 256 x 256 tiles
+//   input_grad_kernel      mma.sync tiles of 64 rows x 128 columns, for the rest: fp32
+//                          (whose sums the tensor cores' long runs would bias),
+//                          rows that the others cannot load
 // With few tiles the contraction is cut over blocks and the fp32 partial sums
 // are added in a fixed order.
 #include <cuda.h>
@@ -709,6 +711,173 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
   return 0;
 }
 
+// ================================================================ few rows
+// Up to 16 rows: what has to be read is w, once.  A block takes 64 columns and a
+// range of the contraction, 128 of it a step, a warp sixteen: w goes from HBM
+// straight into the warp's matrix fragments, two steps ahead (a lane reads eight
+// columns of four rows; which of the tile's columns a fragment column stands for is
+// free to choose), and only the pieces of dy ws pass through shared memory.  The
+// eight warps' sums are joined in order at the end.
+// 4096 -> 4096, a call with its sum: 20.3 us where input_grad_kernel, which stages w
+// in shared memory, takes 26.7.  At 32 rows both take 27 us, at 64 this form 56.
+constexpr int kFewRows = 16, kFewCols = 64, kFewN = 128, kLdFew = kFewN + 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) input_grad_few_kernel(
+    const T* __restrict__ dy, int64_t lddy, const float* __restrict__ ws, int ws_one,
+    const int8_t* __restrict__ w, int64_t ldw, int M, int N, int K, int n_split, int vec_dy,
+    T* __restrict__ dx, int64_t lddx, float* __restrict__ part) {
+  constexpr int kP = Pieces<T>::n, kRows = kFewRows;
+  constexpr int kPlane = kRows * kLdFew;
+  constexpr bool kApart = std::is_same<T, float>::value;
+  constexpr int kBuf = 2 * kP * kPlane * 2, kJoin = kRows * (kFewCols + 1) * 4;
+  __shared__ __align__(16) uint8_t smem[kBuf > kJoin ? kBuf : kJoin];
+  __nv_bfloat16* sa = reinterpret_cast<__nv_bfloat16*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int q = lane & 3, gcol = lane >> 2;
+  const int col = blockIdx.x * kFewCols + 8 * gcol;
+  const bool in_k = col < K;  // K % 8 == 0
+  const int n_lo = blockIdx.y * n_split, n_hi = min(N, n_lo + n_split);
+
+  float acc[8][4] = {};
+  float low[kApart ? 8 : 1][4] = {};
+  uint2 wq[2][4];
+  auto fetch_w = [&](int n0, uint2 (&r)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + warp * 16 + 2 * q + (i & 1) + (i >> 1) * 8;
+      r[i] = in_k && n < n_hi ? __ldg(reinterpret_cast<const uint2*>(w + n * ldw + col)) : make_uint2(0, 0);
+    }
+  };
+  // dy ws of one step: kRows x 128 elements, eight at a time
+  static_assert(kRows * (kFewN / 8) == kThreads, "eight elements a thread");
+  auto lay = [&](int n0, int buf) {
+    {
+      const int r = tid / (kFewN / 8), c = (tid % (kFewN / 8)) * 8;
+      const int valid = r < M ? min(8, n_hi - n0 - c) : 0;
+      Raw8<T> raw;
+      load8(raw, dy + static_cast<int64_t>(r) * lddy + n0 + c, valid, vec_dy != 0);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = j < valid ? to_f(raw.e[j]) * __ldg(ws + (ws_one ? 0 : n0 + c + j)) : 0.0f;
+      store_pieces<kP>(sa + buf * kP * kPlane + r * kLdFew + c, kPlane, v);
+    }
+  };
+  fetch_w(n_lo, wq[0]);
+  fetch_w(n_lo + kFewN, wq[1]);
+  lay(n_lo, 0);
+  __syncthreads();
+  auto step = [&](int n0, int buf, uint2 (&r)[4]) {
+    uint32_t x[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i][0] = r[i].x ^ 0x80808080u;
+      x[i][1] = r[i].y ^ 0x80808080u;
+    }
+    fetch_w(n0 + 2 * kFewN, r);
+    if (n0 + kFewN < n_hi) lay(n0 + kFewN, buf ^ 1);
+    uint32_t a[kP][4];
+#pragma unroll
+    for (int p = 0; p < kP; ++p) ldsm4(a[p], at16(sa + (buf * kP + p) * kPlane, 0, warp * 16, kLdFew, lane));
+    const uint64_t magic = pk(-8388736.0f, -8388736.0f);  // -(2^23 + 128)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t b[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t f =
+            add2(pk(__uint_as_float(__byte_perm(x[2 * h][j >> 2], 0x4B000000u, 0x7540 + (j & 3))),
+                    __uint_as_float(__byte_perm(x[2 * h + 1][j >> 2], 0x4B000000u, 0x7540 + (j & 3)))),
+                 magic);
+        b[h] = pack_bf16(lo(f), hi(f));
+      }
+#pragma unroll
+      for (int p = 0; p < kP; ++p) {
+        if constexpr (kApart) {
+          mma_apart(acc[j], low[j], a[p], b[0], b[1], p == 0);
+        } else {
+          mma(acc[j], a[p], b[0], b[1]);
+        }
+      }
+    }
+    __syncthreads();
+  };
+  int buf = 0;
+  for (int n0 = n_lo; n0 < n_hi; n0 += 2 * kFewN) {
+    step(n0, buf, wq[0]);
+    buf ^= 1;
+    if (n0 + kFewN < n_hi) {
+      step(n0 + kFewN, buf, wq[1]);
+      buf ^= 1;
+    }
+  }
+  if constexpr (kApart) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] += low[j][e];
+  }
+  // the warps' sums, in order
+  float* sum = reinterpret_cast<float*>(smem);
+  for (int v = 0; v < kThreads / 32; ++v) {
+    if (warp == v) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // fragment column 2 q + (e & 1) of tile j stands for column 8 (2 q + (e & 1)) + j
+          const int r = gcol + (e >> 1) * 8, c = 8 * (2 * q + (e & 1)) + j;
+          float* cell = sum + r * (kFewCols + 1) + c;
+          *cell = v ? *cell + acc[j][e] : acc[j][e];
+        }
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < kRows * kFewCols; i += kThreads) {
+    const int r = i / kFewCols, c = blockIdx.x * kFewCols + i % kFewCols;
+    if (r >= M || c >= K) continue;
+    const float v = sum[r * (kFewCols + 1) + i % kFewCols];
+    if (part) {
+      part[(static_cast<int64_t>(blockIdx.y) * M + r) * K + c] = v;
+    } else {
+      dx[static_cast<int64_t>(r) * lddx + c] = from_f<T>(v);
+    }
+  }
+}
+
+// Whether input_grad_few_kernel takes a call, by shape (its operands' alignment apart).
+bool few_shape(int64_t M, int64_t N, int64_t K) { return M <= kFewRows && N > 0 && K % 8 == 0; }
+// Two blocks a multiprocessor, at least two steps each, at most 16 pieces.
+struct FewSplit {
+  int count, per;
+};
+FewSplit few_split(int64_t N, int64_t K) {
+  const int64_t cols = (K + kFewCols - 1) / kFewCols, steps = (N + kFewN - 1) / kFewN;
+  const int64_t want =
+      std::max<int64_t>(1, std::min<int64_t>({2ll * device_sm_count() / cols, 16, steps / 2}));
+  const int64_t per = (steps + want - 1) / want;
+  return {static_cast<int>((steps + per - 1) / per), static_cast<int>(per * kFewN)};
+}
+
+template <typename T>
+int few_typed(const InputGradArgs& g, cudaStream_t stream) {
+  const FewSplit sp = few_split(g.N, g.K);
+  const int M = static_cast<int>(g.M), N = static_cast<int>(g.N), K = static_cast<int>(g.K);
+  const int vec = reinterpret_cast<uintptr_t>(g.dy) % 16 == 0 && (g.lddy * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+  float* part = sp.count > 1 ? static_cast<float*>(g.workspace) : nullptr;
+  const T* dy = static_cast<const T*>(g.dy);
+  T* dx = static_cast<T*>(g.dx);
+  input_grad_few_kernel<T><<<dim3((K + kFewCols - 1) / kFewCols, sp.count), kThreads, 0, stream>>>(
+      dy, g.lddy, g.ws, g.ws_numel == 1, g.w, g.ldw, M, N, K, sp.per, vec, dx, g.lddx, part);
+  if (int rc = launched("input gradient")) return rc;
+  if (part) {
+    sum_parts<T>(part, sp.count, g, stream);
+    return launched("input gradient sum");
+  }
+  return 0;
+}
+
 template <typename T>
 int typed(const InputGradArgs& g, cudaStream_t stream) {
   const int N = static_cast<int>(g.N), K = static_cast<int>(g.K);
@@ -741,6 +910,10 @@ int typed(const InputGradArgs& g, cudaStream_t stream) {
 int64_t input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
   const NSplit sp = n_split_of(M, N, K);
   int64_t bytes = sp.count > 1 ? sp.count * M * K * 4 : 0;
+  if (few_shape(M, N, K)) {
+    const int few = few_split(N, K).count;
+    bytes = std::max(bytes, few > 1 ? few * M * K * 4 : 0);
+  }
   if (tc_shape(M, N, K, dtype)) {
     const TcPlan p = tc_plan(M, N, K, dtype);
     bytes = std::max(bytes, p.pieces_bytes + p.weight_bytes + p.part_bytes);
@@ -750,6 +923,13 @@ int64_t input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
 
 int input_grad_launch(const InputGradArgs& g, cudaStream_t stream) {
   const bool tc = tc_shape(g.M, g.N, g.K, g.dtype) && tc_operands(g);
+  if (few_shape(g.M, g.N, g.K) && reinterpret_cast<uintptr_t>(g.w) % 8 == 0 && g.ldw % 8 == 0) {
+    switch (g.dtype) {
+      case W8A8_BF16: return few_typed<__nv_bfloat16>(g, stream);
+      case W8A8_F16: return few_typed<__half>(g, stream);
+      default: return few_typed<float>(g, stream);
+    }
+  }
   switch (g.dtype) {
     case W8A8_BF16: return tc ? tc_typed<__nv_bfloat16>(g, stream) : typed<__nv_bfloat16>(g, stream);
     case W8A8_F16: return tc ? tc_typed<__half>(g, stream) : typed<__half>(g, stream);
