@@ -1,0 +1,237 @@
+"""The adapters' kernels for long bf16 batches (tiles of 128 rows, TMA operands): mixed tiles,
+ragged ends, every padded rank, and the batches beside them that take the other form.
+Tolerances as in test_gpu_adapters."""
+import pytest
+import torch
+
+from tests.test_gpu_adapters import PIECES, _add_ref, _case, _check, _check_grads, _grad_ref, _sums
+
+pytestmark = pytest.mark.gpu
+
+
+def _ragged(m, s, seed, none=True):
+    """Adapters of ragged requests: runs of rows, some without an adapter."""
+    g = torch.Generator().manual_seed(seed)
+    idx = torch.empty(m, dtype=torch.int32)
+    at = 0
+    while at < m:
+        run = int(torch.randint(1, max(2, m // 3), (1,), generator=g))
+        idx[at:at + run] = int(torch.randint(-1 if none else 0, s, (1,), generator=g))
+        at += run
+    return idx.cuda()
+
+
+def _quiet():
+    import imagine_b200 as W
+
+    assert W.device_error() == 0
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("m,k,n,s,r", [
+    (256, 64, 64, 1, 8), (257, 136, 72, 2, 16), (300, 512, 264, 3, 24), (511, 1032, 520, 5, 32), (640, 192, 1544, 4, 64),
+    (1000, 1024, 776, 7, 40), (777, 256, 512, 2, 128), (384, 2056, 200, 64, 16), (1290, 320, 328, 3, 104)])
+def test_every_rank_and_ragged_ends(m, k, n, s, r, codes):
+    import imagine_b200 as W
+
+    x, y, dy, a, b, c, _ = _case(m, k, n, s, r, torch.bfloat16, seed=2)
+    idx = _ragged(m, s, m + r)
+    if not codes:
+        out = W.lora_add(y, x, a, b, idx, c)
+        _check(out, *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(k, r), "out")
+        assert torch.equal(out[idx < 0], y[idx < 0])
+        assert torch.equal(out, W.lora_add(y.clone(), x, a, b, idx.long(), c, out=y))
+    xs, data = None, x
+    if codes:
+        x, xs = W.quantize_int8_rowwise(x)
+        data = x.double() * xs.double()
+    got = W.lora_backward(dy, x, a, b, idx, c, x_scale=xs)
+    _check_grads(got, data, dy, a, b, c, idx)
+    assert not bool(got[0][idx < 0].any())
+    assert all(torch.equal(p, q) for p, q in zip(got, W.lora_backward(dy, x, a, b, idx, c, x_scale=xs)))
+    base = torch.randn(m, k, device="cuda").bfloat16()
+    dx = W.lora_backward(dy, x, a, b, idx, c, x_scale=xs, dx=base.clone(), need_weights=False)[0]
+    ref, size = _grad_ref(data, dy, a, b, c, idx)["dx"]
+    _check(dx, ref + base.double(), size, 2 * PIECES[dy.dtype] + _sums(n, r), "dx added")
+    assert torch.equal(dx[idx < 0], base[idx < 0])
+    _quiet()
+
+
+@pytest.mark.parametrize("s,r", [(64, 16), (64, 64), (9, 128), (70, 8)])
+def test_every_row_another_adapter(s, r):
+    """Rows of all adapters in every tile (more than there are accumulators for); over 64 adapters
+    the other form runs."""
+    import imagine_b200 as W
+
+    m, k, n = 400, 264, 392
+    x, y, dy, a, b, c, idx = _case(m, k, n, s, r, torch.bfloat16)
+    _check(W.lora_add(y, x, a, b, idx, c), *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(k, r))
+    _check_grads(W.lora_backward(dy, x, a, b, idx, c), x, dy, a, b, c, idx)
+    _quiet()
+
+
+def test_nan_stays_in_its_rows_and_adapters():
+    import imagine_b200 as W
+
+    m, k, n, s, r = 700, 256, 384, 3, 16
+    x, y, dy, a, b, c, _ = _case(m, k, n, s, r, torch.bfloat16)
+    idx = _ragged(m, s, 11)
+    idx[100:140], idx[600:650], idx[300:310] = 1, 1, -1
+    clean, grads = W.lora_add(y, x, a, b, idx, c), W.lora_backward(dy, x, a, b, idx, c)
+    bad = idx == 1
+    for v in (float("nan"), float("inf")):
+        xb, yb, dyb, ab, bb = x.clone(), y.clone(), dy.clone(), a.clone(), b.clone()
+        xb[bad], yb[bad], dyb[bad], ab[1], bb[1] = v, v, v, v, v
+        xb[idx < 0], dyb[idx < 0] = v, v
+        out = W.lora_add(yb, xb, ab, bb, idx, c)
+        assert torch.equal(out[~bad], clean[~bad]) and not bool(out[bad].isfinite().any())
+        dx, da, db = W.lora_backward(dyb, xb, ab, bb, idx, c)
+        assert torch.equal(dx[~bad], grads[0][~bad]) and not bool(dx[bad].isfinite().any())
+        for t, ref in ((da, grads[1]), (db, grads[2])):
+            assert torch.equal(t[[0, 2]], ref[[0, 2]]) and not bool(t[1].isfinite().any())
+    _quiet()
+
+
+def test_operands_that_lie_elsewhere():
+    """Rows apart (16-byte strides: the same form; odd ones: the other), a stack's every second adapter,
+    samples of a batch, and rows of the output's surroundings left as they were."""
+    import imagine_b200 as W
+
+    bt, t, k, n, s, r = 3, 130, 136, 200, 4, 16
+    m = bt * t
+    x, y, dy, a, b, c, _ = _case(m, k, n, s, r, torch.bfloat16)
+    sample = torch.tensor([2, -1, 0], device="cuda")
+    token = sample.repeat_interleave(t)
+    want, grads = W.lora_add(y, x, a, b, token, c), W.lora_backward(dy, x, a, b, token, c)
+    for p, q in zip(W.lora_backward(dy.view(bt, t, n), x.view(bt, t, k), a, b, sample, c), grads):
+        assert torch.equal(p.reshape(q.shape), q)
+    assert torch.equal(W.lora_add(y.view(bt, t, n), x.view(bt, t, k), a, b, sample, c).view(m, n), want)
+
+    def apart(v, pad, at):
+        big = torch.full((v.shape[0], v.shape[1] + pad), float("nan"), dtype=v.dtype, device="cuda")
+        big[:, at:at + v.shape[1]] = v
+        return big[:, at:at + v.shape[1]]
+    a2 = torch.full((2 * s, r, k), float("nan"), dtype=a.dtype, device="cuda")
+    b2 = torch.full((2 * s, n, r), float("nan"), dtype=a.dtype, device="cuda")
+    a2[::2], b2[::2] = a, b
+    xa, ya, dya = apart(x, 24, 8), apart(y, 16, 16), apart(dy, 8, 0)
+    wide = torch.full((m, n + 24), 7.0, dtype=y.dtype, device="cuda")
+    W.lora_add(ya, xa, a2[::2], b2[::2], token, c, out=wide[:, 8:8 + n])
+    assert torch.equal(wide[:, 8:8 + n], want)
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 8 + n:] == 7).all())
+    for p, q in zip(W.lora_backward(dya, xa, a2[::2], b2[::2], token, c), grads):
+        assert torch.equal(p, q)
+    # rows that TMA cannot take: other kernels, the same values up to the order of the sums
+    for p, q in zip(W.lora_backward(apart(dy, 3, 1), apart(x, 5, 2), a, b, token, c), grads):
+        assert float((p.double() - q.double()).norm() / q.double().norm()) < 2.0 ** -8
+    odd = W.lora_add(apart(y, 1, 0), apart(x, 3, 1), a, b, token, c)
+    _check(odd, *_add_ref(x, y, a, b, c, token), 2 * PIECES[x.dtype] + _sums(k, r))
+    assert torch.equal(odd[token < 0], y[token < 0])
+
+
+@pytest.mark.parametrize("rows", [64, 65, 255, 256, 2048 * 64 + 70])
+def test_borders_of_the_forms(rows):
+    """Row counts where another kernel, or another split of a long batch, takes over."""
+    import imagine_b200 as W
+
+    k, n, s, r = 64, 72, 2, 8
+    x, y, dy, a, b, c, _ = _case(rows, k, n, s, r, torch.bfloat16)
+    idx = (torch.arange(rows, device="cuda") * s // rows).int()
+    idx[rows // 3] = -1
+    _check(W.lora_add(y, x, a, b, idx, c), *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(k, r))
+    _check_grads(W.lora_backward(dy, x, a, b, idx, c), x, dy, a, b, c, idx)
+    _quiet()
+
+
+def test_two_streams_and_a_graph():
+    """Two calls at once on two streams, and a captured step whose replay reads new contents."""
+    import imagine_b200 as W
+
+    sets = [_case(500, 512, 640, 3, 32, torch.bfloat16, seed=q) for q in (1, 2)]
+    idx = _ragged(500, 3, 5)
+    w = torch.randint(-127, 128, (640, 512), device="cuda", dtype=torch.int8)
+    ws = torch.rand(640, device="cuda") * 1e-3
+
+    def step(x, y, dy, a, b, c, _):
+        base = W.int8_linear_backward(dy, w, ws)
+        return (W.lora_add(y, x, a, b, idx, c), *W.lora_backward(dy, x, a, b, idx, c, dx=base))
+    want = [step(*q) for q in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for run in got[i]:
+            assert all(torch.equal(p, q) for p, q in zip(run, want[i]))
+    held_in = [t.clone() for t in sets[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(*held_in)
+    for i in (1, 0):
+        for dst, src in zip(held_in, sets[i]):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, want[i]))
+    _quiet()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_long_batches_of_the_other_types(dtype):
+    import imagine_b200 as W
+
+    m, k, n, s, r = 1100, 520, 264, 3, 24
+    x, y, dy, a, b, c, _ = _case(m, k, n, s, r, dtype)
+    idx = _ragged(m, s, 3)
+    _check(W.lora_add(y, x, a, b, idx, c), *_add_ref(x, y, a, b, c, idx), 2 * PIECES[dtype] + _sums(k, r))
+    _check_grads(W.lora_backward(dy, x, a, b, idx, c), x, dy, a, b, c, idx)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_layer_as_it_is_trained(dtype):
+    """MLP up, activation, MLP down with adapters: the run of the operators together, its gradients
+    against the same layer in 64 bits with the inputs that the operators kept."""
+    import imagine_b200 as W
+
+    g = torch.Generator(device="cuda").manual_seed(9)
+    t, k, f, s, r = 320, 256, 512, 2, 16
+    def rn(*shape, std=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+    x = rn(t, k).requires_grad_()
+    up, ups = W.quantize_weight(rn(f, k, std=0.05).bfloat16())
+    down, downs = W.quantize_weight(rn(k, f, std=0.05).bfloat16())
+    leaves = [rn(s, r, k, std=0.05), rn(s, f, r, std=0.1), rn(s, r, f, std=0.05), rn(s, k, r, std=0.1)]
+    for q in leaves:
+        q.requires_grad_()
+    idx = _ragged(t, s, 4)
+    c = torch.tensor([1.0, 0.5], device="cuda")
+    u = W.int8_linear_lora(x, up, ups, None, leaves[0], leaves[1], idx, c)
+    h = W.checkpointed_activation(u)
+    z = W.int8_linear_lora(h, down, downs, None, leaves[2], leaves[3], idx, c)
+    dz = rn(t, k)
+    grads = torch.autograd.grad(z, (x, *leaves), dz)
+    # the same backward in 64 bits, from what was kept
+    def kept(v):
+        q, sc = W.quantize_int8_rowwise(v.detach())
+        return q.double() * sc.double()
+    hk, xk = kept(h), kept(x)
+    uq, us = W.act_checkpoint_int8(u.detach())[1:]
+    uk = (uq.float() * us.repeat_interleave(128, 1)).double().requires_grad_()
+    a1, b1, a2, b2 = (q.detach().double() for q in leaves)
+    dz64 = dz.double()
+
+    def through(d, wq, wsc, a, b, inp):
+        ref = _grad_ref(inp, d, a, b, c, idx)
+        return d @ (wq.double() * wsc.double().view(-1, 1)) + ref["dx"][0], ref["da"][0], ref["db"][0]
+    dh, da2, db2 = through(dz64, down, downs, a2, b2, hk)
+    du = torch.autograd.grad(torch.nn.functional.gelu(uk, approximate="tanh"), uk, dh)[0]
+    dx, da1, db1 = through(du, up, ups, a1, b1, xk)
+    # per operator: its inputs' and its own rounding (u each), seven of them in the longest chain
+    u_ = torch.finfo(dtype).eps / 2
+    for name, got, ref in zip(("x", "a1", "b1", "a2", "b2"), grads, (dx, da1, db1, da2, db2)):
+        off = float((got.double() - ref).norm() / ref.norm())
+        assert off < 7 * u_ + 1e-5, (name, off)
