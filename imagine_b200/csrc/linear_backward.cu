@@ -24,6 +24,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "lora_rows.cuh"
 #include "pieces.cuh"
 #include "quant_common.cuh"
 #include "sm100_ptx.cuh"
@@ -54,7 +55,7 @@ int read_and_clear_input_grad_error(cudaStream_t stream, int* value) {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBM = 64, kBC = 128, kBN = 64;
+constexpr int kBC = 128, kBN = 64;
 constexpr int kLdA = kBN + 8, kLdB = kBC + 8;
 
 template <typename T>
@@ -63,6 +64,7 @@ __global__ void __launch_bounds__(kThreads) input_grad_kernel(
     const int8_t* __restrict__ w, int64_t ldw, int64_t M, int N, int K, int col_tiles, int n_split,
     int vec_dy, int vec_w, int vec_o, T* __restrict__ dx, int64_t lddx, float* __restrict__ part) {
   constexpr int kP = Pieces<T>::n;
+  griddep_launch_dependents();
   constexpr int kPlane = kBM * kLdA;
   constexpr bool kApart = std::is_same<T, float>::value;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -183,6 +185,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) sum_parts_kernel(const float* __restrict__ part,
                                                              int parts, int64_t M, int K, int vec,
                                                              T* __restrict__ dx, int64_t lddx) {
+  griddep_wait();
   const int64_t total = M * K;
   const int64_t start = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) sum_parts_kernel(const float* __rest
     for (int64_t i = start * 4; i < total; i += step * 4) {
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int p = 0; p < parts; ++p) {
-        const float4 o = __ldg(reinterpret_cast<const float4*>(part + p * total + i));
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(part + p * total + i));
         v.x += o.x;
         v.y += o.y;
         v.z += o.z;
@@ -209,20 +212,25 @@ __global__ void __launch_bounds__(kThreads) sum_parts_kernel(const float* __rest
   }
   for (int64_t i = start; i < total; i += step) {
     float v = 0.0f;
-    for (int p = 0; p < parts; ++p) v += __ldg(part + p * total + i);
+    for (int p = 0; p < parts; ++p) v += __ldcg(part + p * total + i);
     const int64_t row = i / K;
     dx[row * lddx + (i - row * K)] = from_f<T>(v);
   }
 }
 
 template <typename T>
-void sum_parts(const float* part, int parts, const InputGradArgs& g, cudaStream_t stream) {
+int sum_parts(const float* part, int parts, const InputGradArgs& g, cudaStream_t stream) {
   const int K = static_cast<int>(g.K);
   const int vec = K % 4 == 0 && reinterpret_cast<uintptr_t>(g.dx) % (4 * sizeof(T)) == 0 && g.lddx % 4 == 0;
   const int64_t items = g.M * K / (vec ? 4 : 1);
   const int64_t blocks = std::min<int64_t>((items + kThreads - 1) / kThreads, 16ll * device_sm_count());
-  sum_parts_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(part, parts, g.M, K, vec,
-                                                                             static_cast<T*>(g.dx), g.lddx);
+  const cudaError_t e = launch_chained(true, sum_parts_kernel<T>, dim3(static_cast<unsigned>(blocks)), kThreads, 0,
+                                       stream, part, parts, g.M, K, vec, static_cast<T*>(g.dx), g.lddx);
+  if (e != cudaSuccess) {
+    set_error("input gradient sum launch failed: %s", cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
 }
 
 // At most two blocks a multiprocessor (all resident), at least four steps each, at
@@ -345,6 +353,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  griddep_launch_dependents();
+  griddep_wait();  // the widened weights
 
   if (warp == kTmaWarp) {
     if (lane == 0) {
@@ -479,6 +489,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 __global__ void __launch_bounds__(kThreads) widen_weights_kernel(
     const int8_t* __restrict__ w, int64_t ldw, const float* __restrict__ ws, int ws_one, int N, int K,
     int n_pad, int k_tiles, int vec, __nv_bfloat16* __restrict__ out) {
+  griddep_launch_dependents();
   __shared__ __align__(16) uint4 tile[64][16];
   const int n0 = static_cast<int>(blockIdx.x / k_tiles) * 128, k0 = static_cast<int>(blockIdx.x % k_tiles) * 64;
   const int kc = threadIdx.x & 15, ng = threadIdx.x >> 4;
@@ -529,6 +540,7 @@ __global__ void __launch_bounds__(kThreads) widen_weights_kernel(
     if (k0 + k < K && n < n_pad)
       *reinterpret_cast<uint4*>(out + static_cast<int64_t>(k0 + k) * n_pad + n) = tile[k][c ^ (k >> 2)];
   }
+  griddep_wait();  // what follows this kernel may then use what the one before it wrote
 }
 
 // bf16 pieces of dy ws as planes [row][piece][n_pad], zero past N: the operand
@@ -538,6 +550,7 @@ __global__ void __launch_bounds__(kThreads) pieces_kernel(const T* __restrict__ 
                                                           const float* __restrict__ ws, int ws_one,
                                                           int64_t M, int N, int n_pad, int vec,
                                                           __nv_bfloat16* __restrict__ out) {
+  griddep_launch_dependents();
   constexpr int kP = Pieces<T>::n;
   const int64_t total = M * (n_pad / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
@@ -647,11 +660,15 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
   }
   uint8_t* wide = work + p.pieces_bytes;
   const int k_tiles = (K + 63) / 64;
-  widen_weights_kernel<<<static_cast<unsigned>(static_cast<int64_t>((N + 127) / 128) * k_tiles), kThreads, 0,
-                         stream>>>(g.w, g.ldw, direct ? g.ws : nullptr, g.ws_numel == 1, N, K, n_pad, k_tiles,
-                                   reinterpret_cast<uintptr_t>(g.w) % 4 == 0 && g.ldw % 4 == 0,
-                                   reinterpret_cast<__nv_bfloat16*>(wide));
-  if (int rc = launched("input gradient weights")) return rc;
+  const cudaError_t we = launch_chained(
+      !direct, widen_weights_kernel, dim3(static_cast<unsigned>(static_cast<int64_t>((N + 127) / 128) * k_tiles)),
+      kThreads, 0, stream, g.w, g.ldw, direct ? g.ws : nullptr, static_cast<int>(g.ws_numel == 1), N, K, n_pad, k_tiles,
+      static_cast<int>(reinterpret_cast<uintptr_t>(g.w) % 4 == 0 && g.ldw % 4 == 0),
+      reinterpret_cast<__nv_bfloat16*>(wide));
+  if (we != cudaSuccess) {
+    set_error("input gradient weights launch failed: %s", cudaGetErrorString(we));
+    return W8A8_ERR_ACCELERATOR;
+  }
   CUtensorMap map_a, map_b;
   const int64_t inner = direct ? g.N : static_cast<int64_t>(kP) * n_pad;
   if (!map_rows(&map_a, direct ? g.dy : work, inner, g.M, direct ? g.lddy : inner) ||
@@ -692,21 +709,22 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
   lc.blockDim = dim3(kTcThreads);
   lc.dynamicSmemBytes = kTcSmem;
   lc.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   lc.attrs = attr;
-  lc.numAttrs = 1;
+  lc.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&lc, kern, map_a, map_b, a);
   if (e != cudaSuccess) {
     set_error("input gradient launch failed: %s", cudaGetErrorString(e));
     return W8A8_ERR_ACCELERATOR;
   }
   if (a.part) {
-    sum_parts<T>(a.part, p.splits, g, stream);
-    return launched("input gradient sum");
+    return sum_parts<T>(a.part, p.splits, g, stream);
   }
   return 0;
 }
@@ -728,6 +746,7 @@ __global__ void __launch_bounds__(kThreads) input_grad_few_kernel(
     const int8_t* __restrict__ w, int64_t ldw, int M, int N, int K, int n_split, int vec_dy,
     T* __restrict__ dx, int64_t lddx, float* __restrict__ part) {
   constexpr int kP = Pieces<T>::n, kRows = kFewRows;
+  griddep_launch_dependents();
   constexpr int kPlane = kRows * kLdFew;
   constexpr bool kApart = std::is_same<T, float>::value;
   constexpr int kBuf = 2 * kP * kPlane * 2, kJoin = kRows * (kFewCols + 1) * 4;
@@ -872,8 +891,7 @@ int few_typed(const InputGradArgs& g, cudaStream_t stream) {
       dy, g.lddy, g.ws, g.ws_numel == 1, g.w, g.ldw, M, N, K, sp.per, vec, dx, g.lddx, part);
   if (int rc = launched("input gradient")) return rc;
   if (part) {
-    sum_parts<T>(part, sp.count, g, stream);
-    return launched("input gradient sum");
+    return sum_parts<T>(part, sp.count, g, stream);
   }
   return 0;
 }
@@ -899,8 +917,7 @@ int typed(const InputGradArgs& g, cudaStream_t stream) {
       vdy, vw, vo, static_cast<T*>(g.dx), g.lddx, part);
   if (int rc = launched("input gradient")) return rc;
   if (part) {
-    sum_parts<T>(part, sp.count, g, stream);
-    return launched("input gradient sum");
+    return sum_parts<T>(part, sp.count, g, stream);
   }
   return 0;
 }

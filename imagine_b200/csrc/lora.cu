@@ -223,12 +223,14 @@ __device__ __forceinline__ void shrink_tile(const ShrinkArgs<TX, TW>& g, const R
 
 template <typename TX, typename TW, int kRank, bool kWRows>
 __global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs<TX, TW> g, Rows rows, int R) {
+  griddep_launch_dependents();
   shrink_tile<TX, TW, kRank, kWRows>(g, rows, R, blockIdx.y);
 }
 // dy times B and x times A in one launch: blockIdx.y below `first` is the former.
 template <typename TX, typename T, int kRank>
 __global__ void __launch_bounds__(kThreads) shrink_pair_kernel(ShrinkArgs<T, T> dy, ShrinkArgs<TX, T> x, int first,
                                                                Rows rows, int R) {
+  griddep_launch_dependents();
   if (static_cast<int>(blockIdx.y) < first) {
     shrink_tile<T, T, kRank, false>(dy, rows, R, blockIdx.y);
   } else {
@@ -255,14 +257,14 @@ __device__ __forceinline__ void load_rank_side(__nv_bfloat16* dst, const float* 
       const float* p = part + (row0 + r) * R + c;
       for (int sp = 0; sp < splits; ++sp, p += plane) {
         if (R % 4 == 0) {
-          const float4 lo = c < R ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
+          const float4 lo = c < R ? __ldcg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
           const float4 hi =
-              c + 4 < R ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
+              c + 4 < R ? __ldcg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
           v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
           v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] += c + i < R ? __ldg(p + i) : 0.0f;
+          for (int i = 0; i < 8; ++i) v[i] += c + i < R ? __ldcg(p + i) : 0.0f;
         }
       }
       const float m = row_mul ? mul * __ldg(row_mul + row0 + r) : mul;
@@ -298,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && kRank <= 64 ? 2 : 
     int cols_part, int vec_w, int vec_o, T* out, int64_t ldo) {
   using Tile = ExpandTile<T, kRank, kWCols>;
   constexpr bool kApart = std::is_same<T, float>::value;
+  griddep_launch_dependents();
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ TileIds ids;
   __nv_bfloat16* sh = reinterpret_cast<__nv_bfloat16*>(smem);
@@ -309,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && kRank <= 64 ? 2 : 
   const int c_lo = static_cast<int>(blockIdx.x % col_parts) * cols_part;
   const int c_hi = min(N, c_lo + cols_part);
   tile_ids(rows, row0, ids);
+  griddep_wait();
 
   // this thread's outputs of a tile: rows tid / 16 + 16 i, eight columns
   constexpr int kRowsT = kBM / 16;
@@ -696,6 +700,8 @@ __device__ __forceinline__ void tokens_tile(const TokensArgs<TX>& g, const float
 template <typename TX, typename T, int kRank>
 __global__ void __launch_bounds__(kThreads) tokens_pair_kernel(TokensArgs<TX> a, TokensArgs<T> b,
                                                                const float* __restrict__ scaling, Rows rows, int R) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int first = a.chunks * a.count;
   const int i = static_cast<int>(blockIdx.x);
   if (i < first) {
@@ -714,21 +720,39 @@ struct SumArgs {
   int64_t per;  // elements of one adapter
   void* out;
 };
+constexpr int kSplitsMost = 1024;  // of the rows of a batch (tokens_split, tokens_tc_split)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sum_splits_kernel(SumArgs ga, SumArgs gb, int S) {
+  griddep_wait();
   const SumArgs g = blockIdx.z ? gb : ga;
   const int s = blockIdx.y;
   const int64_t plane = g.per * S;
   const float* p0 = g.part + s * g.per;
   T* out = static_cast<T*>(g.out) + s * g.per;
+  // the splits that have rows of the adapter, in order
+  __shared__ uint16_t list[kSplitsMost];
+  __shared__ int count;
+  if (threadIdx.x < 32) {
+    int n = 0;
+    for (int base = 0; base < g.splits; base += 32) {
+      const int sp = base + static_cast<int>(threadIdx.x);
+      const bool there = sp < g.splits && __ldcg(g.found + sp * S + s);
+      const unsigned m = __ballot_sync(0xffffffffu, there);
+      if (there) list[n + __popc(m & ((1u << threadIdx.x) - 1u))] = static_cast<uint16_t>(sp);
+      n += __popc(m);
+    }
+    if (threadIdx.x == 0) count = n;
+  }
+  __syncthreads();
+  const int n = count;
   const int64_t start = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
   if (g.per % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % (4 * sizeof(T)) == 0) {
     for (int64_t i = start * 4; i < g.per; i += step * 4) {
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int sp = 0; sp < g.splits; ++sp) {
-        if (!__ldg(g.found + sp * S + s)) continue;
-        const float4 o = __ldg(reinterpret_cast<const float4*>(p0 + sp * plane + i));
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(p0 + list[j] * plane + i));
         v.x += o.x;
         v.y += o.y;
         v.z += o.z;
@@ -745,8 +769,7 @@ __global__ void __launch_bounds__(kThreads) sum_splits_kernel(SumArgs ga, SumArg
   }
   for (int64_t i = start; i < g.per; i += step) {
     float v = 0.0f;
-    for (int sp = 0; sp < g.splits; ++sp)
-      if (__ldg(g.found + sp * S + s)) v += __ldg(p0 + sp * plane + i);
+    for (int j = 0; j < n; ++j) v += __ldcg(p0 + list[j] * plane + i);
     out[i] = from_f<T>(v);
   }
 }
@@ -774,6 +797,14 @@ int prepare(K kernel, int bytes) {
 
 int launched(const char* what) {
   cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error("%s launch failed: %s", what, cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
+}
+
+int chained(const char* what, cudaError_t e) {
   if (e != cudaSuccess) {
     set_error("%s launch failed: %s", what, cudaGetErrorString(e));
     return W8A8_ERR_ACCELERATOR;
@@ -826,7 +857,7 @@ int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 // operands TMA can take (16-byte rows).
 constexpr int64_t kTcRows = 256;
 bool tc_shape(const LoraArgs& g) {
-  return g.dtype == W8A8_BF16 && g.M >= kTcRows && g.S <= 64 && g.K % 8 == 0 && g.N % 8 == 0 && g.R % 8 == 0 &&
+  return g.dtype == W8A8_BF16 && g.M >= kTcRows && g.M <= (1ll << 27) && g.S <= 64 && g.K % 8 == 0 && g.N % 8 == 0 && g.R % 8 == 0 &&
          g.K > 0 && g.N > 0;
 }
 bool tc_rows(const void* p, int64_t ld, int size) {
@@ -845,21 +876,23 @@ Split shrink_tc_split(int64_t M, int K) {
   const int per = static_cast<int>((steps + want - 1) / want);
   return {(steps + per - 1) / per, per * 64};
 }
-// One block a multiprocessor for 256 columns each; a block lists at most 2048 tiles.
-RowSplit tokens_tc_split(int64_t M, int C) {
+// One block a multiprocessor for 256 columns each, at most 256 MiB of partial sums;
+// a block lists at most 2048 tiles.
+RowSplit tokens_tc_split(int64_t M, int C, int S, int R) {
   const int64_t tiles = std::max<int64_t>(1, (M + kBM - 1) / kBM);
   const int64_t chunks = std::max<int64_t>(1, (C + 255) / 256);
-  int64_t want = std::max<int64_t>(1, std::min<int64_t>(device_sm_count() / chunks, tiles));
+  const int64_t one = std::max<int64_t>(1, static_cast<int64_t>(S) * R * C * 4);
+  int64_t want = std::max<int64_t>(1, std::min<int64_t>({device_sm_count() / chunks, tiles, (256ll << 20) / one}));
   want = std::max(want, (tiles + 2047) / 2048);
   const int64_t per = (tiles + want - 1) / want;
   return {static_cast<int>((tiles + per - 1) / per), per * kBM};
 }
 int shrink_tc(const LoraArgs& g, const void* x, int64_t ldx, bool codes, const float* x_scale, const void* w,
-              int64_t slot, bool w_rows, int64_t K, const Split& sp, float* part, int* counts, cudaStream_t stream) {
+              int64_t slot, bool w_rows, int64_t K, const Split& sp, float* part, int* counts, bool first, cudaStream_t stream) {
   const int64_t blocks = (g.M + 127) / 128 * sp.count;
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.S, 2ll * device_sm_count() / blocks));
   return lora_shrink_tc({x, codes, ldx, x_scale, w, w_rows, slot, g.M, K, g.S, g.R, sp.count, sp.per / 64,
-                         static_cast<int>(parts), part, counts},
+                         static_cast<int>(parts), part, counts, first, start_early(g)},
                         {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
 }
 
@@ -915,7 +948,7 @@ int shrink_pair(const ShrinkArgs<T, T>& dy, int splits_dy, const ShrinkArgs<TX, 
 
 template <typename T, bool kWCols>
 int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, int64_t slot,
-           const float* scaling, const Rows& rows, int N, int R, T* out, int64_t ldo,
+           const float* scaling, const Rows& rows, int N, int R, T* out, int64_t ldo, bool early,
            cudaStream_t stream) {
   const int64_t tiles = (rows.M + kBM - 1) / kBM;
   const int col_tiles = (N + kBN - 1) / kBN;
@@ -927,12 +960,13 @@ int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, i
   const int per = (col_tiles + parts - 1) / parts;
   parts = (col_tiles + per - 1) / per;
   const dim3 grid(static_cast<unsigned>(tiles * parts), 1, parts_of(rows.M, rows.S, parts));
+  cudaError_t e = cudaSuccess;
 #define EXPAND(RANK)                                                                              \
   {                                                                                               \
     auto k = expand_kernel<T, RANK, kWCols>;                                                      \
     constexpr int bytes = ExpandTile<T, RANK, kWCols>::kBytes;                                    \
     if (int rc = prepare(k, bytes)) return rc;                                                    \
-    k<<<grid, kThreads, bytes, stream>>>(y, ldy, part, splits, w, slot, scaling, rows, N, R, parts, \
+    e = launch_chained(early, k, grid, kThreads, bytes, stream, y, ldy, part, splits, w, slot, scaling, rows, N, R, parts, \
                                          per * kBN, vw, vo, out, ldo);                            \
   }
   switch (pad_rank(R)) {
@@ -942,23 +976,24 @@ int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, i
     default: EXPAND(128) break;
   }
 #undef EXPAND
-  return launched("lora expand");
+  return chained("lora expand", e);
 }
 
 template <typename TX, typename T>
 int tokens_pair(const TokensArgs<TX>& a, const TokensArgs<T>& b, const float* scaling, const Rows& rows, int R,
-                cudaStream_t stream) {
+                bool early, cudaStream_t stream) {
   const dim3 grid(a.chunks * a.count + b.chunks * b.count, 1, rows.S);
+  cudaError_t e = cudaSuccess;
 #define TOKENS(RANK)                                                       \
   {                                                                        \
     auto k = tokens_pair_kernel<TX, T, RANK>;                              \
     constexpr int bytes = std::max(TokensTile<TX, T, RANK, false>::kBytes, TokensTile<T, T, RANK, true>::kBytes); \
     if (int rc = prepare(k, bytes)) return rc;                             \
-    k<<<grid, kThreads, bytes, stream>>>(a, b, scaling, rows, R);          \
+    e = launch_chained(early, k, grid, kThreads, bytes, stream, a, b, scaling, rows, R); \
   }
   BY_RANK(TOKENS)
 #undef TOKENS
-  return launched("lora tokens");
+  return chained("lora tokens", e);
 }
 
 // Up to one tile of rows.
@@ -975,25 +1010,13 @@ int add_few_rows(const LoraArgs& g, const Rows& rows, float* h, cudaStream_t str
   const unsigned m = static_cast<unsigned>(g.M);
   shrink_row_kernel<T><<<dim3(R, m), kThreads, 0, stream>>>(x, g.ldx, a, g.lda, rows, K, R, vec, h);
   if (int rc = launched("lora shrink")) return rc;
-  cudaLaunchConfig_t lc{};
-  lc.gridDim = dim3((N + kThreads - 1) / kThreads, m);
-  lc.blockDim = dim3(kThreads);
-  lc.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  lc.attrs = attr;
-  lc.numAttrs = 1;
+  const bool early = true;  // one row tile: latency is all
   const bool whole = R % 8 == 0 && aligned(b, R, sizeof(T)) && aligned(b, g.ldb, sizeof(T));
-  const cudaError_t e =
-      cudaLaunchKernelEx(&lc, whole ? expand_row_kernel<T, true> : expand_row_kernel<T, false>, y, g.ldy,
-                         static_cast<const float*>(h), b, g.ldb, g.scaling, rows, N, R,
-                         static_cast<T*>(g.out), g.ldo);
-  if (e != cudaSuccess) {
-    set_error("lora expand launch failed: %s", cudaGetErrorString(e));
-    return W8A8_ERR_ACCELERATOR;
-  }
-  return 0;
+  return chained("lora expand",
+                 launch_chained(early, whole ? expand_row_kernel<T, true> : expand_row_kernel<T, false>,
+                                dim3((N + kThreads - 1) / kThreads, m), kThreads, 0, stream, y, g.ldy,
+                                static_cast<const float*>(h), b, g.ldb, g.scaling, rows, N, R,
+                                static_cast<T*>(g.out), g.ldo));
 }
 
 template <typename T>
@@ -1007,19 +1030,19 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
   if (tc_shape(g) && tc_x(g) && tc_weights(g.a, g.lda, K, g.S)) {
     sp = shrink_tc_split(g.M, K);
     counts = reinterpret_cast<int*>(part + sp.count * g.M * g.R);
-    if (int rc = shrink_tc(g, g.x, g.ldx, false, nullptr, g.a, g.lda, true, K, sp, part, counts, stream)) return rc;
+    if (int rc = shrink_tc(g, g.x, g.ldx, false, nullptr, g.a, g.lda, true, K, sp, part, counts, true, stream)) return rc;
   } else if (int rc = shrink<T>(shrink_args<T, T, true>(static_cast<const T*>(g.x), g.ldx, nullptr,
                                                         static_cast<const T*>(g.a), g.lda, K, R, sp, part),
                                 true, sp.count, rows, R, stream)) {
     return rc;
   }
   if (counts && tc_rows(g.y, g.ldy, 2) && tc_rows(g.out, g.ldo, 2) && tc_weights(g.b, g.ldb, R, g.S)) {
-    return lora_expand_tc({g.y, g.ldy, counts, part, sp.count, g.b, 1, g.ldb, g.scaling, g.out, g.ldo, g.M, g.N, g.S, g.R},
+    return lora_expand_tc({g.y, g.ldy, counts, part, sp.count, g.b, 1, g.ldb, g.scaling, g.out, g.ldo, g.M, g.N, g.S, g.R, start_early(g)},
                           {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
   }
   return expand<T, true>(static_cast<const T*>(g.y), g.ldy, part, sp.count,
                          static_cast<const T*>(g.b), g.ldb, g.scaling, rows, N, R,
-                         static_cast<T*>(g.out), g.ldo, stream);
+                         static_cast<T*>(g.out), g.ldo, start_early(g), stream);
 }
 
 struct BackwardPlan {
@@ -1032,8 +1055,8 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R
   const int r = static_cast<int>(R), s = static_cast<int>(S), k = static_cast<int>(K), n = static_cast<int>(N);
   p.h = tc ? shrink_tc_split(M, k) : shrink_split(M, k);
   p.g = tc ? shrink_tc_split(M, n) : shrink_split(M, n);
-  p.a = tc ? tokens_tc_split(M, k) : tokens_split(M, k, s, r);
-  p.b = tc ? tokens_tc_split(M, n) : tokens_split(M, n, s, r);
+  p.a = tc ? tokens_tc_split(M, k, s, r) : tokens_split(M, k, s, r);
+  p.b = tc ? tokens_tc_split(M, n, s, r) : tokens_split(M, n, s, r);
   p.off_g = up(p.h.count * M * R * 4);
   p.off_a = p.off_g + up(p.g.count * M * R * 4);
   p.off_b = p.off_a + up(p.a.count * S * R * K * 4);
@@ -1052,6 +1075,7 @@ template <typename T, typename TX>
 int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
   const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
+  const bool early = start_early(g);
   const bool tc = tc_shape(g) && tc_x(g) && tc_rows(g.y, g.ldy, 2) && tc_weights(g.a, g.lda, g.K, g.S) &&
                   tc_weights(g.b, g.ldb, g.R, g.S);
   const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R, tc);
@@ -1069,7 +1093,7 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   const T* b = static_cast<const T*>(g.b);
   if (g.M > 0) {
     if (tc) {
-      if (int rc = shrink_tc(g, dy, g.ldy, false, nullptr, b, g.ldb, false, N, p.g, pg, counts, stream)) return rc;
+      if (int rc = shrink_tc(g, dy, g.ldy, false, nullptr, b, g.ldb, false, N, p.g, pg, counts, true, stream)) return rc;
     } else {
       const auto sg = shrink_args<T, T, false>(dy, g.ldy, nullptr, b, g.ldb, N, R, p.g, pg);
       const auto sh = shrink_args<TX, T, true>(x, g.ldx, g.x_scale, a, g.lda, K, R, p.h, ph);
@@ -1080,14 +1104,14 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
     }
     if (g.out && tc && tc_rows(g.out, g.ldo, 2)) {
       if (int rc = lora_expand_tc({g.accumulate ? g.out : nullptr, g.ldo, counts, pg, p.g.count, a, 0, g.lda, g.scaling,
-                                   g.out, g.ldo, g.M, g.K, g.S, g.R},
+                                   g.out, g.ldo, g.M, g.K, g.S, g.R, early},
                                   {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream)) {
         return rc;
       }
     } else if (g.out) {
       if (int rc = expand<T, false>(g.accumulate ? static_cast<const T*>(g.out) : nullptr, g.ldo, pg,
                                     p.g.count, a, g.lda, g.scaling, rows, K, R,
-                                    static_cast<T*>(g.out), g.ldo, stream)) {
+                                    static_cast<T*>(g.out), g.ldo, start_early(g), stream)) {
         return rc;
       }
     }
@@ -1097,16 +1121,16 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
     const LoraRows lr{g.adapter, g.adapter64, g.rows_per_index, g.M, g.S};
     void *qa = ws + p.off_pa, *qb = ws + p.off_pb;
     uint8_t* info = ws + p.off_info;
-    if (int rc = shrink_tc(g, x, g.ldx, g.x_scale != nullptr, g.x_scale, a, g.lda, true, K, p.h, ph, counts, stream)) return rc;
-    if (int rc = lora_rank_pieces({pg, p.g.count, g.x_scale, qa, ph, p.h.count, qb, g.scaling, R, info}, lr, stream)) {
+    if (int rc = shrink_tc(g, x, g.ldx, g.x_scale != nullptr, g.x_scale, a, g.lda, true, K, p.h, ph, nullptr, false, stream)) return rc;
+    if (int rc = lora_rank_pieces({pg, p.g.count, g.x_scale, qa, ph, p.h.count, qb, g.scaling, R, info, early}, lr, stream)) {
       return rc;
     }
     const int per_a = static_cast<int>(p.a.per / kBM), per_b = static_cast<int>(p.b.per / kBM);
     if (int rc = lora_tokens_tc({x, g.x_scale != nullptr, g.ldx, qa, g.M, g.K, g.S, g.R, 0, p.a.count, per_a,
-                                 info, pa, fa}, lr, stream)) {
+                                 info, pa, fa, early}, lr, stream)) {
       return rc;
     }
-    if (int rc = lora_tokens_tc({dy, 0, g.ldy, qb, g.M, g.N, g.S, g.R, 1, p.b.count, per_b, info, pb, fb}, lr,
+    if (int rc = lora_tokens_tc({dy, 0, g.ldy, qb, g.M, g.N, g.S, g.R, 1, p.b.count, per_b, info, pb, fb, early}, lr,
                                 stream)) {
       return rc;
     }
@@ -1115,15 +1139,16 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
                             aligned(x, g.ldx, sizeof(TX)), pa, fa};
     const TokensArgs<T> tb{dy, g.ldy, nullptr, ph, p.h.count, N, p.b.per, p.b.count, (N + kBN - 1) / kBN,
                            aligned(dy, g.ldy, sizeof(T)), pb, fb};
-    if (int rc = tokens_pair<TX, T>(ta, tb, g.scaling, rows, R, stream)) return rc;
+    if (int rc = tokens_pair<TX, T>(ta, tb, g.scaling, rows, R, early, stream)) return rc;
   }
   const SumArgs sa{pa, fa, p.a.count, g.R * g.K, g.da}, sb{pb, fb, p.b.count, g.R * g.N, g.db};
   const int64_t most = std::max(sa.per, sb.per);
   const int64_t want = (most + 4 * kThreads - 1) / (4 * kThreads);
   const int64_t cap = std::max<int64_t>(1, 8ll * device_sm_count() / g.S);
-  sum_splits_kernel<T><<<dim3(static_cast<unsigned>(std::min(want, cap)), static_cast<unsigned>(g.S), 2),
-                         kThreads, 0, stream>>>(sa, sb, static_cast<int>(g.S));
-  return launched("lora gradient sum");
+  return chained("lora gradient sum",
+                 launch_chained(early, sum_splits_kernel<T>,
+                                dim3(static_cast<unsigned>(std::min(want, cap)), static_cast<unsigned>(g.S), 2),
+                                kThreads, 0, stream, sa, sb, static_cast<int>(g.S)));
 }
 
 }  // namespace
@@ -1135,7 +1160,7 @@ int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t
     return up(std::max(shrink_split(M, k).count, shrink_tc_split(M, k).count) * M * R * 4 + (M + 127) / 128 * 4);
   }
   return std::max(backward_plan(M, N, K, S, R, false).bytes,
-                  M >= kTcRows ? backward_plan(M, N, K, S, R, true).bytes : 0);
+                  M >= kTcRows && S <= 64 ? backward_plan(M, N, K, S, R, true).bytes : 0);
 }
 
 int lora_add_launch(const LoraArgs& g, cudaStream_t stream) {

@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
     const float* __restrict__ row_mul, int K, int R, int kb_split, float* __restrict__ part,
     int* __restrict__ counts) {
   using C = ShrinkTc<kCodes, kRank>;
+  griddep_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -225,7 +226,6 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
   }
   __syncthreads();
   const int total = count;
-  if (tid == 0 && blockIdx.y == 0 && blockIdx.z == 0) counts[blockIdx.x] = total;  // for expand_tc_kernel
   const uint32_t tmem = bars->tmem;
   // this block's adapters of the tile: those from blockIdx.z on, gridDim.z apart, kAtOnce a pass
   const int mine_n = total > static_cast<int>(blockIdx.z) ? (total - blockIdx.z + gridDim.z - 1) / gridDim.z : 0;
@@ -307,6 +307,9 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
       }
     }
   } else {
+    // x and W_s are the caller's; what is written may still be in use by the kernel before
+    if (warp < 4) griddep_wait();
+    if (counts && tid == 0 && blockIdx.y == 0 && blockIdx.z == 0) counts[blockIdx.x] = total;  // for expand_tc_kernel
     uint32_t it = 0, pass = 0;
     bool ok = true;
     for (int i0 = 0; ok && i0 < mine_n; i0 += C::kAtOnce, ++pass) {
@@ -395,9 +398,11 @@ __global__ void __launch_bounds__(256) rank_pieces_kernel(RankSide a, RankSide b
                                                           int R, int64_t m_pad, uint8_t* __restrict__ info) {
   __shared__ float v[kTile][kRank + 1];
   __shared__ TileIds ids;
+  griddep_launch_dependents();
   const RankSide g = blockIdx.y ? b : a;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kTile;
   tile_ids(rows, row0, ids);
+  griddep_wait();
   constexpr int kVecs = kRank / 4;
   constexpr int kEach = kTile * kVecs / 256;  // 1 .. 8 vectors a thread
   const int64_t plane = rows.M * R;
@@ -411,7 +416,7 @@ __global__ void __launch_bounds__(256) rank_pieces_kernel(RankSide a, RankSide b
       const float* p = g.part + (row0 + r) * R + c;
 #pragma unroll 4
       for (int sp = 0; sp < g.splits; ++sp) {
-        const float4 q = __ldg(reinterpret_cast<const float4*>(p + sp * plane));
+        const float4 q = __ldcg(reinterpret_cast<const float4*>(p + sp * plane));
         sum.x += q.x;
         sum.y += q.y;
         sum.z += q.z;
@@ -479,6 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
     int tiles, int tiles_split, const uint8_t* __restrict__ info, float* __restrict__ part,
     int* __restrict__ found) {
   using T = TokensTc<kCodes, kRank>;
+  griddep_launch_dependents();
   // two accumulators of 2 kRank columns (the sums with the first pieces, then the second)
   constexpr uint32_t kTokenCols = 4 * kRank;
   extern __shared__ uint8_t smem_raw[];
@@ -506,10 +512,11 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
     bars->abort_flag = 0;
     fence_mbarrier_init();
   }
+  griddep_wait();  // info and the pieces
   // which adapters these rows have
   for (int s = warp; s < rows.S; s += kThreads / 32) {
     int any = 0;
-    for (int i = lane; i < n_tiles; i += 32) any |= __ldg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
+    for (int i = lane; i < n_tiles; i += 32) any |= __ldcg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
     any = __any_sync(0xffffffffu, any);
     if (lane == 0) {
       present[s] = static_cast<uint8_t>(any);
@@ -533,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
   uint32_t it = 0, segment = 0;
   for (int s = 0; s < rows.S; ++s) {
     if (!present[s]) continue;
-    for (int i = tid; i < n_tiles; i += kThreads) live[i] = __ldg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
+    for (int i = tid; i < n_tiles; i += kThreads) live[i] = __ldcg(info + static_cast<int64_t>(s) * tiles + t_lo + i);
     __syncthreads();
     tc_fence_after();
     if (warp == kTmaWarp) {
@@ -726,6 +733,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
     const int* __restrict__ counts, const float* __restrict__ part, int splits, const float* __restrict__ scaling, Rows rows, int N,
     int R) {
   using C = ExpandTc<kRank>;
+  griddep_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -784,13 +792,14 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   uint32_t h_count = 0;  // times h has been laid down
   int to_free = -1;      // the stage whose store may still be reading
 
+  griddep_wait();  // the rank side, and the adapters' counts
   // this block's share [lo, hi) of the whole cost, and the row tile it starts in: a
   // thread adds up a run of row tiles, a scan over the block gives the run's start
   {
     const int64_t run = (row_tiles + kEThreads - 1) / kEThreads;
     const int64_t first = min(row_tiles, tid * run), last = min(row_tiles, first + run);
     int64_t mine = 0;
-    for (int64_t i = first; i < last; ++i) mine += tile_cost(__ldg(counts + i));
+    for (int64_t i = first; i < last; ++i) mine += tile_cost(__ldcg(counts + i));
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -809,7 +818,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
     const int64_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
     int64_t at = before * col_tiles;
     for (int64_t i = first; i < last; ++i) {
-      const int64_t end = at + static_cast<int64_t>(tile_cost(__ldg(counts + i))) * col_tiles;
+      const int64_t end = at + static_cast<int64_t>(tile_cost(__ldcg(counts + i))) * col_tiles;
       if (lo >= at && lo < end) {
         start_tile = i;
         start_at = at;
@@ -826,7 +835,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   int64_t at = start_at;
   for (int64_t rt = start_tile; rt < row_tiles && at < hi; ++rt) {
     // the row tile's tiles that start in the share
-    const int64_t cost = tile_cost(__ldg(counts + rt));
+    const int64_t cost = tile_cost(__ldcg(counts + rt));
     const int t_lo = static_cast<int>(lo <= at ? 0 : min(static_cast<int64_t>(col_tiles), (lo - at + cost - 1) / cost));
     const int t_hi = static_cast<int>(min(static_cast<int64_t>(col_tiles), (hi - at + cost - 1) / cost));
     at += cost * col_tiles;
@@ -932,7 +941,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
 #pragma unroll 3
           for (int sp = 0; sp < splits; ++sp) {
             const float4* q = reinterpret_cast<const float4*>(p0 + sp * rows.M * R + c);
-            const float4 a = __ldg(q), b = __ldg(q + 1);
+            const float4 a = __ldcg(q), b = __ldcg(q + 1);
             x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
             x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
           }
@@ -1098,6 +1107,14 @@ int launched(const char* what) {
   return 0;
 }
 
+int chained(const char* what, cudaError_t e) {
+  if (e != cudaSuccess) {
+    set_error("%s launch failed: %s", what, cudaGetErrorString(e));
+    return W8A8_ERR_ACCELERATOR;
+  }
+  return 0;
+}
+
 template <bool kCodes, int kRank, bool kWRows>
 int shrink_rank(const ShrinkTcArgs& g, const Rows& rows, cudaStream_t stream) {
   CUtensorMap tx, tw;
@@ -1113,9 +1130,12 @@ int shrink_rank(const ShrinkTcArgs& g, const Rows& rows, cudaStream_t stream) {
   constexpr int bytes = ShrinkTc<kCodes, kRank>::kBytes;
   if (int rc = opt_in(k, bytes)) return rc;
   const dim3 grid(static_cast<unsigned>((g.M + kSRows - 1) / kSRows), g.splits, g.parts);
-  k<<<grid, kThreads, bytes, stream>>>(tx, tw, rows, g.x_scale, static_cast<int>(g.K), static_cast<int>(g.R),
+  if (g.first) {
+    k<<<grid, kThreads, bytes, stream>>>(tx, tw, rows, g.x_scale, static_cast<int>(g.K), static_cast<int>(g.R),
                                        g.kb_split, g.part, g.counts);
-  return launched("lora shrink");
+    return launched("lora shrink");
+  }
+  return chained("lora shrink", launch_chained(g.early != 0, k, grid, kThreads, bytes, stream, tx, tw, rows, g.x_scale, static_cast<int>(g.K), static_cast<int>(g.R), g.kb_split, g.part, g.counts));
 }
 
 template <bool kCodes, bool kWRows>
@@ -1141,9 +1161,7 @@ int tokens_rank(const TokensTcArgs& g, const Rows& rows, cudaStream_t stream) {
   constexpr int bytes = TokensTc<kCodes, kRank>::kBytes;
   if (int rc = opt_in(k, bytes)) return rc;
   const dim3 grid(static_cast<unsigned>((g.C + kTCols - 1) / kTCols), g.splits);
-  k<<<grid, kThreads, bytes, stream>>>(tx, th, rows, static_cast<int>(g.C), static_cast<int>(g.R),
-                                       static_cast<int>(tiles), g.tiles_split, g.info, g.part, g.found);
-  return launched("lora tokens");
+  return chained("lora tokens", launch_chained(g.early != 0, k, grid, kThreads, bytes, stream, tx, th, rows, static_cast<int>(g.C), static_cast<int>(g.R), static_cast<int>(tiles), g.tiles_split, g.info, g.part, g.found));
 }
 
 template <bool kCodes, bool kByCol>
@@ -1171,10 +1189,8 @@ int expand_rank(const ExpandTcArgs& g, const Rows& rows, cudaStream_t stream) {
   constexpr int bytes = ExpandTc<kRank>::kBytes;
   if (int rc = opt_in(k, bytes)) return rc;
   const int64_t tiles = (g.M + kERows - 1) / kERows * ((g.N + kECols - 1) / kECols);
-  k<<<static_cast<unsigned>(std::min<int64_t>(tiles, device_sm_count())), kEThreads, bytes, stream>>>(
-      ty, tw, to, static_cast<const __nv_bfloat16*>(g.y), static_cast<__nv_bfloat16*>(g.out), g.counts, g.part,
-      g.splits, g.scaling, rows, static_cast<int>(g.N), static_cast<int>(g.R));
-  return launched("lora expand");
+  return chained("lora expand", launch_chained(g.early != 0, k, dim3(static_cast<unsigned>(std::min<int64_t>(tiles, device_sm_count()))),
+      kEThreads, bytes, stream, ty, tw, to, static_cast<const __nv_bfloat16*>(g.y), static_cast<__nv_bfloat16*>(g.out), g.counts, g.part, g.splits, g.scaling, rows, static_cast<int>(g.N), static_cast<int>(g.R)));
 }
 
 template <bool kWCols>
@@ -1190,9 +1206,8 @@ int pieces_rank(const RankPiecesArgs& g, const Rows& rows, cudaStream_t stream) 
   const int64_t tiles = (rows.M + kTile - 1) / kTile;
   const RankSide a{g.part_a, g.splits_a, g.row_mul_a, static_cast<__nv_bfloat16*>(g.out_a)};
   const RankSide b{g.part_b, g.splits_b, nullptr, static_cast<__nv_bfloat16*>(g.out_b)};
-  rank_pieces_kernel<kRank><<<dim3(static_cast<unsigned>(tiles), 2), 256, 0, stream>>>(
-      a, b, g.scaling, rows, g.R, tiles * kTile, g.info);
-  return launched("lora rank pieces");
+  return chained("lora rank pieces", launch_chained(g.early != 0, rank_pieces_kernel<kRank>, dim3(static_cast<unsigned>(tiles), 2), 256, 0,
+      stream, a, b, g.scaling, rows, g.R, tiles * kTile, g.info));
 }
 
 }  // namespace
