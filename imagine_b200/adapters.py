@@ -205,7 +205,8 @@ def lora_backward(dy: torch.Tensor, x: Optional[torch.Tensor], a: torch.Tensor, 
     ``da[s]`` and ``db[s]`` the sums over the rows of adapter s (zero without
     rows), all in dy's dtype.  ``x`` is the forward input, or with ``x_scale`` the
     int8 codes of ``quantize_int8_rowwise`` (its 8-bit checkpoint; one fp32 scale a
-    row).  A given ``dx`` (the base linear's input gradient) is added to, in place.
+    row).  A given ``dx`` (the base linear's input gradient; no operand's memory) is added
+    to, in place.
     ``need_dx`` / ``need_weights`` False: None in their place (x may then be None)."""
     dev = _cuda("dy", dy).device
     lead, n, k, dtype = dy.shape[:-1], dy.shape[-1], a.shape[-1], dy.dtype
@@ -240,7 +241,7 @@ def lora_backward(dy: torch.Tensor, x: Optional[torch.Tensor], a: torch.Tensor, 
         da = torch.empty_like(a) if slot_a == r * k else dy.new_empty((s, r, k))
         db = torch.empty_like(b) if slot_b == n * r else dy.new_empty((s, n, r))
     with _on(dev):
-        nbytes = _lora_bytes(dev.index, m, n, k, s, r, 1)
+        nbytes = _lora_bytes(dev.index, m, n, k, s, r, 1 if need_weights else 2)
         ws = _workspace(nbytes, dev)
         N.check(N.LIB.w8a8_lora_backward(
             dy2.data_ptr(), lddy, _ptr(x2), ldx, _ptr(xs), code, a.data_ptr(), slot_a, b.data_ptr(),
@@ -305,7 +306,10 @@ class _Int8LinearLora(torch.autograd.Function):
             N.check(N.LIB.w8a8_gemv_dequant(_vp(q), _vp(w), _vp(xs), ctypes.byref(ep), _vp(y),
                                             _code(x.dtype), m, n, k, stream))
         elif m > 0:
-            L._gemm_dequant(q, w, xs.reshape(-1), ep, y, x.dtype, m, n, k, None, None, stream)
+            # the linear's split-K scratch belongs to a stream, and a graph may be replayed
+            # on any: captured, tiles run whole (the same bits)
+            split = 1 if torch.cuda.is_current_stream_capturing() else None
+            L._gemm_dequant(q, w, xs.reshape(-1), ep, y, x.dtype, m, n, k, None, split, stream)
         y = y.reshape(*x.shape[:-1], n)
         lora_add(y, x, a, b, adapter, scaling, out=y)
         kept = (x, None) if keep_input else (q.reshape(x.shape), xs)
@@ -336,7 +340,9 @@ def int8_linear_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
 
     For the backward pass it keeps the int8 codes that the linear made of x
     (half of a bf16 input's bytes), from which da and db are taken; with ``keep_input`` it
-    keeps x itself instead.  Operands as in the two operators."""
+    keeps x itself instead.  Operands as in the two operators.  A training step that is
+    captured into a CUDA graph is captured whole, with no eager graph of the same leaves
+    alive (autograd's accumulation would run on the eager graph's stream)."""
     dev = _cuda("x", x).device
     with _on(dev):
         _cuda("weight", weight, dev)
@@ -351,6 +357,9 @@ def int8_linear_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
             raise ValueError(f"INT8 weight scale must be scalar or per-output-channel, got "
                              f"{tuple(weight_scale.shape)} for weight shape {tuple(weight.shape)}")
         _code(x.dtype)
+        for name, t in (("weight_scale", weight_scale), ("bias", bias), ("scaling", scaling)):
+            if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+                raise ValueError(f"{name} is frozen in int8_linear_lora: detach it")
         _adapters(a, b, k, n, x.dtype, dev)
         scaling = _scaling(scaling, a.shape[0], dev)
         return _Int8LinearLora.apply(x, weight, weight_scale, bias, a, b, adapter, scaling, keep_input)

@@ -935,6 +935,7 @@ int check_lora_common(const LoraArgs& g, int64_t workspace_bytes, int backward) 
 int64_t w8a8_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R,
                                   int backward) {
   if (int rc = check_lora_shape(M, N, K, S, R)) return rc;
+  if (backward < 0 || backward > 2) return fail(W8A8_ERR_VALUE, "lora: backward is 0, 1 or 2");
   return lora_workspace_bytes(M, N, K, S, R, backward);
 }
 
@@ -985,6 +986,7 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
   if ((da == nullptr) != (db == nullptr)) return fail(W8A8_ERR_VALUE, "lora: da and db go together");
   if (N == 0 || K == 0) return fail(W8A8_ERR_VALUE, "lora: gradients need N > 0 and K > 0");
   if (!dx && !da) return finish(0);
+  if (dx && (dx == dy || dx == x)) return fail(W8A8_ERR_VALUE, "lora: dx is an operand's memory");
   if (M > 0) {
     if (!dy || (da && !x)) return fail(W8A8_ERR_VALUE, "NULL tensor pointer");
     if (lddy < N || (da && ldx < K) || (dx && lddx < K)) {
@@ -1019,7 +1021,7 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
   g.S = S;
   g.R = R;
   g.workspace = workspace;
-  if (int rc = check_lora_common(g, workspace_bytes, 1)) return rc;
+  if (int rc = check_lora_common(g, workspace_bytes, da ? 1 : 2)) return rc;
   const int64_t size = float_size(dtype);
   if (bad_align(da, size) || bad_align(db, size)) {
     return fail(W8A8_ERR_VALUE, "lora: pointer not aligned to its element");

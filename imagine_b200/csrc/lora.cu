@@ -470,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && kRank <= 64 ? 2 : 
 // what has to be read is the adapters' weights, once, and latency counts.  The
 // second kernel starts while the first runs (programmatic dependent launch): its
 // weights and y are on their way when h arrives.
-// 64 rows, 32 adapters of rank 32, 4096 -> 12288: see the measurements at few_rows().
+// 64 rows, 32 adapters of rank 32, 4096 -> 12288: 9 and 13 us where the tiles took
+// 16 and 96 (their blocks go through their adapters one after another).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) shrink_row_kernel(const T* __restrict__ x, int64_t ldx,
                                                               const T* __restrict__ a, int64_t slot,
@@ -1048,7 +1049,7 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
 struct BackwardPlan {
   Split h, g;
   RowSplit a, b;
-  int64_t off_g, off_a, off_b, off_found, off_pa, off_pb, off_info, off_counts, bytes;
+  int64_t off_g, off_counts, off_a, off_b, off_found, off_pa, off_pb, off_info, bytes;  // dx alone: up to off_a
 };
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, bool tc) {
   BackwardPlan p;
@@ -1058,7 +1059,8 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R
   p.a = tc ? tokens_tc_split(M, k, s, r) : tokens_split(M, k, s, r);
   p.b = tc ? tokens_tc_split(M, n, s, r) : tokens_split(M, n, s, r);
   p.off_g = up(p.h.count * M * R * 4);
-  p.off_a = p.off_g + up(p.g.count * M * R * 4);
+  p.off_counts = p.off_g + up(p.g.count * M * R * 4);
+  p.off_a = p.off_counts + (tc ? up((M + 127) / 128 * 4) : 0);
   p.off_b = p.off_a + up(p.a.count * S * R * K * 4);
   p.off_found = p.off_b + up(p.b.count * S * R * N * 4);
   p.off_pa = p.off_found + up((p.a.count + p.b.count) * S * 4);
@@ -1066,8 +1068,7 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R
   const int64_t pieces = tc ? up(2 * pad_rank(r) * tiles * kBM * 2) : 0;
   p.off_pb = p.off_pa + pieces;
   p.off_info = p.off_pb + pieces;
-  p.off_counts = p.off_info + (tc ? up(S * tiles) : 0);
-  p.bytes = p.off_counts + (tc ? up((M + 127) / 128 * 4) : 0);
+  p.bytes = p.off_info + (tc ? up(S * tiles) : 0);
   return p;
 }
 
@@ -1159,8 +1160,10 @@ int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t
   if (!backward) {
     return up(std::max(shrink_split(M, k).count, shrink_tc_split(M, k).count) * M * R * 4 + (M + 127) / 128 * 4);
   }
-  return std::max(backward_plan(M, N, K, S, R, false).bytes,
-                  M >= kTcRows && S <= 64 ? backward_plan(M, N, K, S, R, true).bytes : 0);
+  const BackwardPlan plain = backward_plan(M, N, K, S, R, false);
+  const bool tc = M >= kTcRows && S <= 64;
+  const BackwardPlan other = tc ? backward_plan(M, N, K, S, R, true) : plain;
+  return backward == 2 ? std::max(plain.off_a, other.off_a) : std::max(plain.bytes, other.bytes);
 }
 
 int lora_add_launch(const LoraArgs& g, cudaStream_t stream) {

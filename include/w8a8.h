@@ -567,9 +567,11 @@ int w8a8_sampler_step(float* x, const void* out_cond, const void* out_uncond, in
  * quantiser (w8a8_quantize_rowwise): the activation's 8-bit checkpoint.
  * Sums are taken in a fixed order: the same call gives the same bits.
  *
+ * dx may not overlap dy, x, a or b.
+ *
  * workspace: at least w8a8_lora_workspace_bytes(M, N, K, S, R, backward)
- * bytes, 256-byte aligned, any content; calls sharing one must not overlap on
- * the GPU. */
+ * bytes (backward: 0 w8a8_lora_add, 1 w8a8_lora_backward, 2 its dx alone),
+ * 256-byte aligned, any content; calls sharing one must not overlap on the GPU. */
 int64_t w8a8_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R,
                                   int backward);
 int w8a8_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dtype, const void* a,

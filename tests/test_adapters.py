@@ -43,7 +43,7 @@ def test_lora_add_with_nothing_to_do():
 
 def _back(**kw):
     d = dict(dy=P, lddy=64, x=P, ldx=32, xs=None, dtype=N.BF16, a=P, slot_a=256, b=P, slot_b=512, adapter=P, is64=0,
-             per=1, scaling=P, dx=P, lddx=32, acc=0, da=P, db=P, m=10, n=64, k=32, s=2, r=8, ws=P, ws_bytes=1 << 30)
+             per=1, scaling=P, dx=2 * P, lddx=32, acc=0, da=P, db=P, m=10, n=64, k=32, s=2, r=8, ws=P, ws_bytes=1 << 30)
     d.update(kw)
     return N.LIB.w8a8_lora_backward(d["dy"], d["lddy"], d["x"], d["ldx"], d["xs"], d["dtype"], d["a"], d["slot_a"],
                                     d["b"], d["slot_b"], d["adapter"], d["is64"], d["per"], d["scaling"], d["dx"],
@@ -55,8 +55,8 @@ def _back(**kw):
     (dict(r=200), "rank"), (dict(da=None), "go together"), (dict(db=None), "go together"), (dict(n=0), "N > 0"),
     (dict(k=0), "N > 0"), (dict(dy=None), "NULL"), (dict(x=None), "NULL"), (dict(lddy=3), "stride"),
     (dict(ldx=3), "stride"), (dict(lddx=3), "stride"), (dict(dtype=N.E4M3), "floating"), (dict(a=None), "NULL"),
-    (dict(x=P + 1), "aligned"), (dict(xs=P + 1), "aligned"), (dict(dx=P + 1), "aligned"), (dict(da=P + 1), "aligned"),
-    (dict(ws_bytes=100), "workspace")])
+    (dict(x=P + 1), "aligned"), (dict(xs=P + 1), "aligned"), (dict(dx=2 * P + 1), "aligned"), (dict(da=P + 1), "aligned"),
+    (dict(ws_bytes=100), "workspace"), (dict(dx=P + 64, dy=P + 64), "operand"), (dict(dx=P + 64, x=P + 64), "operand")])
 def test_lora_backward_refuses(kw, word):
     assert _back(**kw) == N.ERR_VALUE
     assert word in _err()
@@ -67,6 +67,9 @@ def test_workspace_sizes():
     need = N.LIB.w8a8_lora_workspace_bytes
     assert need(10, 64, 32, 2, 8, 0) >= 10 * 8 * 4
     assert need(10, 64, 32, 2, 200, 0) == N.ERR_VALUE and need(-1, 64, 32, 2, 8, 1) == N.ERR_VALUE
+    assert need(10, 64, 32, 2, 8, 3) == N.ERR_VALUE
+    # the input gradient alone takes no room for the adapters' sums
+    assert need(4096, 4096, 4096, 4, 64, 2) < need(4096, 4096, 4096, 4, 64, 1)
     # partial sums of the adapters' gradients stay bounded
     assert need(100000, 12288, 12288, 64, 128, 1) < 10 << 30
     assert N.LIB.w8a8_input_grad_workspace_bytes(10, 64, 32, N.S8) == N.ERR_VALUE

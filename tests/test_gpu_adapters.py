@@ -307,6 +307,42 @@ def test_int8_linear_lora_trains():
     assert torch.equal(only, q_again)
 
 
+def test_int8_linear_lora_captured_and_frozen():
+    """A captured training step on its own stream, replayed with new contents; what is frozen says so."""
+    import imagine_b200 as W
+
+    g = torch.Generator(device="cuda").manual_seed(12)
+    m, k, n, r = 40, 512, 768, 8
+    x = torch.randn(m, k, generator=g, device="cuda").bfloat16()
+    w, ws = W.quantize_weight((torch.randn(n, k, generator=g, device="cuda") * 0.02).bfloat16())
+    a = (torch.randn(1, r, k, generator=g, device="cuda") * 0.05).bfloat16().requires_grad_()
+    b = (torch.randn(1, n, r, generator=g, device="cuda") * 0.1).bfloat16().requires_grad_()
+    dy = torch.randn(m, n, generator=g, device="cuda").bfloat16()
+
+    def step():
+        y = W.int8_linear_lora(x, w, ws, None, a, b)
+        return (y, *torch.autograd.grad(y, (a, b), dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(2):
+        x.copy_(torch.randn(m, k, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, step()))
+    for kw in (dict(weight_scale=ws.clone().requires_grad_()), dict(bias=torch.zeros(n, device="cuda", requires_grad=True)),
+               dict(scaling=torch.ones(1, device="cuda", requires_grad=True))):
+        args = dict(weight_scale=ws, bias=None, scaling=None)
+        args.update(kw)
+        with pytest.raises(ValueError, match="frozen"):
+            W.int8_linear_lora(x, w, args["weight_scale"], args["bias"], a, b, None, args["scaling"])
+
+
 def test_gradient_against_differences():
     """fp32: the adapters' gradient against differences of the forward operator, which is linear
     in each of x, a and b (so a difference is the slope, up to the rounding of its two ends)."""
