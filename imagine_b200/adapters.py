@@ -162,7 +162,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     is each row's adapter and has x's leading dimensions or the first of them
     ([B] for [B, S, K]: one for each sample); an index outside [0, S), such as
     -1, means no adapter and returns y's row.  None: adapter 0 everywhere.
-    ``scaling``: fp32 [S], or one number.  ``out`` may be ``y``, to add in place.
+    ``scaling``: fp32 [S], or one number.  ``out`` may be ``y``, to add in place, and
+    is no operand's memory otherwise.
 
     The contraction over K and the rank are summed in fp32 and the result is
     rounded once; the same call gives the same bits."""

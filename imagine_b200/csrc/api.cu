@@ -889,6 +889,19 @@ bool bad_align(const void* p, int64_t unit) { return reinterpret_cast<uintptr_t>
 
 int64_t float_size(int dtype) { return dtype == W8A8_F32 ? 4 : 2; }
 
+// Whether M rows of w_p bytes, ld_p apart, share a byte with M rows of w_q bytes, ld_q
+// apart.  Rows of two columns of one tensor do not; different strides in one range
+// count as sharing.
+bool rows_overlap(const void* p, int64_t ld_p, int64_t w_p, const void* q, int64_t ld_q, int64_t w_q, int64_t M) {
+  if (!p || !q || M == 0) return false;
+  const auto a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p));
+  const auto b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q));
+  if (a + (M - 1) * ld_p + w_p <= b || b + (M - 1) * ld_q + w_q <= a) return false;
+  if (ld_p != ld_q || ld_p == 0) return true;
+  const int64_t d = ((b - a) % ld_p + ld_p) % ld_p;
+  return d < w_p || d + w_q > ld_p;
+}
+
 int check_lora_shape(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R) {
   if (M < 0 || N < 0 || K < 0) return fail(W8A8_ERR_VALUE, "lora: negative shape");
   if (R < 1 || R > 128) {
@@ -972,6 +985,11 @@ int w8a8_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dt
   g.R = R;
   g.workspace = workspace;
   if (int rc = check_lora_common(g, workspace_bytes, 0)) return rc;
+  const int64_t size = float_size(dtype);
+  if ((y != out && rows_overlap(out, ldo * size, N * size, y, ldy * size, N * size, M)) ||
+      (K > 0 && rows_overlap(out, ldo * size, N * size, x, ldx * size, K * size, M))) {
+    return fail(W8A8_ERR_VALUE, "lora: out overlaps an operand's memory");
+  }
   return finish(lora_add_launch(g, static_cast<cudaStream_t>(stream)));
 }
 
@@ -986,7 +1004,11 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
   if ((da == nullptr) != (db == nullptr)) return fail(W8A8_ERR_VALUE, "lora: da and db go together");
   if (N == 0 || K == 0) return fail(W8A8_ERR_VALUE, "lora: gradients need N > 0 and K > 0");
   if (!dx && !da) return finish(0);
-  if (dx && (dx == dy || dx == x)) return fail(W8A8_ERR_VALUE, "lora: dx is an operand's memory");
+  const int64_t size = is_float_dtype(dtype) ? float_size(dtype) : 1, size_x = x_scale ? 1 : size;
+  if (dx && (dx == dy || dx == x || rows_overlap(dx, lddx * size, K * size, dy, lddy * size, N * size, M) ||
+             (da && rows_overlap(dx, lddx * size, K * size, x, ldx * size_x, K * size_x, M)))) {
+    return fail(W8A8_ERR_VALUE, "lora: dx is an operand's memory");
+  }
   if (M > 0) {
     if (!dy || (da && !x)) return fail(W8A8_ERR_VALUE, "NULL tensor pointer");
     if (lddy < N || (da && ldx < K) || (dx && lddx < K)) {
@@ -1022,7 +1044,6 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
   g.R = R;
   g.workspace = workspace;
   if (int rc = check_lora_common(g, workspace_bytes, da ? 1 : 2)) return rc;
-  const int64_t size = float_size(dtype);
   if (bad_align(da, size) || bad_align(db, size)) {
     return fail(W8A8_ERR_VALUE, "lora: pointer not aligned to its element");
   }

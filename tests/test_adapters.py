@@ -132,3 +132,20 @@ def test_argument_helpers():
     assert A._rows(torch.zeros(3, 2, 8)[:, :, :4])[1] == 8  # samples whose rows stay one stride apart
     assert A._index(None, (4,), 4, None) == (None, 0, 1)
     assert A._scaling(None, 3, None) is None
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=P + 2 * 64),                         # y a row further
+    dict(y=P, out=P + 64, ldy=128, ldo=128),      # half of y's columns
+    dict(y=P + (1 << 20), out=P + 2 * 16, x=P),   # inside x
+    dict(y=P + 2 * 64, out=P, ldo=70, ldy=64)])   # another stride in one range
+def test_lora_add_refuses_an_output_that_overlaps(kw):
+    assert _add(**{**dict(y=P, x=P + (1 << 21), out=P, m=10, n=64), **kw}) == N.ERR_VALUE
+    assert "operand's memory" in _err()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dx=P + 2 * 32, dy=P, lddy=64), dict(dx=P + 2 * 32, x=P), dict(dx=P + 16, x=P, xs=P)])
+def test_lora_backward_refuses_a_gradient_that_overlaps(kw):
+    assert _back(**{**dict(dy=P + (1 << 20), x=P + (1 << 21), dx=P + (1 << 22)), **kw}) == N.ERR_VALUE
+    assert "operand's memory" in _err()

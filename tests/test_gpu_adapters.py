@@ -395,3 +395,16 @@ def test_other_stream_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(held, step()))
+
+
+def test_output_beside_the_projection_in_one_tensor():
+    """Columns of one tensor as y, out and x: rows interleave and share nothing."""
+    import imagine_b200 as W
+    m, n, k, s, r = 70, 64, 64, 2, 16
+    gen = torch.Generator("cuda").manual_seed(5)
+    big, a, b = (torch.randn(shape, generator=gen, device="cuda", dtype=torch.bfloat16)
+                 for shape in ((m, 3 * 64), (s, r, k), (s, n, r)))
+    y, x, out = big[:, :64], big[:, 64:128], big[:, 128:]
+    want = W.lora_add(y.contiguous(), x.contiguous(), a, b)
+    got = W.lora_add(y, x, a, b, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
