@@ -2,7 +2,7 @@
 //
 // The codes w are exact in bf16, so the product runs as bf16 x bf16 -> fp32
 // with the weight scales folded into dy: dy ws, an fp32 product, is cut into
-// one bf16 piece for a bf16 dy (one rounding of 2^-9, as a dequantised bf16
+// one bf16 piece for a bf16 dy (one rounding of 2^-8 at most, as a dequantised bf16
 // weight would have), two for f16 and three for fp32 (pieces.cuh), which keeps
 // each type's own precision.
 //
@@ -250,8 +250,9 @@ NSplit n_split_of(int64_t M, int64_t N, int64_t K) {
 // ================================================================ tcgen05
 // D[256 x 256] of a CTA pair: rows of dy (or of its pieces) times 256 columns
 // of w, 64 of the contraction a stage, six stages.  The weights come as bf16,
-// transposed to [K][n] once per call by widen_weights_kernel (16 us for 12288 x
-// 4096, against 380 us of products at 5856 rows).  Per CTA:
+// transposed to [K][n] once per call by widen_weights_kernel (30 us for 12288 x
+// 4096, against 395 us of products at 5856 rows, 1.49 PFLOP/s with the tensor pipe
+// active 91 % of the time; under the power cap of a long run 450).  Per CTA:
 //   warp 4     TMA: its 128 rows of dy and its 128 columns of w (both K-major,
 //              128-byte swizzle)
 //   warp 5     MMA issue (the pair's leader), two TMEM accumulators of 256 columns
