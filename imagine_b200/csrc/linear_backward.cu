@@ -58,8 +58,10 @@ constexpr int kThreads = 256;
 constexpr int kBC = 128, kBN = 64;
 constexpr int kLdA = kBN + 8, kLdB = kBC + 8;
 
+// Two blocks a multiprocessor.  With 173 registers an fp32 call had one, and the
+// blocks of a cut contraction ran in two waves (712 x 5584 -> 1152: 294 us, now 201).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) input_grad_kernel(
+__global__ void __launch_bounds__(kThreads, 2) input_grad_kernel(
     const T* __restrict__ dy, int64_t lddy, const float* __restrict__ ws, int ws_one,
     const int8_t* __restrict__ w, int64_t ldw, int64_t M, int N, int K, int col_tiles, int n_split,
     int vec_dy, int vec_w, int vec_o, T* __restrict__ dx, int64_t lddx, float* __restrict__ part) {
@@ -83,8 +85,9 @@ __global__ void __launch_bounds__(kThreads) input_grad_kernel(
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
   float low[kApart ? 8 : 1][4] = {};
 
+  __shared__ __align__(16) float s_ws[kBN];  // the step's weight scales
   Raw8<T> ra[2];
-  float rs[2][8];
+  float next_ws = 0.0f;
   Raw8<int8_t> rb[4];
   auto fetch = [&](int n0) {
 #pragma unroll
@@ -93,9 +96,8 @@ __global__ void __launch_bounds__(kThreads) input_grad_kernel(
       const int r = gi >> 3, c = (gi & 7) * 8;
       const int valid = row0 + r < M ? min(8, n_hi - n0 - c) : 0;
       load8(ra[i], dy + (row0 + r) * lddy + n0 + c, valid, vec_dy != 0);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) rs[i][j] = j < valid ? __ldg(ws + (ws_one ? 0 : n0 + c + j)) : 0.0f;
     }
+    if (tid < kBN) next_ws = n0 + tid < n_hi ? __ldg(ws + (ws_one ? 0 : n0 + tid)) : 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int gi = tid + i * kThreads;
@@ -106,13 +108,14 @@ __global__ void __launch_bounds__(kThreads) input_grad_kernel(
   };
   fetch(n_lo);
   for (int n0 = n_lo; n0 < n_hi; n0 += kBN) {
+    if (tid < kBN) s_ws[tid] = next_ws;  // the step before read its own before its second barrier
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int gi = tid + i * kThreads;
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f(ra[i].e[j]) * rs[i][j];
+      for (int j = 0; j < 8; ++j) v[j] = to_f(ra[i].e[j]) * s_ws[(gi & 7) * 8 + j];  // zeros past n_hi
       store_pieces<kP>(sa + (gi >> 3) * kLdA + (gi & 7) * 8, kPlane, v);
     }
 #pragma unroll
@@ -737,8 +740,8 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
 // columns of four rows; which of the tile's columns a fragment column stands for is
 // free to choose), and only the pieces of dy ws pass through shared memory.  The
 // eight warps' sums are joined in order at the end.
-// 4096 -> 4096, a call with its sum: 20.3 us where input_grad_kernel, which stages w
-// in shared memory, takes 26.7.  At 32 rows both take 27 us, at 64 this form 56.
+// 4096 -> 4096 with its sum: 16.2 us (fp32: 22.7) where input_grad_kernel, which stages
+// w in shared memory, takes 19.3 (39.6).  At 32 rows this form takes 27, that one 21.
 constexpr int kFewRows = 16, kFewCols = 64, kFewN = 128, kLdFew = kFewN + 8;
 
 template <typename T>
@@ -911,7 +914,7 @@ int typed(const InputGradArgs& g, cudaStream_t stream) {
   const int64_t tiles = (g.M + kBM - 1) / kBM;
   float* part = sp.count > 1 ? static_cast<float*>(g.workspace) : nullptr;
   constexpr int bytes = 2 * (Pieces<T>::n * kBM * kLdA + kBN * kLdB);
-  static_assert(bytes <= 48 * 1024, "no opt-in shared memory needed");
+  static_assert(bytes + kBN * 4 <= 48 * 1024, "no opt-in shared memory needed");
   const dim3 grid(static_cast<unsigned>(tiles * cols), sp.count);
   input_grad_kernel<T><<<grid, kThreads, bytes, stream>>>(
       static_cast<const T*>(g.dy), g.lddy, g.ws, g.ws_numel == 1, g.w, g.ldw, g.M, N, K, cols, sp.per,
