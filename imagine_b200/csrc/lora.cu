@@ -222,14 +222,14 @@ __device__ __forceinline__ void shrink_tile(const ShrinkArgs<TX, TW>& g, const R
 }
 
 template <typename TX, typename TW, int kRank, bool kWRows>
-__global__ void __launch_bounds__(kThreads) shrink_kernel(ShrinkArgs<TX, TW> g, Rows rows, int R) {
+__global__ void __launch_bounds__(kThreads, kRank <= 64 ? 2 : 1) shrink_kernel(ShrinkArgs<TX, TW> g, Rows rows, int R) {
   griddep_launch_dependents();
   shrink_tile<TX, TW, kRank, kWRows>(g, rows, R, blockIdx.y);
 }
 // dy times B and x times A in one launch: blockIdx.y below `first` is the former.
 template <typename TX, typename T, int kRank>
-__global__ void __launch_bounds__(kThreads) shrink_pair_kernel(ShrinkArgs<T, T> dy, ShrinkArgs<TX, T> x, int first,
-                                                               Rows rows, int R) {
+__global__ void __launch_bounds__(kThreads, kRank <= 64 ? 2 : 1) shrink_pair_kernel(
+    ShrinkArgs<T, T> dy, ShrinkArgs<TX, T> x, int first, Rows rows, int R) {
   griddep_launch_dependents();
   if (static_cast<int>(blockIdx.y) < first) {
     shrink_tile<T, T, kRank, false>(dy, rows, R, blockIdx.y);
@@ -255,14 +255,18 @@ __device__ __forceinline__ void load_rank_side(__nv_bfloat16* dst, const float* 
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     if (id[r] == s) {
       const float* p = part + (row0 + r) * R + c;
-      for (int sp = 0; sp < splits; ++sp, p += plane) {
-        if (R % 4 == 0) {
-          const float4 lo = c < R ? __ldcg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
-          const float4 hi =
-              c + 4 < R ? __ldcg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
+      if (R % 4 == 0) {
+        const bool has_lo = c < R, has_hi = c + 4 < R;
+        // four splits' loads in flight (the latency of one after the other showed)
+#pragma unroll 4
+        for (int sp = 0; sp < splits; ++sp, p += plane) {
+          const float4 lo = has_lo ? __ldcg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
+          const float4 hi = has_hi ? __ldcg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
           v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
           v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
-        } else {
+        }
+      } else {
+        for (int sp = 0; sp < splits; ++sp, p += plane) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += c + i < R ? __ldcg(p + i) : 0.0f;
         }
@@ -699,7 +703,7 @@ __device__ __forceinline__ void tokens_tile(const TokensArgs<TX>& g, const float
 
 // Both gradients in one launch: blocks below a.chunks * a.count are dA's.
 template <typename TX, typename T, int kRank>
-__global__ void __launch_bounds__(kThreads) tokens_pair_kernel(TokensArgs<TX> a, TokensArgs<T> b,
+__global__ void __launch_bounds__(kThreads, kRank <= 64 ? 2 : 1) tokens_pair_kernel(TokensArgs<TX> a, TokensArgs<T> b,
                                                                const float* __restrict__ scaling, Rows rows, int R) {
   griddep_launch_dependents();
   griddep_wait();
@@ -827,6 +831,17 @@ Split shrink_split(int64_t M, int K) {
   want = std::max<int64_t>(1, std::min<int64_t>({want, 16, (steps + 1) / 2}));
   const int per = static_cast<int>((steps + want - 1) / want);
   return {(steps + per - 1) / per, per * kBK};
+}
+// The same for two shrinks in one launch, which share twice the blocks in proportion to
+// their steps (fp32, 641 rows, 7680 and 1152 at rank 64: 68 us with as many blocks for
+// each, 44 so, with two blocks a multiprocessor).
+void shrink_pair_split(int64_t M, int N, int K, Split& n, Split& k) {
+  const int64_t tiles = std::max<int64_t>(1, (M + kBM - 1) / kBM);
+  const int64_t steps_n = std::max(1, (N + kBK - 1) / kBK), steps_k = std::max(1, (K + kBK - 1) / kBK);
+  const int64_t want = std::max<int64_t>(2, 4 * device_sm_count() / tiles);
+  const int64_t per = std::max<int64_t>({2, (steps_n + steps_k + want - 1) / want, (std::max(steps_n, steps_k) + 15) / 16});
+  n = {static_cast<int>((steps_n + per - 1) / per), static_cast<int>(per * kBK)};
+  k = {static_cast<int>((steps_k + per - 1) / per), static_cast<int>(per * kBK)};
 }
 // Blocks that share out a tile's adapters (a tile of a decode batch has many).
 int parts_of(int64_t M, int S, int blocks) {
@@ -1051,11 +1066,15 @@ struct BackwardPlan {
   RowSplit a, b;
   int64_t off_g, off_counts, off_a, off_b, off_found, off_pa, off_pb, off_info, bytes;  // dx alone: up to off_a
 };
-BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, bool tc) {
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t S, int64_t R, bool tc, bool weights) {
   BackwardPlan p;
   const int r = static_cast<int>(R), s = static_cast<int>(S), k = static_cast<int>(K), n = static_cast<int>(N);
-  p.h = tc ? shrink_tc_split(M, k) : shrink_split(M, k);
-  p.g = tc ? shrink_tc_split(M, n) : shrink_split(M, n);
+  if (tc || !weights) {
+    p.h = tc ? shrink_tc_split(M, k) : shrink_split(M, k);
+    p.g = tc ? shrink_tc_split(M, n) : shrink_split(M, n);
+  } else {
+    shrink_pair_split(M, n, k, p.g, p.h);
+  }
   p.a = tc ? tokens_tc_split(M, k, s, r) : tokens_split(M, k, s, r);
   p.b = tc ? tokens_tc_split(M, n, s, r) : tokens_split(M, n, s, r);
   p.off_g = up(p.h.count * M * R * 4);
@@ -1079,7 +1098,7 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   const bool early = start_early(g);
   const bool tc = tc_shape(g) && tc_x(g) && tc_rows(g.y, g.ldy, 2) && tc_weights(g.a, g.lda, g.K, g.S) &&
                   tc_weights(g.b, g.ldb, g.R, g.S);
-  const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R, tc);
+  const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R, tc, g.da != nullptr);
   uint8_t* ws = static_cast<uint8_t*>(g.workspace);
   float* ph = reinterpret_cast<float*>(ws);
   float* pg = reinterpret_cast<float*>(ws + p.off_g);
@@ -1160,10 +1179,11 @@ int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t
   if (!backward) {
     return up(std::max(shrink_split(M, k).count, shrink_tc_split(M, k).count) * M * R * 4 + (M + 127) / 128 * 4);
   }
-  const BackwardPlan plain = backward_plan(M, N, K, S, R, false);
+  const bool weights = backward == 1;
+  const BackwardPlan plain = backward_plan(M, N, K, S, R, false, weights);
   const bool tc = M >= kTcRows && S <= 64;
-  const BackwardPlan other = tc ? backward_plan(M, N, K, S, R, true) : plain;
-  return backward == 2 ? std::max(plain.off_a, other.off_a) : std::max(plain.bytes, other.bytes);
+  const BackwardPlan other = tc ? backward_plan(M, N, K, S, R, true, weights) : plain;
+  return !weights ? std::max(plain.off_a, other.off_a) : std::max(plain.bytes, other.bytes);
 }
 
 int lora_add_launch(const LoraArgs& g, cudaStream_t stream) {

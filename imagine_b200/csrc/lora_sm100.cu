@@ -130,6 +130,41 @@ __device__ __forceinline__ void let_copies_land() {
   }
 }
 
+// The splits' sums of the rank side, in order, all of a split's loads in flight at once:
+// thread `at` of kThreadsN has the vectors at + i kThreadsN, kV of them a row, of the rows
+// from row0 + r0 on.  What lies past R is zero; rows without an adapter give whatever is
+// there (the caller leaves them out), rows past M the last row.
+template <int kV, int kThreadsN, int kEach>
+__device__ __forceinline__ void rank_sums(const float* __restrict__ part, int splits, const Rows& rows, int64_t row0,
+                                          int r0, int at, int R, float4 (&sum)[kEach]) {
+  const int64_t plane = rows.M * R;
+  const int last = static_cast<int>(min(static_cast<int64_t>(127), rows.M - 1 - row0));
+  const float* p = part + row0 * R;
+  const int c = at % kV * 4;  // kThreadsN % kV == 0: the same for all
+  int rel[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    rel[i] = min(r0 + (at + i * kThreadsN) / kV, last) * R + (c < R ? c : 0);  // R % 8 == 0
+    sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  constexpr int kAhead = kEach > 8 ? 1 : kEach > 4 ? 2 : 4;
+#pragma unroll kAhead
+  for (int sp = 0; sp < splits; ++sp, p += plane) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const float4 q = __ldcg(reinterpret_cast<const float4*>(p + rel[i]));
+      sum[i].x += q.x;
+      sum[i].y += q.y;
+      sum[i].z += q.z;
+      sum[i].w += q.w;
+    }
+  }
+  if (c >= R) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+}
+
 struct Bars {
   uint64_t full[8], ready[8], empty[8], acc[8], w_full[4], w_empty[4], done, drained;
   uint32_t tmem;
@@ -142,8 +177,8 @@ static_assert(sizeof(Bars) <= kBarBytes, "barriers");
 // A tile whose rows have several adapters is multiplied by each of them while it is
 // there, into accumulators of their own, as many at a time as TMEM has columns for.
 // The contraction is cut so that two blocks a multiprocessor are all there are.  Bound
-// by reading x: 11712 x 4096 at rank 64, four adapters, in 30 us (98 MB, 3.3 TB/s; half
-// of it is the start, the first loads and the last sums), 5856 x 4096 at rank 16 in 15.
+// by reading x: 11712 x 4096 at rank 64 in 30 us (98 MB, 3.3 TB/s), 5856 x 4096 at
+// rank 16 in 12 to 15, 11712 x 12288 in 76 (288 MB, 3.8 TB/s).
 constexpr int kSRows = 128, kSK = 64;
 constexpr int kXTile = kSRows * kSK * 2;  // 16 KB
 template <bool kCodes, int kRank>
@@ -407,34 +442,20 @@ __global__ void __launch_bounds__(256) rank_pieces_kernel(RankSide a, RankSide b
   griddep_wait();
   constexpr int kVecs = kRank / 4;
   constexpr int kEach = kTile * kVecs / 256;  // 1 .. 8 vectors a thread
-  const int64_t plane = rows.M * R;
+  float4 sum[kEach];
+  rank_sums<kVecs, 256, kEach>(g.part, g.splits, rows, row0, 0, threadIdx.x, R, sum);
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int at = threadIdx.x + i * 256;
     const int r = at / kVecs, c = (at % kVecs) * 4;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int own = ids.id[r];
-    if (own >= 0 && c < R) {  // R % 8 == 0
-      const float* p = g.part + (row0 + r) * R + c;
-#pragma unroll 4
-      for (int sp = 0; sp < g.splits; ++sp) {
-        const float4 q = __ldcg(reinterpret_cast<const float4*>(p + sp * plane));
-        sum.x += q.x;
-        sum.y += q.y;
-        sum.z += q.z;
-        sum.w += q.w;
-      }
-      float mul = scaling ? __ldg(scaling + own) : 1.0f;
-      if (g.row_mul) mul *= __ldg(g.row_mul + row0 + r);
-      sum.x *= mul;
-      sum.y *= mul;
-      sum.z *= mul;
-      sum.w *= mul;
-    }
-    v[r][c] = sum.x;
-    v[r][c + 1] = sum.y;
-    v[r][c + 2] = sum.z;
-    v[r][c + 3] = sum.w;
+    float mul = 1.0f;
+    if (own >= 0 && scaling) mul = __ldg(scaling + own);
+    if (own >= 0 && g.row_mul) mul *= __ldg(g.row_mul + row0 + r);
+    v[r][c] = own >= 0 ? sum[i].x * mul : 0.0f;
+    v[r][c + 1] = own >= 0 ? sum[i].y * mul : 0.0f;
+    v[r][c + 2] = own >= 0 ? sum[i].z * mul : 0.0f;
+    v[r][c + 3] = own >= 0 ? sum[i].w * mul : 0.0f;
   }
   __syncthreads();
 #pragma unroll
@@ -730,8 +751,11 @@ struct ExpandTc {
 };
 
 // What a tile of rows with so many adapters costs: a second product takes the thread
-// that issues them 1100 cycles, where HBM needs 1260 for the tile.
-__device__ __forceinline__ int tile_cost(int adapters) { return adapters <= 1 ? 4 : 3 * adapters + 1; }
+// that issues them 1100 cycles, where HBM needs 1260 for the tile.  Where every tile
+// has a block (`each`), one: a block with tiles of two row tiles takes twice as long.
+__device__ __forceinline__ int tile_cost(int adapters, bool each) {
+  return each ? 1 : adapters <= 1 ? 4 : 3 * adapters + 1;
+}
 
 template <int kRank, bool kWCols>
 __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
@@ -800,11 +824,12 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   griddep_wait();  // the rank side, and the adapters' counts
   // this block's share [lo, hi) of the whole cost, and the row tile it starts in: a
   // thread adds up a run of row tiles, a scan over the block gives the run's start
+  const bool each = gridDim.x == row_tiles * col_tiles;
   {
     const int64_t run = (row_tiles + kEThreads - 1) / kEThreads;
     const int64_t first = min(row_tiles, tid * run), last = min(row_tiles, first + run);
     int64_t mine = 0;
-    for (int64_t i = first; i < last; ++i) mine += tile_cost(__ldcg(counts + i));
+    for (int64_t i = first; i < last; ++i) mine += tile_cost(__ldcg(counts + i), each);
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -823,7 +848,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
     const int64_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
     int64_t at = before * col_tiles;
     for (int64_t i = first; i < last; ++i) {
-      const int64_t end = at + static_cast<int64_t>(tile_cost(__ldcg(counts + i))) * col_tiles;
+      const int64_t end = at + static_cast<int64_t>(tile_cost(__ldcg(counts + i), each)) * col_tiles;
       if (lo >= at && lo < end) {
         start_tile = i;
         start_at = at;
@@ -840,7 +865,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   int64_t at = start_at;
   for (int64_t rt = start_tile; rt < row_tiles && at < hi; ++rt) {
     // the row tile's tiles that start in the share
-    const int64_t cost = tile_cost(__ldcg(counts + rt));
+    const int64_t cost = tile_cost(__ldcg(counts + rt), each);
     const int t_lo = static_cast<int>(lo <= at ? 0 : min(static_cast<int64_t>(col_tiles), (lo - at + cost - 1) / cost));
     const int t_hi = static_cast<int>(min(static_cast<int64_t>(col_tiles), (hi - at + cost - 1) / cost));
     at += cost * col_tiles;
@@ -936,34 +961,21 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
       const int r = quad * 32 + lane;
       const int64_t row = row0 + r;
       const int own = id[r];
-      // the row's h as pieces, a group half of the rank each (zero without an adapter);
-      // the products with the last one are done (see the barrier below)
-      const float* p0 = part + row * R;
-#pragma unroll 4
-      for (int c = group * (kRank / 2); c < (group + 1) * (kRank / 2); c += 8) {
-        float x[8] = {};
-        if (own >= 0 && c < R) {  // R % 8 == 0
-#pragma unroll 3
-          for (int sp = 0; sp < splits; ++sp) {
-            const float4* q = reinterpret_cast<const float4*>(p0 + sp * rows.M * R + c);
-            const float4 a = __ldcg(q), b = __ldcg(q + 1);
-            x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
-            x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
-          }
-        }
-        uint4 piece[2];
-        uint32_t* u = reinterpret_cast<uint32_t*>(piece);
+      // the rows' h as pieces (zero without an adapter), sixteen rows a warp, a lane a
+      // vector of four of a row: with a lane a row, 14 splits of 2005 x 64 took the kernel
+      // 36 us, now 15.  The products with the last one are done (see the barrier below)
+      constexpr int kV = kRank / 4, kEach = kV / 2;
+      float4 sum[kEach];
+      rank_sums<kV, 32, kEach>(part, splits, rows, row0, warp * 16, lane, R, sum);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x0 = next_piece(x[2 * j]), x1 = next_piece(x[2 * j + 1]);
-          u[j] = pack_bf16(x0, x1);
-          u[4 + j] = pack_bf16(x[2 * j], x[2 * j + 1]);
-        }
-        const int blk = c >> 6, ch = (c >> 3) & 7;
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          *reinterpret_cast<uint4*>(s_h + (p * C::kBlks + blk) * C::kHBlk + r * 128 + ((ch ^ (r & 7)) << 4)) =
-              piece[p];
+      for (int i = 0; i < kEach; ++i) {
+        const int hr = warp * 16 + (lane + i * 32) / kV, c = (lane + i * 32) % kV * 4;
+        float x[4] = {sum[i].x, sum[i].y, sum[i].z, sum[i].w};
+        if (id[hr] < 0) x[0] = x[1] = x[2] = x[3] = 0.0f;
+        const float x0 = next_piece(x[0]), x1 = next_piece(x[1]), x2 = next_piece(x[2]), x3 = next_piece(x[3]);
+        uint8_t* h = s_h + (c >> 6) * C::kHBlk + hr * 128 + ((((c >> 3) & 7) ^ (hr & 7)) << 4) + (c & 4) * 2;
+        *reinterpret_cast<uint2*>(h) = make_uint2(pack_bf16(x0, x1), pack_bf16(x2, x3));
+        *reinterpret_cast<uint2*>(h + C::kBlks * C::kHBlk) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
       }
       fence_proxy_async_smem();
       __syncwarp();
