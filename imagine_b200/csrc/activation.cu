@@ -36,8 +36,25 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroup = 128;
-constexpr int kLanes = 4;   // lanes per group
-constexpr int kChunks = 4;  // chunks of eight elements a lane: lane l has chunks l, l + 4, l + 8, l + 12
+// How a group lies in lanes.
+//   kWhole     rows (or halves) of whole groups on vector boundaries, the usual case, in which
+//              nothing has to be looked at element by element: lane l of four has the chunks of
+//              eight elements l, l + 4, l + 8, l + 12
+//   kVectors   the same with a last group that may be shorter
+//   kElements  rows that vectors cannot take: lane l of sixteen has the pairs of elements l, l + 16,
+//              ..., so that neighbours share the memory sectors that each access touches (GELU,
+//              1837 x 2455 bf16, both passes: 72 us with eight neighbouring elements a lane, 19 so);
+//              pairs, since two elements share a reciprocal: the bits are those of the others
+enum Layout : int { kWhole = 0, kVectors = 1, kElements = 2 };
+template <int kLayout>
+struct Lay {
+  static constexpr int kLanes = kLayout == kElements ? 16 : 4;
+  static constexpr int kChunks = kGroup / (8 * kLanes);
+  static constexpr int kFirst = kLayout == kElements ? 2 : 8;  // from a lane's first element to the next lane's
+  // element i of a lane's chunk
+  static __device__ constexpr int at(int i) { return kLayout == kElements ? (i >> 1) * 2 * kLanes + (i & 1) : i; }
+};
+constexpr int kStep = 32;  // elements from one of a lane's chunks to the next
 
 constexpr float kC0 = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kC1 = 0.044715f;
@@ -200,7 +217,7 @@ __device__ __forceinline__ uint32_t abs_max(const Raw8<T>& r) {
   }
 }
 // The group's, over its lanes.
-template <typename T>
+template <typename T, int kLanes>
 __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) {
@@ -244,8 +261,19 @@ __device__ __forceinline__ void widen_codes(uint64_t (&v)[4], const Raw8<int8_t>
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_two(T* p, const uint64_t (&v)[4], int valid, bool vec) {
+// A lane's chunk; `left`: elements of the row from its first on.
+template <int kLayout, typename T>
+__device__ __forceinline__ void load_chunk(Raw8<T>& r, const T* p, int left) {
+  if constexpr (kLayout == kElements) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.e[i] = Lay<kLayout>::at(i) < left ? p[Lay<kLayout>::at(i)] : T(0.0f);
+  } else {
+    load8(r, p, kLayout == kWhole ? (left > 0 ? 8 : 0) : min(8, left), true);
+  }
+}
+
+template <int kLayout, typename T>
+__device__ __forceinline__ void store_two(T* p, const uint64_t (&v)[4], int left) {
   Raw8<T> o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -256,7 +284,7 @@ __device__ __forceinline__ void store_two(T* p, const uint64_t (&v)[4], int vali
       o.e[2 * i + 1] = from_f<T>(hi(v[i]));
     }
   }
-  if (vec && valid >= 8) {
+  if (kLayout == kWhole || (kLayout == kVectors && left >= 8)) {
 #pragma unroll
     for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) {
       const uint2* s = reinterpret_cast<const uint2*>(o.e) + 2 * q;
@@ -265,17 +293,19 @@ __device__ __forceinline__ void store_two(T* p, const uint64_t (&v)[4], int vali
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < valid) p[i] = o.e[i];
+      if (Lay<kLayout>::at(i) < left) p[Lay<kLayout>::at(i)] = o.e[i];
   }
 }
 
-__device__ __forceinline__ void store_codes(int8_t* p, uint2 w, int valid, bool vec) {
-  if (vec && valid >= 8) {
+template <int kLayout>
+__device__ __forceinline__ void store_codes(int8_t* p, uint2 w, int left) {
+  if (kLayout == kWhole || (kLayout == kVectors && left >= 8)) {
     *reinterpret_cast<uint2*>(p) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < valid) p[i] = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+      if (Lay<kLayout>::at(i) < left)
+        p[Lay<kLayout>::at(i)] = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
   }
 }
 
@@ -306,6 +336,7 @@ struct Item {
   int left;    // elements of the row (or half) from c on, 0 for no item
   uint32_t g;
 };
+template <int kLayout>
 __device__ __forceinline__ Item item_at(uint64_t item, uint32_t items, const Groups& groups, int K) {
   Item t;
   const bool live = item < items;
@@ -313,30 +344,28 @@ __device__ __forceinline__ Item item_at(uint64_t item, uint32_t items, const Gro
   const uint32_t row = groups.row_of(i);
   t.row = row;
   t.g = i - row * groups.count;
-  t.c = static_cast<int>(t.g) * kGroup + (threadIdx.x % kLanes) * 8;
+  t.c = static_cast<int>(t.g) * kGroup + (threadIdx.x % Lay<kLayout>::kLanes) * Lay<kLayout>::kFirst;
   t.left = live ? K - t.c : 0;
   return t;
 }
-constexpr int kStep = kLanes * 8;  // elements from one of a lane's chunks to the next
 
 // Forward.  Item = one group of one row (of both halves when gated).  Every lane
 // of a warp makes the same number of steps (shuffles).
-// kWhole: rows (or halves) of whole groups on vector boundaries, the usual case, in which nothing
-// has to be looked at element by element.
-template <typename T, int kAct, bool kWhole>
+template <typename T, int kAct, int kLayout>
 __global__ void __launch_bounds__(kThreads, kAct == kSwiglu || sizeof(T) == 4 ? 1 : 4) act_checkpoint_kernel(
-    const T* __restrict__ x, int64_t ldx, uint32_t items, int K, Groups groups, int vec,
+    const T* __restrict__ x, int64_t ldx, uint32_t items, int K, Groups groups,
     T* __restrict__ y, int8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int kHalves = kAct == kSwiglu ? 2 : 1;
+  constexpr int kLanes = Lay<kLayout>::kLanes, kChunks = Lay<kLayout>::kChunks;
   constexpr uint32_t kPerBlock = kThreads / kLanes;
-  const Item it = item_at(static_cast<uint64_t>(blockIdx.x) * kPerBlock + threadIdx.x / kLanes, items, groups, K);
+  const Item it = item_at<kLayout>(static_cast<uint64_t>(blockIdx.x) * kPerBlock + threadIdx.x / kLanes, items, groups, K);
   Raw8<T> raw[kHalves][kChunks];
 #pragma unroll
   for (int h = 0; h < kHalves; ++h)
 #pragma unroll
     for (int j = 0; j < kChunks; ++j)
-      load8(raw[h][j], x + it.row * ldx + h * static_cast<int64_t>(K) + it.c + j * kStep,
-            kWhole ? (it.left > 0 ? 8 : 0) : min(8, it.left - j * kStep), kWhole || vec != 0);
+      load_chunk<kLayout>(raw[h][j], x + it.row * ldx + h * static_cast<int64_t>(K) + it.c + j * kStep,
+                          it.left - j * kStep);
   float s[kHalves], recip[kHalves];
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
@@ -346,19 +375,19 @@ __global__ void __launch_bounds__(kThreads, kAct == kSwiglu || sizeof(T) == 4 ? 
       const uint32_t o = abs_max(raw[h][j]);
       m = sizeof(T) == 2 ? __vmaxu2(m, o) : max(m, o);
     }
-    s[h] = group_scale(group_max<T>(m), recip[h]);
+    s[h] = group_scale(group_max<T, kLanes>(m), recip[h]);
     if (it.left > 0 && threadIdx.x % kLanes == 0) scale[(it.row * kHalves + h) * groups.count + it.g] = s[h];
   }
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    const int valid = kWhole ? 8 : it.left - j * kStep;
-    if (kWhole ? it.left <= 0 : valid <= 0) break;
+    const int left = it.left - j * kStep;
+    if (kLayout == kWhole ? it.left <= 0 : left <= 0) break;
     const int c = it.c + j * kStep;
     uint64_t v[kHalves][4], o[4];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       widen(v[h], raw[h][j]);
-      store_codes(q + (it.row * kHalves + h) * K + c, codes_of(v[h], s[h], recip[h]), valid, kWhole || vec != 0);
+      store_codes<kLayout>(q + (it.row * kHalves + h) * K + c, codes_of(v[h], s[h], recip[h]), left);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -370,18 +399,19 @@ __global__ void __launch_bounds__(kThreads, kAct == kSwiglu || sizeof(T) == 4 ? 
       }
       if constexpr (kAct == kSwiglu) o[i] = mul2(o[i], v[kHalves - 1][i]);
     }
-    store_two(y + it.row * K + c, o, valid, kWhole || vec != 0);
+    store_two<kLayout>(y + it.row * K + c, o, left);
   }
 }
 
 // Backward: dx [rows, halves * K] from dy [rows, K] and the checkpoint.
-template <typename T, int kAct, bool kWhole>
+template <typename T, int kAct, int kLayout>
 __global__ void __launch_bounds__(kThreads) act_backward_kernel(
-    const T* __restrict__ dy, int64_t lddy, uint32_t items, int K, Groups groups, int vec,
+    const T* __restrict__ dy, int64_t lddy, uint32_t items, int K, Groups groups,
     const int8_t* __restrict__ q, const float* __restrict__ scale, T* __restrict__ dx) {
   constexpr int kHalves = kAct == kSwiglu ? 2 : 1;
+  constexpr int kLanes = Lay<kLayout>::kLanes, kChunks = Lay<kLayout>::kChunks;
   constexpr uint32_t kPerBlock = kThreads / kLanes;
-  const Item it = item_at(static_cast<uint64_t>(blockIdx.x) * kPerBlock + threadIdx.x / kLanes, items, groups, K);
+  const Item it = item_at<kLayout>(static_cast<uint64_t>(blockIdx.x) * kPerBlock + threadIdx.x / kLanes, items, groups, K);
   Raw8<T> rd[kChunks];
   Raw8<int8_t> rq[kHalves][kChunks];
   float sc[kHalves];
@@ -389,16 +419,15 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(
   for (int h = 0; h < kHalves; ++h) sc[h] = __ldg(scale + (it.row * kHalves + h) * groups.count + it.g);
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    const int valid = kWhole ? (it.left > 0 ? 8 : 0) : min(8, it.left - j * kStep);
-    load8(rd[j], dy + it.row * lddy + it.c + j * kStep, valid, kWhole || vec != 0);
+    load_chunk<kLayout>(rd[j], dy + it.row * lddy + it.c + j * kStep, it.left - j * kStep);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h)
-      load8(rq[h][j], q + (it.row * kHalves + h) * K + it.c + j * kStep, valid, kWhole || vec != 0);
+      load_chunk<kLayout>(rq[h][j], q + (it.row * kHalves + h) * K + it.c + j * kStep, it.left - j * kStep);
   }
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    const int valid = kWhole ? 8 : it.left - j * kStep;
-    if (kWhole ? it.left <= 0 : valid <= 0) break;
+    const int left = it.left - j * kStep;
+    if (kLayout == kWhole ? it.left <= 0 : left <= 0) break;
     uint64_t d[4], v[kHalves][4], o[kHalves][4];
     widen(d, rd[j]);
 #pragma unroll
@@ -424,16 +453,22 @@ __global__ void __launch_bounds__(kThreads) act_backward_kernel(
     }
 #pragma unroll
     for (int h = 0; h < kHalves; ++h)
-      store_two(dx + (it.row * kHalves + h) * K + it.c + j * kStep, o[h], valid, kWhole || vec != 0);
+      store_two<kLayout>(dx + (it.row * kHalves + h) * K + it.c + j * kStep, o[h], left);
   }
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+template <int kLayout>
 unsigned blocks_for(int64_t items) {
-  const int64_t per = kThreads / kLanes;
-  return static_cast<unsigned>((items + per - 1) / per);  // below 2^31 / 64
+  const int64_t per = kThreads / Lay<kLayout>::kLanes;
+  return static_cast<unsigned>((items + per - 1) / per);  // below 2^31 / 16
 }
+
+#define BY_LAYOUT(F, ACT)                \
+  if (!vec) F(ACT, kElements);           \
+  else if (K % kGroup) F(ACT, kVectors); \
+  else F(ACT, kWhole)
 
 int launched(const char* what) {
   cudaError_t e = cudaGetLastError();
@@ -455,19 +490,18 @@ int checkpoint_typed(const void* x, int64_t ldx, int64_t rows, int K, int act, v
   // every group starts on a vector boundary: rows, halves and codes alike
   const int vec = K % 8 == 0 && aligned16(x) && (ldx * static_cast<int64_t>(sizeof(T))) % 16 == 0 &&
                   aligned16(y) && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  const bool whole = vec && K % kGroup == 0;
   const T* xp = static_cast<const T*>(x);
   T* yp = static_cast<T*>(y);
   for (int64_t r = 0; r < rows; r += rows_per_launch(groups)) {
     const uint32_t items = static_cast<uint32_t>(std::min(rows - r, rows_per_launch(groups)) * groups.count);
-#define CHECKPOINT(ACT, WHOLE)                                                                           \
-  act_checkpoint_kernel<T, ACT, WHOLE><<<blocks_for(items), kThreads, 0, stream>>>(      \
-      xp + r * ldx, ldx, items, K, groups, vec, yp + r * K, q + r * halves * K,                   \
+#define CHECKPOINT(ACT, LAYOUT)                                                                   \
+  act_checkpoint_kernel<T, ACT, LAYOUT><<<blocks_for<LAYOUT>(items), kThreads, 0, stream>>>(      \
+      xp + r * ldx, ldx, items, K, groups, yp + r * K, q + r * halves * K,                   \
       scale + r * halves * groups.count)
     switch (act) {
-      case kGelu: if (whole) CHECKPOINT(kGelu, true); else CHECKPOINT(kGelu, false); break;
-      case kSilu: if (whole) CHECKPOINT(kSilu, true); else CHECKPOINT(kSilu, false); break;
-      default: if (whole) CHECKPOINT(kSwiglu, true); else CHECKPOINT(kSwiglu, false); break;
+      case kGelu: BY_LAYOUT(CHECKPOINT, kGelu); break;
+      case kSilu: BY_LAYOUT(CHECKPOINT, kSilu); break;
+      default: BY_LAYOUT(CHECKPOINT, kSwiglu); break;
     }
 #undef CHECKPOINT
     if (int rc = launched("act_checkpoint")) return rc;
@@ -482,19 +516,18 @@ int backward_typed(const void* dy, int64_t lddy, int64_t rows, int K, int act, c
   const int64_t halves = act == kSwiglu ? 2 : 1;
   const int vec = K % 8 == 0 && aligned16(dy) && (lddy * static_cast<int64_t>(sizeof(T))) % 16 == 0 &&
                   aligned16(dx) && reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  const bool whole = vec && K % kGroup == 0;
   const T* dp = static_cast<const T*>(dy);
   T* xp = static_cast<T*>(dx);
   for (int64_t r = 0; r < rows; r += rows_per_launch(groups)) {
     const uint32_t items = static_cast<uint32_t>(std::min(rows - r, rows_per_launch(groups)) * groups.count);
-#define BACKWARD(ACT, WHOLE)                                                                             \
-  act_backward_kernel<T, ACT, WHOLE><<<blocks_for(items), kThreads, 0, stream>>>(        \
-      dp + r * lddy, lddy, items, K, groups, vec, q + r * halves * K,                             \
+#define BACKWARD(ACT, LAYOUT)                                                                   \
+  act_backward_kernel<T, ACT, LAYOUT><<<blocks_for<LAYOUT>(items), kThreads, 0, stream>>>(      \
+      dp + r * lddy, lddy, items, K, groups, q + r * halves * K,                             \
       scale + r * halves * groups.count, xp + r * halves * K)
     switch (act) {
-      case kGelu: if (whole) BACKWARD(kGelu, true); else BACKWARD(kGelu, false); break;
-      case kSilu: if (whole) BACKWARD(kSilu, true); else BACKWARD(kSilu, false); break;
-      default: if (whole) BACKWARD(kSwiglu, true); else BACKWARD(kSwiglu, false); break;
+      case kGelu: BY_LAYOUT(BACKWARD, kGelu); break;
+      case kSilu: BY_LAYOUT(BACKWARD, kSilu); break;
+      default: BY_LAYOUT(BACKWARD, kSwiglu); break;
     }
 #undef BACKWARD
     if (int rc = launched("act_backward")) return rc;
