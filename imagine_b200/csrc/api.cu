@@ -1057,6 +1057,7 @@ int64_t w8a8_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dty
       ((M + 63) / 64) * ((K + 127) / 128) > 0x7fffffffLL) {
     return fail(W8A8_ERR_VALUE, "input_grad: sizes up to %lld", static_cast<long long>(kMaxDim));
   }
+  if (M == 0 || K == 0) return 0;  // dx has no element
   return input_grad_workspace_bytes(M, N, K, dtype);
 }
 

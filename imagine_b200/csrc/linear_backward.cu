@@ -603,7 +603,7 @@ bool map_rows(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, i
 // apart), more rows than one mma.sync tile and, for bf16, rows of dy that TMA
 // can read.
 bool tc_shape(int64_t M, int64_t N, int64_t K, int dtype) {
-  return dtype != W8A8_F32 && M > kBM && N > 0;
+  return dtype != W8A8_F32 && M > kBM && N > 0 && K > 0;
 }
 bool rows_of_16_bytes(const InputGradArgs& g) {
   return reinterpret_cast<uintptr_t>(g.dy) % 16 == 0 && (g.lddy * 2) % 16 == 0;
@@ -870,7 +870,7 @@ __global__ void __launch_bounds__(kThreads) input_grad_few_kernel(
 }
 
 // Whether input_grad_few_kernel takes a call, by shape (its operands' alignment apart).
-bool few_shape(int64_t M, int64_t N, int64_t K) { return M <= kFewRows && N > 0 && K % 8 == 0; }
+bool few_shape(int64_t M, int64_t N, int64_t K) { return M <= kFewRows && N > 0 && K > 0 && K % 8 == 0; }
 // Two blocks a multiprocessor, at least two steps each, at most 16 pieces.
 struct FewSplit {
   int count, per;

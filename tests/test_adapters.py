@@ -149,3 +149,23 @@ def test_lora_add_refuses_an_output_that_overlaps(kw):
 def test_lora_backward_refuses_a_gradient_that_overlaps(kw):
     assert _back(**{**dict(dy=P + (1 << 20), x=P + (1 << 21), dx=P + (1 << 22)), **kw}) == N.ERR_VALUE
     assert "operand's memory" in _err()
+
+
+@pytest.mark.parametrize("dtype", [N.BF16, N.F16, N.F32])
+@pytest.mark.parametrize("m", [0, 1, 10, 16, 30, 65, 100])
+def test_input_grad_of_a_dimension_of_zero(m, dtype):
+    """No output: no workspace and nothing to do, whatever the kernel the row count would choose."""
+    need = N.LIB.w8a8_input_grad_workspace_bytes
+    for n in (0, 64, 4096):
+        assert need(m, n, 0, dtype) == 0 and need(0, n, 64, dtype) == 0
+        assert N.LIB.w8a8_input_grad(P, n, P, 0, P, n, dtype, None, 0, m, n, 0, None, 0, None) == 0
+        assert N.LIB.w8a8_input_grad(None, n, P, 64, P, n, dtype, None, 64, 0, n, 64, None, 0, None) == 0
+    assert need(m, 0, 64, dtype) >= 0  # an empty sum: dx is zero
+
+
+@pytest.mark.parametrize("backward", [0, 1, 2])
+def test_lora_workspace_of_a_dimension_of_zero(backward):
+    need = N.LIB.w8a8_lora_workspace_bytes
+    for m in (0, 1, 64, 100, 300):
+        for n, k in ((0, 64), (64, 0), (0, 0), (64, 64)):
+            assert need(m, n, k, 2, 8, backward) >= 0

@@ -408,3 +408,15 @@ def test_output_beside_the_projection_in_one_tensor():
     want = W.lora_add(y.contiguous(), x.contiguous(), a, b)
     got = W.lora_add(y, x, a, b, out=out)
     assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m", [0, 1, 16, 30, 100])
+def test_input_gradient_of_a_weight_without_rows_or_columns(m, dtype):
+    import imagine_b200 as W
+
+    t = DTYPES[dtype]
+    for n, k in ((64, 0), (0, 40), (0, 0)):
+        w = torch.zeros(n, k, dtype=torch.int8, device="cuda")
+        dx = W.int8_linear_backward(torch.ones(m, n, dtype=t, device="cuda"), w, torch.ones(n, device="cuda"))
+        assert dx.shape == (m, k) and dx.dtype == t and not bool(dx.any())
