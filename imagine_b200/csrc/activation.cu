@@ -18,8 +18,10 @@
 // on pairs, and a group in four lanes of 32 elements each (four 16-byte loads in
 // flight): the scale's two divisions, the index arithmetic and the shuffles are
 // paid once for 32 elements.  With 16 lanes of 8 the forward pass was issue-bound.
-// GELU at 5856 x 12288 bf16: forward 75 us (365 MB, 4.9 TB/s), gradient 60 us (364 MB,
-// 6.1 TB/s), issue slots 67 and 62 % in use; SwiGLU is at the rate of a copy.
+// At 5856 x 12288 bf16: GELU forward 78 us (365 MB, 4.7 TB/s), gradient 63 us (364 MB,
+// 5.7 TB/s), with issue slots two thirds in use; SwiGLU (rows of 2 x 12288) forward 150 us
+// (580 MB, 3.9 TB/s; both halves' chunks take 106 registers a thread, two blocks a
+// multiprocessor where GELU has four), gradient 92 us (580 MB, 6.3 TB/s: the rate of a copy).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -123,11 +125,19 @@ __device__ __forceinline__ uint64_t argument_two(uint64_t x) {
     return mul2(x, both(kLog2e));
   }
 }
-// With e = exp(-|z|): er = e / (1 + e) and r = 1 / (1 + e); the sigmoid is r where z >= 0, else er
+// With e = exp(-|z|): er = e / (1 + e) and r = 1 / (1 + e); the sigmoid is r where z >= 0, else er.
+// kApart: one of the two may be NaN and the other not.  The two share a reciprocal, so a
+// NaN argument is taken as 0 (fminf drops it) and leaves a finite sigmoid; x itself carries the NaN on.
+template <bool kApart>
 __device__ __forceinline__ void exp_recip_two(uint64_t z, uint64_t& er, uint64_t& r, uint64_t& s) {
   // the exponential 2^24 too large, so that flushing its subnormals to zero loses
   // nothing that bf16 holds (ftz: one instruction instead of four)
-  const uint64_t e = mul2(pk(ex2(24.0f - fabsf(lo(z))), ex2(24.0f - fabsf(hi(z)))), both(5.9604644775390625e-8f));
+  float e0 = 24.0f - fabsf(lo(z)), e1 = 24.0f - fabsf(hi(z));
+  if constexpr (kApart) {
+    e0 = fminf(e0, 24.0f);
+    e1 = fminf(e1, 24.0f);
+  }
+  const uint64_t e = mul2(pk(ex2(e0), ex2(e1)), both(5.9604644775390625e-8f));
   const uint64_t d = add2(e, both(1.0f));
   // both reciprocals from that of the product, which lies in [1, 4]: the special
   // function unit (a quarter of the rate) is the busiest
@@ -138,10 +148,11 @@ __device__ __forceinline__ void exp_recip_two(uint64_t z, uint64_t& er, uint64_t
 template <int kAct>
 __device__ __forceinline__ uint64_t act_two(uint64_t x) {
   uint64_t er, r, s;
-  exp_recip_two(argument_two<kAct>(x), er, r, s);
+  exp_recip_two<true>(argument_two<kAct>(x), er, r, s);
   return mul2(x, s);
 }
-// The slope of x sigmoid(z(x)), and sigmoid(z) itself.
+// The slope of x sigmoid(z(x)), and sigmoid(z) itself.  Both elements are of one group, whose scale
+// is NaN for all of it or for none.
 template <int kAct>
 __device__ __forceinline__ uint64_t slope_two(uint64_t x, uint64_t& s) {
   uint64_t er, r;
@@ -151,10 +162,10 @@ __device__ __forceinline__ uint64_t slope_two(uint64_t x, uint64_t& s) {
     constexpr float k = 2.0f * kC0;
     const uint64_t x2 = mul2(x, x);
     const uint64_t m = pk(fminf(lo(x2), 256.0f), fminf(hi(x2), 256.0f));
-    exp_recip_two(mul2(x, fma2(m, both(k * kC1 * kLog2e), both(k * kLog2e))), er, r, s);
+    exp_recip_two<false>(mul2(x, fma2(m, both(k * kC1 * kLog2e), both(k * kLog2e))), er, r, s);
     return fma2(mul2(x, mul2(er, r)), fma2(m, both(3.0f * k * kC1), both(k)), s);
   } else {
-    exp_recip_two(argument_two<kAct>(x), er, r, s);
+    exp_recip_two<false>(argument_two<kAct>(x), er, r, s);
     return fma2(x, mul2(er, r), s);
   }
 }

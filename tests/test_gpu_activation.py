@@ -169,3 +169,68 @@ def test_empty():
     y, q, scale = W.act_checkpoint_int8(torch.empty(0, 256, device="cuda").half(), "swiglu")
     assert y.shape == (0, 128) and q.shape == (0, 256) and scale.shape == (0, 2)
     assert W.act_backward_int8(y, q, scale, "swiglu").shape == (0, 256)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("k", [512, 200, 333])
+def test_output_next_to_nan_and_infinity(k, dtype, act):
+    """y is a function of the element itself: what stands beside a NaN or an infinity, at even and odd
+    places, has the bits of the same row without it; the element itself has the formula's value."""
+    import imagine_b200 as W
+
+    t = DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(24, k * (2 if act == "swiglu" else 1), generator=g, device="cuda").to(t)
+    clean = W.act_checkpoint_int8(x, act)[0]
+    spots = [0, 1, 2, 63, 64, 127, 128, k - 2, k - 1, 31, 100, 165]
+    for half in range(2 if act == "swiglu" else 1):
+        for v in (float("nan"), float("inf"), -float("inf")):
+            z = x.clone()
+            hit = torch.zeros(24, k, dtype=torch.bool, device="cuda")
+            for row in range(24):
+                at = spots[row % len(spots)]
+                z[row, half * k + at] = v
+                hit[row, at] = True
+            y, q, scale = W.act_checkpoint_int8(z, act)
+            assert torch.equal(y[~hit], clean[~hit])
+            want = _forward(z.double(), act)[0][hit]
+            # -inf times a sigmoid of zero is NaN, as in the formula
+            assert torch.equal(y[hit].isnan(), want.isnan())
+            known = ~want.isnan()
+            assert torch.equal(y[hit][known].double(), want[known])
+            # and the gradient of such a group is NaN, of the others finite
+            dx = W.act_backward_int8(torch.ones_like(y), q, scale, act)
+            groups = -(-k // 128)
+            of = scale.isnan().unflatten(-1, (-1, groups)).repeat_interleave(128, -1)[..., :k]
+            assert bool((of.any(1) == dx.unflatten(-1, (-1, k)).isnan().any(1)).all())
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_zeros_tiny_and_huge_values_of_sixteen_bits(dtype, act):
+    import imagine_b200 as W
+
+    t = DTYPES[dtype]
+    fi = torch.finfo(t)
+    x = torch.randn(6, 512, device="cuda").to(t)
+    x[0] = 0
+    x[1] = x[1].sign() * fi.tiny
+    x[2, ::3] = fi.max
+    x[3, 1::3] = -fi.max
+    x[4] *= fi.smallest_normal ** 0.5
+    x[5] *= 60
+    k = 256 if act == "swiglu" else 512
+    y, q, scale = W.act_checkpoint_int8(x, act)
+    want_q, want_s = _codes(x, k)
+    assert torch.equal(scale.cpu(), want_s) and torch.equal(q.cpu(), want_q)
+    ref, err = _forward(x.double(), act)
+    fits = ref.abs() <= float(fi.max)
+    # a value below the type's normal range is off by half of its last place there
+    tol = fi.eps / 2 * ref.abs() * (1 + 2.0 ** -8) + err + 2 * fi.tiny
+    assert bool(((y.double() - ref).abs() <= tol)[fits].all())
+    assert bool((y[~fits].double().sign() == ref[~fits].sign()).all())
+    dx = W.act_backward_int8(torch.ones(6, k, dtype=t, device="cuda"), q, scale, act)
+    want, err = _backward(torch.ones(6, k, device="cuda").double(), _value(q, scale, k), act)
+    fits = want.abs() <= float(fi.max)
+    _check(torch.where(fits, dx, 0), torch.where(fits, want, 0), torch.where(fits, err, 0))
