@@ -889,15 +889,30 @@ bool bad_align(const void* p, int64_t unit) { return reinterpret_cast<uintptr_t>
 
 int64_t float_size(int dtype) { return dtype == W8A8_F32 ? 4 : 2; }
 
+// Whether M rows of w bytes, ld apart, share a byte with `count` blocks of `size` bytes, `slot` apart.
+// Exact: of each block's rows only the first that reaches it is looked at.
+bool rows_meet_blocks(const void* p, int64_t ld, int64_t w, int64_t M, const void* q, int64_t slot, int64_t size,
+                      int64_t count) {
+  if (!p || !q || M == 0 || w == 0 || size == 0 || count == 0) return false;
+  const auto a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p));
+  const auto b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q));
+  if (a + (M - 1) * ld + w <= b || b + (count - 1) * slot + size <= a) return false;
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t lo = b + i * slot;
+    const int64_t row = a + w > lo ? 0 : ld > 0 ? (lo - a - w) / ld + 1 : M;
+    if (row < M && a + row * ld < lo + size) return true;
+  }
+  return false;
+}
+
 // Whether M rows of w_p bytes, ld_p apart, share a byte with M rows of w_q bytes, ld_q
-// apart.  Rows of two columns of one tensor do not; different strides in one range
-// count as sharing.
+// apart.  Rows of two columns of one tensor do not.
 bool rows_overlap(const void* p, int64_t ld_p, int64_t w_p, const void* q, int64_t ld_q, int64_t w_q, int64_t M) {
   if (!p || !q || M == 0) return false;
+  if (ld_p != ld_q || ld_p == 0) return rows_meet_blocks(p, ld_p, w_p, M, q, ld_q, w_q, M);
   const auto a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p));
   const auto b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q));
   if (a + (M - 1) * ld_p + w_p <= b || b + (M - 1) * ld_q + w_q <= a) return false;
-  if (ld_p != ld_q || ld_p == 0) return true;
   const int64_t d = ((b - a) % ld_p + ld_p) % ld_p;
   return d < w_p || d + w_q > ld_p;
 }
@@ -941,6 +956,18 @@ int check_lora_common(const LoraArgs& g, int64_t workspace_bytes, int backward) 
                 static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   }
   return 0;
+}
+
+// Whether what a call writes in rows (out, dx) shares memory with the adapters, their index or their
+// scales, which its kernels read while they write (y, dy and x are looked at by the callers).
+bool output_meets_adapters(const LoraArgs& g, int64_t cols) {
+  const int64_t size = float_size(g.dtype), ld = g.ldo * size, w = cols * size;
+  const int64_t index = g.adapter64 ? 8 : 4, indices = (g.M + g.rows_per_index - 1) / g.rows_per_index;
+  return rows_meet_blocks(g.out, ld, w, g.M, g.a, g.lda * size, g.R * g.K * size, g.S) ||
+         rows_meet_blocks(g.out, ld, w, g.M, g.b, g.ldb * size, g.N * g.R * size, g.S) ||
+         rows_meet_blocks(g.out, ld, w, g.M, g.adapter, 0, indices * index, 1) ||
+         rows_meet_blocks(g.out, ld, w, g.M, g.scaling, 0, g.S * 4, 1) ||
+         rows_meet_blocks(g.out, ld, w, g.M, g.x_scale, 0, g.M * 4, 1);
 }
 
 }  // namespace
@@ -987,7 +1014,7 @@ int w8a8_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int dt
   if (int rc = check_lora_common(g, workspace_bytes, 0)) return rc;
   const int64_t size = float_size(dtype);
   if ((y != out && rows_overlap(out, ldo * size, N * size, y, ldy * size, N * size, M)) ||
-      (K > 0 && rows_overlap(out, ldo * size, N * size, x, ldx * size, K * size, M))) {
+      (K > 0 && rows_overlap(out, ldo * size, N * size, x, ldx * size, K * size, M)) || output_meets_adapters(g, N)) {
     return fail(W8A8_ERR_VALUE, "lora: out overlaps an operand's memory");
   }
   return finish(lora_add_launch(g, static_cast<cudaStream_t>(stream)));
@@ -1047,6 +1074,7 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
   if (bad_align(da, size) || bad_align(db, size)) {
     return fail(W8A8_ERR_VALUE, "lora: pointer not aligned to its element");
   }
+  if (output_meets_adapters(g, K)) return fail(W8A8_ERR_VALUE, "lora: dx is an operand's memory");
   return finish(lora_backward_launch(g, static_cast<cudaStream_t>(stream)));
 }
 
@@ -1081,6 +1109,11 @@ int w8a8_input_grad(const void* dy, int64_t lddy, const int8_t* w, int64_t ldw, 
   if (workspace_bytes < need || (need > 0 && (!workspace || bad_align(workspace, 256)))) {
     return fail(W8A8_ERR_VALUE, "input_grad: workspace of %lld bytes, %lld needed (256-byte aligned)",
                 static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  }
+  if (rows_meet_blocks(dx, lddx * size, K * size, M, dy, lddy * size, N * size, M) ||
+      rows_meet_blocks(dx, lddx * size, K * size, M, w, ldw, K, N) ||
+      rows_meet_blocks(dx, lddx * size, K * size, M, ws, 0, ws_numel * 4, 1)) {
+    return fail(W8A8_ERR_VALUE, "input_grad: dx is an operand's memory");
   }
   InputGradArgs g{dtype, dy, lddy, w, ldw, ws, ws_numel, dx, lddx, M, N, K, workspace};
   return finish(input_grad_launch(g, static_cast<cudaStream_t>(stream)));

@@ -555,7 +555,7 @@ int w8a8_sampler_step(float* x, const void* out_cond, const void* out_uncond, in
  * w8a8_lora_add: out = y + scaling[s] * (x a[s]^T) b[s]^T, x [M, K], y and out
  * [M, N] (row strides in elements), each output rounded once; a row without an
  * adapter is y's row.  out may be y; it may not overlap it otherwise, nor the
- * other operands.
+ * other operands (refused).
  *
  * w8a8_lora_backward, from dy [M, N]:
  *   dx [M, K] = (dx when accumulate) + scaling[s] * (dy b[s]) a[s], zero (or
@@ -567,7 +567,7 @@ int w8a8_sampler_step(float* x, const void* out_cond, const void* out_uncond, in
  * quantiser (w8a8_quantize_rowwise): the activation's 8-bit checkpoint.
  * Sums are taken in a fixed order: the same call gives the same bits.
  *
- * dx may not overlap dy, x, a or b.
+ * dx may not overlap dy, x, a, b, the index or the scales (refused).
  *
  * workspace: at least w8a8_lora_workspace_bytes(M, N, K, S, R, backward)
  * bytes (backward: 0 w8a8_lora_add, 1 w8a8_lora_backward, 2 its dx alone),
@@ -591,7 +591,8 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * No reference counterpart (the reference only infers).  dx [M, K] = dy [M, N]
  * (ws * w) for w int8 [N, K] (row stride ldw) and its scales ws (N or 1); the
  * quantisation of the input passes the gradient through unchanged.  dy, dx:
- * `dtype` (F32/F16/BF16).  workspace: w8a8_input_grad_workspace_bytes(M, N, K,
+ * `dtype` (F32/F16/BF16); dx may not overlap an operand (refused).
+ * workspace: w8a8_input_grad_workspace_bytes(M, N, K,
  * dtype) bytes, 256-byte aligned, any content (may be 0 bytes, then NULL). */
 int64_t w8a8_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
 int w8a8_input_grad(const void* dy, int64_t lddy, const int8_t* w, int64_t ldw, const float* ws,

@@ -169,3 +169,39 @@ def test_lora_workspace_of_a_dimension_of_zero(backward):
     for m in (0, 1, 64, 100, 300):
         for n, k in ((0, 64), (64, 0), (0, 0), (64, 64)):
             assert need(m, n, k, 2, 8, backward) >= 0
+
+
+@pytest.mark.parametrize("kw", [dict(dy=P), dict(dy=P + 2 * 64 * 9 + 2 * 31), dict(w=P + 2 * 32 * 9), dict(w=P - 63 * 32),
+                                dict(ws=P + 16)])
+def test_input_grad_refuses_a_gradient_in_an_operands_memory(kw):
+    d = dict(dy=P + (1 << 22), w=P + (2 << 22), ws=P + (3 << 22))
+    d.update(kw)
+    rc = N.LIB.w8a8_input_grad(d["dy"], 64, d["w"], 32, d["ws"], 64, N.BF16, P, 64, 10, 64, 32, P + (4 << 22), 1 << 22, None)
+    assert rc == N.ERR_VALUE and "operand's memory" in _err()
+
+
+# Addresses far from each other for whatever a case does not name.
+FAR = dict(a=P + (1 << 22), b=P + (2 << 22), adapter=P + (3 << 22), scaling=P + (4 << 22))
+
+
+@pytest.mark.parametrize("name", list(FAR))
+@pytest.mark.parametrize("at", [0, 2 * 64 * 9])  # the output's first row, and its last
+def test_lora_add_refuses_an_output_in_the_adapters_memory(name, at):
+    far = dict(FAR, y=P + (5 << 22), x=P + (6 << 22))
+    assert _add(**{**far, name: P + at, "out": P}) == N.ERR_VALUE
+    assert "operand's memory" in _err()
+    # the second adapter of a stack alone
+    if name in ("a", "b"):
+        assert _add(**{**far, name: P - 2 * 4096, f"slot_{name}": 4096, "out": P}) == N.ERR_VALUE
+        assert "operand's memory" in _err()
+
+
+@pytest.mark.parametrize("name", [*FAR, "xs"])
+@pytest.mark.parametrize("at", [0, 2 * 32 * 9])
+def test_lora_backward_refuses_a_gradient_in_the_adapters_memory(name, at):
+    far = dict(FAR, dy=P + (5 << 22), x=P + (6 << 22), xs=P + (7 << 22))
+    assert _back(**{**far, name: P + at, "dx": P}) == N.ERR_VALUE
+    assert "operand's memory" in _err()
+    if name in ("a", "b"):
+        assert _back(**{**far, name: P - 2 * 4096, f"slot_{name}": 4096, "dx": P}) == N.ERR_VALUE
+        assert "operand's memory" in _err()

@@ -420,3 +420,33 @@ def test_input_gradient_of_a_weight_without_rows_or_columns(m, dtype):
         w = torch.zeros(n, k, dtype=torch.int8, device="cuda")
         dx = W.int8_linear_backward(torch.ones(m, n, dtype=t, device="cuda"), w, torch.ones(n, device="cuda"))
         assert dx.shape == (m, k) and dx.dtype == t and not bool(dx.any())
+
+
+def test_output_beside_the_adapters_in_one_tensor():
+    """Columns between which other operands lie share nothing with them; an operand's own memory is refused."""
+    import imagine_b200 as W
+
+    m, n, k, s, r = 30, 64, 64, 2, 16
+    gen = torch.Generator("cuda").manual_seed(6)
+    x, y, a, b = (torch.randn(shape, generator=gen, device="cuda", dtype=torch.bfloat16)
+                  for shape in ((m, k), (m, n), (s, r, k), (s, n, r)))
+    want = W.lora_add(y, x, a, b)
+    grads = W.lora_backward(y, x, a, b)
+    # a row of the buffer: 64 columns of out, then 2048 in which an adapter's a (rows 0 and 1) and b (2 and 3) lie
+    big = torch.zeros(m, 64 + 2048, dtype=torch.bfloat16, device="cuda")
+    out, tail = big[:, :64], big[:, 64:]
+    tail[:2].copy_(a.flatten(1, 2)[:, :1024].repeat(1, 2))
+    tail[2:4].copy_(b.flatten(1, 2)[:, :1024].repeat(1, 2))
+    ab, bb = tail[:2, :1024].unflatten(1, (r, k)), tail[2:4, :1024].unflatten(1, (n, r))
+    assert not ab.is_contiguous() and ab.data_ptr() == big.data_ptr() + 128
+    assert torch.equal(W.lora_add(y, x, ab, bb, out=out), want)
+    out.zero_()
+    dx, da, db = W.lora_backward(y, x, ab, bb, dx=out)
+    assert torch.equal(dx, grads[0]) and torch.equal(da, grads[1]) and torch.equal(db, grads[2])
+    for t in (a, b):
+        part = t.flatten()[:m * 64].view(-1, 64)
+        if part.shape[0] == m:
+            with pytest.raises(ValueError, match="operand's memory"):
+                W.lora_add(y, x, a, b, out=part)
+            with pytest.raises(ValueError, match="operand's memory"):
+                W.lora_backward(y, x, a, b, dx=part)
