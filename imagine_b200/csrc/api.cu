@@ -883,7 +883,10 @@ int w8a8_mxfp8_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
 // ---- activations with an 8-bit checkpoint
 namespace {
 
-constexpr int64_t kMaxDim = 0x7fffff00LL;
+// Kernels step through a dimension in 32 bits, by whole tiles and by whole splits of one: the last
+// step ends at most 888 tiles of 128 past the dimension (expand_kernel's column ranges, six
+// blocks for each of 148 multiprocessors), and 2^20 keeps that below 2^31.
+constexpr int64_t kMaxDim = (1LL << 31) - (1LL << 20);
 
 bool bad_align(const void* p, int64_t unit) { return reinterpret_cast<uintptr_t>(p) % unit != 0; }
 

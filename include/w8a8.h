@@ -552,6 +552,8 @@ int w8a8_sampler_step(float* x, const void* out_cond, const void* out_uncond, in
  * an index outside [0, S) means no adapter.  scaling: fp32 [S] or NULL (ones).
  * Adapters of smaller rank are padded with zeros.
  *
+ * M, N and K up to 2^31 - 2^20.
+ *
  * w8a8_lora_add: out = y + scaling[s] * (x a[s]^T) b[s]^T, x [M, K], y and out
  * [M, N] (row strides in elements), each output rounded once; a row without an
  * adapter is y's row.  out may be y; it may not overlap it otherwise, nor the
@@ -593,7 +595,8 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * quantisation of the input passes the gradient through unchanged.  dy, dx:
  * `dtype` (F32/F16/BF16); dx may not overlap an operand (refused).
  * workspace: w8a8_input_grad_workspace_bytes(M, N, K,
- * dtype) bytes, 256-byte aligned, any content (may be 0 bytes, then NULL). */
+ * dtype) bytes, 256-byte aligned, any content (may be 0 bytes, then NULL).  M, N
+ * and K up to 2^31 - 2^20. */
 int64_t w8a8_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
 int w8a8_input_grad(const void* dy, int64_t lddy, const int8_t* w, int64_t ldw, const float* ws,
                     int64_t ws_numel, int dtype, void* dx, int64_t lddx, int64_t M, int64_t N,
@@ -606,7 +609,7 @@ int w8a8_input_grad(const void* dy, int64_t lddy, const int8_t* w, int64_t ldw, 
  * int8 codes q and one fp32 scale = max(amax / 127, 1e-30), q = rne(x /
  * scale).  q [rows, halves * cols], scale [rows, halves * ceil(cols / 128)];
  * y, q and scale contiguous.  A group that holds an infinity or a NaN gets the
- * scale NaN.  w8a8_act_backward: dx [rows, halves * cols] (contiguous) = dy act'(q *
+ * scale NaN.  rows up to 2^31 - 2^20, cols half as many.  w8a8_act_backward: dx [rows, halves * cols] (contiguous) = dy act'(q *
  * scale). */
 #define W8A8_CKPT_GROUP 128
 #define W8A8_CKPT_ACT_GELU_TANH 1

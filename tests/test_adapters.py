@@ -205,3 +205,40 @@ def test_lora_backward_refuses_a_gradient_in_the_adapters_memory(name, at):
     if name in ("a", "b"):
         assert _back(**{**far, name: P - 2 * 4096, f"slot_{name}": 4096, "dx": P}) == N.ERR_VALUE
         assert "operand's memory" in _err()
+
+
+def test_sizes_whose_steps_would_pass_31_bits_are_refused():
+    """A block steps through a dimension in 32 bits, by up to 2048 elements at a time."""
+    most = (1 << 31) - (1 << 20)
+    need = N.LIB.w8a8_lora_workspace_bytes
+    grad = N.LIB.w8a8_input_grad_workspace_bytes
+    for big in (most + 1, 0x7fffff00, 1 << 31):
+        for sizes in ((big, 64, 64), (1, big, 64), (1, 64, big)):
+            for backward in (0, 1, 2):
+                assert need(*sizes, 1, 1, backward) == N.ERR_VALUE and "sizes" in _err()
+            for dtype in (N.BF16, N.F16, N.F32):
+                assert grad(*sizes, dtype) == N.ERR_VALUE and "sizes" in _err()
+        assert N.LIB.w8a8_act_checkpoint(P, N.BF16, 64, big, 64, 1, P, P, P, None) == N.ERR_VALUE
+        assert N.LIB.w8a8_act_backward(P, N.BF16, big, 1, big // 2 + 1, 1, P, P, P, None) == N.ERR_VALUE
+    for sizes in ((most, 64, 64), (1, most, 64), (1, 64, most)):
+        assert need(*sizes, 1, 1, 0) >= 0 and grad(*sizes, N.BF16) >= 0
+
+
+@pytest.mark.parametrize("size", [(1 << 31) - (1 << 20), (1 << 31) - (1 << 20) - 1, (1 << 30) + 7, 4096, 1])
+def test_last_steps_of_the_largest_sizes_stay_below_31_bits(size):
+    """The kernels' index arithmetic, restated: each loop's counter after its last step."""
+    top = (1 << 31) - 1
+    sms = 148
+    # few rows: 256 threads of eight elements
+    assert size - 1 + 256 * 8 <= top
+    # contractions cut into at most 16 splits of whole steps of 64 or 128
+    for step in (64, 128):
+        steps = -(-size // step)
+        for want in range(1, 17):
+            per = -(-steps // want)
+            assert -(-steps // per) * per * step + 2 * step <= top
+    # column ranges: up to six blocks a multiprocessor, of whole tiles of 128
+    tiles = -(-size // 128)
+    for want in range(1, 6 * sms + 1):
+        per = -(-tiles // min(want, tiles))
+        assert -(-tiles // per) * per * 128 + 128 <= top
