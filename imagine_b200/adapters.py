@@ -256,7 +256,11 @@ def int8_linear_backward(dy: torch.Tensor, weight: torch.Tensor, weight_scale: t
     """Input gradient of ``int8_linear``: ``dx = dy (weight_scale * weight)`` for
     ``dy`` [..., N] and the int8 ``weight`` [N, K] with its scales (N or 1), dx
     [..., K] in dy's dtype.  The quantisation of the input passes the gradient through
-    unchanged (the straight-through estimate)."""
+    unchanged (the straight-through estimate).
+
+    Products are summed in fp32 and the result is rounded once.  fp32 and f16 keep their
+    own precision in between; bf16 takes the weight as dequantised to bf16 (off by 2^-8 of itself
+    at most), or, where one scale serves the whole weight, as its exact codes."""
     dev = _cuda("dy", dy).device
     _same("weight", weight, dev)
     if weight.dim() != 2 or weight.dtype != torch.int8:

@@ -1,10 +1,15 @@
 // Gradient of the W8A8 linear's input: dx[m, k] = sum_n dy[m, n] ws[n] w[n, k].
 //
-// The codes w are exact in bf16, so the product runs as bf16 x bf16 -> fp32
-// with the weight scales folded into dy: dy ws, an fp32 product, is cut into
-// one bf16 piece for a bf16 dy (one rounding of 2^-8 at most, as a dequantised bf16
-// weight would have), two for f16 and three for fp32 (pieces.cuh), which keeps
-// each type's own precision.
+// The products run as bf16 x bf16 -> fp32; the codes w are exact in bf16.  Where the weight
+// scales go:
+//   f16, fp32   into dy: the fp32 product dy ws is cut into two or three bf16 pieces
+//               (pieces.cuh), which keeps the type's own precision
+//   bf16        one scale for all: onto the fp32 sum, and nothing is rounded on the way.
+//               A scale a row: into the weight, bf16(w ws), a dequantised bf16 weight,
+//               off by 2^-8 of itself at most.  Two pieces of dy ws would keep it exact and cost
+//               as many products again (5856 x 12288 -> 4096 takes 400 us of them).  All
+//               kernels below round the same value, so that a row's gradient does not
+//               depend on which of them its batch goes to, but for the order of the fp32 sum.
 //
 // Three kernels:
 //   input_grad_few_kernel  up to 16 rows: w from HBM straight into mma.sync fragments
@@ -60,6 +65,10 @@ constexpr int kLdA = kBN + 8, kLdB = kBC + 8;
 
 // Two blocks a multiprocessor.  With 173 registers an fp32 call had one, and the
 // blocks of a cut contraction ran in two waves (712 x 5584 -> 1152: 294 us, now 201).
+// Whether the weight's scale is folded into the weight (or, a single one, put on the sum).
+template <typename T>
+constexpr bool kScaleWeight = std::is_same<T, __nv_bfloat16>::value;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) input_grad_kernel(
     const T* __restrict__ dy, int64_t lddy, const float* __restrict__ ws, int ws_one,
@@ -97,7 +106,9 @@ __global__ void __launch_bounds__(kThreads, 2) input_grad_kernel(
       const int valid = row0 + r < M ? min(8, n_hi - n0 - c) : 0;
       load8(ra[i], dy + (row0 + r) * lddy + n0 + c, valid, vec_dy != 0);
     }
-    if (tid < kBN) next_ws = n0 + tid < n_hi ? __ldg(ws + (ws_one ? 0 : n0 + tid)) : 0.0f;
+    if (tid < kBN) {
+      next_ws = kScaleWeight<T> && ws_one ? 1.0f : n0 + tid < n_hi ? __ldg(ws + (ws_one ? 0 : n0 + tid)) : 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int gi = tid + i * kThreads;
@@ -113,15 +124,29 @@ __global__ void __launch_bounds__(kThreads, 2) input_grad_kernel(
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int gi = tid + i * kThreads;
-      float v[8];
+      __nv_bfloat16* to = sa + (gi >> 3) * kLdA + (gi & 7) * 8;
+      if constexpr (kScaleWeight<T>) {
+        store8(to, kPlane, ra[i]);
+      } else {
+        float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f(ra[i].e[j]) * s_ws[(gi & 7) * 8 + j];  // zeros past n_hi
-      store_pieces<kP>(sa + (gi >> 3) * kLdA + (gi & 7) * 8, kPlane, v);
+        for (int j = 0; j < 8; ++j) v[j] = to_f(ra[i].e[j]) * s_ws[(gi & 7) * 8 + j];  // zeros past n_hi
+        store_pieces<kP>(to, kPlane, v);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int gi = tid + i * kThreads;
-      store8(sb + (gi >> 4) * kLdB + (gi & 15) * 8, 0, rb[i]);
+      __nv_bfloat16* to = sb + (gi >> 4) * kLdB + (gi & 15) * 8;
+      if constexpr (kScaleWeight<T>) {
+        const float scale = s_ws[gi >> 4];
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_f(rb[i].e[j]) * scale;
+        store_pieces<1>(to, 0, v);
+      } else {
+        store8(to, 0, rb[i]);
+      }
     }
     __syncthreads();
     if (n0 + kBN < n_hi) fetch(n0 + kBN);
@@ -153,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 2) input_grad_kernel(
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] += low[i][j];
   }
+  const float post = kScaleWeight<T> && ws_one ? __ldg(ws) : 1.0f;
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -160,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2) input_grad_kernel(
       const int64_t row = row0 + wm * 16 + (lane >> 2) + half * 8;
       const int c = col0 + wn * 64 + n * 8 + (lane & 3) * 2;
       if (row >= M) continue;
-      const float v0 = acc[n][2 * half], v1 = acc[n][2 * half + 1];
+      const float v0 = acc[n][2 * half] * post, v1 = acc[n][2 * half + 1] * post;
       if (part) {
         float* p = part + (blockIdx.y * M + row) * K + c;
         if (c < K) p[0] = v0;
@@ -280,7 +306,7 @@ __device__ __forceinline__ void mma_bf16_pair(uint32_t d, uint64_t a, uint64_t b
 
 struct TcArgs {
   int64_t M;
-  int N, K;
+  int K;
   int n_blocks;   // blocks of 64 of N; the contraction runs over pieces * n_blocks
   int kb_total;
   int col_tiles, row_tiles, splits;
@@ -288,6 +314,7 @@ struct TcArgs {
   int64_t lddx;
   int vec_o;
   float* part;    // splits > 1
+  const float* one_scale;  // the single scale of a bf16 call's weight, for the sums; or NULL
 };
 
 // Unit u: split, then tiles in groups of eight row tiles (the CTAs that run
@@ -425,6 +452,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
+    const float post = g.one_scale ? __ldg(g.one_scale) : 1.0f;
     uint32_t tl = 0;
     for (int unit = first; unit < units; unit += step, ++tl) {
       int mb, cb, lo, hi, split;
@@ -441,6 +469,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + acc * kTcCols + c * 32, v);
         tmem_ld_wait();
+        if (g.one_scale) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * post);
+        }
         if (row >= g.M) {
         } else if (g.part) {
           float* p = g.part + (static_cast<int64_t>(split) * g.M + row) * g.K + col;
@@ -491,8 +523,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // the mantissa of 2^23), four 16-byte pieces of output rows, exchanged through
 // shared memory so that the stores run along n.
 __global__ void __launch_bounds__(kThreads) widen_weights_kernel(
-    const int8_t* __restrict__ w, int64_t ldw, const float* __restrict__ ws, int ws_one, int N, int K,
-    int n_pad, int k_tiles, int vec, __nv_bfloat16* __restrict__ out) {
+    const int8_t* __restrict__ w, int64_t ldw, const float* __restrict__ ws, int N, int K, int n_pad,
+    int k_tiles, int vec, __nv_bfloat16* __restrict__ out) {
   griddep_launch_dependents();
   __shared__ __align__(16) uint4 tile[64][16];
   const int n0 = static_cast<int>(blockIdx.x / k_tiles) * 128, k0 = static_cast<int>(blockIdx.x % k_tiles) * 64;
@@ -519,8 +551,7 @@ __global__ void __launch_bounds__(kThreads) widen_weights_kernel(
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int n = n0 + ng * 8 + 2 * j;
-    sc[j] = pk(ws && n < N ? __ldg(ws + (ws_one ? 0 : n)) : 1.0f,
-               ws && n + 1 < N ? __ldg(ws + (ws_one ? 0 : n + 1)) : 1.0f);
+    sc[j] = pk(ws && n < N ? __ldg(ws + n) : 1.0f, ws && n + 1 < N ? __ldg(ws + n + 1) : 1.0f);
   }
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
@@ -652,7 +683,8 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
   constexpr int kP = Pieces<T>::n;
   constexpr bool direct = kP == 1;  // bf16: TMA takes dy as it lies
   uint8_t* work = static_cast<uint8_t*>(g.workspace);
-  // the scales go into the pieces of dy where there are pieces, else into w
+  // the scales go into the pieces of dy where there are pieces, else into w, a single one onto the sums
+  const bool one = direct && g.ws_numel == 1;
   if constexpr (!direct) {
     const int vec = rows_of_16_bytes(g);
     const int64_t total = g.M * (n_pad / 8);
@@ -666,7 +698,7 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
   const int k_tiles = (K + 63) / 64;
   const cudaError_t we = launch_chained(
       !direct, widen_weights_kernel, dim3(static_cast<unsigned>(static_cast<int64_t>((N + 127) / 128) * k_tiles)),
-      kThreads, 0, stream, g.w, g.ldw, direct ? g.ws : nullptr, static_cast<int>(g.ws_numel == 1), N, K, n_pad, k_tiles,
+      kThreads, 0, stream, g.w, g.ldw, direct && !one ? g.ws : nullptr, N, K, n_pad, k_tiles,
       static_cast<int>(reinterpret_cast<uintptr_t>(g.w) % 4 == 0 && g.ldw % 4 == 0),
       reinterpret_cast<__nv_bfloat16*>(wide));
   if (we != cudaSuccess) {
@@ -683,7 +715,6 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
   }
   TcArgs a{};
   a.M = g.M;
-  a.N = N;
   a.K = K;
   a.n_blocks = p.n_blocks;
   a.kb_total = p.kb_total;
@@ -694,6 +725,7 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
   a.lddx = g.lddx;
   a.vec_o = reinterpret_cast<uintptr_t>(g.dx) % 16 == 0 && (g.lddx * 2) % 16 == 0;
   a.part = p.splits > 1 ? reinterpret_cast<float*>(wide + p.weight_bytes) : nullptr;
+  a.one_scale = one ? g.ws : nullptr;
   auto kern = input_grad_tc_kernel<T>;
   static bool set[64] = {};
   int dev = 0;
@@ -738,10 +770,11 @@ int tc_typed(const InputGradArgs& g, cudaStream_t stream) {
 // range of the contraction, 128 of it a step, a warp sixteen: w goes from HBM
 // straight into the warp's matrix fragments, two steps ahead (a lane reads eight
 // columns of four rows; which of the tile's columns a fragment column stands for is
-// free to choose), and only the pieces of dy ws pass through shared memory.  The
+// free to choose), and only dy or the pieces of dy ws pass through shared memory.  The
 // eight warps' sums are joined in order at the end.
-// 4096 -> 4096 with its sum: 16.2 us (fp32: 22.7) where input_grad_kernel, which stages
-// w in shared memory, takes 19.3 (39.6).  At 32 rows this form takes 27, that one 21.
+// A captured call of 16 rows, sum included, memory cold: 4096 -> 4096 in 22.5 us (f16 26.6, fp32
+// 30.7) where input_grad_kernel, which stages w in shared memory, takes 24.5 (32.8, 47.1); 12288 ->
+// 4096 in 45 (57, 68) against 49 (70, 112).  At 32 rows this form took 27, that one 21.
 constexpr int kFewRows = 16, kFewCols = 64, kFewN = 128, kLdFew = kFewN + 8;
 
 template <typename T>
@@ -764,15 +797,21 @@ __global__ void __launch_bounds__(kThreads) input_grad_few_kernel(
 
   float acc[8][4] = {};
   float low[kApart ? 8 : 1][4] = {};
-  uint2 wq[2][4];
-  auto fetch_w = [&](int n0, uint2 (&r)[4]) {
+  // a step's four rows of w: their codes, and their scales where those go into the weight
+  struct Codes {
+    uint2 q[4];
+    float scale[kScaleWeight<T> ? 4 : 1];
+  };
+  Codes wq[2];
+  auto fetch_w = [&](int n0, Codes& r) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = n0 + warp * 16 + 2 * q + (i & 1) + (i >> 1) * 8;
-      r[i] = in_k && n < n_hi ? __ldg(reinterpret_cast<const uint2*>(w + n * ldw + col)) : make_uint2(0, 0);
+      r.q[i] = in_k && n < n_hi ? __ldg(reinterpret_cast<const uint2*>(w + n * ldw + col)) : make_uint2(0, 0);
+      if constexpr (kScaleWeight<T>) r.scale[i] = ws_one || n >= n_hi ? 1.0f : __ldg(ws + n);
     }
   };
-  // dy ws of one step: kRows x 128 elements, eight at a time
+  // dy (times ws) of one step: kRows x 128 elements, eight at a time
   static_assert(kRows * (kFewN / 8) == kThreads, "eight elements a thread");
   auto lay = [&](int n0, int buf) {
     {
@@ -780,23 +819,32 @@ __global__ void __launch_bounds__(kThreads) input_grad_few_kernel(
       const int valid = r < M ? min(8, n_hi - n0 - c) : 0;
       Raw8<T> raw;
       load8(raw, dy + static_cast<int64_t>(r) * lddy + n0 + c, valid, vec_dy != 0);
-      float v[8];
+      if constexpr (kScaleWeight<T>) {
+        store8(sa + buf * kP * kPlane + r * kLdFew + c, kPlane, raw);
+      } else {
+        float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = j < valid ? to_f(raw.e[j]) * __ldg(ws + (ws_one ? 0 : n0 + c + j)) : 0.0f;
-      store_pieces<kP>(sa + buf * kP * kPlane + r * kLdFew + c, kPlane, v);
+        for (int j = 0; j < 8; ++j)
+          v[j] = j < valid ? to_f(raw.e[j]) * __ldg(ws + (ws_one ? 0 : n0 + c + j)) : 0.0f;
+        store_pieces<kP>(sa + buf * kP * kPlane + r * kLdFew + c, kPlane, v);
+      }
     }
   };
   fetch_w(n_lo, wq[0]);
   fetch_w(n_lo + kFewN, wq[1]);
   lay(n_lo, 0);
   __syncthreads();
-  auto step = [&](int n0, int buf, uint2 (&r)[4]) {
+  auto step = [&](int n0, int buf, Codes& r) {
     uint32_t x[4][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[i][0] = r[i].x ^ 0x80808080u;
-      x[i][1] = r[i].y ^ 0x80808080u;
+      x[i][0] = r.q[i].x ^ 0x80808080u;
+      x[i][1] = r.q[i].y ^ 0x80808080u;
+    }
+    uint64_t scale[2];
+    if constexpr (kScaleWeight<T>) {
+      scale[0] = pk(r.scale[0], r.scale[1]);
+      scale[1] = pk(r.scale[2], r.scale[3]);
     }
     fetch_w(n0 + 2 * kFewN, r);
     if (n0 + kFewN < n_hi) lay(n0 + kFewN, buf ^ 1);
@@ -809,10 +857,11 @@ __global__ void __launch_bounds__(kThreads) input_grad_few_kernel(
       uint32_t b[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint64_t f =
+        uint64_t f =
             add2(pk(__uint_as_float(__byte_perm(x[2 * h][j >> 2], 0x4B000000u, 0x7540 + (j & 3))),
                     __uint_as_float(__byte_perm(x[2 * h + 1][j >> 2], 0x4B000000u, 0x7540 + (j & 3)))),
                  magic);
+        if constexpr (kScaleWeight<T>) f = mul2(f, scale[h]);
         b[h] = pack_bf16(lo(f), hi(f));
       }
 #pragma unroll
@@ -857,10 +906,11 @@ __global__ void __launch_bounds__(kThreads) input_grad_few_kernel(
     }
     __syncthreads();
   }
+  const float post = kScaleWeight<T> && ws_one ? __ldg(ws) : 1.0f;
   for (int i = tid; i < kRows * kFewCols; i += kThreads) {
     const int r = i / kFewCols, c = blockIdx.x * kFewCols + i % kFewCols;
     if (r >= M || c >= K) continue;
-    const float v = sum[r * (kFewCols + 1) + i % kFewCols];
+    const float v = sum[r * (kFewCols + 1) + i % kFewCols] * post;
     if (part) {
       part[(static_cast<int64_t>(blockIdx.y) * M + r) * K + c] = v;
     } else {

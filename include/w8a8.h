@@ -592,8 +592,10 @@ int w8a8_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
 /* ---- gradient of the int8 linear's input ----------------------------------
  * No reference counterpart (the reference only infers).  dx [M, K] = dy [M, N]
  * (ws * w) for w int8 [N, K] (row stride ldw) and its scales ws (N or 1); the
- * quantisation of the input passes the gradient through unchanged.  dy, dx:
- * `dtype` (F32/F16/BF16); dx may not overlap an operand (refused).
+ * quantisation of the input passes the gradient through unchanged.  F32 and F16
+ * keep their own precision; BF16 multiplies by the weight dequantised to bf16,
+ * bf16(ws w), or with one scale by w itself, the fp32 sum times ws.  Sums in fp32, the
+ * result rounded once.  dy, dx: `dtype` (F32/F16/BF16); dx may not overlap an operand (refused).
  * workspace: w8a8_input_grad_workspace_bytes(M, N, K,
  * dtype) bytes, 256-byte aligned, any content (may be 0 bytes, then NULL).  M, N
  * and K up to 2^31 - 2^20. */

@@ -450,3 +450,33 @@ def test_output_beside_the_adapters_in_one_tensor():
                 W.lora_add(y, x, a, b, out=part)
             with pytest.raises(ValueError, match="operand's memory"):
                 W.lora_backward(y, x, a, b, dx=part)
+
+
+@pytest.mark.parametrize("scalar", [False, True])
+@pytest.mark.parametrize("k,n", [(264, 4096), (130, 333), (1024, 1040)])
+def test_bf16_input_gradient_is_the_same_product_in_every_form(k, n, scalar):
+    """bf16: dy times the weight dequantised to bf16, whatever the rows and strides (and so the kernel);
+    with one scale for the whole weight, dy times the codes, the scale on the sum: nothing rounded on
+    the way.  What is left beside the output's rounding is the fp32 sum: its products, at most sixteen
+    splits and eight warps joined (2^-24 each) and the scale's product."""
+    import imagine_b200 as W
+
+    g = torch.Generator(device="cuda").manual_seed(k)
+    m = 300
+    dy = torch.randn(m, n, generator=g, device="cuda").bfloat16()
+    w = torch.randint(-128, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    ws = torch.rand(1 if scalar else n, generator=g, device="cuda") * 1e-3 + 1e-4
+    if scalar:
+        wd = w.double() * ws.double()
+    else:
+        wd = (w.float() * ws.view(-1, 1)).bfloat16().double()
+    ref, size = dy.double() @ wd, dy.double().abs() @ wd.abs()
+    rel = _sums(n) + 6 * 2.0 ** -22 + 2.0 ** -23
+    apart = torch.empty(m, n + 3, dtype=dy.dtype, device="cuda")[:, 1:1 + n]
+    apart.copy_(dy)
+    wide = torch.empty(n, k + 5, dtype=torch.int8, device="cuda")[:, 2:2 + k]
+    wide.copy_(w)
+    for rows in (1, 10, 16, 17, 64, 65, 300):
+        for d in (dy, apart):
+            for v in (w, wide):
+                _check(W.int8_linear_backward(d[:rows], v, ws), ref[:rows], size[:rows], rel, f"{rows} rows")
