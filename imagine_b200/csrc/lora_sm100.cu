@@ -387,16 +387,22 @@ __global__ void __launch_bounds__(kThreads) shrink_tc_kernel(
       float* dst = part + (static_cast<int64_t>(blockIdx.y) * rows.M + row) * R;
       for (int i = 0; i < n; ++i) {
         const bool mine = id[r] == adapter(i0 + i);
+        constexpr int kLoad = kRank < 32 ? kRank : 32;  // no further than the block's columns
 #pragma unroll
-        for (int c = 0; c < kRank; c += 32) {
-          uint32_t d[32];
+        for (int c = 0; c < kRank; c += kLoad) {
+          uint32_t d[kLoad];
           __syncwarp();
-          tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + i * kRank + c, d);
+          const uint32_t at = tmem + (static_cast<uint32_t>(warp * 32) << 16) + i * kRank + c;
+          if constexpr (kLoad == 32) {
+            tmem_ld_32x32b_x32(at, d);
+          } else {
+            tmem_ld_32x32b_x16(at, d);
+          }
           tmem_ld_wait();
           if (mine) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {  // R % 8 == 0
-              if (c + j < R && j < kRank) {
+            for (int j = 0; j < kLoad; j += 4) {  // R % 8 == 0
+              if (c + j < R) {
                 *reinterpret_cast<float4*>(dst + c + j) =
                     make_float4(__uint_as_float(d[j]) * mul, __uint_as_float(d[j + 1]) * mul,
                                 __uint_as_float(d[j + 2]) * mul, __uint_as_float(d[j + 3]) * mul);

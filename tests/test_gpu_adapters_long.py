@@ -235,3 +235,36 @@ def test_a_layer_as_it_is_trained(dtype):
     for name, got, ref in zip(("x", "a1", "b1", "a2", "b2"), grads, (dx, da1, db1, da2, db2)):
         off = float((got.double() - ref).norm() / ref.norm())
         assert off < 7 * u_ + 1e-5, (name, off)
+
+
+@pytest.mark.parametrize("r", [8, 16, 24, 32, 64, 128])
+@pytest.mark.parametrize("s", [16, 33, 64])
+@pytest.mark.parametrize("codes", [False, True])
+def test_as_many_adapters_in_a_block_as_tensor_memory_holds(s, r, codes):
+    """A long contraction of rows of many adapters: a block's accumulators take all of its columns, and
+    several passes where there are more adapters."""
+    import imagine_b200 as W
+
+    m, wide, narrow = 1500, 2048, 64
+    x, y, _, a, b, c, idx = _case(m, wide, narrow, s, r, torch.bfloat16, seed=5)
+    _check(W.lora_add(y, x, a, b, idx, c), *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(wide, r))
+    _quiet()
+    x, _, dy, a, b, c, idx = _case(m, narrow, wide, s, r, torch.bfloat16, seed=6)
+    xs, data = None, x
+    if codes:
+        x, xs = W.quantize_int8_rowwise(x)
+        data = x.double() * xs.double()
+    _check_grads(W.lora_backward(dy, x, a, b, idx, c, x_scale=xs), data, dy, a, b, c, idx)
+    _quiet()
+    x, _, dy, a, b, c, idx = _case(m, wide, narrow, s, r, torch.bfloat16, seed=7)
+    if codes:
+        x, xs = W.quantize_int8_rowwise(x)
+        data = x.double() * xs.double()
+    else:
+        data = x
+    ref = _grad_ref(data, dy, a, b, c, idx)
+    dx, da, db = W.lora_backward(dy, x, a, b, idx, c, x_scale=xs, need_dx=False)
+    assert dx is None
+    _check(da, *ref["da"], 2 * PIECES[dy.dtype] + _sums(narrow, m), "da")
+    _check(db, *ref["db"], 2 * PIECES[dy.dtype] + _sums(wide, m), "db")
+    _quiet()
