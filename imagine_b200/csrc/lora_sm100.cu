@@ -732,10 +732,11 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
 // One block a multiprocessor takes an equal share of all 128 x 64 tiles, row tile by
 // row tile, a tile counted as often as it takes (its adapters are counted by the
 // shrink kernel): a segment is its run of columns in one row tile, whose h it keeps as
-// pieces in shared memory.  y arrives by TMA up to eight tiles ahead, W_s four; the
-// products lie in four accumulators; two groups of four warps take the tiles in
-// turn, add the product to y in place in shared memory, and a TMA store takes the
-// tile away.  Bound by reading y and writing out: 11712 x 12288 at rank 64 in 117 us,
+// pieces in shared memory.  y arrives by TMA up to eight tiles ahead, W_s four; two
+// groups of four warps take the tiles in turn, add the product to y in place in shared
+// memory, and a TMA store takes the tile away.  Each group has two accumulators and two
+// pairs of barriers of its own: a wait tells apart only odd and even phases, so a warp has to
+// see every phase of a barrier it waits on, and a tile's products may be any number.  Bound by reading y and writing out: 11712 x 12288 at rank 64 in 117 us,
 // 561 MB of HBM traffic at 4.8 TB/s (a copy reaches 6.2).
 // Three stages and one group of warps, twice a multiprocessor, waited for the loads:
 // 178 us on 11712 x 12288 at rank 64.
@@ -779,7 +780,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   Bars* bars = reinterpret_cast<Bars*>(s_w + C::kWStages * C::kW);
   uint64_t *y_full = bars->full, *y_empty = bars->empty;
   uint64_t *w_full = bars->w_full, *w_empty = bars->w_empty;
-  uint64_t* tfull = bars->acc;         // four accumulators
+  uint64_t* tfull = bars->acc;         // four accumulators, 2 g and 2 g + 1 group g's
   uint64_t* tempty = bars->acc + 4;
   uint64_t* h_there = &bars->done;
   int* id = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + kBarBytes);
@@ -802,7 +803,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
     }
     for (int b = 0; b < 4; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 4);
+      mbar_init(&tempty[b], 4);  // the warps of its group
     }
     mbar_init(h_there, 8);
     bars->abort_flag = 0;
@@ -822,8 +823,9 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
   tc_fence_after();
   griddep_launch_dependents();  // after the allocation, as in shrink_tc_kernel
   const uint32_t tmem = bars->tmem;
-  uint32_t yt = 0;       // tiles this block has gone through
+  uint32_t yt = 0;       // tiles this block has gone through; odd ones are group 1's
   uint32_t wt = 0;       // products (a tile times an adapter)
+  uint32_t made[2] = {0, 0};  // of them, of each group's tiles (epilogue: its own group's alone)
   uint32_t h_count = 0;  // times h has been laid down
   int to_free = -1;      // the stage whose store may still be reading
 
@@ -937,11 +939,21 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
         constexpr uint32_t idesc = idesc_bf16(kECols, 0, kWCols ? 0 : 1);
         bool ok = mbar_wait(h_there, h_count & 1u, abortv, err, kDevTimeoutFull);
         ++h_count;
-        const uint32_t end = wt + static_cast<uint32_t>(t_hi - t_lo) * static_cast<uint32_t>(n);
-        for (; ok && wt != end; ++wt) {
+        const uint32_t tiles = static_cast<uint32_t>(t_hi - t_lo);
+        const uint32_t products = tiles * static_cast<uint32_t>(n);
+        uint32_t left = static_cast<uint32_t>(n);  // of the tile
+        uint32_t group = yt & 1u;
+        yt += tiles;
+        for (uint32_t i = 0; ok && i < products; ++i, ++wt) {
+          if (left == 0) {
+            left = static_cast<uint32_t>(n);
+            group ^= 1u;
+          }
+          --left;
           const int ws = static_cast<int>(wt % C::kWStages);
-          const uint32_t acc = wt & 3u;
-          if (!mbar_wait(&tempty[acc], ((wt >> 2) & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty) ||
+          const uint32_t j = group ? made[1]++ : made[0]++;
+          const uint32_t acc = 2 * group + (j & 1u);
+          if (!mbar_wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u, abortv, err, kDevTimeoutTmemEmpty) ||
               !mbar_wait(&w_full[ws], (wt / C::kWStages) & 1u, abortv, err, kDevTimeoutFull)) {
             break;
           }
@@ -988,7 +1000,7 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
       if (lane == 0) mbar_arrive(h_there);
       const float mul = own >= 0 && scaling ? __ldg(scaling + own) : 1.0f;
       bool ok = true;
-      for (int t = t_lo; ok && t < t_hi; ++t, ++yt, wt += static_cast<uint32_t>(n)) {
+      for (int t = t_lo; ok && t < t_hi; ++t, ++yt) {
         if (static_cast<int>(yt & 1u) != group) continue;
         const int s = static_cast<int>(yt % C::kYStages);
         bool there = mbar_wait(&y_full[s], (yt / C::kYStages) & 1u, abortv, err, kDevTimeoutFull);
@@ -1002,9 +1014,9 @@ __global__ void __launch_bounds__(kEThreads, 1) expand_tc_kernel(
           for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(yr + (c << 4)) = make_uint4(0, 0, 0, 0);
         }
         for (int li = 0; li < n; ++li) {
-          const uint32_t j = wt + static_cast<uint32_t>(li);
-          const uint32_t acc = j & 3u;
-          there = mbar_wait(&tfull[acc], (j >> 2) & 1u, abortv, err, kDevTimeoutTmemFull);
+          const uint32_t j = made[0]++;
+          const uint32_t acc = 2 * static_cast<uint32_t>(group) + (j & 1u);
+          there = mbar_wait(&tfull[acc], (j >> 1) & 1u, abortv, err, kDevTimeoutTmemFull);
           if (!__all_sync(0xffffffffu, there)) {
             ok = false;
             break;

@@ -268,3 +268,32 @@ def test_as_many_adapters_in_a_block_as_tensor_memory_holds(s, r, codes):
     _check(da, *ref["da"], 2 * PIECES[dy.dtype] + _sums(narrow, m), "da")
     _check(db, *ref["db"], 2 * PIECES[dy.dtype] + _sums(wide, m), "db")
     _quiet()
+
+
+@pytest.mark.parametrize("m,k,n,s,r", [
+    (700, 264, 4096, 4, 16), (700, 4096, 512, 16, 64), (1500, 264, 2048, 64, 16), (1500, 2048, 264, 9, 128),
+    (3000, 512, 520, 64, 64), (2000, 1032, 1544, 5, 40)])
+@pytest.mark.parametrize("order", ["mixed", "runs", "some"])
+def test_many_adapters_in_tiles_of_blocks_with_several(m, k, n, s, r, order):
+    """More tiles than multiprocessors, so that a block goes through several, each with as many products
+    as its 128 rows have adapters: every row another one, short runs, or tiles of one, none and many."""
+    import imagine_b200 as W
+
+    x, y, dy, a, b, c, idx = _case(m, k, n, s, r, torch.bfloat16, seed=4)
+    if order == "runs":
+        idx = (torch.arange(m, device="cuda") // 11 % (s + 1) - 1).int()
+    elif order == "some":
+        tile = torch.arange(m, device="cuda") // 128
+        idx = torch.where(tile % 3 == 0, idx, torch.where(tile % 3 == 1, tile.int() % s, -1)).int()
+    out = W.lora_add(y, x, a, b, idx, c)
+    _quiet()
+    _check(out, *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(k, r), "out")
+    assert torch.equal(out, W.lora_add(y.clone(), x, a, b, idx, c, out=y))
+    got = W.lora_backward(dy, x, a, b, idx, c)
+    _quiet()
+    _check_grads(got, x, dy, a, b, c, idx)
+    base = torch.randn(m, k, device="cuda").bfloat16()
+    dx = W.lora_backward(dy, x, a, b, idx, c, dx=base.clone(), need_weights=False)[0]
+    _quiet()
+    ref, size = _grad_ref(x, dy, a, b, c, idx)["dx"]
+    _check(dx, ref + base.double(), size, 2 * PIECES[dy.dtype] + _sums(n, r), "dx added")
