@@ -908,7 +908,7 @@ int shrink_tc(const LoraArgs& g, const void* x, int64_t ldx, bool codes, const f
   const int64_t blocks = (g.M + 127) / 128 * sp.count;
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(g.S, 2ll * device_sm_count() / blocks));
   return lora_shrink_tc({x, codes, ldx, x_scale, w, w_rows, slot, g.M, K, g.S, g.R, sp.count, sp.per / 64,
-                         static_cast<int>(parts), part, counts, first, start_early(g)},
+                         static_cast<int>(parts), part, counts, first},
                         {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
 }
 
@@ -964,7 +964,7 @@ int shrink_pair(const ShrinkArgs<T, T>& dy, int splits_dy, const ShrinkArgs<TX, 
 
 template <typename T, bool kWCols>
 int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, int64_t slot,
-           const float* scaling, const Rows& rows, int N, int R, T* out, int64_t ldo, bool early,
+           const float* scaling, const Rows& rows, int N, int R, T* out, int64_t ldo,
            cudaStream_t stream) {
   const int64_t tiles = (rows.M + kBM - 1) / kBM;
   const int col_tiles = (N + kBN - 1) / kBN;
@@ -982,7 +982,7 @@ int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, i
     auto k = expand_kernel<T, RANK, kWCols>;                                                      \
     constexpr int bytes = ExpandTile<T, RANK, kWCols>::kBytes;                                    \
     if (int rc = prepare(k, bytes)) return rc;                                                    \
-    e = launch_chained(early, k, grid, kThreads, bytes, stream, y, ldy, part, splits, w, slot, scaling, rows, N, R, parts, \
+    e = launch_chained(true, k, grid, kThreads, bytes, stream, y, ldy, part, splits, w, slot, scaling, rows, N, R, parts, \
                                          per * kBN, vw, vo, out, ldo);                            \
   }
   switch (pad_rank(R)) {
@@ -997,7 +997,7 @@ int expand(const T* y, int64_t ldy, const float* part, int splits, const T* w, i
 
 template <typename TX, typename T>
 int tokens_pair(const TokensArgs<TX>& a, const TokensArgs<T>& b, const float* scaling, const Rows& rows, int R,
-                bool early, cudaStream_t stream) {
+                cudaStream_t stream) {
   const dim3 grid(a.chunks * a.count + b.chunks * b.count, 1, rows.S);
   cudaError_t e = cudaSuccess;
 #define TOKENS(RANK)                                                       \
@@ -1005,7 +1005,7 @@ int tokens_pair(const TokensArgs<TX>& a, const TokensArgs<T>& b, const float* sc
     auto k = tokens_pair_kernel<TX, T, RANK>;                              \
     constexpr int bytes = std::max(TokensTile<TX, T, RANK, false>::kBytes, TokensTile<T, T, RANK, true>::kBytes); \
     if (int rc = prepare(k, bytes)) return rc;                             \
-    e = launch_chained(early, k, grid, kThreads, bytes, stream, a, b, scaling, rows, R); \
+    e = launch_chained(true, k, grid, kThreads, bytes, stream, a, b, scaling, rows, R); \
   }
   BY_RANK(TOKENS)
 #undef TOKENS
@@ -1026,10 +1026,9 @@ int add_few_rows(const LoraArgs& g, const Rows& rows, float* h, cudaStream_t str
   const unsigned m = static_cast<unsigned>(g.M);
   shrink_row_kernel<T><<<dim3(R, m), kThreads, 0, stream>>>(x, g.ldx, a, g.lda, rows, K, R, vec, h);
   if (int rc = launched("lora shrink")) return rc;
-  const bool early = true;  // one row tile: latency is all
   const bool whole = R % 8 == 0 && aligned(b, R, sizeof(T)) && aligned(b, g.ldb, sizeof(T));
   return chained("lora expand",
-                 launch_chained(early, whole ? expand_row_kernel<T, true> : expand_row_kernel<T, false>,
+                 launch_chained(true, whole ? expand_row_kernel<T, true> : expand_row_kernel<T, false>,
                                 dim3((N + kThreads - 1) / kThreads, m), kThreads, 0, stream, y, g.ldy,
                                 static_cast<const float*>(h), b, g.ldb, g.scaling, rows, N, R,
                                 static_cast<T*>(g.out), g.ldo));
@@ -1053,12 +1052,12 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
     return rc;
   }
   if (counts && tc_rows(g.y, g.ldy, 2) && tc_rows(g.out, g.ldo, 2) && tc_weights(g.b, g.ldb, R, g.S)) {
-    return lora_expand_tc({g.y, g.ldy, counts, part, sp.count, g.b, 1, g.ldb, g.scaling, g.out, g.ldo, g.M, g.N, g.S, g.R, start_early(g)},
+    return lora_expand_tc({g.y, g.ldy, counts, part, sp.count, g.b, 1, g.ldb, g.scaling, g.out, g.ldo, g.M, g.N, g.S, g.R},
                           {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream);
   }
   return expand<T, true>(static_cast<const T*>(g.y), g.ldy, part, sp.count,
                          static_cast<const T*>(g.b), g.ldb, g.scaling, rows, N, R,
-                         static_cast<T*>(g.out), g.ldo, start_early(g), stream);
+                         static_cast<T*>(g.out), g.ldo, stream);
 }
 
 struct BackwardPlan {
@@ -1095,7 +1094,6 @@ template <typename T, typename TX>
 int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
   const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
-  const bool early = start_early(g);
   const bool tc = tc_shape(g) && tc_x(g) && tc_rows(g.y, g.ldy, 2) && tc_weights(g.a, g.lda, g.K, g.S) &&
                   tc_weights(g.b, g.ldb, g.R, g.S);
   const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R, tc, g.da != nullptr);
@@ -1124,14 +1122,14 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
     }
     if (g.out && tc && tc_rows(g.out, g.ldo, 2)) {
       if (int rc = lora_expand_tc({g.accumulate ? g.out : nullptr, g.ldo, counts, pg, p.g.count, a, 0, g.lda, g.scaling,
-                                   g.out, g.ldo, g.M, g.K, g.S, g.R, early},
+                                   g.out, g.ldo, g.M, g.K, g.S, g.R},
                                   {g.adapter, g.adapter64, g.rows_per_index, g.M, g.S}, stream)) {
         return rc;
       }
     } else if (g.out) {
       if (int rc = expand<T, false>(g.accumulate ? static_cast<const T*>(g.out) : nullptr, g.ldo, pg,
                                     p.g.count, a, g.lda, g.scaling, rows, K, R,
-                                    static_cast<T*>(g.out), g.ldo, start_early(g), stream)) {
+                                    static_cast<T*>(g.out), g.ldo, stream)) {
         return rc;
       }
     }
@@ -1142,15 +1140,15 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
     void *qa = ws + p.off_pa, *qb = ws + p.off_pb;
     uint8_t* info = ws + p.off_info;
     if (int rc = shrink_tc(g, x, g.ldx, g.x_scale != nullptr, g.x_scale, a, g.lda, true, K, p.h, ph, nullptr, false, stream)) return rc;
-    if (int rc = lora_rank_pieces({pg, p.g.count, g.x_scale, qa, ph, p.h.count, qb, g.scaling, R, info, early}, lr, stream)) {
+    if (int rc = lora_rank_pieces({pg, p.g.count, g.x_scale, qa, ph, p.h.count, qb, g.scaling, R, info}, lr, stream)) {
       return rc;
     }
     const int per_a = static_cast<int>(p.a.per / kBM), per_b = static_cast<int>(p.b.per / kBM);
     if (int rc = lora_tokens_tc({x, g.x_scale != nullptr, g.ldx, qa, g.M, g.K, g.S, g.R, 0, p.a.count, per_a,
-                                 info, pa, fa, early}, lr, stream)) {
+                                 info, pa, fa}, lr, stream)) {
       return rc;
     }
-    if (int rc = lora_tokens_tc({dy, 0, g.ldy, qb, g.M, g.N, g.S, g.R, 1, p.b.count, per_b, info, pb, fb, early}, lr,
+    if (int rc = lora_tokens_tc({dy, 0, g.ldy, qb, g.M, g.N, g.S, g.R, 1, p.b.count, per_b, info, pb, fb}, lr,
                                 stream)) {
       return rc;
     }
@@ -1159,14 +1157,14 @@ int backward_typed(const LoraArgs& g, cudaStream_t stream) {
                             aligned(x, g.ldx, sizeof(TX)), pa, fa};
     const TokensArgs<T> tb{dy, g.ldy, nullptr, ph, p.h.count, N, p.b.per, p.b.count, (N + kBN - 1) / kBN,
                            aligned(dy, g.ldy, sizeof(T)), pb, fb};
-    if (int rc = tokens_pair<TX, T>(ta, tb, g.scaling, rows, R, early, stream)) return rc;
+    if (int rc = tokens_pair<TX, T>(ta, tb, g.scaling, rows, R, stream)) return rc;
   }
   const SumArgs sa{pa, fa, p.a.count, g.R * g.K, g.da}, sb{pb, fb, p.b.count, g.R * g.N, g.db};
   const int64_t most = std::max(sa.per, sb.per);
   const int64_t want = (most + 4 * kThreads - 1) / (4 * kThreads);
   const int64_t cap = std::max<int64_t>(1, 8ll * device_sm_count() / g.S);
   return chained("lora gradient sum",
-                 launch_chained(early, sum_splits_kernel<T>,
+                 launch_chained(true, sum_splits_kernel<T>,
                                 dim3(static_cast<unsigned>(std::min(want, cap)), static_cast<unsigned>(g.S), 2),
                                 kThreads, 0, stream, sa, sb, static_cast<int>(g.S)));
 }

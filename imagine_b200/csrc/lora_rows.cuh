@@ -70,18 +70,14 @@ __device__ __forceinline__ void tile_ids(const Rows& rows, int64_t row0, TileIds
   __syncthreads();
 }
 
-// Whether a call's kernels start early (launch_chained): where a call moves little,
-// their launches and prologues are worth hiding (5856 rows, 4096 -> 4096, rank 16:
-// gradients in 82 us against 97); in long calls a kernel's early blocks disturb the one
-// they wait for (11712 rows, 4096 -> 12288, rank 64: forward 161 us against 152,
-// gradients 316 against 303).
-inline bool start_early(const LoraArgs& g) { return g.M * (g.N + g.K) <= (100ll << 20); }
-
 // Launches a kernel of a chain: it may start while the one before it on the stream
 // still runs, waits (griddep_wait) before it reads what that one wrote or writes
 // anything, and lets the next one start in turn (griddep_launch_dependents).  What
 // the call's user wrote is there from the start: the chain's first kernel is
-// launched plainly.  `early` false: every kernel waits for the end of the one before.
+// launched plainly (`early` false).  Hiding launches and prologues is worth it at every size: calls
+// one after another, early against not, gradients of 5856 rows, 4096 -> 4096, rank 16 in 81 us
+// against 98, of 11712 rows, 4096 -> 12288, rank 64 in 237 against 260 (forward 142 against
+// 145), of 40000 rows, 4096 -> 4096, rank 32 in 380 against 405.
 template <typename... P, typename... A>
 cudaError_t launch_chained(bool early, void (*kernel)(P...), dim3 grid, int threads, int bytes, cudaStream_t stream,
                            A... args) {

@@ -1171,7 +1171,7 @@ int shrink_rank(const ShrinkTcArgs& g, const Rows& rows, cudaStream_t stream) {
     return launched("lora shrink");
   }
   return chained("lora shrink",
-                 launch_chained(g.early != 0, k, grid, kThreads, bytes, stream, tx, tw, rows, g.x_scale,
+                 launch_chained(true, k, grid, kThreads, bytes, stream, tx, tw, rows, g.x_scale,
                                 static_cast<int>(g.K), static_cast<int>(g.R), g.kb_split, g.part, g.counts));
 }
 
@@ -1199,7 +1199,7 @@ int tokens_rank(const TokensTcArgs& g, const Rows& rows, cudaStream_t stream) {
   if (int rc = opt_in(k, bytes)) return rc;
   const dim3 grid(static_cast<unsigned>((g.C + kTCols - 1) / kTCols), g.splits);
   return chained("lora tokens",
-                 launch_chained(g.early != 0, k, grid, kThreads, bytes, stream, tx, th, rows, static_cast<int>(g.C),
+                 launch_chained(true, k, grid, kThreads, bytes, stream, tx, th, rows, static_cast<int>(g.C),
                                 static_cast<int>(g.R), static_cast<int>(tiles), g.tiles_split, g.info, g.part, g.found));
 }
 
@@ -1230,7 +1230,7 @@ int expand_rank(const ExpandTcArgs& g, const Rows& rows, cudaStream_t stream) {
   const int64_t tiles = (g.M + kERows - 1) / kERows * ((g.N + kECols - 1) / kECols);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(tiles, device_sm_count())));
   return chained("lora expand",
-                 launch_chained(g.early != 0, k, grid, kEThreads, bytes, stream, ty, tw, to,
+                 launch_chained(true, k, grid, kEThreads, bytes, stream, ty, tw, to,
                                 static_cast<const __nv_bfloat16*>(g.y), static_cast<__nv_bfloat16*>(g.out), g.counts,
                                 g.part, g.splits, g.scaling, rows, static_cast<int>(g.N), static_cast<int>(g.R)));
 }
@@ -1249,7 +1249,7 @@ int pieces_rank(const RankPiecesArgs& g, const Rows& rows, cudaStream_t stream) 
   const RankSide a{g.part_a, g.splits_a, g.row_mul_a, static_cast<__nv_bfloat16*>(g.out_a)};
   const RankSide b{g.part_b, g.splits_b, nullptr, static_cast<__nv_bfloat16*>(g.out_b)};
   return chained("lora rank pieces",
-                 launch_chained(g.early != 0, rank_pieces_kernel<kRank>, dim3(static_cast<unsigned>(tiles), 2), 256, 0,
+                 launch_chained(true, rank_pieces_kernel<kRank>, dim3(static_cast<unsigned>(tiles), 2), 256, 0,
                                 stream, a, b, g.scaling, rows, g.R, tiles * kTile, g.info));
 }
 

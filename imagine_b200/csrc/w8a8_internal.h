@@ -201,7 +201,6 @@ struct ShrinkTcArgs {
   float* part;
   int* counts;    // out: the adapters of every 128 rows (may be NULL)
   int first;      // the call's first kernel
-  int early;      // starts while the kernel before it runs (launch_chained), as below
 };
 struct ExpandTcArgs {
   const void* y;  // or NULL
@@ -216,7 +215,6 @@ struct ExpandTcArgs {
   void* out;
   int64_t ldo;
   int64_t M, N, S, R;
-  int early;
 };
 struct TokensTcArgs {
   const void* x;
@@ -229,7 +227,6 @@ struct TokensTcArgs {
   const uint8_t* info;
   float* part;
   int* found;
-  int early;
 };
 struct RankPiecesArgs {
   const float* part_a;  // the rank side that meets x (its row scale in row_mul_a), and dy
@@ -242,7 +239,6 @@ struct RankPiecesArgs {
   const float* scaling;
   int R;
   uint8_t* info;
-  int early;
 };
 int lora_shrink_tc(const ShrinkTcArgs& g, const LoraRows& rows, cudaStream_t stream);
 int lora_expand_tc(const ExpandTcArgs& g, const LoraRows& rows, cudaStream_t stream);
