@@ -872,9 +872,26 @@ int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 // ---- the tcgen05 form (lora_sm100.cu): long bf16 batches of a few adapters whose
 // operands TMA can take (16-byte rows).
 constexpr int64_t kTcRows = 256;
-bool tc_shape(const LoraArgs& g) {
-  return g.dtype == W8A8_BF16 && g.M >= kTcRows && g.M <= (1ll << 27) && g.S <= 64 && g.K % 8 == 0 && g.N % 8 == 0 && g.R % 8 == 0 &&
-         g.K > 0 && g.N > 0;
+constexpr int64_t kTcAdapters = 64;
+// Whether a call is work enough for it, M (N + K) elements of the batch.  It reads them at a
+// higher rate but has more kernels (a gradient seven against four) and longer prologues, and the
+// mma.sync form goes through a tile's adapters one after another.  Captured calls, memory
+// cold, rank 16 and 64, us (tcgen05 / mma.sync):
+//   gradients  one adapter     256 x 768 -> 256 (0.3 Mi) 35 / 18, 45 / 25;  3000 x 512 -> 512 (2.9 Mi) 45 / 33, 57 / 47;
+//                              1000 x 2048 -> 2048 (3.9 Mi) 41 / 35, 57 / 59;  700 x 4096 -> 4096 (5.5 Mi) 43 / 47, 66 / 80;
+//                              6000 x 4096 -> 4096 (47 Mi) 84 / 160, 104 / 244
+//              32, mixed rows  256 x 4096 -> 4096 (2.0 Mi) 291 / 254, 538 / 504;  1500 x 1024 -> 1024 (2.9 Mi) 313 / 393, 584 / 642
+//   forward    one adapter     6000 x 256 -> 256 (2.9 Mi) 21 / 14, 25 / 18;  2000 x 2048 -> 2048 (7.8 Mi) 25 / 23, 33 / 33;
+//                              2000 x 4096 -> 4096 (16 Mi) 29 / 33, 43 / 47
+//              32, mixed rows  256 x 1024 -> 1024 (0.5 Mi) 41 / 31, 45 / 43;  256 x 4096 -> 4096 (2.0 Mi) 47 / 101, 55 / 162
+bool tc_work(int64_t M, int64_t N, int64_t K, int64_t S, bool backward) {
+  if (M < kTcRows || S > kTcAdapters) return false;
+  const int64_t mi = S <= 8 ? (backward ? 5 : 8) : (backward ? 3 : 2);
+  return M * (N + K) >= mi << 20;
+}
+bool tc_shape(const LoraArgs& g, bool backward) {
+  return g.dtype == W8A8_BF16 && g.M <= (1ll << 27) && g.K % 8 == 0 && g.N % 8 == 0 && g.R % 8 == 0 && g.K > 0 &&
+         g.N > 0 && tc_work(g.M, g.N, g.K, g.S, backward);
 }
 bool tc_rows(const void* p, int64_t ld, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0;
@@ -1042,7 +1059,7 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
   if (few_rows(g.M)) return add_few_rows<T>(g, rows, part, stream);
   Split sp = shrink_split(g.M, K);
   int* counts = nullptr;
-  if (tc_shape(g) && tc_x(g) && tc_weights(g.a, g.lda, K, g.S)) {
+  if (tc_shape(g, false) && tc_x(g) && tc_weights(g.a, g.lda, K, g.S)) {
     sp = shrink_tc_split(g.M, K);
     counts = reinterpret_cast<int*>(part + sp.count * g.M * g.R);
     if (int rc = shrink_tc(g, g.x, g.ldx, false, nullptr, g.a, g.lda, true, K, sp, part, counts, true, stream)) return rc;
@@ -1094,7 +1111,7 @@ template <typename T, typename TX>
 int backward_typed(const LoraArgs& g, cudaStream_t stream) {
   const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
   const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
-  const bool tc = tc_shape(g) && tc_x(g) && tc_rows(g.y, g.ldy, 2) && tc_weights(g.a, g.lda, g.K, g.S) &&
+  const bool tc = tc_shape(g, true) && tc_x(g) && tc_rows(g.y, g.ldy, 2) && tc_weights(g.a, g.lda, g.K, g.S) &&
                   tc_weights(g.b, g.ldb, g.R, g.S);
   const BackwardPlan p = backward_plan(g.M, g.N, g.K, g.S, g.R, tc, g.da != nullptr);
   uint8_t* ws = static_cast<uint8_t*>(g.workspace);
@@ -1179,7 +1196,7 @@ int64_t lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t S, int64_t
   }
   const bool weights = backward == 1;
   const BackwardPlan plain = backward_plan(M, N, K, S, R, false, weights);
-  const bool tc = M >= kTcRows && S <= 64;
+  const bool tc = tc_work(M, N, K, S, true);
   const BackwardPlan other = tc ? backward_plan(M, N, K, S, R, true, weights) : plain;
   return !weights ? std::max(plain.off_a, other.off_a) : std::max(plain.bytes, other.bytes);
 }

@@ -271,8 +271,8 @@ def test_as_many_adapters_in_a_block_as_tensor_memory_holds(s, r, codes):
 
 
 @pytest.mark.parametrize("m,k,n,s,r", [
-    (700, 264, 4096, 4, 16), (700, 4096, 512, 16, 64), (1500, 264, 2048, 64, 16), (1500, 2048, 264, 9, 128),
-    (3000, 512, 520, 64, 64), (2000, 1032, 1544, 5, 40)])
+    (2000, 264, 4096, 4, 16), (700, 4096, 512, 16, 64), (1500, 264, 2048, 64, 16), (1500, 2048, 264, 9, 128),
+    (3100, 512, 520, 64, 64), (3300, 1032, 1544, 5, 40)])
 @pytest.mark.parametrize("order", ["mixed", "runs", "some"])
 def test_many_adapters_in_tiles_of_blocks_with_several(m, k, n, s, r, order):
     """More tiles than multiprocessors, so that a block goes through several, each with as many products
@@ -297,3 +297,127 @@ def test_many_adapters_in_tiles_of_blocks_with_several(m, k, n, s, r, order):
     _quiet()
     ref, size = _grad_ref(x, dy, a, b, c, idx)["dx"]
     _check(dx, ref + base.double(), size, 2 * PIECES[dy.dtype] + _sums(n, r), "dx added")
+
+
+# The tcgen05 form takes batches from 256 rows on of 5 to 8 Mi elements (2 to 3 Mi with more than eight
+# adapters): the smallest and oddest of those, of every padded rank.
+LONG = [
+    (1300, 4104, 2568, 1, 8), (2049, 4096, 72, 2, 16), (2049, 72, 4096, 2, 24), (257, 16400, 16392, 3, 24),
+    (511, 8200, 8328, 5, 32), (1000, 1544, 7000, 4, 64), (777, 5504, 5512, 2, 128), (3001, 2048, 776, 7, 40),
+    (1290, 3208, 3320, 3, 104), (256, 8200, 4200, 64, 16)]
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("m,k,n,s,r", LONG)
+def test_every_rank_and_ragged_ends_of_long_batches(m, k, n, s, r, codes):
+    test_every_rank_and_ragged_ends(m, k, n, s, r, codes)
+
+
+def test_nan_stays_in_its_rows_and_adapters_of_long_batches():
+    import imagine_b200 as W
+
+    m, k, n, s, r = 2100, 2048, 2056, 3, 16
+    x, y, dy, a, b, c, _ = _case(m, k, n, s, r, torch.bfloat16)
+    idx = _ragged(m, s, 11)
+    idx[100:140], idx[600:650], idx[300:310], idx[1900:1905] = 1, 1, -1, 1
+    clean, grads = W.lora_add(y, x, a, b, idx, c), W.lora_backward(dy, x, a, b, idx, c)
+    bad = idx == 1
+    for v in (float("nan"), float("inf")):
+        xb, yb, dyb, ab, bb = x.clone(), y.clone(), dy.clone(), a.clone(), b.clone()
+        xb[bad], yb[bad], dyb[bad], ab[1], bb[1] = v, v, v, v, v
+        xb[idx < 0], dyb[idx < 0] = v, v
+        out = W.lora_add(yb, xb, ab, bb, idx, c)
+        assert torch.equal(out[~bad], clean[~bad]) and not bool(out[bad].isfinite().any())
+        dx, da, db = W.lora_backward(dyb, xb, ab, bb, idx, c)
+        assert torch.equal(dx[~bad], grads[0][~bad]) and not bool(dx[bad].isfinite().any())
+        for t, ref in ((da, grads[1]), (db, grads[2])):
+            assert torch.equal(t[[0, 2]], ref[[0, 2]]) and not bool(t[1].isfinite().any())
+    _quiet()
+
+
+def test_operands_of_long_batches_that_lie_elsewhere():
+    """Rows a multiple of 16 bytes apart, a stack's every second adapter, samples of a batch: the same
+    bits; the output's surroundings left as they were; rows that TMA cannot take: the same values."""
+    import imagine_b200 as W
+
+    bt, t, k, n, s, r = 3, 700, 2056, 2040, 4, 16
+    m = bt * t
+    x, y, dy, a, b, c, _ = _case(m, k, n, s, r, torch.bfloat16)
+    sample = torch.tensor([2, -1, 0], device="cuda")
+    token = sample.repeat_interleave(t)
+    want, grads = W.lora_add(y, x, a, b, token, c), W.lora_backward(dy, x, a, b, token, c)
+    for p, q in zip(W.lora_backward(dy.view(bt, t, n), x.view(bt, t, k), a, b, sample, c), grads):
+        assert torch.equal(p.reshape(q.shape), q)
+    assert torch.equal(W.lora_add(y.view(bt, t, n), x.view(bt, t, k), a, b, sample, c).view(m, n), want)
+
+    def apart(v, pad, at):
+        big = torch.full((v.shape[0], v.shape[1] + pad), float("nan"), dtype=v.dtype, device="cuda")
+        big[:, at:at + v.shape[1]] = v
+        return big[:, at:at + v.shape[1]]
+    a2 = torch.full((2 * s, r, k), float("nan"), dtype=a.dtype, device="cuda")
+    b2 = torch.full((2 * s, n, r), float("nan"), dtype=a.dtype, device="cuda")
+    a2[::2], b2[::2] = a, b
+    xa, ya, dya = apart(x, 24, 8), apart(y, 16, 16), apart(dy, 8, 0)
+    wide = torch.full((m + 1, n + 24), 7.0, dtype=y.dtype, device="cuda")
+    W.lora_add(ya, xa, a2[::2], b2[::2], token, c, out=wide[:m, 8:8 + n])
+    assert torch.equal(wide[:m, 8:8 + n], want) and bool((wide[m] == 7).all())
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 8 + n:] == 7).all())
+    base = torch.full((m + 1, k + 16), 7.0, dtype=y.dtype, device="cuda")
+    base[:m, 8:8 + k] = 0
+    got = W.lora_backward(dya, xa, a2[::2], b2[::2], token, c, dx=base[:m, 8:8 + k])
+    assert all(torch.equal(p, q) for p, q in zip(got, grads))
+    assert bool((base[:, :8] == 7).all()) and bool((base[:, 8 + k:] == 7).all()) and bool((base[m] == 7).all())
+    for p, q in zip(W.lora_backward(apart(dy, 3, 1), apart(x, 5, 2), a, b, token, c), grads):
+        assert float((p.double() - q.double()).norm() / q.double().norm()) < 2.0 ** -8
+    odd = W.lora_add(apart(y, 1, 0), apart(x, 3, 1), a, b, token, c)
+    _check(odd, *_add_ref(x, y, a, b, c, token), 2 * PIECES[x.dtype] + _sums(k, r))
+    # a dx or an out alone that TMA cannot take: the contraction's sums go to the other form's product
+    out = torch.empty(m, n + 3, dtype=y.dtype, device="cuda")[:, 1:1 + n]
+    _check(W.lora_add(y, x, a, b, token, c, out=out), *_add_ref(x, y, a, b, c, token), 2 * PIECES[x.dtype] + _sums(k, r))
+    odd = torch.zeros(m, k + 3, dtype=y.dtype, device="cuda")[:, 1:1 + k]
+    _check_grads(W.lora_backward(dy, x, a, b, token, c, dx=odd), x, dy, a, b, c, token)
+    _quiet()
+
+
+@pytest.mark.parametrize("m,n,k,s", [
+    (1279, 2048, 2048, 1), (1280, 2048, 2048, 1), (2047, 2048, 2048, 8), (2048, 2048, 2048, 8), (767, 2048, 2048, 9),
+    (768, 2048, 2048, 9), (511, 2048, 2048, 9), (512, 2048, 2048, 64), (2048, 2048, 2048, 65), (255, 20000, 20000, 2)])
+def test_borders_between_the_forms_by_work(m, n, k, s):
+    import imagine_b200 as W
+
+    r = 16
+    x, y, dy, a, b, c, idx = _case(m, k, n, s, r, torch.bfloat16, seed=8)
+    _check(W.lora_add(y, x, a, b, idx, c), *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(k, r))
+    _check_grads(W.lora_backward(dy, x, a, b, idx, c), x, dy, a, b, c, idx)
+    _quiet()
+
+
+def test_long_calls_on_three_streams():
+    """Contractions, products and sums over rows of three streams at once, with the linear and its input
+    gradient among them: each run has the bits of the call alone."""
+    import imagine_b200 as W
+
+    steps = []
+    for seed, (m, k, n, s, r) in enumerate(((1500, 4096, 2048, 3, 16), (3100, 512, 2048, 64, 64), (5000, 1024, 1024, 2, 128))):
+        x, y, dy, a, b, c, idx = _case(m, k, n, s, r, torch.bfloat16, seed=seed)
+        w = torch.randint(-127, 128, (n, k), device="cuda", dtype=torch.int8)
+        ws = torch.rand(n, device="cuda") * 1e-3
+        q, xs = W.quantize_int8_rowwise(x)
+
+        def step(x=x, dy=dy, a=a, b=b, c=c, idx=idx, w=w, ws=ws, q=q, xs=xs):
+            base = W.int8_linear_backward(dy, w, ws)
+            z = W.lora_add(W.int8_linear(x, w, ws), x, a, b, idx, c)
+            return (z, *W.lora_backward(dy, q, a, b, idx, c, x_scale=xs, dx=base), *W.act_checkpoint_int8(z))
+        steps.append(step)
+    want = [f() for f in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(4):
+        got = []
+        for f, st in zip(steps, streams):
+            with torch.cuda.stream(st):
+                got.append(f())
+        torch.cuda.synchronize()
+        for run, ref in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(run, ref))
+    _quiet()
