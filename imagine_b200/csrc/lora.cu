@@ -474,8 +474,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && kRank <= 64 ? 2 : 
 // what has to be read is the adapters' weights, once, and latency counts.  The
 // second kernel starts while the first runs (programmatic dependent launch): its
 // weights and y are on their way when h arrives.
-// 64 rows, 32 adapters of rank 32, 4096 -> 12288: 9 and 13 us where the tiles took
-// 16 and 96 (their blocks go through their adapters one after another).
+// 64 rows, 32 adapters of rank 32, 4096 -> 12288: 9 and 13 us.  Which calls: few_rows below.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) shrink_row_kernel(const T* __restrict__ x, int64_t ldx,
                                                               const T* __restrict__ a, int64_t slot,
@@ -1029,8 +1028,20 @@ int tokens_pair(const TokensArgs<TX>& a, const TokensArgs<T>& b, const float* sc
   return chained("lora tokens", e);
 }
 
-// Up to one tile of rows.
-bool few_rows(int64_t M) { return M <= kBM; }
+// Whether up to one tile of rows goes row by row: each reads its adapter again, M R (K + N) elements
+// of weights through L2, where a tile reads an adapter once but goes through its adapters, of which
+// it has min(S, M) at most, one after another.  Captured calls, memory cold, 4096 -> 12288
+// in bf16, us (rows / tiles):
+//   one adapter   16 rows  rank 16 10 / 14, rank 64 20 / 16;  64 rows  rank 16 18 / 16, rank 32 23 / 16, rank 128 86 / 29
+//   four          16 rows  rank 64 21 / 23, rank 128 31 / 33;  64 rows  rank 16 18 / 21, rank 64 49 / 27
+//   thirty-two    64 rows  rank 16 18 / 55, rank 32 27 / 64, rank 128 92 / 203
+// f16 and fp32 tiles multiply pieces and pay later, 4096 -> 4096, one adapter: 32 rows of rank 128
+// 31 / 33 (fp32 37 / 55), 64 rows of rank 64 27 / 27 (37 / 37), of rank 128 46 / 39 (66 / 62).
+bool few_rows(const LoraArgs& g) {
+  if (g.M > kBM) return false;
+  const int64_t adapters = std::min(g.S, g.M);
+  return g.M * g.R <= (g.dtype == W8A8_BF16 ? 256 * (adapters + 3) : 512 * (adapters + 8));
+}
 
 template <typename T>
 int add_few_rows(const LoraArgs& g, const Rows& rows, float* h, cudaStream_t stream) {
@@ -1056,7 +1067,7 @@ int add_typed(const LoraArgs& g, cudaStream_t stream) {
   const Rows rows{g.adapter, g.adapter64, g.rows_per_index, g.M, static_cast<int>(g.S)};
   const int K = static_cast<int>(g.K), N = static_cast<int>(g.N), R = static_cast<int>(g.R);
   float* part = static_cast<float*>(g.workspace);
-  if (few_rows(g.M)) return add_few_rows<T>(g, rows, part, stream);
+  if (few_rows(g)) return add_few_rows<T>(g, rows, part, stream);
   Split sp = shrink_split(g.M, K);
   int* counts = nullptr;
   if (tc_shape(g, false) && tc_x(g) && tc_weights(g.a, g.lda, K, g.S)) {

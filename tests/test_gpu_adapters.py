@@ -480,3 +480,18 @@ def test_bf16_input_gradient_is_the_same_product_in_every_form(k, n, scalar):
         for d in (dy, apart):
             for v in (w, wide):
                 _check(W.int8_linear_backward(d[:rows], v, ws), ref[:rows], size[:rows], rel, f"{rows} rows")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,s,r", [(1, 1, 128), (8, 1, 128), (9, 1, 128), (64, 1, 16), (64, 1, 17), (33, 1, 100), (64, 4, 28),
+                                   (64, 4, 29), (64, 64, 128), (64, 1, 72), (64, 8, 128), (2, 70, 5)])
+def test_lora_add_of_up_to_64_rows_in_either_form(m, s, r, dtype):
+    """Row by row or as a tile, by the rows' share of each adapter; k and n that vectors take and not."""
+    import imagine_b200 as W
+
+    for k, n in ((512, 384), (130, 257)):
+        x, y, _, a, b, c, idx = _case(m, k, n, s, r, DTYPES[dtype], seed=9)
+        out = W.lora_add(y, x, a, b, idx, c)
+        _check(out, *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(k, r), "out")
+        assert torch.equal(out[idx < 0], y[idx < 0])
+        assert torch.equal(out, W.lora_add(y.clone(), x, a, b, idx, c, out=y))
