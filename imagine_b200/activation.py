@@ -100,5 +100,7 @@ class _Checkpointed(torch.autograd.Function):
 
 def checkpointed_activation(x: torch.Tensor, act: str = "gelu_tanh") -> torch.Tensor:
     """``act(x)``, differentiable, keeping x for the backward pass as its 8-bit
-    checkpoint (half of a bf16 input's bytes, and 1/32 more for the scales)."""
+    checkpoint (half of a bf16 input's bytes, and 1/32 of the codes' more for the scales).  A training
+    step that is captured into a CUDA graph is captured whole, with no eager graph of the same
+    leaves alive, as with any differentiable operator."""
     return _Checkpointed.apply(x, act)

@@ -166,7 +166,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     is no operand's memory otherwise.
 
     The contraction over K and the rank are summed in fp32 and the result is
-    rounded once; the same call gives the same bits."""
+    rounded once; the same call gives the same bits.  NaN and infinity stay in the rows (and
+    adapters) that hold them, where an infinity gives an infinity or a NaN."""
     dev = _cuda("x", x).device
     _same("y", y, dev)
     shape, dtype = x.shape, x.dtype
@@ -341,7 +342,8 @@ def int8_linear_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
                      keep_input: bool = False) -> torch.Tensor:
     """``lora_add(int8_linear(x, weight, weight_scale, bias), x, a, b, adapter,
     scaling)`` with gradients for x, a and b (the int8 weight, its scales and the
-    bias are frozen).
+    bias are frozen).  The linear is the plain one, [N, K] codes with N scales or one: no ConvRot
+    weight, input or output activation, or residual.
 
     For the backward pass it keeps the int8 codes that the linear made of x
     (half of a bf16 input's bytes), from which da and db are taken; with ``keep_input`` it

@@ -6,10 +6,13 @@
 //   h = x A[s]^T            out = y + c h B[s]^T
 //   g = dy B[s]             dx  = (dx +) c g A[s]
 //   dA[s] = c sum_m g^T x   dB[s] = c sum_m dy^T h      (m over the rows of s)
-// Three kernels do all of it:
-//   shrink  [rows, K] x [K, R]: contracts a row with an adapter (h and g)
-//   expand  [rows, R] x [R, N]: adds the low-rank product to a row (out, dx)
-//   tokens  [R, rows] x [rows, C]: contracts over the rows of an adapter (dA, dB)
+// Kernels (of long bf16 batches: lora_sm100.cu):
+//   shrink      [rows, K] x [K, R]: contracts a row with an adapter (h and g); both in one launch
+//               in the backward pass (shrink_pair_kernel)
+//   expand      [rows, R] x [R, N]: adds the low-rank product to a row (out, dx)
+//   tokens      [R, rows] x [rows, C]: contracts over the rows of an adapter (dA and dB in one launch)
+//   sum_splits  adds up the pieces of dA and dB that blocks of rows made
+//   shrink_row, expand_row   the first two for few rows, on CUDA cores
 //
 // Arithmetic.  The products run on the tensor cores as bf16 x bf16 -> fp32.  A
 // value that bf16 does not hold is cut into bf16 pieces that add up to it
@@ -20,8 +23,9 @@
 // than the last kept bit are dropped (pair()).  int8 codes are exact in bf16;
 // their row scale multiplies h, or the rank side of dA, in fp32.
 //
-// Rows of other adapters, and rows without one, never enter a product as data:
-// they are not loaded, so NaN or infinity there stays there.
+// Rows of other adapters, and rows without one, are not loaded here, so NaN or infinity there
+// stays there.  An infinity in a row or adapter in use gives an infinity or a NaN: pieces of one
+// factor meet it with either sign.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -14,6 +14,11 @@
 // third of it).  int8 codes (an 8-bit checkpoint as x) land as bytes and are
 // widened to bf16 by four warps on the way.
 //
+// What keeps rows of other adapters apart (NaN and infinity stay in their rows): shrink_tc and
+// expand_tc multiply every row of a tile by every adapter of the tile, but output rows are
+// independent and only the row's own adapter's result is stored; tokens_tc sums over rows, so
+// there the rows of other adapters are zeroed in both operands first.
+//
 // Waits are bounded (sm100_ptx.cuh): a wait that gives up records its code, every
 // role of the block falls through, and TMEM is released.
 #include <cuda.h>
@@ -1257,9 +1262,7 @@ int pieces_rank(const RankPiecesArgs& g, const Rows& rows, cudaStream_t stream) 
 
 int lora_shrink_tc(const ShrinkTcArgs& g, const LoraRows& r, cudaStream_t stream) {
   const Rows rows = rows_of(r);
-  if (g.codes) {
-    return g.w_rows ? shrink_codes<true, true>(g, rows, stream) : shrink_codes<true, false>(g, rows, stream);
-  }
+  if (g.codes) return shrink_codes<true, true>(g, rows, stream);  // codes are x, which meets A
   return g.w_rows ? shrink_codes<false, true>(g, rows, stream) : shrink_codes<false, false>(g, rows, stream);
 }
 

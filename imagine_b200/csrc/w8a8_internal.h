@@ -190,7 +190,7 @@ struct LoraRows {
 };
 struct ShrinkTcArgs {
   const void* x;  // bf16, or int8 codes
-  int codes;
+  int codes;      // with w_rows
   int64_t ldx;
   const float* x_scale;
   const void* w;

@@ -567,7 +567,9 @@ int w8a8_sampler_step(float* x, const void* out_cond, const void* out_uncond, in
  *     contiguous, in `dtype`, zero for an adapter without rows; both NULL: not wanted
  * x is `dtype`, or with x_scale (fp32 [M]) the int8 codes of the forward
  * quantiser (w8a8_quantize_rowwise): the activation's 8-bit checkpoint.
- * Sums are taken in a fixed order: the same call gives the same bits.
+ * Sums are taken in a fixed order: the same call gives the same bits.  NaN and
+ * infinity stay in the rows and adapters that hold them, where an infinity gives an
+ * infinity or a NaN.
  *
  * dx may not overlap dy, x, a, b, the index or the scales (refused).
  *

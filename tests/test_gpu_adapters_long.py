@@ -421,3 +421,32 @@ def test_long_calls_on_three_streams():
         for run, ref in zip(got, want):
             assert all(torch.equal(p, q) for p, q in zip(run, ref))
     _quiet()
+
+
+@pytest.mark.parametrize("m,k,n", [(200000, 512, 12288), (1100000, 2048, 2040)])
+def test_offsets_beyond_32_bits(m, k, n):
+    """Operands of more than 2^31 elements: the last rows against the formula."""
+    import imagine_b200 as W
+
+    s, r = 3, 16
+    x, y, a, b = (torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_(0, std)
+                  for shape, std in (((m, k), 1), ((m, n), 1), ((s, r, k), k ** -0.5), ((s, n, r), 0.5)))
+    assert y.numel() > 1 << 31
+    c = torch.ones(s, device="cuda")
+    idx = torch.arange(m, device="cuda") * s // m
+    last = slice(m - 300, m)
+    out = W.lora_add(y, x, a, b, idx, c)
+    _check(out[last], *_add_ref(x[last], y[last], a, b, c, idx[last]), 2 * PIECES[x.dtype] + _sums(k, r))
+    assert torch.equal(W.lora_add(y, x, a, b, torch.full_like(idx, -1), c, out=out)[last], y[last])
+    del out
+    dx = W.lora_backward(y, None, a, b, idx, c, need_weights=False)[0]
+    ref, size = _grad_ref(x[last], y[last], a, b, c, idx[last])["dx"]
+    _check(dx[last], ref, size, 2 * PIECES[y.dtype] + _sums(n, r))
+    w = torch.randint(-127, 128, (n, k), device="cuda", dtype=torch.int8)
+    dx = W.int8_linear_backward(y, w, torch.ones(1, device="cuda"))
+    _check(dx[last], y[last].double() @ w.double(), y[last].double().abs() @ w.double().abs(), _sums(n) + 8 * 2.0 ** -22)
+    o, q, scale = W.act_checkpoint_int8(y)
+    few = W.act_checkpoint_int8(y[last])
+    assert all(torch.equal(p[last], v) for p, v in zip((o, q, scale), few))
+    assert torch.equal(W.act_backward_int8(y, q, scale)[last], W.act_backward_int8(y[last], *few[1:]))
+    _quiet()
