@@ -19,6 +19,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native as N
 from . import linear as L
@@ -183,7 +184,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     m = math.prod(lead)
     idx, idx64, per = _index(adapter, lead, m, dev)
     c = _scaling(scaling, s, dev)
-    if out is None:
+    given = out is not None
+    if not given:
         out, ldo = (torch.empty_like(y) if y2 is y else y.new_empty(y.shape)), max(n, 1)
     else:
         ldo = _out_rows("out", out, y.shape, dtype, dev)
@@ -194,6 +196,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
             y2.data_ptr(), ldy, x2.data_ptr(), ldx, code, a.data_ptr(), slot_a, b.data_ptr(), slot_b,
             _ptr(idx), idx64, per, _ptr(c), out.data_ptr(), ldo, m, n, k, s, r, _ptr(ws), nbytes,
             _raw_stream(dev.index)))
+    if given:
+        increment_version(out)  # a graph that saved it says so
     return out
 
 
@@ -249,6 +253,8 @@ def lora_backward(dy: torch.Tensor, x: Optional[torch.Tensor], a: torch.Tensor, 
             dy2.data_ptr(), lddy, _ptr(x2), ldx, _ptr(xs), code, a.data_ptr(), slot_a, b.data_ptr(),
             slot_b, _ptr(idx), idx64, per, _ptr(c), _ptr(dx), lddx, accumulate, _ptr(da), _ptr(db), m,
             n, k, s, r, _ptr(ws), nbytes, _raw_stream(dev.index)))
+    if accumulate:
+        increment_version(dx)
     return dx, da, db
 
 

@@ -495,3 +495,25 @@ def test_lora_add_of_up_to_64_rows_in_either_form(m, s, r, dtype):
         _check(out, *_add_ref(x, y, a, b, c, idx), 2 * PIECES[x.dtype] + _sums(k, r), "out")
         assert torch.equal(out[idx < 0], y[idx < 0])
         assert torch.equal(out, W.lora_add(y.clone(), x, a, b, idx, c, out=y))
+
+
+def test_writing_into_a_saved_tensor_is_noticed():
+    """An output written in place counts as a change of it: a graph that saved its old values for the
+    backward pass raises instead of going on with the new ones."""
+    import imagine_b200 as W
+
+    x, y, dy, a, b, c, idx = _case(20, 64, 64, 2, 8, torch.float32)
+    leaf = y.clone().requires_grad_()
+    for write in (lambda t: W.lora_add(t, x, a, b, idx, c, out=t), lambda t: W.lora_backward(dy, x, a, b, idx, c, dx=t)):
+        held = leaf * 2
+        z = held * held
+        before = held._version
+        write(held.detach())
+        assert held._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+    # what is not written stays as it was
+    before = [t._version for t in (x, y, dy, a, b, c, idx)]
+    W.lora_add(y, x, a, b, idx, c)
+    W.lora_backward(dy, x, a, b, idx, c)
+    assert before == [t._version for t in (x, y, dy, a, b, c, idx)]
