@@ -183,7 +183,7 @@ static_assert(sizeof(Bars) <= kBarBytes, "barriers");
 // there, into accumulators of their own, as many at a time as TMEM has columns for.
 // The contraction is cut so that two blocks a multiprocessor are all there are.  Bound
 // by reading x: 11712 x 4096 at rank 64 in 30 us (98 MB, 3.3 TB/s), 5856 x 4096 at
-// rank 16 in 12 to 15, 11712 x 12288 in 76 (288 MB, 3.8 TB/s).
+// rank 16 in 12 to 15, 11712 x 12288 in 70 (288 MB, 4.1 TB/s).
 constexpr int kSRows = 128, kSK = 64;
 constexpr int kXTile = kSRows * kSK * 2;  // 16 KB
 template <bool kCodes, int kRank>
@@ -741,8 +741,8 @@ __global__ void __launch_bounds__(kThreads, 1) tokens_tc_kernel(
 // groups of four warps take the tiles in turn, add the product to y in place in shared
 // memory, and a TMA store takes the tile away.  Each group has two accumulators and two
 // pairs of barriers of its own: a wait tells apart only odd and even phases, so a warp has to
-// see every phase of a barrier it waits on, and a tile's products may be any number.  Bound by reading y and writing out: 11712 x 12288 at rank 64 in 117 us,
-// 561 MB of HBM traffic at 4.8 TB/s (a copy reaches 6.2).
+// see every phase of a barrier it waits on, and a tile's products may be any number.  Bound by reading y and writing out: 11712 x 12288 at rank 64 in 112 us,
+// 561 MB of HBM traffic at 5.0 TB/s (a copy reaches 6.5).
 // Three stages and one group of warps, twice a multiprocessor, waited for the loads:
 // 178 us on 11712 x 12288 at rank 64.
 // Every row of a tile keeps the h of its own adapter; a tile whose rows have
