@@ -18,13 +18,14 @@
 // value that bf16 does not hold is cut into bf16 pieces that add up to it
 // (each piece rounded from what is left): f16 into two, fp32 into three,
 // both exactly.  The rank-side values h and g are sums, kept in fp32, and enter
-// the next product as two pieces (2^-18, far below the rounding of a 16-bit
+// the next product as two pieces (2^-16 at most, far below the rounding of a 16-bit
 // output) or three for fp32 outputs.  Of the products of pieces, those smaller
 // than the last kept bit are dropped (pair()).  int8 codes are exact in bf16;
 // their row scale multiplies h, or the rank side of dA, in fp32.
 //
-// Rows of other adapters, and rows without one, are not loaded here, so NaN or infinity there
-// stays there.  An infinity in a row or adapter in use gives an infinity or a NaN: pieces of one
+// Rows of other adapters, and rows without one, do not enter a product (their values are not loaded,
+// their rank side is zero), and of a product only the adapter's own rows are stored, so NaN or
+// infinity there stays there.  An infinity in a row or adapter in use gives an infinity or a NaN: pieces of one
 // factor meet it with either sign.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
